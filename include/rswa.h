@@ -328,6 +328,124 @@ int rswa_attn_bwd_dkdv_keys(const rswa_attn_params* p);
  * bits either way); a negative status if the call would be refused. */
 int rswa_attn_fwd_blocks_per_cu(const rswa_attn_params* p);
 
+/*
+ * Serving from an 8-bit paged cache.  No counterpart in the upstream package, whose attention is for training and
+ * whole prompts: these calls continue a sequence whose prompt the calls above have computed, token by token, chunk by
+ * chunk, or for a batch of sequences at once.
+ *
+ * Keys and values are held as e4m3 codes (OCP 8-bit floating point: 4 exponent and 3 mantissa bits, no infinity)
+ * times one power of two for each (page, kv head), itself a byte e that stands for 2^(e - 127) (e8m0).  A page holds
+ * page_size tokens (16, 32, 64, 128 or 256) of one sequence:
+ *   k        [num_pages, heads_kv, page_size, head_dim]           one byte an element
+ *   v        [num_pages, heads_kv, page_size / 16, head_dim, 16]  the 16 keys of a group are adjacent
+ *   k_scale, v_scale   [num_pages, heads_kv]                      one byte an element
+ * (V lies as the matrix instruction wants it: 16 bytes are 16 keys of one dimension.)  Page and head strides are the
+ * caller's, in bytes, those of k and v multiples of 16; within a (page, head) the bytes are dense.
+ *
+ * Token t of sequence b is in page page_table[b * page_table_stride + t / page_size] at place t % page_size.  An id
+ * outside [0, num_pages) (-1, say) is a page that is not there: its keys are seen by nobody, tokens that would go
+ * there are not written.  seqlens[b] counts a sequence's tokens; what a row of the table cannot hold is cut off.
+ * Nothing on the device is read by the host.
+ *
+ * Queries are the last rows of their sequence: row i of n is token seqlens[b] - n + i and sees the keys of tokens
+ *   j <= seqlens[b] - n + i  and  (window_left < 0  or  j >= seqlens[b] - n + i - window_left  or  j < num_sink)
+ * which is the rule of rswa_attn_fwd with causal != 0, bottom-right aligned.  Rows that see nothing: out = 0,
+ * lse = -inf.  Dense rows are [batch, seqlen_q, heads, head_dim]; with cu_seqlens_q (int32, batch + 1 entries on the
+ * device) [total_q, heads, head_dim], and rows behind cu_seqlens_q[batch] are left alone.
+ */
+typedef struct rswa_cache_params {
+  int32_t dtype;     /* RSWA_BF16 or RSWA_F16: type of q, out, new_k, new_v */
+  int32_t head_dim;  /* 64 or 128 */
+  int32_t batch;
+  int32_t heads_q;   /* attn, weights: a multiple of heads_kv */
+  int32_t heads_kv;
+  int32_t page_size;
+  int32_t num_pages;
+  int32_t max_pages; /* entries of a row of page_table; max_pages * page_size < 2^28 */
+  void* k;
+  void* v;
+  void* k_scale;
+  void* v_scale;
+  int64_t k_stride[2]; /* page, head */
+  int64_t v_stride[2];
+  int64_t k_scale_stride[2];
+  int64_t v_scale_stride[2];
+  const int32_t* page_table;
+  int64_t page_table_stride;
+  const int32_t* seqlens; /* append: tokens held before the call; else: all tokens, the queries' own among them */
+
+  int32_t seqlen_q; /* dense: rows per sequence */
+  int64_t total_q;  /* packed: rows */
+  const int32_t* cu_seqlens_q;
+
+  /* attn, weights */
+  float softmax_scale;
+  int32_t window_left; /* < 0 (or >= 2^28): unbounded */
+  int32_t num_sink;
+  const void* q;
+  int64_t q_stride[3];   /* batch, row, head; rows 16-byte aligned */
+  void* out;             /* attn */
+  int64_t out_stride[3];
+  float* lse;            /* attn: written (NULL: not wanted); weights: read */
+  int64_t lse_stride[3]; /* batch, head, row */
+  void* workspace;       /* attn: rswa_cache_attn_workspace_bytes(), 16-byte aligned, uninitialised */
+  uint64_t workspace_bytes;
+
+  /* append */
+  const void* new_k;
+  const void* new_v;
+  int64_t new_k_stride[3]; /* batch, row, head; rows 16-byte aligned */
+  int64_t new_v_stride[3];
+
+  /* weights, evict: fp32 [batch, heads_kv, weights_len] running sums */
+  float* weights;
+  int64_t weights_stride[2]; /* batch, head */
+  int32_t weights_len;
+
+  /* evict */
+  int32_t budget;
+  int32_t num_recent;
+  const int32_t* new_page_table;
+  int64_t new_page_table_stride;
+  int32_t new_max_pages;
+  int32_t* new_seqlens;  /* [batch] */
+  float* new_weights;    /* [batch, heads_kv, weights_len], dense */
+  int32_t* kept;         /* [batch, heads_kv, budget], dense */
+} rswa_cache_params;
+
+/*
+ * Writes new_k and new_v [.., heads_kv, head_dim] behind the tokens that the sequences hold.  The scale of a (page,
+ * head) is the least 2^e, -120 <= e <= 120, with max |x| <= 448 * 2^e over the finite values written to the page; where
+ * the page holds tokens from before, the larger of that and its present scale, and if it grows the codes from before
+ * are rounded anew to the nearest (ties to even; exactly, but for what falls below the smallest normal code).  Infinities
+ * and NaN are stored as NaN.  Pages of different sequences of one call must differ.
+ */
+int rswa_cache_append(const rswa_cache_params* p, void* stream);
+
+/* Attention of q over the cache: out, and the natural-log lse if asked for.  fp32 sums whatever the types. */
+int rswa_cache_attn(const rswa_cache_params* p, void* stream);
+/* Scratch of such a call: partial results of rows whose keys several blocks share. */
+uint64_t rswa_cache_attn_workspace_bytes(const rswa_cache_params* p);
+
+/*
+ * Adds to weights[b, kv head, j] the softmax weights exp(softmax_scale * q.k_j - lse) of cached key j, summed over the
+ * call's rows that see it and the q heads of the group; lse as rswa_cache_attn gives it (a row whose lse is -inf adds
+ * nothing).  Keys from weights_len on are passed over.  No atomics: run-to-run deterministic.
+ */
+int rswa_cache_weights(const rswa_cache_params* p, void* stream);
+
+/*
+ * Cuts every sequence to at most `budget` tokens, for each kv head by itself: kept are the first num_sink, the last
+ * num_recent, and of the others those with the largest weights (equal ones: the earlier; NaN: as the least), in their
+ * order.  Their codes go to the pages of new_page_table, from place 0 on, at the scale that fits the values in each new
+ * page; new_seqlens[b] = min(seqlens[b], budget); new_weights gets their weights, zeros behind; kept gets the tokens'
+ * old numbers, -1 behind.  The old pages are only read (they may be shared with other sequences), and no page may be
+ * both.  num_sink + num_recent <= budget.
+ */
+int rswa_cache_evict(const rswa_cache_params* p, void* stream);
+
+uint64_t rswa_sizeof_cache_params(void);
+
 /* Message of the calling thread's last failed call ("" if none). */
 const char* rswa_last_error(void);
 

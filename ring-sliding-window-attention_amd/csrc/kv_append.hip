@@ -1,0 +1,195 @@
+// New keys and values into the 8-bit paged cache.
+//
+// A block takes one page of one kv head, the first half of its threads the keys, the second the values.  A thread has
+// 16 tokens (a group) of 8 dimensions: 16 loads of 16 bytes, all in flight before the first use, hold the whole page in
+// registers, so that its largest value is known before the first code is made and memory is read once.  Keys leave as
+// 8 bytes a row, values as 16 bytes a dimension (the transpose is a choice of registers).
+#include "kv_cache.h"
+
+namespace rswa {
+namespace {
+
+struct AppendArgs {
+  CacheArgs c;
+  const void* x[2];  // new keys, values
+  int64_t x_st[2][3];
+  int32_t pages;     // dense: pages that a sequence's new tokens touch at most
+};
+
+template <typename T, int D>
+__global__ void cache_append_kernel(const AppendArgs a) {
+  using V8 = typename Mma<T>::V8;
+  constexpr int LANES = D / 8;
+  __shared__ uint32_t amax[2];
+  const CacheArgs& c = a.c;
+  const int page_size = 1 << c.page_log2;
+  const int hk = blockIdx.x % c.heads_kv;
+  int u = blockIdx.x / c.heads_kv, b, row0, n;
+  // sequence, and which of its touched pages
+  if (c.cu) {
+    // sequence b owns the slots from cu[b] / page_size + 2 b on: n tokens touch at most n / page_size + 2 pages.
+    // (a search 64 ways at a time, as locate_packed)
+    const int lane = lane_id();
+    int lo = 0, cnt = c.batch;
+    for (;;) {
+      const int step = (cnt + 63) >> 6;
+      const int i = min(lo + lane * step, lo + cnt - 1);
+      const int slot = (max(0, min(c.cu[i], c.total_q)) >> c.page_log2) + 2 * i;
+      const int at = max(__popcll(__builtin_amdgcn_ballot_w64(lane * step < cnt && slot <= u)) - 1, 0);
+      lo += at * step;
+      if (step == 1) break;
+      cnt = min(step, cnt - at * step);
+    }
+    b = __builtin_amdgcn_readfirstlane(lo);
+    rows_of(c, b, row0, n);
+    u -= (row0 >> c.page_log2) + 2 * b;
+  } else {
+    b = u / a.pages;
+    u -= b * a.pages;
+    row0 = 0;
+    n = c.seqlen_q;
+  }
+  if (u < 0) return;
+  const int start = max(0, c.lens[b]);
+  const int in_seq = (start >> c.page_log2) + u;  // page of the sequence
+  if (in_seq >= c.max_pages) return;
+  const int from = u == 0 ? start & (page_size - 1) : 0;     // first place written
+  const int i0 = (in_seq << c.page_log2) + from - start;     // its token among the new ones
+  const int count = min(page_size - from, n - i0);
+  if (count <= 0) return;
+  const int id = c.table[(int64_t)b * c.table_st + in_seq];
+  if ((uint32_t)id >= (uint32_t)c.num_pages) return;
+
+  const int half = blockDim.x / 2;
+  const int which = threadIdx.x >= half;
+  const int t = threadIdx.x - which * half;
+  const int d0 = t % LANES * 8, g = t / LANES;  // 8 dimensions, group of 16 places
+  const bool mine = g < (page_size >> 4);       // (blocks of small pages have threads left over)
+  const int lo = max(0, from - g * 16), hi = min(16, from + count - g * 16);  // its places written: lo <= e < hi
+
+  const T* x = (const T*)a.x[which] + (int64_t)b * a.x_st[which][0] + (int64_t)hk * a.x_st[which][2] + d0;
+  V8 v[16];
+  if (threadIdx.x < 2) amax[threadIdx.x] = 0;
+#pragma unroll
+  for (int e = 0; e < 16; e++)
+    if (mine && e >= lo && e < hi)
+      v[e] = *(const V8*)(x + (int64_t)(row0 + i0 + g * 16 + e - from) * a.x_st[which][1]);
+    else
+      v[e] = V8{};
+  float most = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; e++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float y = __builtin_fabsf((float)v[e][i]);
+      most = y < __builtin_inff() ? fmaxf(most, y) : most;
+    }
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) most = fmaxf(most, __shfl_xor(most, s));  // (a wave has keys or values)
+  __syncthreads();
+  // (a positive float's bits grow with it)
+  if (lane_id() == 0) atomicMax(&amax[which], __builtin_bit_cast(uint32_t, most));
+  __syncthreads();
+  uint8_t* const scale = which ? const_cast<uint8_t*>(c.v_scale) + (int64_t)id * c.vs_st[0] + (int64_t)hk * c.vs_st[1]
+                               : const_cast<uint8_t*>(c.k_scale) + (int64_t)id * c.ks_st[0] + (int64_t)hk * c.ks_st[1];
+  const int was = from > 0 ? *scale : 0;
+  const int e_new = max(was, scale_byte(__builtin_bit_cast(float, amax[which])));
+  const float inv = inverse(e_new);
+  const bool grown = from > 0 && e_new > was;
+  // 2^(was - e_new): zero where that is below the least normal number, as every code times it is
+  const float shrink = grown && e_new - was < 127 ? __builtin_bit_cast(float, (uint32_t)(127 - (e_new - was)) << 23) : 0.f;
+  __syncthreads();  // (all have read the scale)
+  if (!mine) return;
+  if (t == 0) *scale = (uint8_t)e_new;
+
+  uint32_t code[16][2];
+#pragma unroll
+  for (int e = 0; e < 16; e++)
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+      code[e][h] = codes4((float)v[e][4 * h] * inv, (float)v[e][4 * h + 1] * inv, (float)v[e][4 * h + 2] * inv,
+                          (float)v[e][4 * h + 3] * inv);
+  const int old = min(16, from - g * 16);  // places e < old hold tokens from before
+  if (!which) {
+    uint8_t* k = const_cast<uint8_t*>(c.k) + (int64_t)id * c.k_st[0] + (int64_t)hk * c.k_st[1] + g * 16 * D + d0;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      if (e >= lo && e < hi) {
+        *(u32x2*)(k + e * D) = u32x2{code[e][0], code[e][1]};
+      } else if (grown && e < old) {
+        const u32x2 w = *(const u32x2*)(k + e * D);
+        *(u32x2*)(k + e * D) = u32x2{rescale4(w[0], shrink), rescale4(w[1], shrink)};
+      }
+    }
+  } else {
+    uint8_t* vp = const_cast<uint8_t*>(c.v) + (int64_t)id * c.v_st[0] + (int64_t)hk * c.v_st[1] + (g * D + d0) * 16;
+    const bool full = lo == 0 && hi == 16;
+    if (full || (grown && old > 0)) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        u32x4 w = full ? u32x4{0, 0, 0, 0} : *(const u32x4*)(vp + i * 16);
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const uint32_t again = !full && grown ? rescale4(w[q], shrink) : 0u;
+          uint32_t r = 0;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int at = 4 * q + e;
+            const uint32_t fresh = code[at][i / 4] >> (8 * (i % 4));
+            const uint32_t byte = at >= lo && at < hi ? fresh : at < old ? again >> (8 * e) : w[q] >> (8 * e);
+            r |= (byte & 0xffu) << (8 * e);
+          }
+          w[q] = r;
+        }
+        *(u32x4*)(vp + i * 16) = w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; e++)
+        if (e >= lo && e < hi)
+#pragma unroll
+          for (int i = 0; i < 8; i++) vp[i * 16 + e] = (uint8_t)(code[e][i / 4] >> (8 * (i % 4)));
+    }
+  }
+}
+
+}  // namespace
+}  // namespace rswa
+
+extern "C" int rswa_cache_append(const rswa_cache_params* p, void* stream) {
+  using namespace rswa;
+  AppendArgs a;
+  if (int rc = cache_args(p, "cache_append", a.c)) return rc;
+  const int64_t rows = p->cu_seqlens_q ? p->total_q : (int64_t)p->batch * p->seqlen_q;
+  if (rows == 0 || p->batch == 0 || p->max_pages == 0) return RSWA_OK;
+  RSWA_REQUIRE(p->new_k && p->new_v, RSWA_ERR_INVALID, "cache_append: null tensor");
+  a.x[0] = p->new_k;
+  a.x[1] = p->new_v;
+  for (int i = 0; i < 3; i++) {
+    a.x_st[0][i] = p->new_k_stride[i];
+    a.x_st[1][i] = p->new_v_stride[i];
+  }
+  for (int w = 0; w < 2; w++) {
+    RSWA_REQUIRE((uintptr_t)a.x[w] % 16 == 0 && a.x_st[w][0] % 8 == 0 && a.x_st[w][1] % 8 == 0 && a.x_st[w][2] % 8 == 0,
+                 RSWA_ERR_UNSUPPORTED, "cache_append: rows of new_k and new_v must be 16-byte aligned");
+    if (p->cu_seqlens_q) a.x_st[w][0] = 0;
+  }
+  a.pages = (int32_t)((p->seqlen_q + p->page_size - 2) / p->page_size + 1);
+  const int64_t slots =
+      p->cu_seqlens_q ? p->total_q / p->page_size + 2 * (int64_t)p->batch : (int64_t)p->batch * a.pages;
+  const int64_t blocks = slots * p->heads_kv;
+  RSWA_REQUIRE(blocks < (1ll << 31), RSWA_ERR_UNSUPPORTED, "cache_append: %lld blocks", (long long)blocks);
+  const int threads = 2 * std::max(64, p->page_size / 16 * (p->head_dim / 8));
+  clear_launch_error();
+  auto go = [&](auto t, auto d) {
+    hipLaunchKernelGGL((cache_append_kernel<decltype(t), decltype(d)::value>), dim3((unsigned)blocks), dim3(threads), 0,
+                       (hipStream_t)stream, a);
+  };
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
+  if (p->dtype == RSWA_BF16)
+    p->head_dim == 128 ? go(__bf16{}, D128{}) : go(__bf16{}, D64{});
+  else
+    p->head_dim == 128 ? go(_Float16{}, D128{}) : go(_Float16{}, D64{});
+  return check_launch("cache_append");
+}

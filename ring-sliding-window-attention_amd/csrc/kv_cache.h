@@ -1,0 +1,216 @@
+// What the kernels over the 8-bit paged cache share: its layout, the lookup of pages, the range of keys that
+// queries see, and how a launch's blocks find their work without the host knowing any length.
+//
+// Register layouts of v_mfma_f32_16x16x32 (wave64): A (16 x 32): lane l holds row l%16, k = 8*(l/16) .. +7;
+// B (32 x 16): lane l holds column l%16, the same k; C (16 x 16): lane l holds column l%16, rows 4*(l/16) .. +3.
+#pragma once
+
+#include "attn_common.h"
+
+namespace rswa {
+
+constexpr int kTileKeys = 64;   // keys that a wave takes at a time
+constexpr int kGroupKeys = 16;  // keys of a group: 16 consecutive bytes for each dimension of V; never in two pages
+
+// Kernel-side view of rswa_cache_params.
+struct CacheArgs {
+  const uint8_t* k;
+  const uint8_t* v;
+  const uint8_t* k_scale;
+  const uint8_t* v_scale;
+  int64_t k_st[2], v_st[2];    // page, head (bytes)
+  int64_t ks_st[2], vs_st[2];  // page, head
+  const int32_t* table;
+  int64_t table_st;
+  const int32_t* lens;
+  const int32_t* cu;  // null: dense
+  int32_t num_pages, max_pages, page_log2;
+  int32_t batch, heads_q, heads_kv, group;
+  int32_t seqlen_q;  // dense
+  int32_t total_q;   // packed
+  int32_t window, n_sink;  // window < 0: unbounded
+  FastDiv by_group;
+  // rows
+  const void* q;
+  void* out;
+  float* lse;
+  int64_t q_st[3], o_st[3], lse_st[3];
+  float scale_log2;  // softmax_scale * log2(e)
+  // how the work is cut (see Plan)
+  int32_t row_tile;   // rows (token x grouped head) of a unit
+  int32_t min_chunk;  // least tiles of a unit
+  float per_unit;     // heads_kv / units wanted
+  // partial results of units whose rows have several (workspace)
+  float* part;        // [unit][row][D]
+  float* part_ml;     // [unit][row][2]: maximum in base 2, sum
+  int32_t part_units;
+  // running sums of softmax weights
+  float* weights;
+  int64_t w_st[2];
+  int32_t w_len;
+};
+
+__device__ __forceinline__ int lane_id() {
+  return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+}
+
+// Tokens that a sequence's row of the page table can hold at most bound its length: no lookup passes its end.
+__device__ __forceinline__ int held_tokens(const CacheArgs& a, int b) {
+  return max(0, min(a.lens[b], a.max_pages << a.page_log2));
+}
+
+// First row and number of rows of sequence b (a pack's: within the tensor whatever cu_seqlens holds).
+__device__ __forceinline__ void rows_of(const CacheArgs& a, int b, int& row0, int& n) {
+  if (a.cu) {
+    row0 = max(0, min(a.cu[b], a.total_q));
+    n = max(row0, min(a.cu[b + 1], a.total_q)) - row0;
+  } else {
+    row0 = 0;
+    n = a.seqlen_q;
+  }
+}
+
+// The tiles that rows at positions first .. last (the end of the sequence) see: those of the sink keys ahead of the
+// band, from tile 0 on, then n_band from tile t_lo on.
+struct SeenTiles {
+  int n_sink, t_lo, n_band;
+  __device__ __forceinline__ int count() const { return n_sink + n_band; }
+};
+__device__ __forceinline__ SeenTiles seen_tiles(const CacheArgs& a, int first, int last) {
+  SeenTiles t{0, 0, 0};
+  if (last < 0) return t;
+  const int lo = a.window < 0 ? 0 : max(0, first - a.window);
+  t.t_lo = lo / kTileKeys;
+  t.n_band = last / kTileKeys - t.t_lo + 1;
+  t.n_sink = min((min(a.n_sink, lo) + kTileKeys - 1) / kTileKeys, t.t_lo);
+  return t;
+}
+
+// Which sequence, row tile and share of its key tiles is unit `u`'s?
+//
+// The host knows no length.  Every wave reads all of them (64 at a time), sums the tiles of the whole call, and cuts
+// the tiles of every row tile into chunks of as many as give the launch about the units it was sized for: sequences
+// of any lengths make units of nearly one size, which the hardware then deals.  The grid is sized for the bound
+//   sum over sequences of row_tiles * ceil(tiles / chunk) <= units wanted / heads_kv + sum of row_tiles
+// and what is beyond the last unit ends at once.  Rows of sequences with several chunks are joined from partial
+// results; those sequences have at most twice the units wanted (ceil(x) <= 2 x for x > 1), which bounds the workspace.
+struct Unit {
+  int b, row_tile, chunk_idx, n_chunks;
+  int row0, n_rows, len;
+  int chunk;  // tiles
+  int part;   // first of the row tile's n_chunks partial results
+  SeenTiles tiles;
+};
+
+// JOIN: units are whole row tiles (chunk_idx stays 0).
+template <bool JOIN>
+__device__ __forceinline__ bool find_unit(const CacheArgs& a, int u, Unit& x) {
+  const int lane = lane_id();
+  int row0 = 0, n = 0, len = 0, row_tiles = 0;
+  SeenTiles t{0, 0, 0};
+  auto load = [&](int b) {
+    row_tiles = 0;
+    t = SeenTiles{0, 0, 0};
+    if (b < a.batch) {
+      rows_of(a, b, row0, n);
+      len = held_tokens(a, b);
+      row_tiles = (int)(((int64_t)n * a.group + a.row_tile - 1) / a.row_tile);
+      if (n > 0) t = seen_tiles(a, len - n, len - 1);
+    }
+  };
+  uint64_t total = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    load(b0 + lane);
+    total += (uint64_t)row_tiles * (uint64_t)t.count();
+  }
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) total += __shfl_xor(total, s);
+  x.chunk = max(a.min_chunk, (int)__builtin_ceilf((float)total * a.per_unit));
+  int before = 0, before_part = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    if (a.batch > 64) load(b0 + lane);
+    const int chunks = max(1, (t.count() + x.chunk - 1) / x.chunk);
+    const int units = JOIN ? row_tiles : row_tiles * chunks;
+    const int parts = chunks > 1 ? row_tiles * chunks : 0;
+    int su = units, sp = parts;  // inclusive sums
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const int tu = __shfl_up(su, s), tp = __shfl_up(sp, s);
+      if (lane >= s) {
+        su += tu;
+        sp += tp;
+      }
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(before + su > u);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+      x.b = b0 + at;
+      x.n_chunks = of(chunks);
+      const int in_seq = u - before - (of(su) - of(units));
+      x.row_tile = JOIN ? in_seq : in_seq / x.n_chunks;
+      x.chunk_idx = JOIN ? 0 : in_seq - x.row_tile * x.n_chunks;
+      x.part = before_part + of(sp) - of(parts) + x.row_tile * x.n_chunks;
+      x.row0 = of(row0);
+      x.n_rows = of(n);
+      x.len = of(len);
+      x.tiles.n_sink = of(t.n_sink);
+      x.tiles.t_lo = of(t.t_lo);
+      x.tiles.n_band = of(t.n_band);
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(su, 63);
+    before_part += __builtin_amdgcn_readlane(sp, 63);
+  }
+  return false;
+}
+
+// Two e4m3 codes (the low or the high half of a word) times a power of two, in the matrix operand's type: one
+// instruction, exact as long as the value fits the type.
+template <typename T, bool HIGH>
+__device__ __forceinline__ uint32_t widen2(uint32_t codes, float scale) {
+  if constexpr (std::is_same_v<T, __bf16>)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, HIGH));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, HIGH));
+}
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::V8 widen8(uint32_t lo, uint32_t hi, float scale) {
+  u32x4 r = {widen2<T, false>(lo, scale), widen2<T, true>(lo, scale), widen2<T, false>(hi, scale),
+             widen2<T, true>(hi, scale)};
+  return __builtin_bit_cast(typename Mma<T>::V8, r);
+}
+
+// Half of the power of two that scale byte `e` stands for.  Operands are taken at half their value (and scores and
+// outputs doubled, which costs nothing): rounding to e4m3 can raise a value just below the 16-bit type's largest
+// past it, and half of that is always there.
+__device__ __forceinline__ float half_scale(int e) {
+  return __builtin_bit_cast(float, (uint32_t)(max(e, 1) - 1) << 23);
+}
+
+// Byte of the least 2^e with amax <= 448 * 2^e (448 = 1.75 * 2^8), -120 <= e <= 120.
+__device__ __forceinline__ int scale_byte(float amax) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, amax);
+  const int e = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u);
+  return max(7, min(247, e));
+}
+__device__ __forceinline__ float inverse(int e) {  // 2^(127 - e)
+  return __builtin_bit_cast(float, (uint32_t)max(0, 254 - e) << 23);
+}
+
+// Four codes of fp32 values within +-448 (rounded to the nearest, ties to even; non-finite ones to NaN).
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+// Four codes times f <= 1, rounded anew.
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float f) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  return codes4(lo[0] * f, lo[1] * f, hi[0] * f, hi[1] * f);
+}
+
+// Checks of rswa_cache_params that every call makes, and the kernels' view of them.
+int cache_args(const rswa_cache_params* p, const char* who, CacheArgs& a);
+int cache_query_args(const rswa_cache_params* p, const char* who, CacheArgs& a);
+
+}  // namespace rswa

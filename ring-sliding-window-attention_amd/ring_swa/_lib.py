@@ -87,6 +87,65 @@ class AttnParams(Structure):
         ("dkdv_form", c_int32),
     ]
 
+
+_I64x2 = c_int64 * 2
+
+
+class CacheParams(Structure):
+    """Mirror of ``rswa_cache_params`` (include/rswa.h); field order is the ABI."""
+
+    _fields_ = [
+        ("dtype", c_int32),
+        ("head_dim", c_int32),
+        ("batch", c_int32),
+        ("heads_q", c_int32),
+        ("heads_kv", c_int32),
+        ("page_size", c_int32),
+        ("num_pages", c_int32),
+        ("max_pages", c_int32),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("k_scale", c_void_p),
+        ("v_scale", c_void_p),
+        ("k_stride", _I64x2),
+        ("v_stride", _I64x2),
+        ("k_scale_stride", _I64x2),
+        ("v_scale_stride", _I64x2),
+        ("page_table", c_void_p),
+        ("page_table_stride", c_int64),
+        ("seqlens", c_void_p),
+        ("seqlen_q", c_int32),
+        ("total_q", c_int64),
+        ("cu_seqlens_q", c_void_p),
+        ("softmax_scale", c_float),
+        ("window_left", c_int32),
+        ("num_sink", c_int32),
+        ("q", c_void_p),
+        ("q_stride", _I64x3),
+        ("out", c_void_p),
+        ("out_stride", _I64x3),
+        ("lse", c_void_p),
+        ("lse_stride", _I64x3),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_uint64),
+        ("new_k", c_void_p),
+        ("new_v", c_void_p),
+        ("new_k_stride", _I64x3),
+        ("new_v_stride", _I64x3),
+        ("weights", c_void_p),
+        ("weights_stride", _I64x2),
+        ("weights_len", c_int32),
+        ("budget", c_int32),
+        ("num_recent", c_int32),
+        ("new_page_table", c_void_p),
+        ("new_page_table_stride", c_int64),
+        ("new_max_pages", c_int32),
+        ("new_seqlens", c_void_p),
+        ("new_weights", c_void_p),
+        ("kept", c_void_p),
+    ]
+
+
 WIDE_OUT, WIDE_DQ, WIDE_DKV = 1, 2, 4
 DKDV_FORMS = {"wide": 1, "short": 2}
 
@@ -147,6 +206,19 @@ def load(path: str) -> ctypes.CDLL:
     L.rswa_attn_fwd_blocks_per_cu.argtypes = [POINTER(AttnParams)]
     L.rswa_attn_bwd_dkdv_keys.restype = c_int
     L.rswa_attn_bwd_dkdv_keys.argtypes = [POINTER(AttnParams)]
+    for name in ("rswa_cache_append", "rswa_cache_attn", "rswa_cache_weights", "rswa_cache_evict"):
+        fn = getattr(L, name)
+        fn.restype = c_int
+        fn.argtypes = [POINTER(CacheParams), c_void_p]
+    L.rswa_cache_attn_workspace_bytes.restype = c_uint64
+    L.rswa_cache_attn_workspace_bytes.argtypes = [POINTER(CacheParams)]
+    L.rswa_sizeof_cache_params.restype = c_uint64
+    if L.rswa_sizeof_cache_params() != ctypes.sizeof(CacheParams):
+        raise ImportError(
+            "rswa_cache_params layout mismatch between librswa.so "
+            f"({L.rswa_sizeof_cache_params()} bytes) and the Python binding "
+            f"({ctypes.sizeof(CacheParams)} bytes): rebuild the library"
+        )
     if L.rswa_sizeof_attn_params() != ctypes.sizeof(AttnParams):
         raise ImportError(
             "rswa_attn_params layout mismatch between librswa.so "

@@ -14,6 +14,7 @@ from .band_attn import (
     wrapped_flash_attn_fwd,
     wrapped_flash_attn_fwd_varlen,
 )
+from .kv_cache import KVCache, kv_cache_append, kv_cache_attn, kv_cache_evict, kv_cache_weights
 from .lse_merge import merge_attn_out
 from .p2p import (
     broadcast_tensor_to_group,
@@ -35,6 +36,11 @@ __all__ = [
     "flash_attn_varlen_fwd_func",
     "flash_attn_varlen_bwd_func",
     "merge_attn_out",
+    "KVCache",
+    "kv_cache_append",
+    "kv_cache_attn",
+    "kv_cache_weights",
+    "kv_cache_evict",
     "ring_attn_p2p_communicate",
     "broadcast_tensor_to_group",
     "reduce_sum_tesnsor_to_rank",

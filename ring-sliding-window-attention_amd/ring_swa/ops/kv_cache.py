@@ -1,0 +1,294 @@
+"""Serving from an 8-bit paged cache: the token-by-token continuation of a sequence whose prompt the
+sliding-window and streaming-LLM functions have computed.  No counterpart in the upstream package,
+which computes whole sequences only.
+
+A cache holds e4m3 codes times one power of two per (page, kv head); a page holds ``page_size``
+tokens of one sequence, and the caller's ``page_table`` (int32 ``[batch, max_pages]``, on the device)
+says which::
+
+    cache = KVCache.empty(num_pages, heads_kv, head_dim, device="cuda")
+    out = ring_streaming_llm_attn(q, k, v, window, num_sink_tokens=4)           # the prompt
+    kv_cache_append(cache, k, v, page_table, held)                              # held = 0
+    held += k.shape[1]
+    while True:                                                                 # a token at a time
+        kv_cache_append(cache, k, v, page_table, held)
+        held += 1
+        out, lse = kv_cache_attn(q, cache, page_table, held, window, num_sink_tokens=4, return_lse=True)
+        kv_cache_weights(q, cache, page_table, held, lse, weights, window, num_sink_tokens=4)
+        ...                                                                     # now and then:
+        held, weights, kept = kv_cache_evict(cache, weights, page_table, held, new_page_table, budget)
+
+Lengths and page ids stay on the device, nothing is read back.  Rows are ``[batch, seq, heads, dim]``,
+or packed ``[tokens, heads, dim]`` with ``cu_seqlens`` (int32 ``[batch + 1]``; sequences may bring
+different numbers of rows, none among them), as in the attention functions.  The new rows' keys are
+in the cache already when their queries attend: row ``i`` of ``n`` is token ``seqlens - n + i``.  A
+page id outside the cache (``-1``) is a page that is not there: seen by nobody, never written, so the
+pages that a window has left behind can be given back.  There is no backward.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from .. import _lib
+
+PAGE_SIZES = (16, 32, 64, 128, 256)
+
+
+class KVCache(NamedTuple):
+    """The tensors of a cache: ``k`` e4m3 ``[pages, kv_heads, page_size, dim]``, ``v`` e4m3 ``[pages,
+    kv_heads, page_size / 16, dim, 16]`` (the 16 keys of a group are adjacent: what the matrix
+    instruction reads), ``k_scale`` and ``v_scale`` e8m0 ``[pages, kv_heads]``.  Strides of pages and
+    heads are free (multiples of 16 for ``k`` and ``v``), so several layers' caches may share a tensor."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+    @classmethod
+    def empty(cls, num_pages: int, heads_kv: int, head_dim: int, page_size: int = 64,
+              device=None) -> "KVCache":
+        """A cache of ``num_pages`` pages with nothing in them."""
+        assert page_size in PAGE_SIZES, f"page_size must be one of {PAGE_SIZES}"
+        k = torch.empty(num_pages, heads_kv, page_size, head_dim, dtype=torch.float8_e4m3fn, device=device)
+        v = torch.empty(num_pages, heads_kv, page_size // 16, head_dim, 16, dtype=torch.float8_e4m3fn,
+                        device=device)
+        scales = (torch.zeros(num_pages, heads_kv, dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+                  for _ in range(2))
+        return cls(k, v, *scales)
+
+    @property
+    def page_size(self) -> int:
+        return self.k.shape[2]
+
+
+def _dense_from(t: torch.Tensor, dim: int) -> bool:
+    """Are the dimensions of ``t`` from ``dim`` on without gaps?  (A stride over one element is never used.)"""
+    step = 1
+    for d in range(t.dim() - 1, dim - 1, -1):
+        if t.shape[d] != 1 and t.stride(d) != step:
+            return False
+        step *= t.shape[d]
+    return True
+
+
+def _no_grad(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("the cache has no backward: call this under torch.no_grad()")
+
+
+def _cache_params(cache, page_table, seqlens, rows, cu_seqlens):
+    """The fields that every call sets, from its cache, table, lengths and rows (a tensor, or None)."""
+    k, v, k_scale, v_scale = cache
+    assert k.dim() == 4 and v.dim() == 5, "expected k [pages, heads, page, dim], v [pages, heads, page / 16, dim, 16]"
+    pages, heads, size, dim = k.shape
+    assert size in PAGE_SIZES, f"page_size must be one of {PAGE_SIZES}"
+    assert v.shape == (pages, heads, size // 16, dim, 16), "v must be [pages, heads, page / 16, dim, 16]"
+    assert k_scale.shape == v_scale.shape == (pages, heads), "scales must be [pages, heads]"
+    assert k.dtype == v.dtype == torch.float8_e4m3fn, "k and v must be float8_e4m3fn"
+    assert k_scale.dtype == v_scale.dtype == torch.float8_e8m0fnu, "scales must be float8_e8m0fnu"
+    assert _dense_from(k, 2) and _dense_from(v, 2), "the rows of a (page, head) must be dense"
+    assert page_table.dim() == 2 and page_table.dtype == torch.int32, "page_table must be int32 [batch, max_pages]"
+    assert _dense_from(page_table, 1), "the entries of a row of page_table must be adjacent"
+    batch = page_table.shape[0]
+    assert seqlens.dtype == torch.int32 and seqlens.shape == (batch,) and seqlens.is_contiguous(), (
+        "seqlens must be a contiguous int32 tensor [batch]")
+    dev = _lib.require_device(k, v, k_scale, v_scale, page_table, seqlens)
+    p = _lib.CacheParams()  # (zero-initialised)
+    p.head_dim, p.batch, p.heads_q, p.heads_kv = dim, batch, heads, heads
+    p.page_size, p.num_pages, p.max_pages = size, pages, page_table.shape[1]
+    p.k, p.v, p.k_scale, p.v_scale = k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()
+    p.k_stride, p.v_stride = k.stride()[:2], v.stride()[:2]
+    p.k_scale_stride, p.v_scale_stride = k_scale.stride(), v_scale.stride()
+    p.page_table, p.page_table_stride = page_table.data_ptr(), page_table.stride(0)
+    p.seqlens = seqlens.data_ptr()
+    if rows is not None:
+        assert rows.shape[-1] == dim, "head_dim mismatch"
+        _lib.require_device(k, rows)
+        p.dtype = _lib.dtype_code(rows)
+        if cu_seqlens is None:
+            assert rows.dim() == 4, "expected [batch, seq, heads, dim]"
+            assert rows.shape[0] == batch, "batch mismatch"
+            p.seqlen_q = rows.shape[1]
+        else:
+            assert rows.dim() == 3, "expected [tokens, heads, dim]"
+            assert cu_seqlens.dtype == torch.int32 and cu_seqlens.shape == (batch + 1,) and \
+                cu_seqlens.is_contiguous(), "cu_seqlens must be a contiguous int32 tensor [batch + 1]"
+            _lib.require_device(k, cu_seqlens)
+            p.total_q = rows.shape[0]
+            p.cu_seqlens_q = cu_seqlens.data_ptr()
+    return p, dev
+
+
+def _strides3(t: torch.Tensor, packed: bool):
+    st = t.stride()
+    return (0, st[0], st[1]) if packed else st[:3]
+
+
+def _query_params(p, q, heads_kv, softmax_scale, window_size, num_sink_tokens, packed):
+    assert q.shape[-2] % heads_kv == 0, "Number of query heads must be divisible by number of key/value heads"
+    assert q.stride(-1) == 1, "last dimension must be contiguous"
+    assert num_sink_tokens >= 0
+    p.heads_q = q.shape[-2]
+    p.softmax_scale = float(q.shape[-1] ** (-0.5) if softmax_scale is None else softmax_scale)
+    p.window_left = max(-1, min(int(window_size), 1 << 28))
+    p.num_sink = min(int(num_sink_tokens), 1 << 28)
+    p.q, p.q_stride = q.data_ptr(), _strides3(q, packed)
+
+
+def kv_cache_append(
+    cache: KVCache,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    page_table: torch.Tensor,
+    seqlens: torch.Tensor,
+    cu_seqlens: Optional[torch.Tensor] = None,
+) -> None:
+    """Write the keys and values of new tokens behind the ``seqlens`` tokens that the sequences hold.
+
+    ``k``, ``v``: ``[batch, seq, kv_heads, dim]``, or packed ``[tokens, kv_heads, dim]`` with
+    ``cu_seqlens``; bf16 or fp16.  The scale of a (page, head) is the smallest power of two at which
+    its largest finite value is within e4m3's range of 448; where the page holds tokens from before it
+    never shrinks, and if it grows their codes are rounded anew (only those that fall below the
+    smallest normal code change).  Infinities and NaN are stored as NaN.  Tokens beyond the last page
+    of ``page_table``, or whose page is not there, are dropped.  ``seqlens`` is left alone; two
+    sequences of one call must not have a page written in common."""
+    _no_grad(k, v)
+    p, dev = _cache_params(cache, page_table, seqlens, k, cu_seqlens)
+    assert k.shape == v.shape and k.dtype == v.dtype, "k and v must have the same shape and dtype"
+    assert k.shape[-2] == p.heads_kv, "k and v must have the cache's heads"
+    _lib.require_device(k, v)
+    assert k.stride(-1) == 1 and v.stride(-1) == 1, "last dimension must be contiguous"
+    packed = cu_seqlens is not None
+    p.new_k, p.new_v = k.data_ptr(), v.data_ptr()
+    p.new_k_stride, p.new_v_stride = _strides3(k, packed), _strides3(v, packed)
+    _lib.launch(dev, _lib.lib().rswa_cache_append, p)
+
+
+def kv_cache_attn(
+    q: torch.Tensor,
+    cache: KVCache,
+    page_table: torch.Tensor,
+    seqlens: torch.Tensor,
+    window_size: int = -1,
+    cu_seqlens: Optional[torch.Tensor] = None,
+    softmax_scale: Optional[float] = None,
+    *,
+    num_sink_tokens: int = 0,
+    return_lse: bool = False,
+):
+    """Attention of the sequences' last tokens over their caches; same mask as ``ring_streaming_llm_attn``.
+
+    ``q``: ``[batch, seq, heads, dim]``, or packed ``[tokens, heads, dim]`` with ``cu_seqlens``; bf16 or
+    fp16.  ``seqlens`` counts all tokens of a sequence, those of ``q`` among them.  Each query sees its
+    own token and the ``window_size`` before it (negative: all) and the first ``num_sink_tokens``.
+    Returns the output, shape and dtype of ``q``, and with ``return_lse`` the log-sum-exp, fp32
+    ``[batch, heads, seq]`` (``[heads, tokens]`` of a pack), as ``merge_attn_out`` takes it.  Rows that
+    see nothing: 0 and ``-inf``."""
+    _no_grad(q)
+    p, dev = _cache_params(cache, page_table, seqlens, q, cu_seqlens)
+    packed = cu_seqlens is not None
+    _query_params(p, q, p.heads_kv, softmax_scale, window_size, num_sink_tokens, packed)
+    out = q.new_empty(q.shape)
+    lse = None
+    if return_lse:
+        qs = q.shape
+        lse = q.new_empty((qs[1], qs[0]) if packed else (qs[0], qs[2], qs[1]), dtype=torch.float32)
+    if q.numel() > 0:
+        if p.max_pages == 0:  # no keys at all
+            out.zero_()
+            if lse is not None:
+                lse.fill_(float("-inf"))
+            return (out, lse) if return_lse else out
+        p.out, p.out_stride = out.data_ptr(), _strides3(out, packed)
+        if lse is not None:
+            p.lse, p.lse_stride = lse.data_ptr(), _strides3(lse, packed)
+        L = _lib.lib()
+        size = int(L.rswa_cache_attn_workspace_bytes(p))
+        if size:
+            workspace = q.new_empty(size, dtype=torch.uint8)
+            p.workspace, p.workspace_bytes = workspace.data_ptr(), size
+        _lib.launch(dev, L.rswa_cache_attn, p)
+    return (out, lse) if return_lse else out
+
+
+def kv_cache_weights(
+    q: torch.Tensor,
+    cache: KVCache,
+    page_table: torch.Tensor,
+    seqlens: torch.Tensor,
+    lse: torch.Tensor,
+    weights: torch.Tensor,
+    window_size: int = -1,
+    cu_seqlens: Optional[torch.Tensor] = None,
+    softmax_scale: Optional[float] = None,
+    *,
+    num_sink_tokens: int = 0,
+) -> None:
+    """Add to ``weights`` how much attention each cached key got from ``q``: the softmax weights
+    summed over the rows that see it and the query heads of its kv head's group.
+
+    ``lse`` is what ``kv_cache_attn(..., return_lse=True)`` returned for the same arguments; ``weights``
+    fp32 ``[batch, kv_heads, n]``, entry ``j`` that of token ``j`` (tokens from ``n`` on are passed over)."""
+    _no_grad(q)
+    p, dev = _cache_params(cache, page_table, seqlens, q, cu_seqlens)
+    packed = cu_seqlens is not None
+    _query_params(p, q, p.heads_kv, softmax_scale, window_size, num_sink_tokens, packed)
+    qs = q.shape
+    assert lse.dtype == torch.float32 and tuple(lse.shape) == (
+        (qs[1], qs[0]) if packed else (qs[0], qs[2], qs[1])), (
+        "lse must be fp32 [batch, heads, seq] ([heads, tokens] when packed)")
+    _weights_params(p, cache, weights)
+    _lib.require_device(q, lse)
+    if q.numel() > 0 and p.max_pages > 0:
+        p.lse, p.lse_stride = lse.data_ptr(), _strides3(lse, packed)
+        _lib.launch(dev, _lib.lib().rswa_cache_weights, p)
+
+
+def _weights_params(p, cache, weights):
+    assert weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (p.batch, p.heads_kv), (
+        "weights must be fp32 [batch, kv_heads, n]")
+    assert _dense_from(weights, 2), "last dimension must be contiguous"
+    _lib.require_device(cache.k, weights)
+    p.weights, p.weights_stride, p.weights_len = weights.data_ptr(), weights.stride()[:2], weights.shape[2]
+
+
+def kv_cache_evict(
+    cache: KVCache,
+    weights: torch.Tensor,
+    page_table: torch.Tensor,
+    seqlens: torch.Tensor,
+    new_page_table: torch.Tensor,
+    budget: int,
+    *,
+    num_sink_tokens: int = 0,
+    num_recent: int = 0,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Cut every sequence to at most ``budget`` tokens, for each kv head by itself.
+
+    Kept are the first ``num_sink_tokens``, the last ``num_recent``, and of the others those with the
+    largest ``weights`` (of equal ones the earlier; NaN counts as the least), in their order.  They move
+    to the pages of ``new_page_table`` (int32 ``[batch, n]``, room for ``budget`` tokens), each page at the
+    scale that fits its values; the old pages are only read, so that sequences may share them, and none
+    of them may be among the new ones.  Returns the new ``seqlens``, the kept tokens' weights (shape of
+    ``weights``, zeros behind) and their old numbers, int32 ``[batch, kv_heads, budget]`` (``-1`` behind).
+    From then on a token's number is its place among the kept ones, for windows too."""
+    assert budget > 0 and num_sink_tokens >= 0 and num_recent >= 0
+    assert num_sink_tokens + num_recent <= budget, "budget must hold the sinks and the recent tokens"
+    p, dev = _cache_params(cache, page_table, seqlens, None, None)
+    _weights_params(p, cache, weights)
+    assert new_page_table.dim() == 2 and new_page_table.dtype == torch.int32 and \
+        new_page_table.shape[0] == p.batch, "new_page_table must be int32 [batch, n]"
+    assert _dense_from(new_page_table, 1), "the entries of a row of new_page_table must be adjacent"
+    _lib.require_device(cache.k, new_page_table)
+    new_seqlens = torch.empty_like(seqlens)
+    new_weights = weights.new_empty(weights.shape)
+    kept = seqlens.new_empty(p.batch, p.heads_kv, int(budget))
+    p.num_sink, p.num_recent, p.budget = int(num_sink_tokens), int(num_recent), int(budget)
+    p.new_page_table, p.new_page_table_stride = new_page_table.data_ptr(), new_page_table.stride(0)
+    p.new_max_pages = new_page_table.shape[1]
+    p.new_seqlens, p.new_weights, p.kept = new_seqlens.data_ptr(), new_weights.data_ptr(), kept.data_ptr()
+    _lib.launch(dev, _lib.lib().rswa_cache_evict, p)
+    return new_seqlens, new_weights, kept
