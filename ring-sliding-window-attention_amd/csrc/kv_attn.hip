@@ -63,7 +63,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_kernel(const CacheArgs
   const int col = lane & 15, hi = lane >> 4;
   const int hk = blockIdx.x % a.heads_kv;
   Unit x;
-  if (!find_unit<false>(a, blockIdx.x / a.heads_kv, x)) return;
+  if (!find_unit<0>(a, blockIdx.x / a.heads_kv, x)) return;
 
   const int wr = wave / KW, kw = wave % KW;
   const int r0 = x.row_tile * ROWS + wr * (NT * 16);  // the wave's first row
@@ -206,8 +206,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_kernel(const CacheArgs
       for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int e = 0; e < 4; e++) top = fmaxf(top, s[nt][t][e]);
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
+      top = columns_max(top);
       if (__builtin_amdgcn_ballot_w64(top > m[nt])) {
         const float m_new = fmaxf(m[nt], top);
         const float shrink = m[nt] == m_new ? 1.f : __builtin_amdgcn_exp2f((m[nt] - m_new) * sc);
@@ -264,10 +263,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_kernel(const CacheArgs
   }
 
 #pragma unroll
-  for (int nt = 0; nt < NT; nt++) {
-    l[nt] += __shfl_xor(l[nt], 16);
-    l[nt] += __shfl_xor(l[nt], 32);
-  }
+  for (int nt = 0; nt < NT; nt++) l[nt] = columns_sum(l[nt]);
 
   // Row r's result: written if the row has one chunk, else left for the join.  d0: first of 4 dimensions.
   const bool direct = x.n_chunks == 1;
@@ -327,40 +323,64 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_kernel(const CacheArgs
   }
 }
 
-// Rows of several chunks: the partial results' sum with the weights of their maxima.
-template <typename T, int D>
+// Rows of several chunks: the partial results' sum with the weights of their maxima.  A thread has 4 dimensions of
+// every P-th chunk of a row, 4 chunks at a time; where rows have many chunks (on average) P threads share a row and
+// meet in LDS.  (A thread that went over all chunks one by one waited for each: 7.4 us for the 16 chunks of one token
+// over 4001, 17 for 16 drafts of 5.)
+template <typename T, int D, int P>
 __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheArgs a) {
+  constexpr int LANES = D / 4, ROWS = kThreads / LANES / P, N = 4;
+  __shared__ f32x4 lds_o[P > 1 ? P : 1][ROWS * LANES];
+  __shared__ f32x2 lds_ml[P > 1 ? P : 1][ROWS];
   const int hk = blockIdx.x % a.heads_kv;
   Unit x;
-  if (!find_unit<true>(a, blockIdx.x / a.heads_kv, x)) return;
+  if (!find_unit<ROWS>(a, blockIdx.x / a.heads_kv, x)) return;
   if (x.n_chunks == 1 || x.part + x.n_chunks > a.part_units) return;
-  const int n_flat = x.n_rows * a.group;
-  for (int at = threadIdx.x; at < a.row_tile * (D / 4); at += kThreads) {
-    const int row = at / (D / 4), d0 = at % (D / 4) * 4;
-    const int r = x.row_tile * a.row_tile + row;
-    if (r >= n_flat) break;
-    float mx = -__builtin_inff(), sum = 0.f;
-    f32x4 o = {0, 0, 0, 0};
-    for (int c = 0; c < x.n_chunks; c++) {
-      const int64_t p = ((int64_t)(x.part + c) * a.heads_kv + hk) * a.row_tile + row;
-      const f32x2 ml = *(const f32x2*)(a.part_ml + p * 2);
-      const f32x4 oc = *(const f32x4*)(a.part + p * D + d0);
-      if (ml[0] == -__builtin_inff()) continue;
-      const float m_new = fmaxf(mx, ml[0]);
-      const float f0 = __builtin_amdgcn_exp2f(mx - m_new), f1 = __builtin_amdgcn_exp2f(ml[0] - m_new);
-      mx = m_new;
-      sum = sum * f0 + ml[1] * f1;
+  const int lane = threadIdx.x % LANES, r = threadIdx.x / LANES % ROWS, part = threadIdx.x / LANES / ROWS;
+  const int d0 = lane * 4;
+  const int row = x.row + r - x.row_tile * a.row_tile;
+  const bool mine = x.row + r < x.n_rows * a.group;
+  float mx = -__builtin_inff(), sum = 0.f;
+  f32x4 o = {0, 0, 0, 0};
+  // (mx, sum, o) of the chunks so far joined with others'
+  auto add = [&](float m, float l, f32x4 v) {
+    if (m == -__builtin_inff()) return;  // (nothing seen: v was not written)
+    const float m_new = fmaxf(mx, m);
+    const float f0 = __builtin_amdgcn_exp2f(mx - m_new), f1 = __builtin_amdgcn_exp2f(m - m_new);
+    mx = m_new;
+    sum = sum * f0 + l * f1;
 #pragma unroll
-      for (int e = 0; e < 4; e++) o[e] = o[e] * f0 + oc[e] * f1;
+    for (int e = 0; e < 4; e++) o[e] = o[e] * f0 + v[e] * f1;
+  };
+  for (int c = mine ? part : x.n_chunks; c < x.n_chunks; c += P * N) {
+    f32x2 ml[N];
+    f32x4 v[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int64_t at = ((int64_t)(x.part + min(c + i * P, x.n_chunks - 1)) * a.heads_kv + hk) * a.row_tile + row;
+      ml[i] = *(const f32x2*)(a.part_ml + at * 2);
+      v[i] = *(const f32x4*)(a.part + at * D + d0);
     }
-    const int tok = quotient(r, a.by_group), head = hk * a.group + r - tok * a.group;
-    const float inv = sum == 0.f ? 0.f : 2.f / sum;
-    T* out = (T*)a.out + (int64_t)x.b * a.o_st[0] + (int64_t)(x.row0 + tok) * a.o_st[1] + (int64_t)head * a.o_st[2];
-    *(typename Mma<T>::V4*)(out + d0) = Mma<T>::pack4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-    if (d0 == 0 && a.lse)
-      a.lse[(int64_t)x.b * a.lse_st[0] + (int64_t)head * a.lse_st[1] + (int64_t)(x.row0 + tok) * a.lse_st[2]] =
-          sum == 0.f ? -__builtin_inff() : (mx - kLift<T> + __log2f(sum)) * (1.f / kLog2e);
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      if (c + i * P < x.n_chunks) add(ml[i][0], ml[i][1], v[i]);
   }
+  if constexpr (P > 1) {
+    lds_o[part][r * LANES + lane] = o;
+    if (lane == 0) lds_ml[part][r] = f32x2{mx, sum};
+    __syncthreads();
+    if (part != 0) return;
+#pragma unroll
+    for (int i = 1; i < P; i++) add(lds_ml[i][r][0], lds_ml[i][r][1], lds_o[i][r * LANES + lane]);
+  }
+  if (!mine) return;
+  const int tok = quotient(x.row + r, a.by_group), head = hk * a.group + x.row + r - tok * a.group;
+  const float inv = sum == 0.f ? 0.f : 2.f / sum;
+  T* out = (T*)a.out + (int64_t)x.b * a.o_st[0] + (int64_t)(x.row0 + tok) * a.o_st[1] + (int64_t)head * a.o_st[2];
+  *(typename Mma<T>::V4*)(out + d0) = Mma<T>::pack4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  if (d0 == 0 && a.lse)
+    a.lse[(int64_t)x.b * a.lse_st[0] + (int64_t)head * a.lse_st[1] + (int64_t)(x.row0 + tok) * a.lse_st[2]] =
+        sum == 0.f ? -__builtin_inff() : (mx - kLift<T> + __log2f(sum)) * (1.f / kLog2e);
 }
 
 // How a call is cut.  Rows of a sequence (on average, of a pack): up to 16 in one tile of a wave, up to 32 in two;
@@ -406,7 +426,15 @@ int launch_attn(CacheArgs& a, const Cut& c, hipStream_t stream) {
     hipLaunchKernelGGL((cache_attn_kernel<T, D, 2, 4>), grid, block, 0, stream, a);
   if (int rc = check_launch("cache_attn")) return rc;
   if (c.part_units == 0) return RSWA_OK;
-  hipLaunchKernelGGL((cache_join_kernel<T, D>), dim3((unsigned)(c.row_tiles * a.heads_kv)), block, 0, stream, a);
+  // as many chunks a row (on average) as threads that may share one, or one thread for all
+  constexpr int P = kThreads / (D / 4);
+  const int64_t rows = a.cu ? a.total_q : (int64_t)a.batch * a.seqlen_q;
+  if (c.row_tiles * a.heads_kv * P <= c.wanted) {
+    hipLaunchKernelGGL((cache_join_kernel<T, D, P>), dim3((unsigned)(rows * a.heads_q)), block, 0, stream, a);
+  } else {
+    const int64_t groups = a.cu ? rows * a.group / P + a.batch : a.batch * ceil_div((int64_t)a.seqlen_q * a.group, P);
+    hipLaunchKernelGGL((cache_join_kernel<T, D, 1>), dim3((unsigned)(groups * a.heads_kv)), block, 0, stream, a);
+  }
   return check_launch("cache_attn join");
 }
 

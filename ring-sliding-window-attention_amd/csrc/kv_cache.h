@@ -54,6 +54,46 @@ __device__ __forceinline__ int lane_id() {
   return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
 }
 
+// Sums over the lanes up to each (wave64), in the vector pipe: an exchange through LDS takes some 100 cycles, and a
+// scan has six in a row.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or_zero(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, true);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+  x += dpp_or_zero<0x111, 0xf>(x);  // from 1, 2, 4, 8 lanes below, within 16
+  x += dpp_or_zero<0x112, 0xf>(x);
+  x += dpp_or_zero<0x114, 0xf>(x);
+  x += dpp_or_zero<0x118, 0xf>(x);
+  x += dpp_or_zero<0x142, 0xa>(x);  // lane 15 of rows 0 and 2 to rows 1 and 3
+  x += dpp_or_zero<0x143, 0xc>(x);  // lane 31 to rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ float wave_scan(float v) {
+  auto from = [](int moved) { return __builtin_bit_cast(float, moved); };
+  auto bits = [](float f) { return __builtin_bit_cast(int, f); };
+  v += from(dpp_or_zero<0x111, 0xf>(bits(v)));
+  v += from(dpp_or_zero<0x112, 0xf>(bits(v)));
+  v += from(dpp_or_zero<0x114, 0xf>(bits(v)));
+  v += from(dpp_or_zero<0x118, 0xf>(bits(v)));
+  v += from(dpp_or_zero<0x142, 0xa>(bits(v)));
+  v += from(dpp_or_zero<0x143, 0xc>(bits(v)));
+  return v;
+}
+__device__ __forceinline__ float last_lane(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
+// Lanes l, l^16, l^32, l^48 with each other (the four that have a column of a 16 x 16 product).
+__device__ __forceinline__ float columns_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return halfwave_max(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+}
+__device__ __forceinline__ float columns_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return halfwave_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
+}
+
 // Tokens that a sequence's row of the page table can hold at most bound its length: no lookup passes its end.
 __device__ __forceinline__ int held_tokens(const CacheArgs& a, int b) {
   return max(0, min(a.lens[b], a.max_pages << a.page_log2));
@@ -94,22 +134,23 @@ __device__ __forceinline__ SeenTiles seen_tiles(const CacheArgs& a, int first, i
 //   sum over sequences of row_tiles * ceil(tiles / chunk) <= units wanted / heads_kv + sum of row_tiles
 // and what is beyond the last unit ends at once.  Rows of sequences with several chunks are joined from partial
 // results; those sequences have at most twice the units wanted (ceil(x) <= 2 x for x > 1), which bounds the workspace.
+// (The sum of tiles is taken in floating point, within 2^-16 of its value: less than the one unit that the host adds.)
 struct Unit {
-  int b, row_tile, chunk_idx, n_chunks;
+  int b, row, row_tile, chunk_idx, n_chunks;
   int row0, n_rows, len;
   int chunk;  // tiles
   int part;   // first of the row tile's n_chunks partial results
   SeenTiles tiles;
 };
 
-// JOIN: units are whole row tiles (chunk_idx stays 0).
-template <bool JOIN>
+// JOIN > 0: units are JOIN rows from x.row on (a divisor of the row tile), and chunk_idx stays 0.
+template <int JOIN>
 __device__ __forceinline__ bool find_unit(const CacheArgs& a, int u, Unit& x) {
   const int lane = lane_id();
   int row0 = 0, n = 0, len = 0, row_tiles = 0;
   SeenTiles t{0, 0, 0};
   auto load = [&](int b) {
-    row_tiles = 0;
+    n = row_tiles = 0;
     t = SeenTiles{0, 0, 0};
     if (b < a.batch) {
       rows_of(a, b, row0, n);
@@ -118,29 +159,21 @@ __device__ __forceinline__ bool find_unit(const CacheArgs& a, int u, Unit& x) {
       if (n > 0) t = seen_tiles(a, len - n, len - 1);
     }
   };
-  uint64_t total = 0;
+  // (fused by hand: attention and join must come to the same chunk)
+  float total = 0.f;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     load(b0 + lane);
-    total += (uint64_t)row_tiles * (uint64_t)t.count();
+    total = __builtin_fmaf((float)row_tiles, (float)t.count(), total);
   }
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) total += __shfl_xor(total, s);
-  x.chunk = max(a.min_chunk, (int)__builtin_ceilf((float)total * a.per_unit));
+  total = last_lane(wave_scan(total));
+  x.chunk = max(a.min_chunk, (int)__builtin_ceilf(total * a.per_unit));
   int before = 0, before_part = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     if (a.batch > 64) load(b0 + lane);
     const int chunks = max(1, (t.count() + x.chunk - 1) / x.chunk);
-    const int units = JOIN ? row_tiles : row_tiles * chunks;
+    const int units = JOIN ? (n * a.group + JOIN - 1) / JOIN : row_tiles * chunks;
     const int parts = chunks > 1 ? row_tiles * chunks : 0;
-    int su = units, sp = parts;  // inclusive sums
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const int tu = __shfl_up(su, s), tp = __shfl_up(sp, s);
-      if (lane >= s) {
-        su += tu;
-        sp += tp;
-      }
-    }
+    const int su = wave_scan(units), sp = wave_scan(parts);
     const uint64_t past = __builtin_amdgcn_ballot_w64(before + su > u);
     if (past) {
       const int at = __builtin_ctzll(past);
@@ -148,7 +181,8 @@ __device__ __forceinline__ bool find_unit(const CacheArgs& a, int u, Unit& x) {
       x.b = b0 + at;
       x.n_chunks = of(chunks);
       const int in_seq = u - before - (of(su) - of(units));
-      x.row_tile = JOIN ? in_seq : in_seq / x.n_chunks;
+      x.row = in_seq * JOIN;
+      x.row_tile = JOIN ? x.row / a.row_tile : in_seq / x.n_chunks;
       x.chunk_idx = JOIN ? 0 : in_seq - x.row_tile * x.n_chunks;
       x.part = before_part + of(sp) - of(parts) + x.row_tile * x.n_chunks;
       x.row0 = of(row0);

@@ -21,7 +21,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
   const int col = lane & 15, hi = lane >> 4;
   const int hk = blockIdx.x % a.heads_kv;
   Unit x;
-  if (!find_unit<false>(a, blockIdx.x / a.heads_kv, x)) return;
+  if (!find_unit<0>(a, blockIdx.x / a.heads_kv, x)) return;
   const int shift = x.len - x.n_rows, n_flat = x.n_rows * a.group;
   const int rw = wave / KW, kw = wave % KW;
   const float sc = 2.f * a.scale_log2;
@@ -100,10 +100,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
       }
     }
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-      sum[t] += __shfl_xor(sum[t], 16);
-      sum[t] += __shfl_xor(sum[t], 32);
-    }
+    for (int t = 0; t < 4; t++) sum[t] = columns_sum(sum[t]);
     // lane l takes key l of the tile
     float mine = hi == 0 ? sum[0] : hi == 1 ? sum[1] : hi == 2 ? sum[2] : sum[3];
     if constexpr (RW > 1) {
