@@ -1,9 +1,6 @@
 // Eviction from the 8-bit paged cache by running sums of softmax weights.
 //
-// Two launches.  The first chooses, a block per (sequence, kv head): the least weight that stays is found by its bits,
-// eight at a time from the highest (counts in LDS), then each wave walks a part of the sequence in order and writes
-// the kept tokens' numbers behind those of the waves before it.  The second moves: a block makes a new page of one kv
-// head, gathers its tokens from wherever they lie, and writes them at the scale that fits them.
+// Two launches: the first chooses, for each sequence and kv head, the second moves what stays into the new pages.
 #include "kv_cache.h"
 
 namespace rswa {
@@ -22,18 +19,29 @@ struct EvictArgs {
   int32_t* kept;
 };
 
-// A weight's bits as an unsigned number that grows with it; NaN below everything.
+// Weights as unsigned numbers that grow with them.  0: no token, 1: NaN, the largest: a token that stays whatever its
+// weight (none is that of a weight).
+constexpr uint32_t kStays = ~0u;
 __device__ __forceinline__ uint32_t ordered(float w) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.f);  // (-0 as 0)
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0;
+  const uint32_t u = __float_as_uint(w + 0.f);  // (-0 as 0)
+  if ((u & 0x7fffffffu) > 0x7f800000u) return 1;
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// A block has one sequence's kv head, a wave of it a part of the tokens in a row, which it keeps in registers (those
+// beyond 32 a lane are read again in each pass).  The bits of the least weight that stays are found from the highest
+// down: a histogram of the first 11 (sign, exponent and two more: with eight, all weights meet in a few counters), a
+// list of the weights that share the digit found, and two more digits from that list.  What bounds it is the one
+// compute unit that a block runs on, some 40 instructions for each token; parts of one sequence on several would need
+// a launch for each step.
 __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const EvictArgs a) {
-  constexpr int WAVES = kSelectThreads / 64;
-  __shared__ uint32_t hist[256];
+  constexpr int WAVES = kSelectThreads / 64, N = 32, BINS = 2048, COPIES = 4, LIST = 8192;
+  __shared__ __attribute__((aligned(16))) uint32_t hist[COPIES][BINS];
+  __shared__ uint32_t list[LIST];
+  __shared__ uint32_t listed;
   __shared__ uint32_t chosen[2];  // digit, how many are still to be found among its weights
   __shared__ int count[WAVES][2];
+  __shared__ uint32_t sums[WAVES];
   const CacheArgs& c = a.c;
   const int b = blockIdx.x / c.heads_kv, hk = blockIdx.x % c.heads_kv;
   const int len = held_tokens(c, b);
@@ -41,87 +49,117 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const Evic
   const float* w = c.weights + (int64_t)b * c.w_st[0] + (int64_t)hk * c.w_st[1];
   int32_t* kept = a.kept + (int64_t)blockIdx.x * a.budget;
   float* new_w = a.new_weights + (int64_t)blockIdx.x * c.w_len;
-  // (tokens without a weight of their own have none)
-  auto weight = [&](int j) { return j < c.w_len ? w[j] : 0.f; };
 
   if (hk == 0 && threadIdx.x == 0) a.new_lens[b] = stay;
   for (int r = stay + threadIdx.x; r < a.budget; r += kSelectThreads) kept[r] = -1;
-  for (int r = stay + threadIdx.x; r < c.w_len; r += kSelectThreads) new_w[r] = 0.f;
+  for (int r = stay + threadIdx.x; r < c.w_len; r += kSelectThreads) new_w[r] = 0.f;  // (the others: see the move)
   if (len <= a.budget) {
-    for (int j = threadIdx.x; j < len; j += kSelectThreads) {
-      kept[j] = j;
-      if (j < c.w_len) new_w[j] = weight(j);
-    }
+    for (int j = threadIdx.x; j < len; j += kSelectThreads) kept[j] = j;
     return;
   }
-  // of tokens c0 .. c1 - 1 the `find` with the largest weights
-  const int c0 = c.n_sink, c1 = len - a.n_recent;
-  int find = a.budget - c.n_sink - a.n_recent;
-  uint32_t least = 0;  // bits of the least weight that stays, known from the top
-  if (find > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = threadIdx.x; i < 256; i += kSelectThreads) hist[i] = 0;
-      __syncthreads();
-      for (int j = c0 + threadIdx.x; j < c1; j += kSelectThreads) {
-        const uint32_t o = ordered(weight(j));
-        if (shift == 24 || (o >> (shift + 8)) == (least >> (shift + 8))) atomicAdd(&hist[(o >> shift) & 255], 1u);
-      }
-      __syncthreads();
-      if (threadIdx.x < 64) {
-        // lane l: digits 255 - 4 l - 0 .. 3, from the largest down
-        uint32_t n[4], sum = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          n[i] = hist[255 - 4 * threadIdx.x - i];
-          sum += n[i];
-        }
-        uint32_t incl = sum;
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-          const uint32_t t = __shfl_up(incl, s);
-          if ((int)threadIdx.x >= s) incl += t;
-        }
-        uint32_t above = incl - sum;
-        if (above < (uint32_t)find && incl >= (uint32_t)find) {
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            if (above < (uint32_t)find && above + n[i] >= (uint32_t)find) {
-              chosen[0] = 255 - 4 * threadIdx.x - i;
-              chosen[1] = find - above;
-            }
-            above += n[i];
-          }
-        }
-      }
-      __syncthreads();
-      least |= chosen[0] << shift;
-      find = chosen[1];
-      __syncthreads();
-    }
-  }
-  // `find` of the weights equal to `least` stay: the earliest
-  const bool any = a.budget > c.n_sink + a.n_recent;
-  const int lane = lane_id(), wave = threadIdx.x / 64;
-  const int part = ((len + WAVES - 1) / WAVES + 63) & ~63;
-  const int p0 = min(len, wave * part), p1 = min(len, p0 + part);
-  auto kind = [&](int j, bool& sure, bool& equal) {
-    sure = equal = false;
-    if (j >= p1) return;
-    if (j < c0 || j >= c1) {
-      sure = true;
-    } else if (any) {
-      const uint32_t o = ordered(weight(j));
-      sure = o > least;
-      equal = o == least;
-    }
+  const int c0 = c.n_sink, c1 = len - a.n_recent;  // the others
+  int find = a.budget - c.n_sink - a.n_recent;     // of which so many stay
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int steps = (len + kSelectThreads - 1) / kSelectThreads;
+  const int p0 = wave * steps * 64 + lane;  // a lane's first token
+  // (loads first and without branches, so that they are all in flight; tokens without a weight of their own have 0)
+  const int last = max(0, c.w_len - 1);
+  if (c.w_len == 0) w = (const float*)c.lens;  // (any place that can be read)
+  auto load = [&](int i) { return w[min(p0 + i * 64, last)]; };
+  auto number = [&](int i, float x) -> uint32_t {
+    const int j = p0 + i * 64;
+    uint32_t o = ordered(j < c.w_len ? x : 0.f);
+    o = (uint32_t)(j - c0) < (uint32_t)(c1 - c0) ? o : kStays;
+    return j < len ? o : 0;
   };
-  int n_sure = 0, n_equal = 0;
-  for (int j = p0; j < p1; j += 64) {
-    bool sure, equal;
-    kind(j + lane, sure, equal);
-    n_sure += __popcll(__builtin_amdgcn_ballot_w64(sure));
-    n_equal += __popcll(__builtin_amdgcn_ballot_w64(equal));
+  uint32_t mine[N];
+  float raw[N];
+#pragma unroll
+  for (int i0 = 0; i0 < N; i0 += 8)
+    if (i0 < steps)
+#pragma unroll
+      for (int i = i0; i < i0 + 8; i++) raw[i] = load(i);
+  for (int i = threadIdx.x; i < COPIES * BINS / 4; i += kSelectThreads) ((u32x4*)hist)[i] = u32x4{0, 0, 0, 0};
+  if (threadIdx.x == 0) listed = 0;
+#pragma unroll
+  for (int i0 = 0; i0 < N; i0 += 8)
+    if (i0 < steps)
+#pragma unroll
+      for (int i = i0; i < i0 + 8; i++) mine[i] = i < steps ? number(i, raw[i]) : 0;
+  // all of a wave's weights, eight steps without a branch at a time (those beyond its part are 0)
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int i0 = 0; i0 < N; i0 += 8)
+      if (i0 < steps)
+#pragma unroll
+        for (int i = i0; i < i0 + 8; i++) f(i, mine[i]);
+    for (int i = N; i < steps; i++) f(i, number(i, load(i)));
+  };
+
+  uint32_t least = kStays - 1;  // above every weight: none of the others stays
+  if (find > 0) {
+    // the digit of the find-th largest from the counts of COUNT copies
+    auto choose = [&](int copies) {
+      uint32_t n0 = 0, n1 = 0;
+      const int top = BINS - 1 - 2 * (int)threadIdx.x;  // thread t: bins BINS - 1 - 2 t and the one below
+      for (int i = 0; i < copies; i++) {
+        n0 += hist[i][top];
+        n1 += hist[i][top - 1];
+      }
+      uint32_t incl = (uint32_t)wave_scan((int)(n0 + n1));
+      if (lane == 63) sums[wave] = incl;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < WAVES; i++) incl += i < wave ? sums[i] : 0;
+      const uint32_t above = incl - n0 - n1;
+      if (above < (uint32_t)find && incl >= (uint32_t)find) {
+        const bool first = above + n0 >= (uint32_t)find;
+        chosen[0] = first ? top : top - 1;
+        chosen[1] = find - above - (first ? 0 : n0);
+      }
+      __syncthreads();
+      find = chosen[1];
+      return chosen[0];
+    };
+    auto weighs = [](uint32_t o) { return o - 1 < kStays - 1; };
+    __syncthreads();
+    each([&](int, uint32_t o) {
+      if (weighs(o)) atomicAdd(&hist[wave % COPIES][o >> 21], 1u);
+    });
+    __syncthreads();
+    const uint32_t digit = choose(COPIES);
+    each([&](int, uint32_t o) {
+      if (weighs(o) && o >> 21 == digit) {
+        const uint32_t at = atomicAdd(&listed, 1u);  // (in any order: only counted)
+        if (at < LIST) list[at] = o;
+      }
+    });
+    least = digit << 21;
+#pragma unroll 1
+    for (int shift = 10; shift >= 0; shift -= 10) {
+      const uint32_t mask = shift ? 2047 : 1023;
+      for (int i = threadIdx.x; i < BINS / 4; i += kSelectThreads) ((u32x4*)hist)[i] = u32x4{0, 0, 0, 0};
+      __syncthreads();
+      const uint32_t known = shift ? ~0u << 21 : ~0u << 10;
+      auto tally = [&](uint32_t o) {
+        if ((o & known) == least) atomicAdd(&hist[0][(o >> shift) & mask], 1u);
+      };
+      if (listed <= LIST)
+        for (uint32_t i = threadIdx.x; i < listed; i += kSelectThreads) tally(list[i]);
+      else
+        each([&](int, uint32_t o) {
+          if (weighs(o)) tally(o);
+        });
+      __syncthreads();
+      least |= choose(1) << shift;
+    }
   }
+  // stays: a larger weight; and `find` of the equal ones, the earliest
+  int n_sure = 0, n_equal = 0;
+  each([&](int, uint32_t o) {
+    n_sure += __popcll(__builtin_amdgcn_ballot_w64(o > least));
+    n_equal += __popcll(__builtin_amdgcn_ballot_w64(o == least));
+  });
   if (lane == 0) {
     count[wave][0] = n_sure;
     count[wave][1] = n_equal;
@@ -133,114 +171,248 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const Evic
     equals += count[i][1];
   }
   at += min(equals, find);
-  const uint64_t below = (1ull << lane) - 1;
-  for (int j = p0; j < p1; j += 64) {
-    bool sure, equal;
-    kind(j + lane, sure, equal);
-    const uint64_t eq = __builtin_amdgcn_ballot_w64(equal);
-    const bool keep = sure || (equal && equals + __popcll(eq & below) < find);
-    const uint64_t k = __builtin_amdgcn_ballot_w64(keep);
-    const int r = at + __popcll(k & below);
-    if (keep && r < a.budget) {
-      kept[r] = j + lane;
-      if (r < c.w_len) new_w[r] = weight(j + lane);
+  auto below = [](uint64_t m, int n) {  // n and the lanes of m below this one
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, n));
+  };
+  each([&](int i, uint32_t o) {
+    bool keep = o > least;
+    const uint64_t eq = __builtin_amdgcn_ballot_w64(o == least);
+    if (eq) {
+      keep = keep || (o == least && below(eq, equals) < find);
+      equals += __popcll(eq);
     }
+    const uint64_t k = __builtin_amdgcn_ballot_w64(keep);
+    const int r = below(k, at);
+    if (keep && r < a.budget) kept[r] = p0 + i * 64;
     at += __popcll(k);
-    equals += __popcll(eq);
-  }
+  });
 }
 
-// One new page of one kv head.  Keys, then values: lane l of a wave has place l%16 of a group, so that tokens that
-// lay side by side are read from the same 16 bytes and written to the same 16 bytes.
+// Largest finite magnitude among codes.  A magnitude's code grows with it; one more than the seven bits, modulo 128,
+// is 0 for NaN and 1 .. 127 for the others, and two such bytes are compared at a time.
+struct LargestCode {
+  uint32_t even = 0, odd = 0;
+  typedef __attribute__((__vector_size__(2 * sizeof(uint16_t)))) uint16_t u16x2;
+  static __device__ __forceinline__ uint32_t max2(uint32_t x, uint32_t y) {
+    const u16x2 p = __builtin_bit_cast(u16x2, x), q = __builtin_bit_cast(u16x2, y);
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(p, q));
+  }
+  __device__ __forceinline__ void add(uint32_t codes) {
+    even = max2(even, ((codes & 0x007f007fu) + 0x00010001u) & 0x007f007fu);
+    odd = max2(odd, (((codes >> 8) & 0x007f007fu) + 0x00010001u) & 0x007f007fu);
+  }
+  // ... times the power of two of scale byte e
+  __device__ __forceinline__ float value(int e) const {
+    const uint32_t m = max2(even, odd), code = max(m & 0xffffu, m >> 16);
+    return __builtin_ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)(code == 0 ? 0 : code - 1), 0), e - 127);
+  }
+};
+
+// Moves the kept tokens into new pages.  A block makes one new page of one kv head; a wave has 64 tokens of its keys or
+// of its values.  Keys are rows to copy.  Of the values a lane has one or two dimensions, 16 tokens of which are 16
+// bytes: it reads the old groups that hold kept tokens one after the other, and since which bytes of a word stay is
+// the same for all lanes, one byte permutation with a scalar selector closes the gaps and one shift appends what is
+// left.  The words wait in LDS until the page's largest value, and with it the new scale, is known.
+// (Reading the values byte by byte, twice, and storing them so, took 195 us for 32 sequences cut from 2176 to 2048.)
 template <int D>
-__global__ __launch_bounds__(256) void cache_move_kernel(const EvictArgs a) {
+__global__ __launch_bounds__(512, 4) void cache_move_kernel(const EvictArgs a) {
+  constexpr int DL = D / 64;          // dimensions of a lane of a value wave
+  constexpr int ROW = 16 + 1;         // words of 64 tokens, and one against bank conflicts
+  constexpr int PIECES = D / 16, PER = 64 / PIECES, STEPS = 64 / PER;  // 16-byte pieces of a key row; rows of a load
+  extern __shared__ uint32_t packed[];
+  __shared__ int64_t base[8][64];     // keys: of each row; values: of each old group.  -1: its page is not there
+  __shared__ uint32_t info[8][64];    // keys: scale byte; values: which tokens of the group stay, scale byte << 16
   __shared__ uint32_t amax[2];
-  __shared__ int64_t from[256];     // (source page << 8) + place, -1: none
-  __shared__ uint8_t ks[256], vs[256];
   const CacheArgs& c = a.c;
   const int page_size = 1 << c.page_log2;
   const int hk = blockIdx.x % c.heads_kv;
   const int b = blockIdx.x / c.heads_kv / a.new_max_pages, np = blockIdx.x / c.heads_kv % a.new_max_pages;
   const int len = held_tokens(c, b), stay = min(len, a.budget);
   const int r0 = np << c.page_log2;
-  const int n = min(page_size, stay - r0);  // tokens of the page
-  if (n <= 0) return;
+  const int n_page = min(page_size, stay - r0);  // tokens of the page
+  if (n_page <= 0) return;
   const int id = a.new_table[(int64_t)b * a.new_table_st + np];
-  if ((uint32_t)id >= (uint32_t)c.num_pages) return;
-  const int t = threadIdx.x;
-  if (t < 2) amax[t] = 0;
-  if (t < n) {
-    const int j = a.kept[((int64_t)b * c.heads_kv + hk) * a.budget + r0 + t];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int half = blockDim.x / 128;
+  const bool values = wave >= half;
+  const int sub = (values ? wave - half : wave) * 64;  // first place of the wave's tokens
+  const int n = max(0, min(64, n_page - sub));
+
+  // lane l: the wave's token l
+  int j = -1, sp = -1, e = 0;
+  if (threadIdx.x < 2) amax[threadIdx.x] = 0;
+  info[wave][lane] = 0;
+  if (lane < n) {
+    j = a.kept[((int64_t)b * c.heads_kv + hk) * a.budget + r0 + sub + lane];
     // (weights that another stream changes during the choice may leave numbers out: nothing is looked up by those)
-    const int sp = (uint32_t)j < (uint32_t)len ? c.table[(int64_t)b * c.table_st + (j >> c.page_log2)] : -1;
-    const bool here = (uint32_t)sp < (uint32_t)c.num_pages;
-    from[t] = here ? ((int64_t)sp << 8) + (j & (page_size - 1)) : -1;
-    ks[t] = here ? c.k_scale[(int64_t)sp * c.ks_st[0] + (int64_t)hk * c.ks_st[1]] : 0;
-    vs[t] = here ? c.v_scale[(int64_t)sp * c.vs_st[0] + (int64_t)hk * c.vs_st[1]] : 0;
+    const bool one = (uint32_t)j < (uint32_t)len;
+    if (one) sp = c.table[(int64_t)b * c.table_st + (j >> c.page_log2)];
+    const int r = r0 + sub + lane;
+    if (!values && r < c.w_len)
+      a.new_weights[((int64_t)b * c.heads_kv + hk) * c.w_len + r] =
+          one && j < c.w_len ? c.weights[(int64_t)b * c.w_st[0] + (int64_t)hk * c.w_st[1] + j] : 0.f;
+    if ((uint32_t)sp >= (uint32_t)c.num_pages) sp = -1;
+    if (sp >= 0)
+      e = values ? c.v_scale[(int64_t)sp * c.vs_st[0] + (int64_t)hk * c.vs_st[1]]
+                 : c.k_scale[(int64_t)sp * c.ks_st[0] + (int64_t)hk * c.ks_st[1]];
+  }
+  if ((uint32_t)id >= (uint32_t)c.num_pages) return;
+  const int slot = j & (page_size - 1);
+  uint64_t starts = 0;  // values: tokens that are the first of their old group
+  if (!values) {
+    if (lane < n) {
+      base[wave][lane] = sp < 0 ? -1 : (int64_t)sp * c.k_st[0] + slot * D;
+      info[wave][lane] = (uint32_t)e;
+    }
+  } else {
+    const int before = __shfl_up(j, 1);
+    const bool start = lane < n && (lane == 0 || (j >> 4) != (before >> 4));
+    starts = __builtin_amdgcn_ballot_w64(start);
+    const int group = __popcll(starts & (~0ull >> (63 - lane))) - 1;
+    if (start) base[wave][group] = sp < 0 ? -1 : (int64_t)sp * c.v_st[0] + (slot >> 4) * (16 * D);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");  // (the zeros above)
+    if (lane < n) atomicOr(&info[wave][group], (1u << (j & 15)) | ((uint32_t)e << 16));
   }
   __syncthreads();
-  const uint8_t* const k_head = c.k + (int64_t)hk * c.k_st[1];
-  const uint8_t* const v_head = c.v + (int64_t)hk * c.v_st[1];
-  // largest finite magnitude: of a code the bits without the sign, NaN (0x7f) passed over
-  auto value = [](uint32_t code, int e) {
-    const uint32_t m = code & 0x7fu;
-    const float f = __builtin_amdgcn_cvt_f32_fp8((int)(m == 0x7fu ? 0u : m), 0);
-    return __builtin_ldexpf(f, e - 127);
-  };
-  float mk = 0.f, mv = 0.f;
-  for (int i = t; i < n * (D / 4); i += 256) {
-    const int r = i / (D / 4), d = i % (D / 4) * 4;
-    const int64_t f = from[r];
-    if (f < 0) continue;
-    const uint32_t w = *(const uint32_t*)(k_head + (f >> 8) * c.k_st[0] + (f & 255) * D + d);
+
+  float most = 0.f;
+  u32x4 rows[STEPS];
+  uint32_t* const words = packed + (values ? wave - half : 0) * (D * ROW);
+  const uint8_t* const head = values ? c.v + (int64_t)hk * c.v_st[1] : c.k + (int64_t)hk * c.k_st[1];
+  if (!values) {
+    const int piece = lane % PIECES * 16;
 #pragma unroll
-    for (int e = 0; e < 4; e++) mk = fmaxf(mk, value(w >> (8 * e), ks[r]));
-  }
-  for (int i = t; i < ((n + 15) & ~15) * D; i += 256) {
-    const int r = i / (16 * D) * 16 + (i & 15), d = i / 16 % D;
-    if (r >= n || from[r] < 0) continue;
-    const int64_t f = from[r];
-    const int s = (int)(f & 255);
-    mv = fmaxf(mv, value(v_head[(f >> 8) * c.v_st[0] + (s >> 4) * (16 * D) + d * 16 + (s & 15)], vs[r]));
+    for (int i = 0; i < STEPS; i++) {
+      const int r = i * PER + lane / PIECES;
+      rows[i] = u32x4{0, 0, 0, 0};
+      if (r < n && base[wave][r] >= 0) rows[i] = *(const u32x4*)(head + base[wave][r] + piece);
+    }
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+      const int r = i * PER + lane / PIECES;
+      LargestCode top;
+#pragma unroll
+      for (int q = 0; q < 4; q++) top.add(rows[i][q]);
+      if (r < n) most = fmaxf(most, top.value((int)info[wave][r]));
+    }
+  } else {
+    // lane m: selector that closes the gaps of a word of which the tokens of the mask m stay
+    uint32_t closes = 0;
+    int taken = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (lane >> i & 1) closes |= (uint32_t)i << (8 * taken++);
+    closes |= 0x0c0c0c0cu << (8 * (taken & 3)) & (taken == 4 ? 0u : ~0u);
+    const int groups = __popcll(starts);
+    const int64_t at = base[wave][lane];  // (lane g: old group g)
+    const uint32_t inf = info[wave][lane];
+    u32x4 x[DL], next[DL];
+    auto load = [&](int g, u32x4(&y)[DL]) {
+      const int64_t from = ((int64_t)__builtin_amdgcn_readlane((int)(at >> 32), g) << 32) |
+                           (uint32_t)__builtin_amdgcn_readlane((int)at, g);
+#pragma unroll
+      for (int i = 0; i < DL; i++)
+        y[i] = from < 0 ? u32x4{0, 0, 0, 0} : *(const u32x4*)(head + from + (lane + 64 * i) * 16);
+    };
+    uint32_t part[DL] = {};
+    int fill = 0, word = 0;  // bytes in `part`, words written
+    if (groups > 0) load(0, x);
+    for (int g = 0; g < groups; g++) {
+      if (g + 1 < groups) load(g + 1, next);
+      const uint32_t which = (uint32_t)__builtin_amdgcn_readlane((int)inf, g);
+      LargestCode top;
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const int m = which >> (4 * q) & 15;
+        if (m == 0) continue;
+        const uint32_t sel = (uint32_t)__builtin_amdgcn_readlane((int)closes, m);
+        const int bytes = __builtin_popcount(m);
+#pragma unroll
+        for (int i = 0; i < DL; i++) {
+          const uint32_t y = __builtin_amdgcn_perm(0u, x[i][q], sel);
+          top.add(y);
+          const uint64_t wide = ((uint64_t)y << (8 * fill)) | part[i];
+          part[i] = (uint32_t)wide;
+          if (fill + bytes >= 4) {
+            words[(lane + 64 * i) * ROW + word] = part[i];
+            part[i] = (uint32_t)(wide >> 32);
+          }
+        }
+        fill += bytes;
+        if (fill >= 4) {
+          fill -= 4;
+          word++;
+        }
+      }
+      most = fmaxf(most, top.value((int)(which >> 16)));
+#pragma unroll
+      for (int i = 0; i < DL; i++) x[i] = next[i];
+    }
+    if (fill > 0)
+#pragma unroll
+      for (int i = 0; i < DL; i++) words[(lane + 64 * i) * ROW + word] = part[i];
   }
 #pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    mk = fmaxf(mk, __shfl_xor(mk, s));
-    mv = fmaxf(mv, __shfl_xor(mv, s));
-  }
-  if (lane_id() == 0) {
-    atomicMax(&amax[0], __builtin_bit_cast(uint32_t, mk));
-    atomicMax(&amax[1], __builtin_bit_cast(uint32_t, mv));
-  }
+  for (int s = 1; s < 64; s <<= 1) most = fmaxf(most, __shfl_xor(most, s));
+  if (lane == 0) atomicMax(&amax[values], __float_as_uint(most));
   __syncthreads();
-  const int ke = scale_byte(__builtin_bit_cast(float, amax[0])), ve = scale_byte(__builtin_bit_cast(float, amax[1]));
-  if (t == 0) {
-    const_cast<uint8_t*>(c.k_scale)[(int64_t)id * c.ks_st[0] + (int64_t)hk * c.ks_st[1]] = (uint8_t)ke;
-    const_cast<uint8_t*>(c.v_scale)[(int64_t)id * c.vs_st[0] + (int64_t)hk * c.vs_st[1]] = (uint8_t)ve;
-  }
-  uint8_t* const k_new = const_cast<uint8_t*>(k_head) + (int64_t)id * c.k_st[0];
-  uint8_t* const v_new = const_cast<uint8_t*>(v_head) + (int64_t)id * c.v_st[0];
-  for (int i = t; i < n * (D / 4); i += 256) {
-    const int r = i / (D / 4), d = i % (D / 4) * 4;
-    const int64_t f = from[r];
-    uint32_t w = 0;
-    if (f >= 0) {
-      w = *(const uint32_t*)(k_head + (f >> 8) * c.k_st[0] + (f & 255) * D + d);
-      if (ks[r] != ke) w = rescale4(w, __builtin_ldexpf(1.f, ks[r] - ke));
+  const int e_new = scale_byte(__uint_as_float(amax[values]));
+  if (!values) {
+    if (threadIdx.x == 0)
+      const_cast<uint8_t*>(c.k_scale)[(int64_t)id * c.ks_st[0] + (int64_t)hk * c.ks_st[1]] = (uint8_t)e_new;
+    uint8_t* const to = const_cast<uint8_t*>(head) + (int64_t)id * c.k_st[0] + (int64_t)sub * D + lane % PIECES * 16;
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+      const int r = i * PER + lane / PIECES;
+      if (r >= n) continue;
+      const int was = (int)info[wave][r];
+      if (was != e_new) {
+        const float f = __builtin_ldexpf(1.f, was - e_new);
+#pragma unroll
+        for (int q = 0; q < 4; q++) rows[i][q] = rescale4(rows[i][q], f);
+      }
+      *(u32x4*)(to + r * D) = rows[i];
     }
-    *(uint32_t*)(k_new + r * D + d) = w;
+    return;
   }
-  for (int i = t; i < ((n + 15) & ~15) * D; i += 256) {
-    const int r = i / (16 * D) * 16 + (i & 15), d = i / 16 % D;
-    if (r >= n) continue;
-    const int64_t f = from[r];
-    uint32_t w = 0;
-    if (f >= 0) {
-      const int s = (int)(f & 255);
-      w = v_head[(f >> 8) * c.v_st[0] + (s >> 4) * (16 * D) + d * 16 + (s & 15)];
-      if (vs[r] != ve) w = rescale4(w, __builtin_ldexpf(1.f, vs[r] - ve));
+  if (wave == half && lane == 0)
+    const_cast<uint8_t*>(c.v_scale)[(int64_t)id * c.vs_st[0] + (int64_t)hk * c.vs_st[1]] = (uint8_t)e_new;
+  uint8_t* const to = const_cast<uint8_t*>(head) + (int64_t)id * c.v_st[0] + (int64_t)(sub / 16) * (16 * D);
+  const float f = __builtin_ldexpf(1.f, e - e_new);  // lane l: token l's
+  const bool change = __builtin_amdgcn_ballot_w64(lane < n && e != e_new) != 0;
+  for (int g = 0; g * 16 < n; g++) {
+    u32x4 y[DL];
+#pragma unroll
+    for (int i = 0; i < DL; i++)
+#pragma unroll
+      for (int q = 0; q < 4; q++) y[i][q] = words[(lane + 64 * i) * ROW + g * 4 + q];
+    if (change) {
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        float ft[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+          ft[t] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), g * 16 + q * 4 + t));
+#pragma unroll
+        for (int i = 0; i < DL; i++) {
+          const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)y[i][q], false);
+          const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)y[i][q], true);
+          y[i][q] = codes4(lo[0] * ft[0], lo[1] * ft[1], hi[0] * ft[2], hi[1] * ft[3]);
+        }
+      }
     }
-    v_new[(r >> 4) * (16 * D) + d * 16 + (r & 15)] = (uint8_t)w;
+    const int left = n - g * 16;
+#pragma unroll
+    for (int i = 0; i < DL; i++) {
+      uint8_t* const p = to + g * (16 * D) + (lane + 64 * i) * 16;
+      if (left >= 16) {
+        *(u32x4*)p = y[i];
+      } else {  // places behind the last token stay as they are
+#pragma unroll
+        for (int t = 0; t < 16; t++)
+          if (t < left) p[t] = (uint8_t)(y[i][t / 4] >> (8 * (t % 4)));
+      }
+    }
   }
 }
 
@@ -286,9 +458,11 @@ extern "C" int rswa_cache_evict(const rswa_cache_params* p, void* stream) {
   hipLaunchKernelGGL(cache_select_kernel, dim3((unsigned)heads), dim3(kSelectThreads), 0, st, a);
   if (int rc = check_launch("cache_evict select")) return rc;
   if (blocks == 0) return RSWA_OK;
+  const int waves = std::max(1, p->page_size / 64);  // of keys, and as many of values
+  const size_t lds = (size_t)waves * p->head_dim * 17 * 4;
   if (p->head_dim == 128)
-    hipLaunchKernelGGL((cache_move_kernel<128>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((cache_move_kernel<128>), dim3((unsigned)blocks), dim3(waves * 128), lds, st, a);
   else
-    hipLaunchKernelGGL((cache_move_kernel<64>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((cache_move_kernel<64>), dim3((unsigned)blocks), dim3(waves * 128), lds, st, a);
   return check_launch("cache_evict move");
 }
