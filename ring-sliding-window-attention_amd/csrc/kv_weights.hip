@@ -1,9 +1,11 @@
 // Sums of the softmax weights of every cached key over a call's rows, added to running sums.
 //
-// A wave keeps 64 keys as matrix operands in registers and goes over the rows, 16 at a time: S = Q K^T with the keys as
-// columns, exp2(S - lse), and a sum over rows that needs no exchange until the end.  K is read once, V not at all.
-// Few rows (one tile of 16): each wave has keys of its own.  More: the four waves of a block share the keys and take
-// every fourth row tile; their sums meet in LDS, in a fixed order.
+// A wave keeps up to 16 NR rows as matrix operands in registers and goes over the keys, 64 at a time: S = Q K^T with
+// the keys as columns, exp2(S - lse), and a sum over rows that needs no exchange until a tile's end.  V is not read.
+// Few rows: each wave has keys of its own, and K is read once.  More: the four waves of a block share the keys, with
+// rows of their own; their sums meet in LDS, in a fixed order, and rows beyond 64 NR come in further rounds over the
+// block's keys.  (Keys in registers and rows from memory instead took 64 us for 64 tokens of 32 / 8 heads against 32001
+// keys, waiting for rows 16 at a time.)
 #include "kv_cache.h"
 
 namespace rswa {
@@ -11,12 +13,12 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <typename T, int D, int RW>
+template <typename T, int D, int NR, int RW>
 __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheArgs a) {
   using V8 = typename Mma<T>::V8;
   constexpr int KW = 4 / RW;  // waves with keys of their own
   constexpr int C = D / 64;
-  __shared__ float lds[RW > 1 ? RW * kTileKeys : 1];
+  __shared__ float lds[2][RW > 1 ? RW * kTileKeys : 1];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int col = lane & 15, hi = lane >> 4;
   const int hk = blockIdx.x % a.heads_kv;
@@ -31,96 +33,134 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
   const uint8_t* const k_head = a.k + (int64_t)hk * a.k_st[1];
   const uint8_t* const ks_head = a.k_scale + (int64_t)hk * a.ks_st[1];
   float* const w = a.weights + (int64_t)x.b * a.w_st[0] + (int64_t)hk * a.w_st[1];
-  const T* const q_seq = (const T*)a.q + (int64_t)x.b * a.q_st[0] + (int64_t)x.row0 * a.q_st[1];
+  const T* const q_seq = (const T*)a.q + (int64_t)x.b * a.q_st[0] + (int64_t)x.row0 * a.q_st[1] + hi * 16;
   const float* const lse_seq = a.lse + (int64_t)x.b * a.lse_st[0] + (int64_t)x.row0 * a.lse_st[2];
 
   const int s0 = x.chunk_idx * x.chunk, s1 = min(s0 + x.chunk, x.tiles.count());
-  for (int slot = s0 + kw; slot < s1; slot += KW) {
-    const int tile = slot < x.tiles.n_sink ? slot : x.tiles.t_lo + slot - x.tiles.n_sink;
-    const int j0 = tile * kTileKeys;
-    // column `col` of the t-th product is key j0 + 16 t + col: one group, one page, one scale
-    V8 kf[4][C][2];
-    bool here[4];
+  auto tile_of = [&](int slot) { return slot < x.tiles.n_sink ? slot : x.tiles.t_lo + slot - x.tiles.n_sink; };
+
+  // B: column `col` of the t-th product is key 16 (col/4) + 4 t + col%4 of the tile, so that a lane's keys are of one
+  // group: one page id and one scale
+  auto page_id = [&](int slot) {
+    return table[min(tile_of(min(slot, s1 - 1)) * 4 + (col >> 2), n_groups - 1) >> per_page];
+  };
+  u32x4 kb[4][C];
+  int ke;
+  auto load_keys = [&](int tile, int id) {
+    const int page = (uint32_t)id < (uint32_t)a.num_pages ? id : 0;
+    const int g = min(tile * 4 + (col >> 2), n_groups - 1) & in_page;
+    const uint8_t* p = k_head + (int64_t)page * a.k_st[0] + (g * kGroupKeys + (col & 3)) * D + hi * 16;
+    ke = ks_head[(int64_t)page * a.ks_st[0]];
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-      const int g = min(tile * 4 + t, n_groups - 1);
-      const int id = table[g >> per_page];
-      here[t] = (uint32_t)id < (uint32_t)a.num_pages;
-      const int page = here[t] ? id : 0;
-      const uint8_t* p = k_head + (int64_t)page * a.k_st[0] + ((g & in_page) * kGroupKeys + col) * D + hi * 16;
-      const float scale = half_scale(ks_head[(int64_t)page * a.ks_st[0]]);
+    for (int t = 0; t < 4; t++)
 #pragma unroll
-      for (int c = 0; c < C; c++) {
-        const u32x4 r = *(const u32x4*)(p + c * 64);
-        kf[t][c][0] = widen8<T>(r[0], r[1], scale);
-        kf[t][c][1] = widen8<T>(r[2], r[3], scale);
-      }
-    }
-    float sum[4] = {0, 0, 0, 0};
-    // rows whose token sees the tile's first key or a later one
-    const int tok_first = max(0, j0 - shift);
-    const bool sinks = j0 < a.n_sink;
-    const int tok_last = a.window < 0 || sinks ? x.n_rows - 1
-                                               : (int)min((int64_t)x.n_rows - 1, (int64_t)j0 + kTileKeys - 1 + a.window - shift);
-    const int rt0 = tok_first * a.group / 16, rt1 = tok_last < 0 ? 0 : ((tok_last + 1) * a.group + 15) / 16;
-    for (int rt = rt0 + rw; rt < rt1; rt += RW) {
-      // A: row r = 16 rt + l%16;  the lane's results are rows 16 rt + 4 (l/16) .. +3
-      const int r = min(rt * 16 + col, n_flat - 1);
-      const int tok = quotient(r, a.by_group);
-      const T* q = q_seq + (int64_t)tok * a.q_st[1] + (int64_t)(hk * a.group + r - tok * a.group) * a.q_st[2] + hi * 16;
-      V8 qf[C][2];
+      for (int c = 0; c < C; c++) kb[t][c] = *(const u32x4*)(p + t * 4 * D + c * 64);
+  };
+
+  for (int round = 0; round < n_flat; round += 16 * NR * RW) {
+    // A: lane l has row l%16 of each row tile; its results are rows 4 (l/16) .. +3
+    const int first_row = round + rw * (16 * NR);
+    V8 q[NR][C][2];
+    float base[NR][4];
+    int tok0[NR], tok1[NR];  // first and last token (tok1 < 0: no rows)
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+      const int r0 = first_row + 16 * i, r = min(r0 + col, n_flat - 1);
+      const int tok = quotient(r, a.by_group), head = hk * a.group + r - tok * a.group;
+      const T* p = q_seq + (int64_t)tok * a.q_st[1] + (int64_t)head * a.q_st[2];
 #pragma unroll
       for (int c = 0; c < C; c++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) qf[c][h] = *(const V8*)(q + c * 64 + h * 8);
-      float base[4];
-      int pos[4];
+        for (int h = 0; h < 2; h++) q[i][c][h] = *(const V8*)(p + c * 64 + h * 8);
+      // rows that are none, or saw nothing, add nothing: exp2(x - inf)
+      const float lse = lse_seq[(int64_t)head * a.lse_st[1] + (int64_t)tok * a.lse_st[2]];
+      const float mine = r0 + col < n_flat && lse != -__builtin_inff() ? lse * kLog2e : __builtin_inff();
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int re = rt * 16 + hi * 4 + e, rc = min(re, n_flat - 1);
-        const int te = quotient(rc, a.by_group);
-        const float lse = lse_seq[(int64_t)(hk * a.group + rc - te * a.group) * a.lse_st[1] + (int64_t)te * a.lse_st[2]];
-        pos[e] = re < n_flat && lse != -__builtin_inff() ? shift + te : -1;
-        base[e] = lse * kLog2e;
-      }
+      for (int e = 0; e < 4; e++) base[i][e] = __shfl(mine, hi * 4 + e);
+      tok0[i] = quotient(min(r0, n_flat - 1), a.by_group);
+      tok1[i] = r0 < n_flat ? quotient(min(r0 + 15, n_flat - 1), a.by_group) : -1;
+    }
+
+    int slot = s0 + kw;
+    if (slot >= s1) return;  // (RW > 1: all waves or none)
+    int id = page_id(slot), id_next = page_id(slot + KW);
+    load_keys(tile_of(slot), id);
+    for (; slot < s1; slot += KW) {
+      const int tile = tile_of(slot), j0 = tile * kTileKeys;
+      const int id_after = page_id(slot + 2 * KW);
+      const bool here = (uint32_t)id < (uint32_t)a.num_pages;
+      const bool all = __builtin_amdgcn_ballot_w64(!here) == 0;
+      const float scale = half_scale(ke);
+      const int key = j0 + 16 * (col >> 2) + (col & 3);  // of product 0
+      float sum[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int t = 0; t < 4; t++) {
-        f32x4 s = {0, 0, 0, 0};
+        V8 kf[C][2];
 #pragma unroll
-        for (int c = 0; c < C; c++)
+        for (int c = 0; c < C; c++) {
+          kf[c][0] = widen8<T>(kb[t][c][0], kb[t][c][1], scale);
+          kf[c][1] = widen8<T>(kb[t][c][2], kb[t][c][3], scale);
+        }
+        f32x4 s[NR];
 #pragma unroll
-          for (int h = 0; h < 2; h++) s = Mma<T>::mfma16(qf[c][h], kf[t][c][h], s);
-        const int j = j0 + 16 * t + col;
+        for (int i = 0; i < NR; i++) {
+          s[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const bool see = here[t] && j <= pos[e] && (a.window < 0 || j >= pos[e] - a.window || j < a.n_sink);
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], sc, -base[e]));
-          sum[t] += see ? p : 0.f;
+          for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) s[i] = Mma<T>::mfma16(q[i][c][h], kf[c][h], s[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+          const bool whole = all && j0 + kTileKeys - 1 <= shift + tok0[i] &&
+                             (a.window < 0 || j0 >= shift + tok1[i] - a.window);
+          if (!whole) {
+            const int j = key + 4 * t;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const int pos = shift + quotient(min(first_row + 16 * i + hi * 4 + e, n_flat - 1), a.by_group);
+              const bool see = here && j <= pos && (a.window < 0 || j >= pos - a.window || j < a.n_sink);
+              s[i][e] = see ? s[i][e] : -__builtin_inff();
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; e++) sum[t] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], sc, -base[i][e]));
         }
       }
-    }
+      if (slot + KW < s1) load_keys(tile_of(slot + KW), id_next);
+      id = id_next;
+      id_next = id_after;
 #pragma unroll
-    for (int t = 0; t < 4; t++) sum[t] = columns_sum(sum[t]);
-    // lane l takes key l of the tile
-    float mine = hi == 0 ? sum[0] : hi == 1 ? sum[1] : hi == 2 ? sum[2] : sum[3];
-    if constexpr (RW > 1) {
-      lds[rw * kTileKeys + lane] = mine;
-      __syncthreads();
-      mine = 0.f;
+      for (int t = 0; t < 4; t++) sum[t] = columns_sum(sum[t]);
+      // lane l takes product l/16's column
+      const int at = 16 * (col >> 2) + 4 * hi + (col & 3);
+      float mine = hi == 0 ? sum[0] : hi == 1 ? sum[1] : hi == 2 ? sum[2] : sum[3];
+      if constexpr (RW > 1) {
+        // (two buffers: a wave that writes the next tile's has passed the barrier behind the reads of this one's last)
+        float* const buf = lds[(slot - s0) & 1];
+        buf[rw * kTileKeys + lane] = mine;
+        __syncthreads();
+        mine = 0.f;
+        if (rw == 0)
 #pragma unroll
-      for (int i = 0; i < RW; i++) mine += lds[i * kTileKeys + lane];
-      __syncthreads();
+          for (int i = 0; i < RW; i++) mine += buf[i * kTileKeys + lane];
+      }
+      if (rw == 0 && j0 + at < min(x.len, a.w_len)) w[j0 + at] += mine;
     }
-    if (rw == 0 && j0 + lane < min(x.len, a.w_len)) w[j0 + lane] += mine;
+    if constexpr (RW > 1) __syncthreads();
   }
 }
 
+// Rows of a sequence (on average, of a pack): up to 16, up to 64, more.
 template <typename T, int D>
-void launch_weights(const CacheArgs& a, bool share, int64_t grid, hipStream_t stream) {
-  if (share)
-    hipLaunchKernelGGL((cache_weights_kernel<T, D, 4>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
+void launch_weights(const CacheArgs& a, int64_t rows, int64_t grid, hipStream_t stream) {
+  const dim3 blocks((unsigned)grid), threads(kThreads);
+  if (rows <= 16)
+    hipLaunchKernelGGL((cache_weights_kernel<T, D, 1, 1>), blocks, threads, 0, stream, a);
+  else if (rows <= 64)
+    hipLaunchKernelGGL((cache_weights_kernel<T, D, 4, 1>), blocks, threads, 0, stream, a);
   else
-    hipLaunchKernelGGL((cache_weights_kernel<T, D, 1>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((cache_weights_kernel<T, D, 4, 4>), blocks, threads, 0, stream, a);
 }
 
 }  // namespace
@@ -143,9 +183,9 @@ extern "C" int rswa_cache_weights(const rswa_cache_params* p, void* stream) {
   a.w_st[1] = p->weights_stride[1];
   a.w_len = p->weights_len;
   a.row_tile = INT32_MAX;  // a unit has all rows of its sequence
-  const bool share = ceil_div(rows, p->batch) * a.group > 16;
-  const int64_t wanted = kComputeUnits * 6;
-  a.min_chunk = share ? 1 : 4;
+  const int64_t per_seq = ceil_div(rows, p->batch) * a.group;
+  const int64_t wanted = kComputeUnits * (per_seq <= 16 ? 6 : 2);
+  a.min_chunk = per_seq > 64 ? 1 : 4;
   a.per_unit = (float)p->heads_kv / (float)wanted;
   const int64_t per_head = ceil_div(wanted, p->heads_kv) + 1;
   const int64_t most_tiles = ceil_div((int64_t)p->max_pages * p->page_size, kTileKeys);
@@ -154,9 +194,9 @@ extern "C" int rswa_cache_weights(const rswa_cache_params* p, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   clear_launch_error();
   if (p->dtype == RSWA_BF16)
-    p->head_dim == 128 ? launch_weights<__bf16, 128>(a, share, grid, st) : launch_weights<__bf16, 64>(a, share, grid, st);
+    p->head_dim == 128 ? launch_weights<__bf16, 128>(a, per_seq, grid, st) : launch_weights<__bf16, 64>(a, per_seq, grid, st);
   else
-    p->head_dim == 128 ? launch_weights<_Float16, 128>(a, share, grid, st)
-                       : launch_weights<_Float16, 64>(a, share, grid, st);
+    p->head_dim == 128 ? launch_weights<_Float16, 128>(a, per_seq, grid, st)
+                       : launch_weights<_Float16, 64>(a, per_seq, grid, st);
   return check_launch("cache_weights");
 }
