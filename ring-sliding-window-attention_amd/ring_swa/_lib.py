@@ -273,6 +273,11 @@ def _load_torch_calls():
     mod.bind(*[ctypes.cast(fn, c_void_p).value
                for fn in (L.rswa_attn_fwd, L.rswa_attn_bwd, L.rswa_attn_bwd_workspace_bytes)],
              check, band_backward)
+    if mod.cache_params_bytes() != ctypes.sizeof(CacheParams):
+        raise ImportError(f"{path} was built for another rswa_cache_params: rebuild it")
+    mod.bind_cache(*[ctypes.cast(fn, c_void_p).value
+                     for fn in (L.rswa_cache_append, L.rswa_cache_attn, L.rswa_cache_weights, L.rswa_cache_evict,
+                                L.rswa_cache_attn_workspace_bytes)])
     return mod
 
 

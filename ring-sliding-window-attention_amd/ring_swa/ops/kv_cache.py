@@ -74,6 +74,13 @@ def _dense_from(t: torch.Tensor, dim: int) -> bool:
     return True
 
 
+def _calls(cache):
+    """The native module where it may take the call (it answers None to what it leaves to Python)."""
+    if cache[0].is_cuda and not torch.compiler.is_compiling():
+        return _lib.torch_calls()
+    return None
+
+
 def _no_grad(*tensors) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError("the cache has no backward: call this under torch.no_grad()")
@@ -84,7 +91,7 @@ def _cache_params(cache, page_table, seqlens, rows, cu_seqlens):
     k, v, k_scale, v_scale = cache
     assert k.dim() == 4 and v.dim() == 5, "expected k [pages, heads, page, dim], v [pages, heads, page / 16, dim, 16]"
     pages, heads, size, dim = k.shape
-    assert size in PAGE_SIZES, f"page_size must be one of {PAGE_SIZES}"
+    assert heads > 0 and size in PAGE_SIZES, f"expected heads, and page_size one of {PAGE_SIZES}"
     assert v.shape == (pages, heads, size // 16, dim, 16), "v must be [pages, heads, page / 16, dim, 16]"
     assert k_scale.shape == v_scale.shape == (pages, heads), "scales must be [pages, heads]"
     assert k.dtype == v.dtype == torch.float8_e4m3fn, "k and v must be float8_e4m3fn"
@@ -155,6 +162,9 @@ def kv_cache_append(
     smallest normal code change).  Infinities and NaN are stored as NaN.  Tokens beyond the last page
     of ``page_table``, or whose page is not there, are dropped.  ``seqlens`` is left alone; two
     sequences of one call must not have a page written in common."""
+    calls = _calls(cache)
+    if calls is not None and calls.cache_append(cache, k, v, page_table, seqlens, cu_seqlens):
+        return
     _no_grad(k, v)
     p, dev = _cache_params(cache, page_table, seqlens, k, cu_seqlens)
     assert k.shape == v.shape and k.dtype == v.dtype, "k and v must have the same shape and dtype"
@@ -187,6 +197,12 @@ def kv_cache_attn(
     Returns the output, shape and dtype of ``q``, and with ``return_lse`` the log-sum-exp, fp32
     ``[batch, heads, seq]`` (``[heads, tokens]`` of a pack), as ``merge_attn_out`` takes it.  Rows that
     see nothing: 0 and ``-inf``."""
+    calls = _calls(cache)
+    if calls is not None:
+        got = calls.cache_attn(q, cache, page_table, seqlens, window_size, cu_seqlens, softmax_scale,
+                               num_sink_tokens, return_lse)
+        if got is not None:
+            return got
     _no_grad(q)
     p, dev = _cache_params(cache, page_table, seqlens, q, cu_seqlens)
     packed = cu_seqlens is not None
@@ -232,6 +248,10 @@ def kv_cache_weights(
 
     ``lse`` is what ``kv_cache_attn(..., return_lse=True)`` returned for the same arguments; ``weights``
     fp32 ``[batch, kv_heads, n]``, entry ``j`` that of token ``j`` (tokens from ``n`` on are passed over)."""
+    calls = _calls(cache)
+    if calls is not None and calls.cache_weights(q, cache, page_table, seqlens, lse, weights, window_size, cu_seqlens,
+                                                 softmax_scale, num_sink_tokens):
+        return
     _no_grad(q)
     p, dev = _cache_params(cache, page_table, seqlens, q, cu_seqlens)
     packed = cu_seqlens is not None
@@ -275,6 +295,12 @@ def kv_cache_evict(
     of them may be among the new ones.  Returns the new ``seqlens``, the kept tokens' weights (shape of
     ``weights``, zeros behind) and their old numbers, int32 ``[batch, kv_heads, budget]`` (``-1`` behind).
     From then on a token's number is its place among the kept ones, for windows too."""
+    calls = _calls(cache)
+    if calls is not None:
+        got = calls.cache_evict(cache, weights, page_table, seqlens, new_page_table, budget, num_sink_tokens,
+                                num_recent)
+        if got is not None:
+            return got
     assert budget > 0 and num_sink_tokens >= 0 and num_recent >= 0
     assert num_sink_tokens + num_recent <= budget, "budget must hold the sinks and the recent tokens"
     p, dev = _cache_params(cache, page_table, seqlens, None, None)
