@@ -90,8 +90,8 @@ __global__ void cache_append_kernel(const AppendArgs a) {
   // (a positive float's bits grow with it)
   if (lane_id() == 0) atomicMax(&amax[which], __builtin_bit_cast(uint32_t, most));
   __syncthreads();
-  uint8_t* const scale = which ? const_cast<uint8_t*>(c.v_scale) + (int64_t)id * c.vs_st[0] + (int64_t)hk * c.vs_st[1]
-                               : const_cast<uint8_t*>(c.k_scale) + (int64_t)id * c.ks_st[0] + (int64_t)hk * c.ks_st[1];
+  uint8_t* const scale = which ? const_cast<uint8_t*>(c.v_scale) + times(id, c.vs_st[0]) + times(hk, c.vs_st[1])
+                               : const_cast<uint8_t*>(c.k_scale) + times(id, c.ks_st[0]) + times(hk, c.ks_st[1]);
   const int was = from > 0 ? *scale : 0;
   const int e_new = max(was, scale_byte(__builtin_bit_cast(float, amax[which])));
   const float inv = inverse(e_new);
@@ -111,7 +111,7 @@ __global__ void cache_append_kernel(const AppendArgs a) {
                           (float)v[e][4 * h + 3] * inv);
   const int old = min(16, from - g * 16);  // places e < old hold tokens from before
   if (!which) {
-    uint8_t* k = const_cast<uint8_t*>(c.k) + (int64_t)id * c.k_st[0] + (int64_t)hk * c.k_st[1] + g * 16 * D + d0;
+    uint8_t* k = const_cast<uint8_t*>(c.k) + times(id, c.k_st[0]) + times(hk, c.k_st[1]) + g * 16 * D + d0;
 #pragma unroll
     for (int e = 0; e < 16; e++) {
       if (e >= lo && e < hi) {
@@ -122,7 +122,7 @@ __global__ void cache_append_kernel(const AppendArgs a) {
       }
     }
   } else {
-    uint8_t* vp = const_cast<uint8_t*>(c.v) + (int64_t)id * c.v_st[0] + (int64_t)hk * c.v_st[1] + (g * D + d0) * 16;
+    uint8_t* vp = const_cast<uint8_t*>(c.v) + times(id, c.v_st[0]) + times(hk, c.v_st[1]) + (g * D + d0) * 16;
     const bool full = lo == 0 && hi == 16;
     if (full || (grown && old > 0)) {
 #pragma unroll

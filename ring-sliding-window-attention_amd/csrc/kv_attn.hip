@@ -4,7 +4,7 @@
 //   S^T = K Q^T    A = K, straight from memory: lane l loads 16 bytes of key row l%16, widened in registers
 //   P^T = exp2(S^T - max)
 //   O^T += V^T P^T A = V^T, straight from memory too: a lane's 16 bytes are 16 keys of one dimension
-// Nothing goes through LDS: which of the 64 keys is row m of the t-th S^T tile is free to choose, and key
+// Which of the 64 keys is row m of the t-th S^T tile is free to choose, and key
 // 16 (m/4) + 4 t + m%4 is the choice by which a lane's 16 scores are 16 consecutive keys -- those of its 16 bytes of
 // V -- and already lie as the B operand of the second product wants them.  All 16 are of one group, so that a page's
 // scale is one value per lane, folded into the widening.
@@ -49,172 +49,138 @@ struct Pages {
   int k, v;  // ids as the table has them
 };
 
-template <typename T, int D, int NT, int WR>
-__global__ __launch_bounds__(kThreads, 2) void cache_attn_kernel(const CacheArgs a) {
-  using V8 = typename Mma<T>::V8;
-  constexpr int KW = 4 / WR;  // waves that share a row tile's keys
-  constexpr int ROWS = NT * 16 * WR;
-  constexpr int C = D / 64;   // 16-byte pieces of a lane's key row
-  constexpr int ND = D / 16;
-  constexpr int LD = D + 4;
-  __shared__ float lds[KW > 1 ? KW * ROWS * (LD + 2) : 1];
-
-  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const int col = lane & 15, hi = lane >> 4;
-  const int hk = blockIdx.x % a.heads_kv;
-  Unit x;
-  if (!find_unit<0>(a, blockIdx.x / a.heads_kv, x)) return;
-
-  const int wr = wave / KW, kw = wave % KW;
-  const int r0 = x.row_tile * ROWS + wr * (NT * 16);  // the wave's first row
-  const int shift = x.len - x.n_rows;                 // position of token 0
-  const int n_flat = x.n_rows * a.group;
-
-  // its rows' tokens, first and last
-  const int tok0 = quotient(min(r0, n_flat - 1), a.by_group);
-  const int tok1 = quotient(min(r0 + NT * 16, n_flat) - 1, a.by_group);
-  const bool some = r0 < n_flat;
-  const int first = shift + tok0, last = some ? shift + tok1 : -1;
-  const TileList list = chunk_tiles(a, x, first, last);
-  const int lo_all = a.window < 0 ? 0 : max(0, first - a.window);
-
-  // B operand: rows of Q, the dimensions in the order in which a lane of A holds K's
-  V8 qf[NT][C][2];
-  int pos[NT], lo[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; nt++) {
-    const int r = r0 + nt * 16 + col;
-    const int tok = quotient(min(r, n_flat - 1), a.by_group);
-    const int head = hk * a.group + min(r, n_flat - 1) - tok * a.group;
-    pos[nt] = r < n_flat ? shift + tok : -1;
-    lo[nt] = a.window < 0 ? 0 : pos[nt] - a.window;
-    const T* q = (const T*)a.q + (int64_t)x.b * a.q_st[0] + (int64_t)(x.row0 + tok) * a.q_st[1] +
-                 (int64_t)head * a.q_st[2] + hi * 16;
-#pragma unroll
-    for (int c = 0; c < C; c++)
-#pragma unroll
-      for (int h = 0; h < 2; h++) qf[nt][c][h] = *(const V8*)(q + c * 64 + h * 8);
-  }
-
-  const int32_t* table = a.table + (int64_t)x.b * a.table_st;
-  const int n_groups = (x.len + kGroupKeys - 1) / kGroupKeys;
-  const int per_page = a.page_log2 - 4;
-  auto page_ids = [&](int tile) {
+// Where a kv head's keys and values of one sequence are.
+template <int D>
+struct Keys {
+  const CacheArgs& a;
+  const int32_t* table;
+  const uint8_t *k, *v, *k_scale, *v_scale;
+  int n_groups, per_page, col, hi;
+  __device__ __forceinline__ Keys(const CacheArgs& args, const Unit& x, int hk, int lane)
+      : a(args), table(args.table + (int64_t)x.b * args.table_st), k(args.k + times(hk, args.k_st[1])),
+        v(args.v + times(hk, args.v_st[1])), k_scale(args.k_scale + times(hk, args.ks_st[1])),
+        v_scale(args.v_scale + times(hk, args.vs_st[1])), n_groups((x.len + kGroupKeys - 1) / kGroupKeys),
+        per_page(args.page_log2 - 4), col(lane & 15), hi(lane >> 4) {}
+  __device__ __forceinline__ Pages pages(int tile) const {
     const int g = tile * 4;
-    Pages p;
-    p.k = table[min(g + (col >> 2), n_groups - 1) >> per_page];
-    p.v = table[min(g + hi, n_groups - 1) >> per_page];
-    return p;
-  };
-  const uint8_t* const k_head = a.k + (int64_t)hk * a.k_st[1];
-  const uint8_t* const v_head = a.v + (int64_t)hk * a.v_st[1];
-  const uint8_t* const ks_head = a.k_scale + (int64_t)hk * a.ks_st[1];
-  const uint8_t* const vs_head = a.v_scale + (int64_t)hk * a.vs_st[1];
+    return {table[min(g + (col >> 2), n_groups - 1) >> per_page], table[min(g + hi, n_groups - 1) >> per_page]};
+  }
   // (a page that is not there is read as page 0: within the pool, and masked)
-  auto there = [&](int id) { return (uint32_t)id < (uint32_t)a.num_pages; };
-  const int in_page = (1 << per_page) - 1;
+  __device__ __forceinline__ bool there(int id) const { return (uint32_t)id < (uint32_t)a.num_pages; }
+  // row l%16 of the t-th product, 16 bytes from hi * 16 on (and every 64 further)
+  __device__ __forceinline__ const uint8_t* key_row(int tile, int t, int id) const {
+    const int g = min(tile * 4 + (col >> 2), n_groups - 1) & ((1 << per_page) - 1);
+    return k + times(there(id) ? id : 0, a.k_st[0]) + (g * kGroupKeys + 4 * t + (col & 3)) * D + hi * 16;
+  }
+  __device__ __forceinline__ int key_scale(int id) const { return k_scale[times(there(id) ? id : 0, a.ks_st[0])]; }
+  // dimension l%16 (and every 16th further, 256 bytes each), the 16 keys of group hi
+  __device__ __forceinline__ const uint8_t* values(int tile, int id) const {
+    const int g = min(tile * 4 + hi, n_groups - 1) & ((1 << per_page) - 1);
+    return v + times(there(id) ? id : 0, a.v_st[0]) + g * (kGroupKeys * D) + col * 16;
+  }
+  __device__ __forceinline__ int value_scale(int id) const { return v_scale[times(there(id) ? id : 0, a.vs_st[0])]; }
+};
 
-  u32x4 kb[4][C], vb[ND];
-  int ke, ve;
-  auto load_k = [&](int tile, int id) {
-    const int page = there(id) ? id : 0;
-    const int g = min(tile * 4 + (col >> 2), n_groups - 1) & in_page;
-    const uint8_t* p = k_head + (int64_t)page * a.k_st[0] + (g * kGroupKeys + (col & 3)) * D + hi * 16;
-    ke = ks_head[(int64_t)page * a.ks_st[0]];
+// Bytes of a lane's 16 keys (from j on) that some row at positions first .. last sees.
+__device__ __forceinline__ u32x4 seen_bytes(const CacheArgs& a, int j, bool here, int first, int last) {
+  const int lo = a.window < 0 ? 0 : max(0, first - a.window);
+  u32x4 keep;
 #pragma unroll
-    for (int t = 0; t < 4; t++)
+  for (int w = 0; w < 4; w++) {
+    uint32_t mask = 0;
 #pragma unroll
-      for (int c = 0; c < C; c++) kb[t][c] = *(const u32x4*)(p + t * 4 * D + c * 64);
-  };
-  auto load_v = [&](int tile, int id) {
-    const int page = there(id) ? id : 0;
-    const int g = min(tile * 4 + hi, n_groups - 1) & in_page;
-    const uint8_t* p = v_head + (int64_t)page * a.v_st[0] + g * (kGroupKeys * D) + col * 16;
-    ve = vs_head[(int64_t)page * a.vs_st[0]];
-#pragma unroll
-    for (int d = 0; d < ND; d++) vb[d] = *(const u32x4*)(p + d * 256);
-  };
+    for (int e = 0; e < 4; e++) {
+      const int jj = j + 4 * w + e;
+      mask |= here && jj <= last && (jj >= lo || jj < a.n_sink) ? 0xffu << (8 * e) : 0u;
+    }
+    keep[w] = mask;
+  }
+  return keep;
+}
 
+// 16 NT rows of a wave from row r0 of the sequence on: B operands of Q (the dimensions in the order in which a lane of
+// A holds K's), what each row sees, and the running softmax and output, O^T.
+template <typename T, int D, int NT>
+struct Rows {
+  using V8 = typename Mma<T>::V8;
+  static constexpr int C = D / 64;  // 16-byte pieces of a lane's key row
+  static constexpr int ND = D / 16;
+  V8 q[NT][C][2];
+  int pos[NT];
+  int first, last;  // positions of the first and the last row (last < 0: no rows)
   f32x4 acc[ND][NT];
   float m[NT], l[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; nt++) {
-    m[nt] = -__builtin_inff();
-    l[nt] = 0.f;
-#pragma unroll
-    for (int d = 0; d < ND; d++) acc[d][nt] = f32x4{0, 0, 0, 0};
-  }
-  const float sc = 2.f * a.scale_log2;  // (K at half its value)
+  float sc;
 
-  const int n = list.count();
-  int i = kw;
-  Pages now{0, 0}, next{0, 0};
-  if (i < n) {
-    now = page_ids(list[i]);
-    next = page_ids(list[min(i + KW, n - 1)]);
-    load_k(list[i], now.k);
-    load_v(list[i], now.v);
-  }
-  for (; i < n; i += KW) {
-    const int tile = list[i], tile_next = list[min(i + KW, n - 1)];
-    const Pages after = page_ids(list[min(i + 2 * KW, n - 1)]);
-
-    // S^T
-    f32x4 s[NT][4];
-    const float kscale = half_scale(ke);
+  __device__ __forceinline__ Rows(const CacheArgs& a, const Unit& x, int hk, int r0, int col, int hi) {
+    const int shift = x.len - x.n_rows, n_flat = x.n_rows * a.group;  // shift: position of token 0
+    first = shift + quotient(min(r0, n_flat - 1), a.by_group);
+    last = r0 < n_flat ? shift + quotient(min(r0 + NT * 16, n_flat) - 1, a.by_group) : -1;
+    sc = 2.f * a.scale_log2;  // (K at half its value)
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) s[nt][t] = f32x4{0, 0, 0, 0};
+    for (int nt = 0; nt < NT; nt++) {
+      const int r = r0 + nt * 16 + col;
+      const int tok = quotient(min(r, n_flat - 1), a.by_group);
+      const int head = hk * a.group + min(r, n_flat - 1) - tok * a.group;
+      pos[nt] = r < n_flat ? shift + tok : -1;
+      const T* p = (const T*)a.q + (int64_t)x.b * a.q_st[0] + (int64_t)(x.row0 + tok) * a.q_st[1] +
+                   (int64_t)head * a.q_st[2] + hi * 16;
 #pragma unroll
       for (int c = 0; c < C; c++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const V8 kf = widen8<T>(kb[t][c][2 * h], kb[t][c][2 * h + 1], kscale);
+        for (int h = 0; h < 2; h++) q[nt][c][h] = *(const V8*)(p + c * 64 + h * 8);
+      m[nt] = -__builtin_inff();
+      l[nt] = 0.f;
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) s[nt][t] = Mma<T>::mfma16(kf, qf[nt][c][h], s[nt][t]);
-        }
+      for (int d = 0; d < ND; d++) acc[d][nt] = f32x4{0, 0, 0, 0};
     }
-    const bool here = there(now.v);
-    const bool more = i + KW < n;
-    if (more) load_k(tile_next, next.k);
-
-    // masks, where a row sees part of the tile or a page is missing
-    const int j0 = tile * kTileKeys;
-    const bool whole = j0 + kTileKeys - 1 <= first && (a.window < 0 || j0 >= last - a.window) &&
-                       __builtin_amdgcn_ballot_w64(!here) == 0;
-    if (!whole) {
-      const int j = j0 + hi * 16;
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int jj = j + 4 * t + e;
-            const bool see = here && jj <= pos[nt] && (jj >= lo[nt] || jj < a.n_sink);
-            s[nt][t][e] = see ? s[nt][t][e] : -__builtin_inff();
-          }
-    }
-
-    // softmax: a row's scores are in the four lanes of its column
-    V8 pf[NT][2];
+  }
+  // does every row see the whole tile? (`here`: the lane's group has its page)
+  __device__ __forceinline__ bool whole(const CacheArgs& a, int j0, bool here) const {
+    return j0 + kTileKeys - 1 <= first && (a.window < 0 || j0 >= last - a.window) &&
+           __builtin_amdgcn_ballot_w64(!here) == 0;
+  }
+  // scores of what a row does not see become -inf; j: the lane's first key
+  __device__ __forceinline__ void mask(const CacheArgs& a, f32x4 (&s)[NT][4], int j, bool here) const {
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
+      const int lo = a.window < 0 ? 0 : pos[nt] - a.window;
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int jj = j + 4 * t + e;
+          const bool see = here && jj <= pos[nt] && (jj >= lo || jj < a.n_sink);
+          s[nt][t][e] = see ? s[nt][t][e] : -__builtin_inff();
+        }
+    }
+  }
+  // One tile's step of the running softmax (a row's scores are in the four lanes of its column): the maximum, with
+  // what it changes ...
+  __device__ __forceinline__ void raise(const f32x4 (&s)[NT][4]) {
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      // (NaN stays NaN, and its weights are: the other maximum would first quiet each score, an instruction apiece)
       float top = s[nt][0][0];
 #pragma unroll
       for (int t = 0; t < 4; t++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) top = fmaxf(top, s[nt][t][e]);
+        for (int e = 0; e < 4; e++) top = __builtin_elementwise_maximum(top, s[nt][t][e]);
       top = columns_max(top);
       if (__builtin_amdgcn_ballot_w64(top > m[nt])) {
-        const float m_new = fmaxf(m[nt], top);
+        const float m_new = __builtin_elementwise_maximum(m[nt], top);
         const float shrink = m[nt] == m_new ? 1.f : __builtin_amdgcn_exp2f((m[nt] - m_new) * sc);
         m[nt] = m_new;
         l[nt] *= shrink;
 #pragma unroll
         for (int d = 0; d < ND; d++) acc[d][nt] *= shrink;
       }
+    }
+  }
+  // ... and the weights, P^T
+  __device__ __forceinline__ void weigh(const f32x4 (&s)[NT][4], V8 (&pf)[NT][2]) {
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
       const float base = m[nt] == -__builtin_inff() ? 0.f : __builtin_fmaf(m[nt], sc, -kLift<T>);
       float sum = 0.f;
 #pragma unroll
@@ -230,21 +196,113 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_kernel(const CacheArgs
       }
       l[nt] += sum;
     }
+  }
+};
 
+// The kernel's arguments read again: those of the epilogue alone would be loaded ahead of the loop, where they crowd
+// others out of the scalar registers.
+__device__ __forceinline__ const CacheArgs& arguments_again() {
+  auto p = (const __attribute__((address_space(4))) CacheArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const CacheArgs*)p;
+}
+
+// Row r's result: written if the row has one chunk, else left for the join.  d0: first of 4 dimensions; mx in base 2.
+template <typename T, int D>
+__device__ __forceinline__ void store_row(const CacheArgs& a, const Unit& x, int hk, int r, int d0, f32x4 o, float mx,
+                                          float sum) {
+  if (r >= x.n_rows * a.group) return;
+  if (x.n_chunks == 1) {
+    const int tok = quotient(r, a.by_group), head = hk * a.group + r - tok * a.group;
+    const float inv = sum == 0.f ? 0.f : 2.f / sum;  // (V at half its value)
+    T* out = (T*)a.out + (int64_t)x.b * a.o_st[0] + (int64_t)(x.row0 + tok) * a.o_st[1] + (int64_t)head * a.o_st[2];
+    *(typename Mma<T>::V4*)(out + d0) = Mma<T>::pack4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (d0 == 0 && a.lse)
+      a.lse[(int64_t)x.b * a.lse_st[0] + (int64_t)head * a.lse_st[1] + (int64_t)(x.row0 + tok) * a.lse_st[2]] =
+          sum == 0.f ? -__builtin_inff() : (mx - kLift<T> + __log2f(sum)) * (1.f / kLog2e);
+  } else {
+    if (x.part + x.n_chunks > a.part_units) return;  // (cu_seqlens that overlap: more units than rows make)
+    const int64_t at = (((int64_t)(x.part + x.chunk_idx) * a.heads_kv + hk) << a.row_log2) + (r - (x.row_tile << a.row_log2));
+    *(f32x4*)(a.part + at * D + d0) = o;
+    if (d0 == 0) *(f32x2*)(a.part_ml + at * 2) = f32x2{mx, sum};
+  }
+}
+
+// Few rows: the four waves of a block have the same rows, each its own keys, and everything from memory to the output
+// stays in registers; the waves meet in LDS at the end.
+template <typename T, int D, int NT>
+__global__ __launch_bounds__(kThreads, 2) void cache_attn_kernel(const CacheArgs a) {
+  using R = Rows<T, D, NT>;
+  using V8 = typename Mma<T>::V8;
+  constexpr int KW = 4, ROWS = NT * 16, C = R::C, ND = R::ND;
+  constexpr int LD = D + 4;
+  __shared__ float lds[KW * ROWS * (LD + 2)];
+
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int col = lane & 15, hi = lane >> 4;
+  const int hk = blockIdx.x % a.heads_kv;
+  Unit x;
+  if (!find_unit<0>(a, blockIdx.x / a.heads_kv, x)) return;
+  R w(a, x, hk, x.row_tile * ROWS, col, hi);
+  const TileList list = chunk_tiles(a, x, w.first, w.last);
+  const Keys<D> keys(a, x, hk, lane);
+
+  u32x4 kb[4][C], vb[ND];
+  int ke, ve;
+  auto load_k = [&](int tile, int id) {
+    ke = keys.key_scale(id);
+    const uint8_t* p = keys.key_row(tile, 0, id);
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+      for (int c = 0; c < C; c++) kb[t][c] = *(const u32x4*)(p + t * 4 * D + c * 64);
+  };
+  auto load_v = [&](int tile, int id) {
+    ve = keys.value_scale(id);
+    const uint8_t* p = keys.values(tile, id);
+#pragma unroll
+    for (int d = 0; d < ND; d++) vb[d] = *(const u32x4*)(p + d * 256);
+  };
+
+  const int n = list.count();
+  int i = wave;
+  Pages next{0, 0};
+  bool here = false;  // the lane's group of the tile has its page
+  if (i < n) {
+    const Pages now = keys.pages(list[i]);
+    here = keys.there(now.v);
+    next = keys.pages(list[min(i + KW, n - 1)]);
+    load_k(list[i], now.k);
+    load_v(list[i], now.v);
+  }
+  for (; i < n; i += KW) {
+    const int j0 = list[i] * kTileKeys, tile_next = list[min(i + KW, n - 1)];
+    const Pages after = keys.pages(list[min(i + 2 * KW, n - 1)]);
+    f32x4 s[NT][4];
+    const float kscale = half_scale(ke);
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) s[nt][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const V8 kf = widen8<T>(kb[t][c][2 * h], kb[t][c][2 * h + 1], kscale);
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) s[nt][t] = Mma<T>::mfma16(kf, w.q[nt][c][h], s[nt][t]);
+        }
+    }
+    const bool more = i + KW < n;
+    if (more) load_k(tile_next, next.k);
+    const bool whole = w.whole(a, j0, here);
+    if (!whole) w.mask(a, s, j0 + hi * 16, here);
+    V8 pf[NT][2];
+    w.raise(s);
+    w.weigh(s, pf);
     // what no row of the wave sees may hold anything, NaN codes included: a weight of zero does not cancel those
     if (!whole) {
-      const int j = j0 + hi * 16;
-      u32x4 keep;
-#pragma unroll
-      for (int wd = 0; wd < 4; wd++) {
-        uint32_t mask = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int jj = j + 4 * wd + e;
-          mask |= here && jj <= last && (jj >= lo_all || jj < a.n_sink) ? 0xffu << (8 * e) : 0u;
-        }
-        keep[wd] = mask;
-      }
+      const u32x4 keep = seen_bytes(a, j0 + hi * 16, here, w.first, w.last);
 #pragma unroll
       for (int d = 0; d < ND; d++) vb[d] &= keep;
     }
@@ -255,71 +313,228 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_kernel(const CacheArgs
       for (int h = 0; h < 2; h++) {
         const V8 vf = widen8<T>(vb[d][2 * h], vb[d][2 * h + 1], vscale);
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) acc[d][nt] = Mma<T>::mfma16(vf, pf[nt][h], acc[d][nt]);
+        for (int nt = 0; nt < NT; nt++) w.acc[d][nt] = Mma<T>::mfma16(vf, pf[nt][h], w.acc[d][nt]);
       }
     if (more) load_v(tile_next, next.v);
-    now = next;
+    here = keys.there(next.v);
     next = after;
   }
 
+  const CacheArgs& late = arguments_again();
+  float* ml = lds + KW * ROWS * LD;
 #pragma unroll
-  for (int nt = 0; nt < NT; nt++) l[nt] = columns_sum(l[nt]);
+  for (int nt = 0; nt < NT; nt++) {
+    w.l[nt] = columns_sum(w.l[nt]);
+    const int row = wave * ROWS + nt * 16 + col;
+#pragma unroll
+    for (int d = 0; d < ND; d++) *(f32x4*)(lds + row * LD + d * 16 + hi * 4) = w.acc[d][nt];
+    if (hi == 0) *(f32x2*)(ml + row * 2) = f32x2{w.m[nt], w.l[nt]};
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int at = threadIdx.x; at < ROWS * (D / 4); at += kThreads) {
+    const int row = at / (D / 4), d0 = at % (D / 4) * 4;
+    float mx = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < KW; k++) mx = fmaxf(mx, ml[(k * ROWS + row) * 2]);
+    f32x4 o = {0, 0, 0, 0};
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < KW; k++) {
+      const float mk = ml[(k * ROWS + row) * 2];
+      const float f = mk == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((mk - mx) * w.sc);
+      const f32x4 ok = *(const f32x4*)(lds + (k * ROWS + row) * LD + d0);
+      sum += f * ml[(k * ROWS + row) * 2 + 1];
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[e] += f * ok[e];
+    }
+    store_row<T, D>(late, x, hk, x.row_tile * ROWS + row, d0, o, mx * w.sc, sum);
+  }
+}
 
-  // Row r's result: written if the row has one chunk, else left for the join.  d0: first of 4 dimensions.
-  const bool direct = x.n_chunks == 1;
-  if (!direct && x.part + x.n_chunks > a.part_units) return;  // (cu_seqlens that overlap: more units than rows make)
-  const int unit = (x.part + x.chunk_idx) * a.heads_kv + hk;
-  auto store = [&](int r, int d0, f32x4 o, float mx, float sum) {
-    if (r >= n_flat) return;
-    if (direct) {
-      const int tok = quotient(r, a.by_group), head = hk * a.group + r - tok * a.group;
-      const float inv = sum == 0.f ? 0.f : 2.f / sum;  // (V at half its value)
-      T* out = (T*)a.out + (int64_t)x.b * a.o_st[0] + (int64_t)(x.row0 + tok) * a.o_st[1] + (int64_t)head * a.o_st[2];
-      *(typename Mma<T>::V4*)(out + d0) = Mma<T>::pack4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-      if (d0 == 0 && a.lse)
-        a.lse[(int64_t)x.b * a.lse_st[0] + (int64_t)head * a.lse_st[1] + (int64_t)(x.row0 + tok) * a.lse_st[2]] =
-            sum == 0.f ? -__builtin_inff() : (mx * sc - kLift<T> + __log2f(sum)) * (1.f / kLog2e);
-    } else {
-      const int64_t at = (int64_t)unit * ROWS + (r - x.row_tile * ROWS);
-      *(f32x4*)(a.part + at * D + d0) = o;
-      if (d0 == 0) *(f32x2*)(a.part_ml + at * 2) = f32x2{mx * sc, sum};
+// Many rows: each wave has 16 NT of its own, and the block goes over the keys together.  A wave widens a quarter of
+// each tile and leaves it in LDS as operands (lane after lane, so that reads and writes have no bank conflicts).  The
+// loop is skewed so that matrix and vector work of a wave can run side by side: while the weights of tile i are
+// computed the scores of tile i + 1 are multiplied, and while tile i's weights meet its values the next operands are
+// widened: K two tiles ahead, V one; one barrier a tile.
+// 2048 tokens of 32 / 8 heads against 32768 keys: 1135 us, 943 TFLOP/s (each wave widening all of a tile for itself
+// 1253, unskewed 1240).  Bound by the vector pipe: some 250 instructions for 64 products of 16 cycles.
+template <typename T, int D, int NT>
+__global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const CacheArgs a) {
+  using R = Rows<T, D, NT>;
+  using V8 = typename Mma<T>::V8;
+  constexpr int C = R::C, ND = R::ND, NV = ND / 4;
+  constexpr int KF = 4 * C * 2, VF = ND * 2;  // operands of a tile
+  __shared__ V8 k_ops[2][KF][64], v_ops[2][VF][64];
+
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int col = lane & 15, hi = lane >> 4;
+  const int hk = blockIdx.x % a.heads_kv;
+  Unit x;
+  if (!find_unit<0>(a, blockIdx.x / a.heads_kv, x)) return;
+  const int r0 = x.row_tile * (4 * NT * 16);
+  R w(a, x, hk, r0 + wave * (NT * 16), col, hi);
+  // the block's rows
+  const int shift = x.len - x.n_rows, n_flat = x.n_rows * a.group;
+  const int first = shift + quotient(r0, a.by_group);
+  const int last = shift + quotient(min(r0 + 4 * NT * 16, n_flat) - 1, a.by_group);
+  const TileList list = chunk_tiles(a, x, first, last);
+  const Keys<D> keys(a, x, hk, lane);
+  const int n = list.count();
+  auto tile_at = [&](int i) { return list[min(i, n - 1)]; };  // (loads run past the end on the last tile)
+
+  // the wave's quarter: product `wave` of K, dimensions 16 (NV wave) .. of V
+  u32x4 kb[C], vb[NV];
+  int ke = 0, ve = 0;
+  auto load_k = [&](int tile, int id) {
+    ke = keys.key_scale(id);
+    const uint8_t* p = keys.key_row(tile, wave, id);
+#pragma unroll
+    for (int c = 0; c < C; c++) kb[c] = *(const u32x4*)(p + c * 64);
+  };
+  auto load_v = [&](int tile, int id) {
+    ve = keys.value_scale(id);
+    const uint8_t* p = keys.values(tile, id) + wave * (NV * 256);
+#pragma unroll
+    for (int d = 0; d < NV; d++) vb[d] = *(const u32x4*)(p + d * 256);
+  };
+  auto widen_k = [&](V8 (&to)[KF][64]) {
+    const float f = half_scale(ke);
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) to[(wave * C + c) * 2 + h][lane] = widen8<T>(kb[c][2 * h], kb[c][2 * h + 1], f);
+  };
+  // (what no row of the block sees may hold anything, NaN codes included: a weight of zero does not cancel those)
+  auto seen = [&](int tile, int id) {
+    const int j0 = tile * kTileKeys;
+    const bool here = keys.there(id);
+    if (j0 + kTileKeys - 1 <= first && (a.window < 0 || j0 >= last - a.window) &&
+        __builtin_amdgcn_ballot_w64(!here) == 0)
+      return u32x4{~0u, ~0u, ~0u, ~0u};
+    return seen_bytes(a, j0 + hi * 16, here, first, last);
+  };
+  auto widen_v = [&](V8 (&to)[VF][64], u32x4 keep) {
+    const float f = half_scale(ve);
+#pragma unroll
+    for (int d = 0; d < NV; d++) {
+      vb[d] &= keep;
+#pragma unroll
+      for (int h = 0; h < 2; h++) to[(wave * NV + d) * 2 + h][lane] = widen8<T>(vb[d][2 * h], vb[d][2 * h + 1], f);
     }
   };
 
-  if constexpr (KW == 1) {
+  f32x4 s0[NT][4], s1[NT][4];
+  V8 kf[2][2], vf[2][2];
+  // S^T of the tile whose operands are in `op`; they are read four products ahead, the first two before the call
+  auto scores = [&](const V8 (&op)[KF][64], f32x4 (&z)[NT][4]) {
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
+    for (int i = 0; i < 4 * C; i++) {
+      const int t = i / C, c = i % C;
+      if (i + 1 < 4 * C)
 #pragma unroll
-      for (int d = 0; d < ND; d++) store(r0 + nt * 16 + col, d * 16 + hi * 4, acc[d][nt], m[nt], l[nt]);
-  } else {
-    float* ml = lds + KW * ROWS * LD;
+        for (int h = 0; h < 2; h++) kf[(i + 1) & 1][h] = op[(i + 1) * 2 + h][lane];
+      if (c == 0)
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      const int row = (kw * WR + wr) * (NT * 16) + nt * 16 + col;
+        for (int nt = 0; nt < NT; nt++) z[nt][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int d = 0; d < ND; d++) *(f32x4*)(lds + row * LD + d * 16 + hi * 4) = acc[d][nt];
-      if (hi == 0) *(f32x2*)(ml + row * 2) = f32x2{m[nt], l[nt]};
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) z[nt][t] = Mma<T>::mfma16(kf[i & 1][h], w.q[nt][c][h], z[nt][t]);
     }
+  };
+
+  Pages p[4] = {};  // of tiles i .. i + 3
+  if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) p[i] = keys.pages(tile_at(i));
+    load_k(tile_at(0), p[0].k);
+    load_v(tile_at(0), p[0].v);
+    widen_k(k_ops[0]);
+    load_k(tile_at(1), p[1].k);
+    widen_v(v_ops[0], seen(tile_at(0), p[0].v));
+    load_v(tile_at(1), p[1].v);
+    widen_k(k_ops[1]);
+    load_k(tile_at(2), p[2].k);
     __syncthreads();
-#pragma unroll 1
-    for (int at = threadIdx.x; at < ROWS * (D / 4); at += kThreads) {
-      const int row = at / (D / 4), d0 = at % (D / 4) * 4;
-      float mx = -__builtin_inff();
 #pragma unroll
-      for (int w = 0; w < KW; w++) mx = fmaxf(mx, ml[(w * ROWS + row) * 2]);
-      f32x4 o = {0, 0, 0, 0};
-      float sum = 0.f;
+    for (int h = 0; h < 2; h++) kf[0][h] = k_ops[0][h][lane];
+    scores(k_ops[0], s0);
+  }
+  // tile i, whose scores are in s; those of the next go to z
+  auto step = [&](int i, f32x4 (&s)[NT][4], f32x4 (&z)[NT][4]) {
+    const int j0 = list[i] * kTileKeys;
+    const Pages after = keys.pages(tile_at(i + 4));
+    const u32x4 keep = seen(tile_at(i + 1), p[1].v);
+    // K of tile i + 1 and V of tile i are there; K of tile i and V of tile i - 1, in whose places the next go, are read
+    __syncthreads();
+    const auto& k_op = k_ops[(i + 1) & 1];
+    const auto& v_op = v_ops[i & 1];
 #pragma unroll
-      for (int w = 0; w < KW; w++) {
-        const float mw = ml[(w * ROWS + row) * 2];
-        const float f = mw == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((mw - mx) * sc);
-        const f32x4 ow = *(const f32x4*)(lds + (w * ROWS + row) * LD + d0);
-        sum += f * ml[(w * ROWS + row) * 2 + 1];
+    for (int h = 0; h < 2; h++) kf[0][h] = k_op[h][lane];
+    const bool here = keys.there(p[0].v);
+    if (!w.whole(a, j0, here)) w.mask(a, s, j0 + hi * 16, here);
+    w.raise(s);
+
+    __builtin_amdgcn_sched_barrier(0);
+    V8 pf[NT][2];
+    scores(k_op, z);
+    w.weigh(s, pf);
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[e] += f * ow[e];
+    for (int h = 0; h < 2; h++) vf[0][h] = v_op[h][lane];
+    // (a product, then vector work of the time it takes)
+#pragma unroll
+    for (int t = 0; t < 4 * C; t++) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+      for (int e = 0; e < 2 * NT; e++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
       }
-      store(x.row_tile * ROWS + row, d0, o, mx, sum);
     }
+    __builtin_amdgcn_sched_barrier(0);
+
+#pragma unroll
+    for (int d = 0; d < ND; d++) {
+      if (d + 1 < ND)
+#pragma unroll
+        for (int h = 0; h < 2; h++) vf[(d + 1) & 1][h] = v_op[(d + 1) * 2 + h][lane];
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) w.acc[d][nt] = Mma<T>::mfma16(vf[d & 1][h], pf[nt][h], w.acc[d][nt]);
+    }
+    widen_k(k_ops[i & 1]);
+    widen_v(v_ops[(i + 1) & 1], keep);
+    load_k(tile_at(i + 3), p[3].k);
+    load_v(tile_at(i + 2), p[2].v);
+#pragma unroll
+    for (int d = 0; d < ND; d++) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+      for (int e = 0; e < 2 * NT; e++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    p[0] = p[1];
+    p[1] = p[2];
+    p[2] = p[3];
+    p[3] = after;
+  };
+  for (int i = 0; i < n; i += 2) {
+    step(i, s0, s1);
+    if (i + 1 < n) step(i + 1, s1, s0);
+  }
+  const CacheArgs& late = arguments_again();
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    w.l[nt] = columns_sum(w.l[nt]);
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+      store_row<T, D>(late, x, hk, r0 + wave * (NT * 16) + nt * 16 + col, d * 16 + hi * 4, w.acc[d][nt], w.m[nt] * w.sc,
+                      w.l[nt]);
   }
 }
 
@@ -338,7 +553,7 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheArgs a)
   if (x.n_chunks == 1 || x.part + x.n_chunks > a.part_units) return;
   const int lane = threadIdx.x % LANES, r = threadIdx.x / LANES % ROWS, part = threadIdx.x / LANES / ROWS;
   const int d0 = lane * 4;
-  const int row = x.row + r - x.row_tile * a.row_tile;
+  const int row = x.row + r - (x.row_tile << a.row_log2);
   const bool mine = x.row + r < x.n_rows * a.group;
   float mx = -__builtin_inff(), sum = 0.f;
   f32x4 o = {0, 0, 0, 0};
@@ -357,7 +572,7 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheArgs a)
     f32x4 v[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const int64_t at = ((int64_t)(x.part + min(c + i * P, x.n_chunks - 1)) * a.heads_kv + hk) * a.row_tile + row;
+      const int64_t at = (((int64_t)(x.part + min(c + i * P, x.n_chunks - 1)) * a.heads_kv + hk) << a.row_log2) + row;
       ml[i] = *(const f32x2*)(a.part_ml + at * 2);
       v[i] = *(const f32x4*)(a.part + at * D + d0);
     }
@@ -398,9 +613,14 @@ Cut cut_call(const rswa_cache_params* p) {
   c.nt = rows <= 16 ? 1 : 2;
   c.wr = rows <= 64 ? 1 : 4;
   c.row_tile = c.nt * 16 * c.wr;
-  c.wanted = kComputeUnits * (c.nt == 1 ? 3 : 2) * 2;
   c.row_tiles = p->cu_seqlens_q ? p->total_q * group / c.row_tile + p->batch
                                 : p->batch * ceil_div(p->seqlen_q * group, c.row_tile);
+  // Units wanted.  Few rows: what the chip holds at once (two blocks a compute unit), or half as many again where a
+  // tile is 16 KB for little other work (64 ragged sequences, head_dim 128: 512 units 215 us, 768 206, 1536 208; 128 of
+  // head_dim 64: 50, 54, 51; 16 x 5 drafts: 33, 33, 38, most of it the join).  Many rows: whole rounds of what it holds.
+  const int resident = 2 * kComputeUnits;
+  c.wanted = c.wr > 1 ? (int)std::min<int64_t>(4, ceil_div(c.row_tiles * p->heads_kv, resident)) * resident
+             : c.nt == 1 && p->head_dim == 128 ? resident * 3 / 2 : resident;
   const int64_t per_head = ceil_div(c.wanted, p->heads_kv) + 1;
   const int64_t most_tiles = ceil_div((int64_t)p->max_pages * p->page_size, kTileKeys);
   const int64_t at_most = std::min(2 * per_head, c.row_tiles * most_tiles);
@@ -419,11 +639,11 @@ int launch_attn(CacheArgs& a, const Cut& c, hipStream_t stream) {
   const dim3 grid((unsigned)c.grid), block(kThreads);
   clear_launch_error();
   if (c.nt == 1)
-    hipLaunchKernelGGL((cache_attn_kernel<T, D, 1, 1>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((cache_attn_kernel<T, D, 1>), grid, block, 0, stream, a);
   else if (c.wr == 1)
-    hipLaunchKernelGGL((cache_attn_kernel<T, D, 2, 1>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((cache_attn_kernel<T, D, 2>), grid, block, 0, stream, a);
   else
-    hipLaunchKernelGGL((cache_attn_kernel<T, D, 2, 4>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((cache_attn_rows_kernel<T, D, 2>), grid, block, 0, stream, a);
   if (int rc = check_launch("cache_attn")) return rc;
   if (c.part_units == 0) return RSWA_OK;
   // as many chunks a row (on average) as threads that may share one, or one thread for all
@@ -471,7 +691,7 @@ extern "C" int rswa_cache_attn(const rswa_cache_params* p, void* stream) {
     a.lse_st[i] = p->lse_stride[i];
   }
   if (a.cu) a.o_st[0] = a.lse_st[0] = 0;
-  a.row_tile = c.row_tile;
+  a.row_log2 = __builtin_ctz((unsigned)c.row_tile);
   a.min_chunk = kMinChunk;
   a.per_unit = (float)p->heads_kv / (float)c.wanted;
   a.part_units = (int)c.part_units;

@@ -18,8 +18,10 @@ struct CacheArgs {
   const uint8_t* v;
   const uint8_t* k_scale;
   const uint8_t* v_scale;
-  int64_t k_st[2], v_st[2];    // page, head (bytes)
-  int64_t ks_st[2], vs_st[2];  // page, head
+  // page, head (bytes); below 2^32, so that a page's place is one 32 x 32 -> 64 bit product, where one with a 64-bit
+  // stride is three multiplications of 16 cycles
+  uint32_t k_st[2], v_st[2];
+  uint32_t ks_st[2], vs_st[2];
   const int32_t* table;
   int64_t table_st;
   const int32_t* lens;
@@ -37,7 +39,7 @@ struct CacheArgs {
   int64_t q_st[3], o_st[3], lse_st[3];
   float scale_log2;  // softmax_scale * log2(e)
   // how the work is cut (see Plan)
-  int32_t row_tile;   // rows (token x grouped head) of a unit
+  int32_t row_log2;   // a unit's row tile has 2^row_log2 rows (token x grouped head)
   int32_t min_chunk;  // least tiles of a unit
   float per_unit;     // heads_kv / units wanted
   // partial results of units whose rows have several (workspace)
@@ -84,15 +86,20 @@ __device__ __forceinline__ float last_lane(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-// Lanes l, l^16, l^32, l^48 with each other (the four that have a column of a 16 x 16 product).
+// Lanes l, l^16, l^32, l^48 with each other (the four that have a column of a 16 x 16 product).  A NaN stays one: the
+// maximum that passes over NaN would first quiet its arguments, an instruction for each.
 __device__ __forceinline__ float columns_max(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return halfwave_max(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  const float m = __builtin_elementwise_maximum(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float columns_sum(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return halfwave_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
 }
+
+__device__ __forceinline__ uint64_t times(int n, uint32_t stride) { return (uint64_t)(uint32_t)n * stride; }
 
 // Tokens that a sequence's row of the page table can hold at most bound its length: no lookup passes its end.
 __device__ __forceinline__ int held_tokens(const CacheArgs& a, int b) {
@@ -131,9 +138,9 @@ __device__ __forceinline__ SeenTiles seen_tiles(const CacheArgs& a, int first, i
 // The host knows no length.  Every wave reads all of them (64 at a time), sums the tiles of the whole call, and cuts
 // the tiles of every row tile into chunks of as many as give the launch about the units it was sized for: sequences
 // of any lengths make units of nearly one size, which the hardware then deals.  The grid is sized for the bound
-//   sum over sequences of row_tiles * ceil(tiles / chunk) <= units wanted / heads_kv + sum of row_tiles
+//   sum over sequences of row_tiles * chunks <= units wanted / heads_kv + sum of row_tiles
 // and what is beyond the last unit ends at once.  Rows of sequences with several chunks are joined from partial
-// results; those sequences have at most twice the units wanted (ceil(x) <= 2 x for x > 1), which bounds the workspace.
+// results; those sequences have at most twice the units wanted (chunks <= 2 tiles / chunk), which bounds the workspace.
 // (The sum of tiles is taken in floating point, within 2^-16 of its value: less than the one unit that the host adds.)
 struct Unit {
   int b, row, row_tile, chunk_idx, n_chunks;
@@ -155,7 +162,7 @@ __device__ __forceinline__ bool find_unit(const CacheArgs& a, int u, Unit& x) {
     if (b < a.batch) {
       rows_of(a, b, row0, n);
       len = held_tokens(a, b);
-      row_tiles = (int)(((int64_t)n * a.group + a.row_tile - 1) / a.row_tile);
+      row_tiles = (n * a.group + (1 << a.row_log2) - 1) >> a.row_log2;  // (below 2^30 rows)
       if (n > 0) t = seen_tiles(a, len - n, len - 1);
     }
   };
@@ -170,7 +177,8 @@ __device__ __forceinline__ bool find_unit(const CacheArgs& a, int u, Unit& x) {
   int before = 0, before_part = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     if (a.batch > 64) load(b0 + lane);
-    const int chunks = max(1, (t.count() + x.chunk - 1) / x.chunk);
+    // (up to a quarter more in one chunk rather than a small one behind it)
+    const int chunks = max(1, (t.count() + x.chunk - 1 - x.chunk / 4) / x.chunk);
     const int units = JOIN ? (n * a.group + JOIN - 1) / JOIN : row_tiles * chunks;
     const int parts = chunks > 1 ? row_tiles * chunks : 0;
     const int su = wave_scan(units), sp = wave_scan(parts);
@@ -182,8 +190,9 @@ __device__ __forceinline__ bool find_unit(const CacheArgs& a, int u, Unit& x) {
       x.n_chunks = of(chunks);
       const int in_seq = u - before - (of(su) - of(units));
       x.row = in_seq * JOIN;
-      x.row_tile = JOIN ? x.row / a.row_tile : in_seq / x.n_chunks;
+      x.row_tile = JOIN ? x.row >> a.row_log2 : in_seq / x.n_chunks;
       x.chunk_idx = JOIN ? 0 : in_seq - x.row_tile * x.n_chunks;
+      x.chunk = (of(t.count()) + x.n_chunks - 1) / x.n_chunks;
       x.part = before_part + of(sp) - of(parts) + x.row_tile * x.n_chunks;
       x.row0 = of(row0);
       x.n_rows = of(n);

@@ -27,6 +27,9 @@ int cache_args(const rswa_cache_params* p, const char* who, CacheArgs& a) {
   RSWA_REQUIRE(p->num_pages == 0 || (p->k && p->v && p->k_scale && p->v_scale), RSWA_ERR_INVALID, "%s: null cache", who);
   RSWA_REQUIRE((uintptr_t)p->k % 16 == 0 && (uintptr_t)p->v % 16 == 0, RSWA_ERR_UNSUPPORTED,
                "%s: k and v must be 16-byte aligned", who);
+  for (const int64_t* st : {p->k_stride, p->v_stride, p->k_scale_stride, p->v_scale_stride})
+    RSWA_REQUIRE(st[0] >= 0 && st[0] < (1ll << 32) && st[1] >= 0 && st[1] < (1ll << 32), RSWA_ERR_UNSUPPORTED,
+                 "%s: strides of the cache must be below 4 GiB", who);
   for (int i = 0; i < 2; i++)
     RSWA_REQUIRE(p->k_stride[i] % 16 == 0 && p->v_stride[i] % 16 == 0, RSWA_ERR_UNSUPPORTED,
                  "%s: strides of k and v must be multiples of 16 bytes", who);
@@ -37,10 +40,10 @@ int cache_args(const rswa_cache_params* p, const char* who, CacheArgs& a) {
   a.k_scale = (const uint8_t*)p->k_scale;
   a.v_scale = (const uint8_t*)p->v_scale;
   for (int i = 0; i < 2; i++) {
-    a.k_st[i] = p->k_stride[i];
-    a.v_st[i] = p->v_stride[i];
-    a.ks_st[i] = p->k_scale_stride[i];
-    a.vs_st[i] = p->v_scale_stride[i];
+    a.k_st[i] = (uint32_t)p->k_stride[i];
+    a.v_st[i] = (uint32_t)p->v_stride[i];
+    a.ks_st[i] = (uint32_t)p->k_scale_stride[i];
+    a.vs_st[i] = (uint32_t)p->v_scale_stride[i];
   }
   a.table = p->page_table;
   a.table_st = p->page_table_stride;

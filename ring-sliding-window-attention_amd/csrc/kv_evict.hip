@@ -253,15 +253,15 @@ __global__ __launch_bounds__(512, 4) void cache_move_kernel(const EvictArgs a) {
           one && j < c.w_len ? c.weights[(int64_t)b * c.w_st[0] + (int64_t)hk * c.w_st[1] + j] : 0.f;
     if ((uint32_t)sp >= (uint32_t)c.num_pages) sp = -1;
     if (sp >= 0)
-      e = values ? c.v_scale[(int64_t)sp * c.vs_st[0] + (int64_t)hk * c.vs_st[1]]
-                 : c.k_scale[(int64_t)sp * c.ks_st[0] + (int64_t)hk * c.ks_st[1]];
+      e = values ? c.v_scale[times(sp, c.vs_st[0]) + times(hk, c.vs_st[1])]
+                 : c.k_scale[times(sp, c.ks_st[0]) + times(hk, c.ks_st[1])];
   }
   if ((uint32_t)id >= (uint32_t)c.num_pages) return;
   const int slot = j & (page_size - 1);
   uint64_t starts = 0;  // values: tokens that are the first of their old group
   if (!values) {
     if (lane < n) {
-      base[wave][lane] = sp < 0 ? -1 : (int64_t)sp * c.k_st[0] + slot * D;
+      base[wave][lane] = sp < 0 ? -1 : (int64_t)times(sp, c.k_st[0]) + slot * D;
       info[wave][lane] = (uint32_t)e;
     }
   } else {
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(512, 4) void cache_move_kernel(const EvictArgs a) {
     const bool start = lane < n && (lane == 0 || (j >> 4) != (before >> 4));
     starts = __builtin_amdgcn_ballot_w64(start);
     const int group = __popcll(starts & (~0ull >> (63 - lane))) - 1;
-    if (start) base[wave][group] = sp < 0 ? -1 : (int64_t)sp * c.v_st[0] + (slot >> 4) * (16 * D);
+    if (start) base[wave][group] = sp < 0 ? -1 : (int64_t)times(sp, c.v_st[0]) + (slot >> 4) * (16 * D);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");  // (the zeros above)
     if (lane < n) atomicOr(&info[wave][group], (1u << (j & 15)) | ((uint32_t)e << 16));
   }
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(512, 4) void cache_move_kernel(const EvictArgs a) {
   float most = 0.f;
   u32x4 rows[STEPS];
   uint32_t* const words = packed + (values ? wave - half : 0) * (D * ROW);
-  const uint8_t* const head = values ? c.v + (int64_t)hk * c.v_st[1] : c.k + (int64_t)hk * c.k_st[1];
+  const uint8_t* const head = values ? c.v + times(hk, c.v_st[1]) : c.k + times(hk, c.k_st[1]);
   if (!values) {
     const int piece = lane % PIECES * 16;
 #pragma unroll
@@ -359,8 +359,8 @@ __global__ __launch_bounds__(512, 4) void cache_move_kernel(const EvictArgs a) {
   const int e_new = scale_byte(__uint_as_float(amax[values]));
   if (!values) {
     if (threadIdx.x == 0)
-      const_cast<uint8_t*>(c.k_scale)[(int64_t)id * c.ks_st[0] + (int64_t)hk * c.ks_st[1]] = (uint8_t)e_new;
-    uint8_t* const to = const_cast<uint8_t*>(head) + (int64_t)id * c.k_st[0] + (int64_t)sub * D + lane % PIECES * 16;
+      const_cast<uint8_t*>(c.k_scale)[times(id, c.ks_st[0]) + times(hk, c.ks_st[1])] = (uint8_t)e_new;
+    uint8_t* const to = const_cast<uint8_t*>(head) + times(id, c.k_st[0]) + (int64_t)sub * D + lane % PIECES * 16;
 #pragma unroll
     for (int i = 0; i < STEPS; i++) {
       const int r = i * PER + lane / PIECES;
@@ -376,8 +376,8 @@ __global__ __launch_bounds__(512, 4) void cache_move_kernel(const EvictArgs a) {
     return;
   }
   if (wave == half && lane == 0)
-    const_cast<uint8_t*>(c.v_scale)[(int64_t)id * c.vs_st[0] + (int64_t)hk * c.vs_st[1]] = (uint8_t)e_new;
-  uint8_t* const to = const_cast<uint8_t*>(head) + (int64_t)id * c.v_st[0] + (int64_t)(sub / 16) * (16 * D);
+    const_cast<uint8_t*>(c.v_scale)[times(id, c.vs_st[0]) + times(hk, c.vs_st[1])] = (uint8_t)e_new;
+  uint8_t* const to = const_cast<uint8_t*>(head) + times(id, c.v_st[0]) + (int64_t)(sub / 16) * (16 * D);
   const float f = __builtin_ldexpf(1.f, e - e_new);  // lane l: token l's
   const bool change = __builtin_amdgcn_ballot_w64(lane < n && e != e_new) != 0;
   for (int g = 0; g * 16 < n; g++) {

@@ -30,8 +30,8 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
   const int32_t* table = a.table + (int64_t)x.b * a.table_st;
   const int n_groups = (x.len + kGroupKeys - 1) / kGroupKeys;
   const int per_page = a.page_log2 - 4, in_page = (1 << per_page) - 1;
-  const uint8_t* const k_head = a.k + (int64_t)hk * a.k_st[1];
-  const uint8_t* const ks_head = a.k_scale + (int64_t)hk * a.ks_st[1];
+  const uint8_t* const k_head = a.k + times(hk, a.k_st[1]);
+  const uint8_t* const ks_head = a.k_scale + times(hk, a.ks_st[1]);
   float* const w = a.weights + (int64_t)x.b * a.w_st[0] + (int64_t)hk * a.w_st[1];
   const T* const q_seq = (const T*)a.q + (int64_t)x.b * a.q_st[0] + (int64_t)x.row0 * a.q_st[1] + hi * 16;
   const float* const lse_seq = a.lse + (int64_t)x.b * a.lse_st[0] + (int64_t)x.row0 * a.lse_st[2];
@@ -49,8 +49,8 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
   auto load_keys = [&](int tile, int id) {
     const int page = (uint32_t)id < (uint32_t)a.num_pages ? id : 0;
     const int g = min(tile * 4 + (col >> 2), n_groups - 1) & in_page;
-    const uint8_t* p = k_head + (int64_t)page * a.k_st[0] + (g * kGroupKeys + (col & 3)) * D + hi * 16;
-    ke = ks_head[(int64_t)page * a.ks_st[0]];
+    const uint8_t* p = k_head + times(page, a.k_st[0]) + (g * kGroupKeys + (col & 3)) * D + hi * 16;
+    ke = ks_head[times(page, a.ks_st[0])];
 #pragma unroll
     for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -182,7 +182,7 @@ extern "C" int rswa_cache_weights(const rswa_cache_params* p, void* stream) {
   a.w_st[0] = p->weights_stride[0];
   a.w_st[1] = p->weights_stride[1];
   a.w_len = p->weights_len;
-  a.row_tile = INT32_MAX;  // a unit has all rows of its sequence
+  a.row_log2 = 30;  // a unit has all rows of its sequence
   const int64_t per_seq = ceil_div(rows, p->batch) * a.group;
   const int64_t wanted = kComputeUnits * (per_seq <= 16 ? 6 : 2);
   a.min_chunk = per_seq > 64 ? 1 : 4;
