@@ -14,6 +14,8 @@ struct AppendArgs {
   const void* x[2];  // new keys, values
   int64_t x_st[2][3];
   int32_t pages;     // dense: pages that a sequence's new tokens touch at most
+  int32_t work;      // blocks with work
+  FastDiv by_pages, by_heads;
 };
 
 template <typename T, int D>
@@ -23,8 +25,12 @@ __global__ void cache_append_kernel(const AppendArgs a) {
   __shared__ uint32_t amax[2];
   const CacheArgs& c = a.c;
   const int page_size = 1 << c.page_log2;
-  const int hk = blockIdx.x % c.heads_kv;
-  int u = blockIdx.x / c.heads_kv, b, row0, n;
+  // Hardware deals block ids to the 8 XCDs in turn; each takes an eighth of the work in a row here, so that the heads of
+  // a page, whose rows of the input lie side by side, are read by one.
+  const int id0 = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+  if (id0 >= a.work) return;
+  int u = quotient(id0, a.by_heads), b, row0, n;
+  const int hk = id0 - u * c.heads_kv;
   // sequence, and which of its touched pages
   if (c.cu) {
     // sequence b owns the slots from cu[b] / page_size + 2 b on: n tokens touch at most n / page_size + 2 pages.
@@ -44,7 +50,7 @@ __global__ void cache_append_kernel(const AppendArgs a) {
     rows_of(c, b, row0, n);
     u -= (row0 >> c.page_log2) + 2 * b;
   } else {
-    b = u / a.pages;
+    b = quotient(u, a.by_pages);
     u -= b * a.pages;
     row0 = 0;
     n = c.seqlen_q;
@@ -58,7 +64,6 @@ __global__ void cache_append_kernel(const AppendArgs a) {
   const int count = min(page_size - from, n - i0);
   if (count <= 0) return;
   const int id = c.table[(int64_t)b * c.table_st + in_seq];
-  if ((uint32_t)id >= (uint32_t)c.num_pages) return;
 
   const int half = blockDim.x / 2;
   const int which = threadIdx.x >= half;
@@ -67,15 +72,25 @@ __global__ void cache_append_kernel(const AppendArgs a) {
   const bool mine = g < (page_size >> 4);       // (blocks of small pages have threads left over)
   const int lo = max(0, from - g * 16), hi = min(16, from + count - g * 16);  // its places written: lo <= e < hi
 
-  const T* x = (const T*)a.x[which] + (int64_t)b * a.x_st[which][0] + (int64_t)hk * a.x_st[which][2] + d0;
+  // (read ahead of the page's number, on which nothing of it depends)
+  const T* x = (const T*)a.x[which] + (int64_t)b * a.x_st[which][0] + (int64_t)hk * a.x_st[which][2] + d0 +
+               (int64_t)(row0 + i0 + g * 16 - from) * a.x_st[which][1];  // (of place 0, which may be none of them)
   V8 v[16];
-  if (threadIdx.x < 2) amax[threadIdx.x] = 0;
+  if (mine && lo == 0 && hi == 16) {
 #pragma unroll
-  for (int e = 0; e < 16; e++)
-    if (mine && e >= lo && e < hi)
-      v[e] = *(const V8*)(x + (int64_t)(row0 + i0 + g * 16 + e - from) * a.x_st[which][1]);
-    else
+    for (int e = 0; e < 16; e++) v[e] = __builtin_nontemporal_load((const V8*)(x + e * a.x_st[which][1]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
       v[e] = V8{};
+      if (mine && e >= lo && e < hi) v[e] = *(const V8*)(x + e * a.x_st[which][1]);
+    }
+  }
+  if ((uint32_t)id >= (uint32_t)c.num_pages) return;
+  uint8_t* const scale = which ? const_cast<uint8_t*>(c.v_scale) + times(id, c.vs_st[0]) + times(hk, c.vs_st[1])
+                               : const_cast<uint8_t*>(c.k_scale) + times(id, c.ks_st[0]) + times(hk, c.ks_st[1]);
+  const int was = from > 0 ? *scale : 0;
+  if (threadIdx.x < 2) amax[threadIdx.x] = 0;
   float most = 0.f;
 #pragma unroll
   for (int e = 0; e < 16; e++)
@@ -90,9 +105,6 @@ __global__ void cache_append_kernel(const AppendArgs a) {
   // (a positive float's bits grow with it)
   if (lane_id() == 0) atomicMax(&amax[which], __builtin_bit_cast(uint32_t, most));
   __syncthreads();
-  uint8_t* const scale = which ? const_cast<uint8_t*>(c.v_scale) + times(id, c.vs_st[0]) + times(hk, c.vs_st[1])
-                               : const_cast<uint8_t*>(c.k_scale) + times(id, c.ks_st[0]) + times(hk, c.ks_st[1]);
-  const int was = from > 0 ? *scale : 0;
   const int e_new = max(was, scale_byte(__builtin_bit_cast(float, amax[which])));
   const float inv = inverse(e_new);
   const bool grown = from > 0 && e_new > was;
@@ -124,13 +136,31 @@ __global__ void cache_append_kernel(const AppendArgs a) {
   } else {
     uint8_t* vp = const_cast<uint8_t*>(c.v) + times(id, c.v_st[0]) + times(hk, c.v_st[1]) + (g * D + d0) * 16;
     const bool full = lo == 0 && hi == 16;
-    if (full || (grown && old > 0)) {
+    if (full) {
+      // 4 tokens x 4 dimensions are transposed by byte permutations
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        u32x4 w = full ? u32x4{0, 0, 0, 0} : *(const u32x4*)(vp + i * 16);
+      for (int h = 0; h < 2; h++) {
+        u32x4 w[4];
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-          const uint32_t again = !full && grown ? rescale4(w[q], shrink) : 0u;
+          const uint32_t c0 = code[4 * q][h], c1 = code[4 * q + 1][h], c2 = code[4 * q + 2][h], c3 = code[4 * q + 3][h];
+          const uint32_t lo01 = __builtin_amdgcn_perm(c1, c0, 0x05010400u), hi01 = __builtin_amdgcn_perm(c1, c0, 0x07030602u);
+          const uint32_t lo23 = __builtin_amdgcn_perm(c3, c2, 0x05010400u), hi23 = __builtin_amdgcn_perm(c3, c2, 0x07030602u);
+          w[0][q] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
+          w[1][q] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
+          w[2][q] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
+          w[3][q] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) *(u32x4*)(vp + (4 * h + i) * 16) = w[i];
+      }
+    } else if (grown && old > 0) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        u32x4 w = *(const u32x4*)(vp + i * 16);
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const uint32_t again = rescale4(w[q], shrink);
           uint32_t r = 0;
 #pragma unroll
           for (int e = 0; e < 4; e++) {
@@ -150,6 +180,58 @@ __global__ void cache_append_kernel(const AppendArgs a) {
 #pragma unroll
           for (int i = 0; i < 8; i++) vp[i * 16 + e] = (uint8_t)(code[e][i / 4] >> (8 * (i % 4)));
     }
+  }
+}
+
+// One token per sequence (dense): a wave has the key or the value of one head.  The same as above in a tenth of the
+// code: such a launch waits for little but memory, and that includes its instructions.
+template <typename T, int D>
+__global__ __launch_bounds__(64) void cache_append_token_kernel(const AppendArgs a) {
+  constexpr int E = D / 64;  // elements of a lane
+  typedef __attribute__((__vector_size__(E * sizeof(T)))) T VE;
+  const CacheArgs& c = a.c;
+  const int which = blockIdx.x & 1, u = blockIdx.x >> 1, lane = threadIdx.x;
+  const int b = quotient(u, a.by_heads), hk = u - b * c.heads_kv;
+  const int start = max(0, c.lens[b]);
+  const VE x = *(const VE*)((const T*)a.x[which] + (int64_t)b * a.x_st[which][0] + (int64_t)hk * a.x_st[which][2] +
+                            lane * E);
+  const int page_size = 1 << c.page_log2, in_seq = start >> c.page_log2, from = start & (page_size - 1);
+  if (in_seq >= c.max_pages) return;
+  const int id = c.table[(int64_t)b * c.table_st + in_seq];
+  if ((uint32_t)id >= (uint32_t)c.num_pages) return;
+  uint8_t* const scale = which ? const_cast<uint8_t*>(c.v_scale) + times(id, c.vs_st[0]) + times(hk, c.vs_st[1])
+                               : const_cast<uint8_t*>(c.k_scale) + times(id, c.ks_st[0]) + times(hk, c.ks_st[1]);
+  uint8_t* const page = which ? const_cast<uint8_t*>(c.v) + times(id, c.v_st[0]) + times(hk, c.v_st[1])
+                              : const_cast<uint8_t*>(c.k) + times(id, c.k_st[0]) + times(hk, c.k_st[1]);
+  const int was = from > 0 ? *scale : 0;
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < E; i++) {
+    const float y = __builtin_fabsf((float)x[i]);
+    most = y < __builtin_inff() ? fmaxf(most, y) : most;
+  }
+  const int e_new = max(was, scale_byte(wave_max(most)));
+  const float inv = inverse(e_new);
+  const uint32_t code = codes4((float)x[0] * inv, (float)x[E - 1] * inv, 0.f, 0.f);
+  if (from > 0 && e_new > was) {  // the tokens from before at the new scale
+    const float f = e_new - was < 127 ? __builtin_bit_cast(float, (uint32_t)(127 - (e_new - was)) << 23) : 0.f;
+    const int words = which ? (from + 15) / 16 * 4 * D : from * D / 4;
+#pragma unroll 1
+    for (int i = lane; i < words; i += 64) {
+      const int left = which ? from - (i / (4 * D) * 16 + (i & 3) * 4) : 4;  // tokens from before in this word
+      uint32_t* const w = (uint32_t*)page + i;
+      const uint32_t again = left > 0 ? rescale4(*w, f) : 0u;
+      if (left >= 4) *w = again;
+#pragma unroll
+      for (int k = 0; k < 3; k++)
+        if (left < 4 && k < left) ((uint8_t*)w)[k] = (uint8_t)(again >> (8 * k));
+    }
+  }
+  if (lane == 0) *scale = (uint8_t)e_new;
+#pragma unroll
+  for (int i = 0; i < E; i++) {
+    const int d = lane * E + i;
+    page[which ? from / 16 * (16 * D) + d * 16 + from % 16 : from * D + d] = (uint8_t)(code >> (8 * i));
   }
 }
 
@@ -178,11 +260,20 @@ extern "C" int rswa_cache_append(const rswa_cache_params* p, void* stream) {
   const int64_t slots =
       p->cu_seqlens_q ? p->total_q / p->page_size + 2 * (int64_t)p->batch : (int64_t)p->batch * a.pages;
   const int64_t blocks = slots * p->heads_kv;
-  RSWA_REQUIRE(blocks < (1ll << 31), RSWA_ERR_UNSUPPORTED, "cache_append: %lld blocks", (long long)blocks);
+  RSWA_REQUIRE(blocks < (1ll << 30), RSWA_ERR_UNSUPPORTED, "cache_append: %lld blocks", (long long)blocks);
+  a.work = (int32_t)blocks;
+  a.by_pages = fast_div((uint32_t)a.pages);
+  a.by_heads = fast_div((uint32_t)p->heads_kv);
   const int threads = 2 * std::max(64, p->page_size / 16 * (p->head_dim / 8));
   clear_launch_error();
+  const bool tokens = !p->cu_seqlens_q && p->seqlen_q == 1;
   auto go = [&](auto t, auto d) {
-    hipLaunchKernelGGL((cache_append_kernel<decltype(t), decltype(d)::value>), dim3((unsigned)blocks), dim3(threads), 0,
+    if (tokens) {
+      hipLaunchKernelGGL((cache_append_token_kernel<decltype(t), decltype(d)::value>), dim3((unsigned)(2 * blocks)),
+                         dim3(64), 0, (hipStream_t)stream, a);
+      return;
+    }
+    hipLaunchKernelGGL((cache_append_kernel<decltype(t), decltype(d)::value>), dim3((unsigned)(ceil_div(blocks, 8) * 8)), dim3(threads), 0,
                        (hipStream_t)stream, a);
   };
   using D64 = std::integral_constant<int, 64>;

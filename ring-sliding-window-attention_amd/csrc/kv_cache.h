@@ -82,6 +82,17 @@ __device__ __forceinline__ float wave_scan(float v) {
   v += from(dpp_or_zero<0x143, 0xc>(bits(v)));
   return v;
 }
+// The largest of all lanes' values, none below 0.
+__device__ __forceinline__ float wave_max(float v) {
+  int x = __float_as_int(v);  // (a positive float's bits grow with it)
+  x = max(x, dpp_or_zero<0x111, 0xf>(x));
+  x = max(x, dpp_or_zero<0x112, 0xf>(x));
+  x = max(x, dpp_or_zero<0x114, 0xf>(x));
+  x = max(x, dpp_or_zero<0x118, 0xf>(x));
+  x = max(x, dpp_or_zero<0x142, 0xa>(x));
+  x = max(x, dpp_or_zero<0x143, 0xc>(x));
+  return __int_as_float(__builtin_amdgcn_readlane(x, 63));
+}
 __device__ __forceinline__ float last_lane(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
