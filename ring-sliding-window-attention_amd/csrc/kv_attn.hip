@@ -207,26 +207,39 @@ __device__ __forceinline__ const CacheArgs& arguments_again() {
   return *(const CacheArgs*)p;
 }
 
-// Row r's result: written if the row has one chunk, else left for the join.  d0: first of 4 dimensions; mx in base 2.
+// Where row r's result goes: to the output, or to the join if the row has several chunks.
 template <typename T, int D>
-__device__ __forceinline__ void store_row(const CacheArgs& a, const Unit& x, int hk, int r, int d0, f32x4 o, float mx,
-                                          float sum) {
-  if (r >= x.n_rows * a.group) return;
-  if (x.n_chunks == 1) {
-    const int tok = quotient(r, a.by_group), head = hk * a.group + r - tok * a.group;
-    const float inv = sum == 0.f ? 0.f : 2.f / sum;  // (V at half its value)
-    T* out = (T*)a.out + (int64_t)x.b * a.o_st[0] + (int64_t)(x.row0 + tok) * a.o_st[1] + (int64_t)head * a.o_st[2];
-    *(typename Mma<T>::V4*)(out + d0) = Mma<T>::pack4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-    if (d0 == 0 && a.lse)
-      a.lse[(int64_t)x.b * a.lse_st[0] + (int64_t)head * a.lse_st[1] + (int64_t)(x.row0 + tok) * a.lse_st[2]] =
-          sum == 0.f ? -__builtin_inff() : (mx - kLift<T> + __log2f(sum)) * (1.f / kLog2e);
-  } else {
-    if (x.part + x.n_chunks > a.part_units) return;  // (cu_seqlens that overlap: more units than rows make)
-    const int64_t at = (((int64_t)(x.part + x.chunk_idx) * a.heads_kv + hk) << a.row_log2) + (r - (x.row_tile << a.row_log2));
-    *(f32x4*)(a.part + at * D + d0) = o;
-    if (d0 == 0) *(f32x2*)(a.part_ml + at * 2) = f32x2{mx, sum};
+struct RowOut {
+  T* out = nullptr;
+  float* lse = nullptr;
+  float* part = nullptr;
+  float* part_ml = nullptr;
+  __device__ __forceinline__ RowOut(const CacheArgs& a, const Unit& x, int hk, int r, bool direct) {
+    if (r >= x.n_rows * a.group) return;
+    if (direct) {
+      const int tok = quotient(r, a.by_group), head = hk * a.group + r - tok * a.group;
+      out = (T*)a.out + (int64_t)x.b * a.o_st[0] + (int64_t)(x.row0 + tok) * a.o_st[1] + (int64_t)head * a.o_st[2];
+      if (a.lse)
+        lse = a.lse + (int64_t)x.b * a.lse_st[0] + (int64_t)head * a.lse_st[1] + (int64_t)(x.row0 + tok) * a.lse_st[2];
+    } else if (x.part + x.n_chunks <= a.part_units) {  // (more: cu_seqlens that overlap; more units than rows make)
+      const int64_t at =
+          (((int64_t)(x.part + x.chunk_idx) * a.heads_kv + hk) << a.row_log2) + (r - (x.row_tile << a.row_log2));
+      part = a.part + at * D;
+      part_ml = a.part_ml + at * 2;
+    }
   }
-}
+  // four dimensions from d0 on
+  __device__ __forceinline__ void put(int d0, f32x4 o, float inv) const {
+    if (out) *(typename Mma<T>::V4*)(out + d0) = Mma<T>::pack4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (part) *(f32x4*)(part + d0) = o;
+  }
+  // the row's maximum in base 2, and the sum of its weights
+  __device__ __forceinline__ void finish(float mx, float sum) const {
+    if (lse) *lse = sum == 0.f ? -__builtin_inff() : (mx - kLift<T> + __log2f(sum)) * (1.f / kLog2e);
+    if (part) *(f32x2*)part_ml = f32x2{mx, sum};
+  }
+  static __device__ __forceinline__ float inverse_of(float sum) { return sum == 0.f ? 0.f : 2.f / sum; }  // (V halved)
+};
 
 // Few rows: the four waves of a block have the same rows, each its own keys, and everything from memory to the output
 // stays in registers; the waves meet in LDS at the end.
@@ -348,7 +361,9 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_kernel(const CacheArgs
 #pragma unroll
       for (int e = 0; e < 4; e++) o[e] += f * ok[e];
     }
-    store_row<T, D>(late, x, hk, x.row_tile * ROWS + row, d0, o, mx * w.sc, sum);
+    const RowOut<T, D> to(late, x, hk, x.row_tile * ROWS + row, x.n_chunks == 1);
+    to.put(d0, o, to.inverse_of(sum));
+    if (d0 == 0) to.finish(mx * w.sc, sum);
   }
 }
 
@@ -531,71 +546,74 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
     w.l[nt] = columns_sum(w.l[nt]);
+    const RowOut<T, D> to(late, x, hk, r0 + wave * (NT * 16) + nt * 16 + col, x.n_chunks == 1);
+    const float inv = to.inverse_of(w.l[nt]);
 #pragma unroll
-    for (int d = 0; d < ND; d++)
-      store_row<T, D>(late, x, hk, r0 + wave * (NT * 16) + nt * 16 + col, d * 16 + hi * 4, w.acc[d][nt], w.m[nt] * w.sc,
-                      w.l[nt]);
+    for (int d = 0; d < ND; d++) to.put(d * 16 + hi * 4, w.acc[d][nt], inv);
+    if (hi == 0) to.finish(w.m[nt] * w.sc, w.l[nt]);
   }
 }
 
 // Rows of several chunks: the partial results' sum with the weights of their maxima.  A thread has 4 dimensions of
 // every P-th chunk of a row, 4 chunks at a time; where rows have many chunks (on average) P threads share a row and
 // meet in LDS.  (A thread that went over all chunks one by one waited for each: 7.4 us for the 16 chunks of one token
-// over 4001, 17 for 16 drafts of 5.)
-template <typename T, int D, int P>
+// over 4001, 17 for 16 drafts of 5.)  A block does GROUPS groups of rows in turn: with chunks of a prompt, which mostly
+// are not split, most blocks find nothing to do, and 4 groups are 5 us instead of 9; with drafts 7.5 instead of 4.
+template <typename T, int D, int P, int GROUPS>
 __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheArgs a) {
   constexpr int LANES = D / 4, ROWS = kThreads / LANES / P, N = 4;
   __shared__ f32x4 lds_o[P > 1 ? P : 1][ROWS * LANES];
   __shared__ f32x2 lds_ml[P > 1 ? P : 1][ROWS];
   const int hk = blockIdx.x % a.heads_kv;
   Unit x;
-  if (!find_unit<ROWS>(a, blockIdx.x / a.heads_kv, x)) return;
-  if (x.n_chunks == 1 || x.part + x.n_chunks > a.part_units) return;
-  const int lane = threadIdx.x % LANES, r = threadIdx.x / LANES % ROWS, part = threadIdx.x / LANES / ROWS;
-  const int d0 = lane * 4;
-  const int row = x.row + r - (x.row_tile << a.row_log2);
-  const bool mine = x.row + r < x.n_rows * a.group;
-  float mx = -__builtin_inff(), sum = 0.f;
-  f32x4 o = {0, 0, 0, 0};
-  // (mx, sum, o) of the chunks so far joined with others'
-  auto add = [&](float m, float l, f32x4 v) {
-    if (m == -__builtin_inff()) return;  // (nothing seen: v was not written)
-    const float m_new = fmaxf(mx, m);
-    const float f0 = __builtin_amdgcn_exp2f(mx - m_new), f1 = __builtin_amdgcn_exp2f(m - m_new);
-    mx = m_new;
-    sum = sum * f0 + l * f1;
+  if (!find_unit<ROWS * GROUPS>(a, blockIdx.x / a.heads_kv, x)) return;
+  if (x.n_chunks == 1) return;
+  const int lane = threadIdx.x % LANES, r0 = threadIdx.x / LANES % ROWS, part = threadIdx.x / LANES / ROWS, d0 = lane * 4;
+#pragma unroll 1
+  for (int g = 0; g < GROUPS; g++) {
+    const int row = x.row + g * ROWS + r0;
+    const int first = x.part + (row >> a.row_log2) * x.n_chunks;  // the row's first partial result
+    const bool mine = row < x.n_rows * a.group && first + x.n_chunks <= a.part_units;
+    float mx = -__builtin_inff(), sum = 0.f;
+    f32x4 o = {0, 0, 0, 0};
+    // (mx, sum, o) of the chunks so far joined with others'
+    auto add = [&](float m, float l, f32x4 v) {
+      if (m == -__builtin_inff()) return;
+      const float m_new = fmaxf(mx, m);
+      const float f0 = __builtin_amdgcn_exp2f(mx - m_new), f1 = __builtin_amdgcn_exp2f(m - m_new);
+      mx = m_new;
+      sum = sum * f0 + l * f1;
 #pragma unroll
-    for (int e = 0; e < 4; e++) o[e] = o[e] * f0 + v[e] * f1;
-  };
-  for (int c = mine ? part : x.n_chunks; c < x.n_chunks; c += P * N) {
-    f32x2 ml[N];
-    f32x4 v[N];
+      for (int e = 0; e < 4; e++) o[e] = o[e] * f0 + v[e] * f1;
+    };
+    for (int c = mine ? part : x.n_chunks; c < x.n_chunks; c += P * N) {
+      f32x2 ml[N];
+      f32x4 v[N];
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const int64_t at = (((int64_t)(x.part + min(c + i * P, x.n_chunks - 1)) * a.heads_kv + hk) << a.row_log2) + row;
-      ml[i] = *(const f32x2*)(a.part_ml + at * 2);
-      v[i] = *(const f32x4*)(a.part + at * D + d0);
+      for (int i = 0; i < N; i++) {
+        const int64_t at = (((int64_t)(first + min(c + i * P, x.n_chunks - 1)) * a.heads_kv + hk) << a.row_log2) +
+                           (row & ((1 << a.row_log2) - 1));
+        ml[i] = *(const f32x2*)(a.part_ml + at * 2);
+        v[i] = *(const f32x4*)(a.part + at * D + d0);
+      }
+#pragma unroll
+      for (int i = 0; i < N; i++)
+        if (c + i * P < x.n_chunks) add(ml[i][0], ml[i][1], v[i]);
     }
+    if constexpr (P > 1) {
+      lds_o[part][r0 * LANES + lane] = o;
+      if (lane == 0) lds_ml[part][r0] = f32x2{mx, sum};
+      __syncthreads();
+      if (part != 0) return;
 #pragma unroll
-    for (int i = 0; i < N; i++)
-      if (c + i * P < x.n_chunks) add(ml[i][0], ml[i][1], v[i]);
+      for (int i = 1; i < P; i++) add(lds_ml[i][r0][0], lds_ml[i][r0][1], lds_o[i][r0 * LANES + lane]);
+    }
+    if (mine) {
+      const RowOut<T, D> to(a, x, hk, row, true);
+      to.put(d0, o, to.inverse_of(sum));
+      if (d0 == 0) to.finish(mx, sum);
+    }
   }
-  if constexpr (P > 1) {
-    lds_o[part][r * LANES + lane] = o;
-    if (lane == 0) lds_ml[part][r] = f32x2{mx, sum};
-    __syncthreads();
-    if (part != 0) return;
-#pragma unroll
-    for (int i = 1; i < P; i++) add(lds_ml[i][r][0], lds_ml[i][r][1], lds_o[i][r * LANES + lane]);
-  }
-  if (!mine) return;
-  const int tok = quotient(x.row + r, a.by_group), head = hk * a.group + x.row + r - tok * a.group;
-  const float inv = sum == 0.f ? 0.f : 2.f / sum;
-  T* out = (T*)a.out + (int64_t)x.b * a.o_st[0] + (int64_t)(x.row0 + tok) * a.o_st[1] + (int64_t)head * a.o_st[2];
-  *(typename Mma<T>::V4*)(out + d0) = Mma<T>::pack4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-  if (d0 == 0 && a.lse)
-    a.lse[(int64_t)x.b * a.lse_st[0] + (int64_t)head * a.lse_st[1] + (int64_t)(x.row0 + tok) * a.lse_st[2]] =
-        sum == 0.f ? -__builtin_inff() : (mx - kLift<T> + __log2f(sum)) * (1.f / kLog2e);
 }
 
 // How a call is cut.  Rows of a sequence (on average, of a pack): up to 16 in one tile of a wave, up to 32 in two;
@@ -649,12 +667,16 @@ int launch_attn(CacheArgs& a, const Cut& c, hipStream_t stream) {
   // as many chunks a row (on average) as threads that may share one, or one thread for all
   constexpr int P = kThreads / (D / 4);
   const int64_t rows = a.cu ? a.total_q : (int64_t)a.batch * a.seqlen_q;
-  if (c.row_tiles * a.heads_kv * P <= c.wanted) {
-    hipLaunchKernelGGL((cache_join_kernel<T, D, P>), dim3((unsigned)(rows * a.heads_q)), block, 0, stream, a);
-  } else {
-    const int64_t groups = a.cu ? rows * a.group / P + a.batch : a.batch * ceil_div((int64_t)a.seqlen_q * a.group, P);
-    hipLaunchKernelGGL((cache_join_kernel<T, D, 1>), dim3((unsigned)(groups * a.heads_kv)), block, 0, stream, a);
-  }
+  auto join_blocks = [&](int64_t n) {  // of n rows each
+    const int64_t per_head = a.cu ? rows * a.group / n + a.batch : a.batch * ceil_div((int64_t)a.seqlen_q * a.group, n);
+    return dim3((unsigned)(per_head * a.heads_kv));
+  };
+  if (c.row_tiles * a.heads_kv * P <= c.wanted)
+    hipLaunchKernelGGL((cache_join_kernel<T, D, P, 1>), join_blocks(1), block, 0, stream, a);
+  else if (c.wr == 1)
+    hipLaunchKernelGGL((cache_join_kernel<T, D, 1, 1>), join_blocks(P), block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((cache_join_kernel<T, D, 1, 4>), join_blocks(4 * P), block, 0, stream, a);
   return check_launch("cache_attn join");
 }
 

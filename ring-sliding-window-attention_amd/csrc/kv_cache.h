@@ -161,7 +161,7 @@ struct Unit {
   SeenTiles tiles;
 };
 
-// JOIN > 0: units are JOIN rows from x.row on (a divisor of the row tile), and chunk_idx stays 0.
+// JOIN > 0: units are JOIN rows from x.row on, and `part` is the sequence's first partial result.
 template <int JOIN>
 __device__ __forceinline__ bool find_unit(const CacheArgs& a, int u, Unit& x) {
   const int lane = lane_id();
@@ -201,7 +201,7 @@ __device__ __forceinline__ bool find_unit(const CacheArgs& a, int u, Unit& x) {
       x.n_chunks = of(chunks);
       const int in_seq = u - before - (of(su) - of(units));
       x.row = in_seq * JOIN;
-      x.row_tile = JOIN ? x.row >> a.row_log2 : in_seq / x.n_chunks;
+      x.row_tile = JOIN ? 0 : in_seq / x.n_chunks;
       x.chunk_idx = JOIN ? 0 : in_seq - x.row_tile * x.n_chunks;
       x.chunk = (of(t.count()) + x.n_chunks - 1) / x.n_chunks;
       x.part = before_part + of(sp) - of(parts) + x.row_tile * x.n_chunks;
