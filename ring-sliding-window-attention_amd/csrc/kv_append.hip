@@ -47,7 +47,7 @@ __global__ void cache_append_kernel(const AppendArgs a) {
       cnt = min(step, cnt - at * step);
     }
     b = __builtin_amdgcn_readfirstlane(lo);
-    rows_of(c, b, row0, n);
+    Sequence(c, b).rows(c, row0, n);
     u -= (row0 >> c.page_log2) + 2 * b;
   } else {
     b = quotient(u, a.by_pages);

@@ -221,7 +221,7 @@ struct RowOut {
       out = (T*)a.out + (int64_t)x.b * a.o_st[0] + (int64_t)(x.row0 + tok) * a.o_st[1] + (int64_t)head * a.o_st[2];
       if (a.lse)
         lse = a.lse + (int64_t)x.b * a.lse_st[0] + (int64_t)head * a.lse_st[1] + (int64_t)(x.row0 + tok) * a.lse_st[2];
-    } else if (x.part + x.n_chunks <= a.part_units) {  // (more: cu_seqlens that overlap; more units than rows make)
+    } else if (x.part >= 0 && x.part <= a.part_units - x.n_chunks) {  // (more: cu_seqlens that overlap; more units than rows make)
       const int64_t at =
           (((int64_t)(x.part + x.chunk_idx) * a.heads_kv + hk) << a.row_log2) + (r - (x.row_tile << a.row_log2));
       part = a.part + at * D;
@@ -244,7 +244,7 @@ struct RowOut {
 // Few rows: the four waves of a block have the same rows, each its own keys, and everything from memory to the output
 // stays in registers; the waves meet in LDS at the end.
 template <typename T, int D, int NT>
-__global__ __launch_bounds__(kThreads, 2) void cache_attn_kernel(const CacheArgs a) {
+__global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(const CacheArgs a) {
   using R = Rows<T, D, NT>;
   using V8 = typename Mma<T>::V8;
   constexpr int KW = 4, ROWS = NT * 16, C = R::C, ND = R::ND;
@@ -259,7 +259,6 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_kernel(const CacheArgs
   R w(a, x, hk, x.row_tile * ROWS, col, hi);
   const TileList list = chunk_tiles(a, x, w.first, w.last);
   const Keys<D> keys(a, x, hk, lane);
-
   u32x4 kb[4][C], vb[ND];
   int ke, ve;
   auto load_k = [&](int tile, int id) {
@@ -294,18 +293,20 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_kernel(const CacheArgs
     f32x4 s[NT][4];
     const float kscale = half_scale(ke);
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) s[nt][t] = f32x4{0, 0, 0, 0};
+      for (int t = 0; t < 4; t++) s[nt][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int c = 0; c < C; c++)
+    for (int c = 0; c < C; c++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
+      for (int h = 0; h < 2; h++) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
           const V8 kf = widen8<T>(kb[t][c][2 * h], kb[t][c][2 * h + 1], kscale);
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) s[nt][t] = Mma<T>::mfma16(kf, w.q[nt][c][h], s[nt][t]);
         }
-    }
+      }
     const bool more = i + KW < n;
     if (more) load_k(tile_next, next.k);
     const bool whole = w.whole(a, j0, here);
@@ -345,7 +346,8 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_kernel(const CacheArgs
   }
   __syncthreads();
 #pragma unroll 1
-  for (int at = threadIdx.x; at < ROWS * (D / 4); at += kThreads) {
+  // (the thread's number anew: kept over the loop it would be the one register too many for a third block on the unit)
+  for (int at = wave * 64 + lane_id(); at < ROWS * (D / 4); at += kThreads) {
     const int row = at / (D / 4), d0 = at % (D / 4) * 4;
     float mx = -__builtin_inff();
 #pragma unroll
@@ -573,7 +575,7 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheArgs a)
   for (int g = 0; g < GROUPS; g++) {
     const int row = x.row + g * ROWS + r0;
     const int first = x.part + (row >> a.row_log2) * x.n_chunks;  // the row's first partial result
-    const bool mine = row < x.n_rows * a.group && first + x.n_chunks <= a.part_units;
+    const bool mine = row < x.n_rows * a.group && first >= 0 && first <= a.part_units - x.n_chunks;
     float mx = -__builtin_inff(), sum = 0.f;
     f32x4 o = {0, 0, 0, 0};
     // (mx, sum, o) of the chunks so far joined with others'
@@ -616,10 +618,14 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheArgs a)
   }
 }
 
-// How a call is cut.  Rows of a sequence (on average, of a pack): up to 16 in one tile of a wave, up to 32 in two;
-// the four waves of a block then share the keys.  More: each wave has 32 rows of its own.
+// How a call is cut.  Rows of a sequence (on average, of a pack): up to 16 in one tile of a wave, more in two; the four
+// waves of a block share the keys.  Above 64, if tiles of 128 rows are a block for every compute unit: each wave has 32
+// rows of its own (us, shared keys / own rows, 32 / 8 heads: 32 sequences of 64 tokens against 1000 keys 78 / 52; 2 of
+// 512 against 4096 96 / 90; half as many tiles as units: 1 of 512 52 / 55, 16 of 32 against 8000 97 / 94; fewer: 4 of 64
+// against 1000 20 / 34, 1 of 64 16 / 22).
+constexpr int kMinChunk = 4;
 struct Cut {
-  int nt, wr, row_tile, wanted;
+  int nt, wr, row_tile, wanted, min_chunk;
   int64_t row_tiles;   // at most, over all sequences
   int64_t part_units;  // at most
   int64_t grid;
@@ -629,25 +635,34 @@ Cut cut_call(const rswa_cache_params* p) {
   const int64_t group = p->heads_q / p->heads_kv;
   const int64_t rows = p->cu_seqlens_q ? ceil_div(p->total_q * group, std::max(1, p->batch)) : p->seqlen_q * group;
   c.nt = rows <= 16 ? 1 : 2;
-  c.wr = rows <= 64 ? 1 : 4;
+  const int64_t all_rows = (p->cu_seqlens_q ? p->total_q : (int64_t)p->batch * p->seqlen_q) * p->heads_q;
+  c.wr = rows <= 64 || all_rows < 128 * kComputeUnits ? 1 : 4;
   c.row_tile = c.nt * 16 * c.wr;
   c.row_tiles = p->cu_seqlens_q ? p->total_q * group / c.row_tile + p->batch
                                 : p->batch * ceil_div(p->seqlen_q * group, c.row_tile);
-  // Units wanted.  Few rows: what the chip holds at once (two blocks a compute unit), or half as many again where a
-  // tile is 16 KB for little other work (64 ragged sequences, head_dim 128: 512 units 215 us, 768 206, 1536 208; 128 of
-  // head_dim 64: 50, 54, 51; 16 x 5 drafts: 33, 33, 38, most of it the join).  Many rows: whole rounds of what it holds.
+  // Units wanted: two for each compute unit, which holds three blocks of up to 16 rows (us, 512 / 1024 / 1536 / 2048 units:
+  // one sequence of 131072 48 / 50 / 53 / 55, 128 of head_dim 64 56 / 59 / 62 / 60, 8 of 8192 28 / 28 / 30 / 30, 64 ragged
+  // ones, which finer shares even out, 217 / 218 / 207 / 207) and two of more (16 x 5 drafts 37 / 43 / 45 / 46); where those
+  // have more row tiles than that, whole rounds.
   const int resident = 2 * kComputeUnits;
-  c.wanted = c.wr > 1 ? (int)std::min<int64_t>(4, ceil_div(c.row_tiles * p->heads_kv, resident)) * resident
-             : c.nt == 1 && p->head_dim == 128 ? resident * 3 / 2 : resident;
+  c.wanted =
+      c.nt == 1 ? resident : (int)std::min<int64_t>(4, ceil_div(c.row_tiles * p->heads_kv, resident)) * resident;
   const int64_t per_head = ceil_div(c.wanted, p->heads_kv) + 1;
-  const int64_t most_tiles = ceil_div((int64_t)p->max_pages * p->page_size, kTileKeys);
-  const int64_t at_most = std::min(2 * per_head, c.row_tiles * most_tiles);
-  c.part_units = most_tiles <= 4 ? 0 : at_most;
+  // tiles that a sequence's rows see at most: what its pages hold, or its rows' windows and the sinks
+  int64_t most_tiles = ceil_div((int64_t)p->max_pages * p->page_size, kTileKeys);
+  if (p->window_left >= 0) {
+    const int64_t rows_seq = p->cu_seqlens_q ? p->total_q : p->seqlen_q;
+    most_tiles = std::min(most_tiles, (p->window_left + rows_seq + kTileKeys - 2) / kTileKeys + 1 +
+                                          ceil_div(p->num_sink, kTileKeys));
+  }
+  const int64_t at_most = std::min(ceil_div(8 * per_head, 5), c.row_tiles * most_tiles);
+  // few tiles are not split: the join costs what a wave's third tile does (one token: 512 keys 8.0 us whole, 10.1 in two
+  // launches, 768 9.2 / 10.2, 1024 10.5 / 10.3; own rows: 500 keys 21.9 / 25.2, 1000 33.2 / 32.7)
+  c.min_chunk = most_tiles <= (c.wr == 1 ? 12 : 8) ? (int)most_tiles : kMinChunk;
+  c.part_units = most_tiles <= c.min_chunk ? 0 : at_most;
   c.grid = (c.row_tiles + std::min(per_head, c.row_tiles * most_tiles)) * p->heads_kv;
   return c;
 }
-constexpr int kMinChunk = 4;
-
 uint64_t part_bytes(const Cut& c, const rswa_cache_params* p) {
   return (uint64_t)c.part_units * p->heads_kv * c.row_tile * (p->head_dim + 2) * 4;
 }
@@ -714,7 +729,7 @@ extern "C" int rswa_cache_attn(const rswa_cache_params* p, void* stream) {
   }
   if (a.cu) a.o_st[0] = a.lse_st[0] = 0;
   a.row_log2 = __builtin_ctz((unsigned)c.row_tile);
-  a.min_chunk = kMinChunk;
+  a.min_chunk = c.min_chunk;
   a.per_unit = (float)p->heads_kv / (float)c.wanted;
   a.part_units = (int)c.part_units;
   a.part = (float*)p->workspace;

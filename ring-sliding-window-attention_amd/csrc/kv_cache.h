@@ -113,20 +113,26 @@ __device__ __forceinline__ float columns_sum(float v) {
 __device__ __forceinline__ uint64_t times(int n, uint32_t stride) { return (uint64_t)(uint32_t)n * stride; }
 
 // Tokens that a sequence's row of the page table can hold at most bound its length: no lookup passes its end.
-__device__ __forceinline__ int held_tokens(const CacheArgs& a, int b) {
-  return max(0, min(a.lens[b], a.max_pages << a.page_log2));
+__device__ __forceinline__ int held_tokens(const CacheArgs& a, int len) {
+  return max(0, min(len, a.max_pages << a.page_log2));
 }
 
-// First row and number of rows of sequence b (a pack's: within the tensor whatever cu_seqlens holds).
-__device__ __forceinline__ void rows_of(const CacheArgs& a, int b, int& row0, int& n) {
-  if (a.cu) {
-    row0 = max(0, min(a.cu[b], a.total_q));
-    n = max(row0, min(a.cu[b + 1], a.total_q)) - row0;
-  } else {
-    row0 = 0;
-    n = a.seqlen_q;
+// A sequence as the device's tensors have it, and what it is taken for: a length that the table can hold, rows within
+// the tensor whatever cu_seqlens holds.
+struct Sequence {
+  int len, cu0, cu1;
+  __device__ __forceinline__ Sequence(const CacheArgs& a, int b) : len(a.lens[b]), cu0(0), cu1(0) {
+    if (a.cu) {
+      cu0 = a.cu[b];
+      cu1 = a.cu[b + 1];
+    }
   }
-}
+  __device__ __forceinline__ int tokens(const CacheArgs& a) const { return held_tokens(a, len); }
+  __device__ __forceinline__ void rows(const CacheArgs& a, int& row0, int& n) const {
+    row0 = a.cu ? max(0, min(cu0, a.total_q)) : 0;
+    n = a.cu ? max(row0, min(cu1, a.total_q)) - row0 : a.seqlen_q;
+  }
+};
 
 // The tiles that rows at positions first .. last (the end of the sequence) see: those of the sink keys ahead of the
 // band, from tile 0 on, then n_band from tile t_lo on.
@@ -151,7 +157,8 @@ __device__ __forceinline__ SeenTiles seen_tiles(const CacheArgs& a, int first, i
 // of any lengths make units of nearly one size, which the hardware then deals.  The grid is sized for the bound
 //   sum over sequences of row_tiles * chunks <= units wanted / heads_kv + sum of row_tiles
 // and what is beyond the last unit ends at once.  Rows of sequences with several chunks are joined from partial
-// results; those sequences have at most twice the units wanted (chunks <= 2 tiles / chunk), which bounds the workspace.
+// results; those sequences have at most 8/5 of the units wanted (with x = tiles / chunk, which is above 5/4 there,
+// chunks < x + 3/4), which bounds the workspace.
 // (The sum of tiles is taken in floating point, within 2^-16 of its value: less than the one unit that the host adds.)
 struct Unit {
   int b, row, row_tile, chunk_idx, n_chunks;
@@ -167,27 +174,33 @@ __device__ __forceinline__ bool find_unit(const CacheArgs& a, int u, Unit& x) {
   const int lane = lane_id();
   int row0 = 0, n = 0, len = 0, row_tiles = 0;
   SeenTiles t{0, 0, 0};
-  auto load = [&](int b) {
-    n = row_tiles = 0;
-    t = SeenTiles{0, 0, 0};
-    if (b < a.batch) {
-      rows_of(a, b, row0, n);
-      len = held_tokens(a, b);
-      row_tiles = (n * a.group + (1 << a.row_log2) - 1) >> a.row_log2;  // (below 2^30 rows)
-      if (n > 0) t = seen_tiles(a, len - n, len - 1);
-    }
+  auto load = [&](int b) { return Sequence(a, min(b, a.batch - 1)); };
+  auto take = [&](const Sequence& s, int b) {
+    s.rows(a, row0, n);
+    len = s.tokens(a);
+    n = b < a.batch ? n : 0;
+    row_tiles = (n * a.group + (1 << a.row_log2) - 1) >> a.row_log2;  // (below 2^30 rows)
+    t = n > 0 ? seen_tiles(a, len - n, len - 1) : SeenTiles{0, 0, 0};
   };
   // (fused by hand: attention and join must come to the same chunk)
   float total = 0.f;
+  Sequence next = load(lane);
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    load(b0 + lane);
+    const Sequence s = next;
+    if (a.batch > 64) next = load(b0 + 64 + lane);
+    take(s, b0 + lane);
     total = __builtin_fmaf((float)row_tiles, (float)t.count(), total);
   }
   total = last_lane(wave_scan(total));
   x.chunk = max(a.min_chunk, (int)__builtin_ceilf(total * a.per_unit));
   int before = 0, before_part = 0;
+  if (a.batch > 64) next = load(lane);
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    if (a.batch > 64) load(b0 + lane);
+    if (a.batch > 64) {
+      const Sequence s = next;
+      next = load(b0 + 64 + lane);
+      take(s, b0 + lane);
+    }
     // (up to a quarter more in one chunk rather than a small one behind it)
     const int chunks = max(1, (t.count() + x.chunk - 1 - x.chunk / 4) / x.chunk);
     const int units = JOIN ? (n * a.group + JOIN - 1) / JOIN : row_tiles * chunks;
@@ -200,6 +213,8 @@ __device__ __forceinline__ bool find_unit(const CacheArgs& a, int u, Unit& x) {
       x.b = b0 + at;
       x.n_chunks = of(chunks);
       const int in_seq = u - before - (of(su) - of(units));
+      // (not so only of cu_seqlens that overlap, whose units can be more than 31 bits count)
+      if (in_seq < 0 || in_seq >= of(units)) return false;
       x.row = in_seq * JOIN;
       x.row_tile = JOIN ? 0 : in_seq / x.n_chunks;
       x.chunk_idx = JOIN ? 0 : in_seq - x.row_tile * x.n_chunks;

@@ -44,7 +44,7 @@ __global__ __launch_bounds__(THREADS) void cache_select_kernel(const EvictArgs a
   __shared__ uint32_t sums[WAVES];
   const CacheArgs& c = a.c;
   const int b = blockIdx.x / c.heads_kv, hk = blockIdx.x % c.heads_kv;
-  const int len = held_tokens(c, b);
+  const int len = held_tokens(c, c.lens[b]);
   const int stay = min(len, a.budget);
   const float* w = c.weights + (int64_t)b * c.w_st[0] + (int64_t)hk * c.w_st[1];
   int32_t* kept = a.kept + (int64_t)blockIdx.x * a.budget;
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(512, 4) void cache_move_kernel(const EvictArgs a) {
   const int page_size = 1 << c.page_log2;
   const int hk = blockIdx.x % c.heads_kv;
   const int b = blockIdx.x / c.heads_kv / a.new_max_pages, np = blockIdx.x / c.heads_kv % a.new_max_pages;
-  const int len = held_tokens(c, b), stay = min(len, a.budget);
+  const int len = held_tokens(c, c.lens[b]), stay = min(len, a.budget);
   const int r0 = np << c.page_log2;
   const int n_page = min(page_size, stay - r0);  // tokens of the page
   if (n_page <= 0) return;
