@@ -110,7 +110,6 @@ __global__ void cache_append_kernel(const AppendArgs a) {
   const bool grown = from > 0 && e_new > was;
   // 2^(was - e_new): zero where that is below the least normal number, as every code times it is
   const float shrink = grown && e_new - was < 127 ? __builtin_bit_cast(float, (uint32_t)(127 - (e_new - was)) << 23) : 0.f;
-  __syncthreads();  // (all have read the scale)
   if (!mine) return;
   if (t == 0) *scale = (uint8_t)e_new;
 

@@ -226,9 +226,13 @@ __global__ __launch_bounds__(512, 4) void cache_move_kernel(const EvictArgs a) {
   constexpr int DL = D / 64;          // dimensions of a lane of a value wave
   constexpr int ROW = 16 + 1;         // words of 64 tokens, and one against bank conflicts
   constexpr int PIECES = D / 16, PER = 64 / PIECES, STEPS = 64 / PER;  // 16-byte pieces of a key row; rows of a load
-  extern __shared__ uint32_t packed[];
-  __shared__ int64_t base[8][64];     // keys: of each row; values: of each old group.  -1: its page is not there
-  __shared__ uint32_t info[8][64];    // keys: scale byte; values: which tokens of the group stay, scale byte << 16
+  // of each wave, base: keys: of each row; values: of each old group; -1: its page is not there.  info: keys: scale byte;
+  // values: which tokens of the group stay, scale byte << 16.  Behind them the words of the value waves.
+  extern __shared__ int64_t shared[];
+  const int waves = blockDim.x / 64;
+  int64_t(*const base)[64] = (int64_t(*)[64])shared;
+  uint32_t(*const info)[64] = (uint32_t(*)[64])(shared + waves * 64);
+  uint32_t* const packed = (uint32_t*)(shared + waves * 96);
   __shared__ uint32_t amax[2];
   const CacheArgs& c = a.c;
   const int page_size = 1 << c.page_log2;
@@ -240,7 +244,7 @@ __global__ __launch_bounds__(512, 4) void cache_move_kernel(const EvictArgs a) {
   if (n_page <= 0) return;
   const int id = a.new_table[(int64_t)b * a.new_table_st + np];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const int half = blockDim.x / 128;
+  const int half = waves / 2;
   const bool values = wave >= half;
   const int sub = (values ? wave - half : wave) * 64;  // first place of the wave's tokens
   const int n = max(0, min(64, n_page - sub));
@@ -313,7 +317,8 @@ __global__ __launch_bounds__(512, 4) void cache_move_kernel(const EvictArgs a) {
     const int groups = __popcll(starts);
     const int64_t at = base[wave][lane];  // (lane g: old group g)
     const uint32_t inf = info[wave][lane];
-    u32x4 x[DL], next[DL];
+    constexpr int AHEAD = 4;
+    u32x4 x[AHEAD][DL];  // groups g .. g + 3, in turn
     auto load = [&](int g, u32x4(&y)[DL]) {
       const int64_t from = ((int64_t)__builtin_amdgcn_readlane((int)(at >> 32), g) << 32) |
                            (uint32_t)__builtin_amdgcn_readlane((int)at, g);
@@ -323,9 +328,10 @@ __global__ __launch_bounds__(512, 4) void cache_move_kernel(const EvictArgs a) {
     };
     uint32_t part[DL] = {};
     int fill = 0, word = 0;  // bytes in `part`, words written
-    if (groups > 0) load(0, x);
-    for (int g = 0; g < groups; g++) {
-      if (g + 1 < groups) load(g + 1, next);
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++)
+      if (k < groups) load(k, x[k]);
+    auto group = [&](int g, u32x4(&x)[DL]) {
       const uint32_t which = (uint32_t)__builtin_amdgcn_readlane((int)inf, g);
       LargestCode top;
 #pragma unroll
@@ -352,9 +358,12 @@ __global__ __launch_bounds__(512, 4) void cache_move_kernel(const EvictArgs a) {
         }
       }
       most = fmaxf(most, top.value((int)(which >> 16)));
+      if (g + AHEAD < groups) load(g + AHEAD, x);
+    };
+    for (int g = 0; g < groups; g += AHEAD)
 #pragma unroll
-      for (int i = 0; i < DL; i++) x[i] = next[i];
-    }
+      for (int k = 0; k < AHEAD; k++)
+        if (g + k < groups) group(g + k, x[k]);
     if (fill > 0)
 #pragma unroll
       for (int i = 0; i < DL; i++) words[(lane + 64 * i) * ROW + word] = part[i];
@@ -471,7 +480,7 @@ extern "C" int rswa_cache_evict(const rswa_cache_params* p, void* stream) {
   if (int rc = check_launch("cache_evict select")) return rc;
   if (blocks == 0) return RSWA_OK;
   const int waves = std::max(1, p->page_size / 64);  // of keys, and as many of values
-  const size_t lds = (size_t)waves * p->head_dim * 17 * 4;
+  const size_t lds = (size_t)waves * (2 * 64 * (8 + 4) + p->head_dim * 17 * 4);
   if (p->head_dim == 128)
     hipLaunchKernelGGL((cache_move_kernel<128>), dim3((unsigned)blocks), dim3(waves * 128), lds, st, a);
   else
