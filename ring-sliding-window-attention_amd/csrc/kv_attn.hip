@@ -580,7 +580,7 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheArgs a)
     f32x4 o = {0, 0, 0, 0};
     // (mx, sum, o) of the chunks so far joined with others'
     auto add = [&](float m, float l, f32x4 v) {
-      if (m == -__builtin_inff()) return;
+      if (l == 0.f) return;  // (saw nothing; a maximum of -inf may also be that of scores that are all NaN, which l is then)
       const float m_new = fmaxf(mx, m);
       const float f0 = __builtin_amdgcn_exp2f(mx - m_new), f1 = __builtin_amdgcn_exp2f(m - m_new);
       mx = m_new;
