@@ -114,7 +114,9 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
         for (int i = 0; i < NR; i++) {
           const bool whole = all && j0 + kTileKeys - 1 <= shift + tok0[i] &&
                              (a.window < 0 || j0 >= shift + tok1[i] - a.window);
-          if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[i][e] = __builtin_fmaf(s[i][e], sc, -base[i][e]);
+          if (!whole) {  // (last of all: a row whose lse is NaN leaves the keys alone that it does not see)
             const int j = key + 4 * t;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -124,7 +126,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
             }
           }
 #pragma unroll
-          for (int e = 0; e < 4; e++) sum[t] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], sc, -base[i][e]));
+          for (int e = 0; e < 4; e++) sum[t] += __builtin_amdgcn_exp2f(s[i][e]);
         }
       }
       if (slot + KW < s1) load_keys(tile_of(slot + KW), id_next);

@@ -77,3 +77,21 @@ def test_a_key_of_nan_is_for_the_rows_that_see_it(case):
     bad = bad.cuda()
     assert bool(out[bad].isnan().all()) and bool(lse.transpose(1, 2)[bad].isnan().all())
     assert torch.equal(out[~bad], want[~bad]) and torch.equal(lse.transpose(1, 2)[~bad], want_lse.transpose(1, 2)[~bad])
+
+
+@pytest.mark.parametrize("case", range(len(CALLS)))
+def test_a_query_of_nan_adds_to_the_weights_of_the_keys_that_it_sees(case):
+    from ring_swa import kv_cache_attn, kv_cache_weights
+
+    q, cache, table, lens, window, sinks = call(case)
+    n, group = q.shape[1], q.shape[2] // cache.k.shape[1]
+    longest = int(lens.max())
+    bad = torch.zeros(len(lens), cache.k.shape[1], longest + 9, dtype=torch.bool)
+    for b, row, head in ((0, n - 1, 1), (1, 0, 0), (1, n // 2, 0)):
+        q[b, row, head, 3] = math.nan
+        for j in range(int(lens[b])):
+            bad[b, head // group, j] |= bool(sees(n, int(lens[b]), window, sinks, j)[row])
+    _, lse = kv_cache_attn(q, cache, table, lens, window, num_sink_tokens=sinks, return_lse=True)
+    w = torch.zeros(bad.shape, device="cuda")
+    kv_cache_weights(q, cache, table, lens, lse, w, window, num_sink_tokens=sinks)
+    assert torch.equal(w.isnan().cpu(), bad)
