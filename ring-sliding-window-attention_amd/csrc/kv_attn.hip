@@ -81,6 +81,12 @@ struct Keys {
   __device__ __forceinline__ int value_scale(int id) const { return v_scale[times(there(id) ? id : 0, a.vs_st[0])]; }
 };
 
+// Do all rows at positions first .. last see the whole tile from key j0 on?  (`here`: the lane's group has its page)
+__device__ __forceinline__ bool whole_tile(const CacheArgs& a, int j0, bool here, int first, int last) {
+  return j0 + kTileKeys - 1 <= first && (a.window < 0 || j0 >= last - a.window) &&
+         __builtin_amdgcn_ballot_w64(!here) == 0;
+}
+
 // Bytes of a lane's 16 keys (from j on) that some row at positions first .. last sees.
 __device__ __forceinline__ u32x4 seen_bytes(const CacheArgs& a, int j, bool here, int first, int last) {
   const int lo = a.window < 0 ? 0 : max(0, first - a.window);
@@ -96,6 +102,27 @@ __device__ __forceinline__ u32x4 seen_bytes(const CacheArgs& a, int j, bool here
     keep[w] = mask;
   }
   return keep;
+}
+
+// A value that is NaN makes those rows NaN that see its key, and no others; but a weight of zero does not cancel it.  So
+// in tiles that some rows see and others do not, the product is taken without such values, and where there were any,
+// spoil() below gives them to their rows afterwards.  (In the loop there are no registers for that.)
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {  // 0xff for each byte that is NaN
+  const uint32_t h = ((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  return h | (h - (h >> 7));
+}
+template <int N>
+__device__ __forceinline__ bool take_out_nan(u32x4 (&codes)[N]) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int d = 0; d < N; d++)
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const uint32_t nan = nan_bytes(codes[d][q]);
+      codes[d][q] &= ~nan;
+      any |= nan;
+    }
+  return __builtin_amdgcn_ballot_w64(any != 0) != 0;
 }
 
 // 16 NT rows of a wave from row r0 of the sequence on: B operands of Q (the dimensions in the order in which a lane of
@@ -135,10 +162,8 @@ struct Rows {
       for (int d = 0; d < ND; d++) acc[d][nt] = f32x4{0, 0, 0, 0};
     }
   }
-  // does every row see the whole tile? (`here`: the lane's group has its page)
   __device__ __forceinline__ bool whole(const CacheArgs& a, int j0, bool here) const {
-    return j0 + kTileKeys - 1 <= first && (a.window < 0 || j0 >= last - a.window) &&
-           __builtin_amdgcn_ballot_w64(!here) == 0;
+    return whole_tile(a, j0, here, first, last);
   }
   // scores of what a row does not see become -inf; j: the lane's first key
   __device__ __forceinline__ void mask(const CacheArgs& a, f32x4 (&s)[NT][4], int j, bool here) const {
@@ -198,6 +223,53 @@ struct Rows {
     }
   }
 };
+
+// NaN for the rows that see a NaN among the values of tiles i, i + step, .., of those that rows at positions
+// first .. last do not all see: a product of ones, 1 where a value is NaN and 1 where a row sees its key.
+template <typename T, int D, int NT>
+__device__ __forceinline__ void spoil(const CacheArgs& a, Rows<T, D, NT>& w, const Keys<D>& keys, const TileList& list,
+                                      int i, int step, int first, int last) {
+  using V8 = typename Mma<T>::V8;
+  const int n = list.count();
+#pragma unroll 1
+  for (; i < n; i += step) {
+    const int tile = list[i], j = tile * kTileKeys + keys.hi * 16, id = keys.pages(tile).v;
+    const bool here = keys.there(id);
+    if (whole_tile(a, tile * kTileKeys, here, first, last)) continue;
+    V8 sees[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const int lo = a.window < 0 ? 0 : w.pos[nt] - a.window;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int jj = j + 8 * h + e;
+          p[e] = here && jj <= w.pos[nt] && (jj >= lo || jj < a.n_sink) ? 1.f : 0.f;
+        }
+        sees[nt][h] = Mma<T>::pack(p);
+      }
+    }
+    const uint8_t* const from = keys.values(tile, id);
+#pragma unroll
+    for (int d = 0; d < Rows<T, D, NT>::ND; d++) {
+      const u32x4 codes = *(const u32x4*)(from + d * 256);
+      V8 nan[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++)  // (0x38 is the code of 1)
+        nan[h] = widen8<T>(nan_bytes(codes[2 * h]) & 0x38383838u, nan_bytes(codes[2 * h + 1]) & 0x38383838u, 1.f);
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        f32x4 of = {0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < 2; h++) of = Mma<T>::mfma16(nan[h], sees[nt][h], of);
+#pragma unroll
+        for (int e = 0; e < 4; e++) w.acc[d][nt][e] = of[e] > 0.f ? __builtin_nanf("") : w.acc[d][nt][e];
+      }
+    }
+  }
+}
 
 // The kernel's arguments read again: those of the epilogue alone would be loaded ahead of the loop, where they crowd
 // others out of the scalar registers.
@@ -287,6 +359,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(c
     load_k(list[i], now.k);
     load_v(list[i], now.v);
   }
+  bool spoiled = false;  // (one token's rows see the same keys: nothing to tell apart)
   for (; i < n; i += KW) {
     const int j0 = list[i] * kTileKeys, tile_next = list[min(i + KW, n - 1)];
     const Pages after = keys.pages(list[min(i + 2 * KW, n - 1)]);
@@ -319,6 +392,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(c
       const u32x4 keep = seen_bytes(a, j0 + hi * 16, here, w.first, w.last);
 #pragma unroll
       for (int d = 0; d < ND; d++) vb[d] &= keep;
+      if (w.first != w.last) spoiled |= take_out_nan(vb);
     }
     const float vscale = half_scale(ve);
 #pragma unroll
@@ -335,6 +409,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(c
   }
 
   const CacheArgs& late = arguments_again();
+  if (spoiled) spoil(late, w, keys, list, wave, KW, w.first, w.last);
   float* ml = lds + KW * ROWS * LD;
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
@@ -383,6 +458,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
   constexpr int C = R::C, ND = R::ND, NV = ND / 4;
   constexpr int KF = 4 * C * 2, VF = ND * 2;  // operands of a tile
   __shared__ V8 k_ops[2][KF][64], v_ops[2][VF][64];
+  __shared__ uint32_t any_nan;
 
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int col = lane & 15, hi = lane >> 4;
@@ -423,19 +499,20 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
       for (int h = 0; h < 2; h++) to[(wave * C + c) * 2 + h][lane] = widen8<T>(kb[c][2 * h], kb[c][2 * h + 1], f);
   };
   // (what no row of the block sees may hold anything, NaN codes included: a weight of zero does not cancel those)
-  auto seen = [&](int tile, int id) {
+  bool spoiled = false;
+  auto prepare_v = [&](int tile, int id) {
     const int j0 = tile * kTileKeys;
     const bool here = keys.there(id);
-    if (j0 + kTileKeys - 1 <= first && (a.window < 0 || j0 >= last - a.window) &&
-        __builtin_amdgcn_ballot_w64(!here) == 0)
-      return u32x4{~0u, ~0u, ~0u, ~0u};
-    return seen_bytes(a, j0 + hi * 16, here, first, last);
+    if (whole_tile(a, j0, here, first, last)) return;
+    const u32x4 keep = seen_bytes(a, j0 + hi * 16, here, first, last);
+#pragma unroll
+    for (int d = 0; d < NV; d++) vb[d] &= keep;
+    spoiled |= take_out_nan(vb);
   };
-  auto widen_v = [&](V8 (&to)[VF][64], u32x4 keep) {
+  auto widen_v = [&](V8 (&to)[VF][64]) {
     const float f = half_scale(ve);
 #pragma unroll
     for (int d = 0; d < NV; d++) {
-      vb[d] &= keep;
 #pragma unroll
       for (int h = 0; h < 2; h++) to[(wave * NV + d) * 2 + h][lane] = widen8<T>(vb[d][2 * h], vb[d][2 * h + 1], f);
     }
@@ -469,10 +546,12 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
     load_v(tile_at(0), p[0].v);
     widen_k(k_ops[0]);
     load_k(tile_at(1), p[1].k);
-    widen_v(v_ops[0], seen(tile_at(0), p[0].v));
+    prepare_v(tile_at(0), p[0].v);
+    widen_v(v_ops[0]);
     load_v(tile_at(1), p[1].v);
     widen_k(k_ops[1]);
     load_k(tile_at(2), p[2].k);
+    if (threadIdx.x == 0) any_nan = 0;
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < 2; h++) kf[0][h] = k_ops[0][h][lane];
@@ -482,7 +561,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
   auto step = [&](int i, f32x4 (&s)[NT][4], f32x4 (&z)[NT][4]) {
     const int j0 = list[i] * kTileKeys;
     const Pages after = keys.pages(tile_at(i + 4));
-    const u32x4 keep = seen(tile_at(i + 1), p[1].v);
+    prepare_v(tile_at(i + 1), p[1].v);
     // K of tile i + 1 and V of tile i are there; K of tile i and V of tile i - 1, in whose places the next go, are read
     __syncthreads();
     const auto& k_op = k_ops[(i + 1) & 1];
@@ -522,7 +601,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
         for (int nt = 0; nt < NT; nt++) w.acc[d][nt] = Mma<T>::mfma16(vf[d & 1][h], pf[nt][h], w.acc[d][nt]);
     }
     widen_k(k_ops[i & 1]);
-    widen_v(v_ops[(i + 1) & 1], keep);
+    widen_v(v_ops[(i + 1) & 1]);
     load_k(tile_at(i + 3), p[3].k);
     load_v(tile_at(i + 2), p[2].v);
 #pragma unroll
@@ -545,6 +624,11 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
     if (i + 1 < n) step(i + 1, s1, s0);
   }
   const CacheArgs& late = arguments_again();
+  if (n > 0) {  // (each wave has looked at its quarter of the values)
+    if (spoiled && lane == 0) any_nan = 1;
+    __syncthreads();
+    if (__builtin_amdgcn_readfirstlane(any_nan)) spoil(late, w, keys, list, 0, 1, first, last);
+  }
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
     w.l[nt] = columns_sum(w.l[nt]);

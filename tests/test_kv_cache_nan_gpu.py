@@ -95,3 +95,28 @@ def test_a_query_of_nan_adds_to_the_weights_of_the_keys_that_it_sees(case):
     w = torch.zeros(bad.shape, device="cuda")
     kv_cache_weights(q, cache, table, lens, lse, w, window, num_sink_tokens=sinks)
     assert torch.equal(w.isnan().cpu(), bad)
+
+
+@pytest.mark.parametrize("whole_token", [True, False])
+@pytest.mark.parametrize("case", range(len(CALLS)))
+def test_a_value_of_nan_is_for_the_rows_that_see_it(case, whole_token):
+    """... and, where it is one dimension, for that one alone."""
+    from ring_swa import kv_cache_attn
+
+    q, cache, table, lens, window, sinks = call(case)
+    n, group, dim = q.shape[1], q.shape[2] // cache.k.shape[1], q.shape[3]
+    want, want_lse = kv_cache_attn(q, cache, table, lens, window, num_sink_tokens=sinks, return_lse=True)
+    bad = torch.zeros(q.shape, dtype=torch.bool)
+    for b, length in enumerate(lens.tolist()):
+        for i, j in enumerate((length - 1, length - n // 2 - 1, max(0, length - n - 40), length - n - 150, sinks - 1)):
+            if j < 0:
+                continue
+            dims = slice(None) if whole_token else slice(dim - 1 - 21 * i, dim - 21 * i)
+            plant(cache, 1, table, b, b, j, dims)
+            mine = torch.zeros(dim, dtype=torch.bool)
+            mine[dims] = True
+            bad[b, :, b * group:(b + 1) * group] |= sees(n, length, window, sinks, j)[:, None, None] & mine
+    out, lse = kv_cache_attn(q, cache, table, lens, window, num_sink_tokens=sinks, return_lse=True)
+    assert torch.equal(out.isnan().cpu(), bad)
+    bad = bad.cuda()
+    assert torch.equal(out[~bad], want[~bad]) and torch.equal(lse, want_lse)
