@@ -114,19 +114,20 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
         for (int i = 0; i < NR; i++) {
           const bool whole = all && j0 + kTileKeys - 1 <= shift + tok0[i] &&
                              (a.window < 0 || j0 >= shift + tok1[i] - a.window);
+          auto weight = [&](int e) { return __builtin_fmaf(s[i][e], sc, -base[i][e]); };
+          if (whole) {
 #pragma unroll
-          for (int e = 0; e < 4; e++) s[i][e] = __builtin_fmaf(s[i][e], sc, -base[i][e]);
-          if (!whole) {  // (last of all: a row whose lse is NaN leaves the keys alone that it does not see)
+            for (int e = 0; e < 4; e++) sum[t] += __builtin_amdgcn_exp2f(weight(e));
+          } else {
             const int j = key + 4 * t;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               const int pos = shift + quotient(min(first_row + 16 * i + hi * 4 + e, n_flat - 1), a.by_group);
               const bool see = here && j <= pos && (a.window < 0 || j >= pos - a.window || j < a.n_sink);
-              s[i][e] = see ? s[i][e] : -__builtin_inff();
+              // (masked last of all: a row whose lse is NaN leaves the keys alone that it does not see)
+              sum[t] += __builtin_amdgcn_exp2f(see ? weight(e) : -__builtin_inff());
             }
           }
-#pragma unroll
-          for (int e = 0; e < 4; e++) sum[t] += __builtin_amdgcn_exp2f(s[i][e]);
         }
       }
       if (slot + KW < s1) load_keys(tile_of(slot + KW), id_next);
