@@ -413,8 +413,12 @@ struct CacheCall {
     if (!w || w->scalar_type() != at::kFloat || w->dim() != 3 || w->size(0) != p.batch || w->size(1) != p.heads_kv ||
         !dense_from(*w, 2) || w->device() != device || w->size(2) >= INT32_MAX)
       return false;
-    for (int d = 0; d < 2; d++)
-      if (w->size(d) != 1 && w->stride(d) < w->size(2)) return false;  // (sums of different heads overlap)
+    int64_t span = w->size(2);  // of what the inner of the two strides has walked over
+    const int inner = w->stride(0) < w->stride(1) ? 0 : 1;
+    for (const int d : {inner, 1 - inner}) {
+      if (w->size(d) > 1 && w->stride(d) < span) return false;  // (sums of different heads overlap)
+      span += std::max<int64_t>(0, w->size(d) - 1) * w->stride(d);
+    }
     p.weights = (float*)w->data_ptr();
     p.weights_stride[0] = w->stride(0);
     p.weights_stride[1] = w->stride(1);

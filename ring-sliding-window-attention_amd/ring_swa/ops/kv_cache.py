@@ -271,8 +271,10 @@ def _weights_params(p, cache, weights):
     assert weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (p.batch, p.heads_kv), (
         "weights must be fp32 [batch, kv_heads, n]")
     assert _dense_from(weights, 2), "last dimension must be contiguous"
-    assert all(weights.shape[d] == 1 or weights.stride(d) >= weights.shape[2] for d in (0, 1)), (
-        "the sums of different heads overlap")
+    span = weights.shape[2]  # of what the inner of the two strides has walked over
+    for size, step in sorted(zip(weights.shape[:2], weights.stride()), key=lambda d: d[1]):
+        assert size <= 1 or step >= span, "the sums of different heads overlap"
+        span += max(0, size - 1) * step
     _lib.require_device(cache.k, weights)
     p.weights, p.weights_stride, p.weights_len = weights.data_ptr(), weights.stride()[:2], weights.shape[2]
 

@@ -130,6 +130,18 @@ def params(fill):
     return p
 
 
+def test_running_sums_that_overlap_are_refused(on_cpu):
+    cache, table, lens, q = args()
+    lse = torch.zeros(q.shape[0], q.shape[2], q.shape[1])
+    batch, heads = table.shape[0], cache.k.shape[1]
+    room = torch.zeros(10000)
+    for strides, fine in (((20 * heads, 20, 1), True), ((20, 20 * batch, 1), True), ((30, 20, 1), False),
+                          ((20, 20, 1), False), ((0, 20, 1), False), ((20 * heads, 19, 1), False)):
+        w = room.as_strided((batch, heads, 20), strides)
+        with pytest.raises(AssertionError, match="launched" if fine else "overlap"):
+            ring_swa.kv_cache_weights(q, cache, table, lens, lse, w)
+
+
 @pytest.mark.parametrize("call", ["append", "attn", "weights", "evict"])
 @pytest.mark.parametrize("fill,status", [
     ({"dtype": 2}, -2), ({"head_dim": 96}, -2), ({"page_size": 48}, -2), ({"page_size": 8}, -2), ({"page_size": 512}, -2),

@@ -124,6 +124,22 @@ def test_running_sums_that_share_memory_are_refused():
         ring_swa.kv_cache_weights(q, cache, table, lens, lse, w)
 
 
+def test_running_sums_whose_strides_interleave():
+    """Rows of one tensor in either order; as far apart in one direction as in the other they would meet."""
+    import ring_swa
+
+    cache, table, lens, _ = make([40, 40], 2, 64, 16, 813)
+    q = randn(torch.Generator().manual_seed(34), torch.bfloat16, 2, 1, 4, 64)
+    _, lse = ring_swa.kv_cache_attn(q, cache, table, lens, return_lse=True)
+    want = torch.zeros(2, 2, 40, device="cuda")
+    ring_swa.kv_cache_weights(q, cache, table, lens, lse, want)
+    w = torch.zeros(2, 2, 40, device="cuda").transpose(0, 1)
+    ring_swa.kv_cache_weights(q, cache, table, lens, lse, w)
+    assert torch.equal(w, want)
+    with pytest.raises(AssertionError, match="overlap"):
+        ring_swa.kv_cache_weights(q, cache, table, lens, lse, torch.zeros(120, device="cuda").as_strided((2, 2, 40), (40, 40, 1)))
+
+
 def test_calls_under_no_grad_and_with_a_gradient():
     import ring_swa
 
