@@ -176,8 +176,9 @@ extern "C" int rswa_cache_weights(const rswa_cache_params* p, void* stream) {
   const int64_t rows = p->cu_seqlens_q ? p->total_q : (int64_t)p->batch * p->seqlen_q;
   if (rows == 0 || p->batch == 0 || p->max_pages == 0) return RSWA_OK;
   if (int rc = cache_query_args(p, "cache_weights", a)) return rc;
-  RSWA_REQUIRE(p->lse && p->weights, RSWA_ERR_INVALID, "cache_weights: null tensor");
   RSWA_REQUIRE(p->weights_len >= 0, RSWA_ERR_INVALID, "cache_weights: negative size");
+  RSWA_REQUIRE(p->lse && (p->weights || p->weights_len == 0), RSWA_ERR_INVALID, "cache_weights: null tensor");
+  if (p->weights_len == 0) return RSWA_OK;
   a.lse = p->lse;
   for (int i = 0; i < 3; i++) a.lse_st[i] = p->lse_stride[i];
   if (a.cu) a.lse_st[0] = 0;

@@ -179,6 +179,10 @@ def test_nothing_to_do_is_no_error():
         assert getattr(L, "rswa_cache_" + call)(params({"batch": 0}), None) == 0
 
 
+def test_running_sums_of_no_tokens_need_no_memory():
+    assert _lib.lib().rswa_cache_weights(params({"weights_len": 0, "weights": None}), None) == 0
+
+
 def test_workspace_is_bounded_and_grows_with_what_is_shared():
     L = _lib.lib()
     size = lambda **kw: int(L.rswa_cache_attn_workspace_bytes(params(kw)))  # noqa: E731

@@ -140,6 +140,20 @@ def test_running_sums_whose_strides_interleave():
         ring_swa.kv_cache_weights(q, cache, table, lens, lse, torch.zeros(120, device="cuda").as_strided((2, 2, 40), (40, 40, 1)))
 
 
+def test_running_sums_of_no_tokens():
+    """Nothing to add to, and every weight 0 for the eviction: the earliest stay."""
+    import ring_swa
+
+    cache, table, lens, _ = make([40, 9], 2, 64, 16, 814)
+    q = randn(torch.Generator().manual_seed(35), torch.bfloat16, 2, 1, 4, 64)
+    _, lse = ring_swa.kv_cache_attn(q, cache, table, lens, return_lse=True)
+    w = torch.zeros(2, 2, 0, device="cuda")
+    ring_swa.kv_cache_weights(q, cache, table, lens, lse, w)
+    n, w, kept = ring_swa.kv_cache_evict(cache, w, table, lens, ints([[-1], [-1]]), 10, num_recent=2)
+    assert n.tolist() == [10, 9] and w.shape == (2, 2, 0)
+    assert kept[0, 1].tolist() == [0, 1, 2, 3, 4, 5, 6, 7, 38, 39] and kept[1, 0].tolist() == list(range(9)) + [-1]
+
+
 def test_calls_under_no_grad_and_with_a_gradient():
     import ring_swa
 
