@@ -30,6 +30,8 @@
  *                         same internally -- and which route a backward call takes)
  *   rswa_stream_copy      (no upstream counterpart: the copy kernel the merge kernel's
  *                         rate is measured against)
+ *   rswa_cache_append, rswa_cache_attn, rswa_cache_weights, rswa_cache_evict  (no upstream
+ *                         counterpart: serving from an 8-bit paged cache; see rswa_cache_params)
  * The accumulating forms of the block operators, ring_swa/ops/attn.py:12-196 with the
  * fp32 / fp64 / fp32 accumulators of ring_swa/sliding_window/nonvarlen.py:53-59, 203-206,
  * are served by the fields out_accumulate, dq_accumulate, wide and dkv_accumulate of
@@ -340,7 +342,9 @@ int rswa_attn_fwd_blocks_per_cu(const rswa_attn_params* p);
  *   v        [num_pages, heads_kv, page_size / 16, head_dim, 16]  the 16 keys of a group are adjacent
  *   k_scale, v_scale   [num_pages, heads_kv]                      one byte an element
  * (V lies as the matrix instruction wants it: 16 bytes are 16 keys of one dimension.)  Page and head strides are the
- * caller's, in bytes, those of k and v multiples of 16; within a (page, head) the bytes are dense.
+ * caller's, in bytes, below 2^32 (a pool may span any number of bytes), those of k and v multiples of 16; within a
+ * (page, head) the bytes are dense.  Attention and weights take the codes' values in the type of q, so that what bf16
+ * rows have written beyond fp16's range is infinite to fp16 queries.
  *
  * Token t of sequence b is in page page_table[b * page_table_stride + t / page_size] at place t % page_size.  An id
  * outside [0, num_pages) (-1, say) is a page that is not there: its keys are seen by nobody, tokens that would go
@@ -350,7 +354,7 @@ int rswa_attn_fwd_blocks_per_cu(const rswa_attn_params* p);
  * Queries are the last rows of their sequence: row i of n is token seqlens[b] - n + i and sees the keys of tokens
  *   j <= seqlens[b] - n + i  and  (window_left < 0  or  j >= seqlens[b] - n + i - window_left  or  j < num_sink)
  * which is the rule of rswa_attn_fwd with causal != 0, bottom-right aligned.  Rows that see nothing: out = 0,
- * lse = -inf.  Dense rows are [batch, seqlen_q, heads, head_dim]; with cu_seqlens_q (int32, batch + 1 entries on the
+ * lse = -inf.  A NaN reaches the results that the formula takes it into and no others.  Dense rows are [batch, seqlen_q, heads, head_dim]; with cu_seqlens_q (int32, batch + 1 entries on the
  * device) [total_q, heads, head_dim], and rows behind cu_seqlens_q[batch] are left alone.
  */
 typedef struct rswa_cache_params {
@@ -437,10 +441,10 @@ int rswa_cache_weights(const rswa_cache_params* p, void* stream);
 /*
  * Cuts every sequence to at most `budget` tokens, for each kv head by itself: kept are the first num_sink, the last
  * num_recent, and of the others those with the largest weights (equal ones: the earlier; NaN: as the least), in their
- * order.  Their codes go to the pages of new_page_table, from place 0 on, at the scale that fits the values in each new
- * page; new_seqlens[b] = min(seqlens[b], budget); new_weights gets their weights, zeros behind; kept gets the tokens'
- * old numbers, -1 behind.  The old pages are only read (they may be shared with other sequences), and no page may be
- * both.  num_sink + num_recent <= budget.
+ * order.  (Tokens from weights_len on weigh 0.)  Their codes go to the pages of new_page_table, from place 0 on, at the
+ * scale that fits the values in each new page; new_seqlens[b] = min(seqlens[b], budget); new_weights gets their weights, zeros behind; kept gets the tokens'
+ * old numbers, -1 behind.  The old pages are only read (they may be shared with other sequences); a page may not be
+ * old and new, or new for two sequences.  num_sink + num_recent <= budget.
  */
 int rswa_cache_evict(const rswa_cache_params* p, void* stream);
 

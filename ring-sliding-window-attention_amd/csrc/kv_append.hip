@@ -3,7 +3,8 @@
 // A block takes one page of one kv head, the first half of its threads the keys, the second the values.  A thread has
 // 16 tokens (a group) of 8 dimensions: 16 loads of 16 bytes, all in flight before the first use, hold the whole page in
 // registers, so that its largest value is known before the first code is made and memory is read once.  Keys leave as
-// 8 bytes a row, values as 16 bytes a dimension (the transpose is a choice of registers).
+// 8 bytes a row, values as 16 bytes a dimension (the transpose is byte permutations).  Bound by memory: prompts of
+// 31500 tokens together, 8 heads of 128, 194 MB in 43 us, 4.5 TB/s (values stored a byte at a time 60 us).
 #include "kv_cache.h"
 
 namespace rswa {
@@ -183,7 +184,8 @@ __global__ void cache_append_kernel(const AppendArgs a) {
 }
 
 // One token per sequence (dense): a wave has the key or the value of one head.  The same as above in a tenth of the
-// code: such a launch waits for little but memory, and that includes its instructions.
+// code: such a launch waits for little but memory, and that includes its instructions (one sequence or 128 of 8 heads:
+// 3.5 us, the kernel above 7.5).
 template <typename T, int D>
 __global__ __launch_bounds__(64) void cache_append_token_kernel(const AppendArgs a) {
   constexpr int E = D / 64;  // elements of a lane
@@ -272,8 +274,8 @@ extern "C" int rswa_cache_append(const rswa_cache_params* p, void* stream) {
                          dim3(64), 0, (hipStream_t)stream, a);
       return;
     }
-    hipLaunchKernelGGL((cache_append_kernel<decltype(t), decltype(d)::value>), dim3((unsigned)(ceil_div(blocks, 8) * 8)), dim3(threads), 0,
-                       (hipStream_t)stream, a);
+    hipLaunchKernelGGL((cache_append_kernel<decltype(t), decltype(d)::value>),
+                       dim3((unsigned)(ceil_div(blocks, 8) * 8)), dim3(threads), 0, (hipStream_t)stream, a);
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;

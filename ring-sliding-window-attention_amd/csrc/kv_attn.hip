@@ -8,6 +8,9 @@
 // 16 (m/4) + 4 t + m%4 is the choice by which a lane's 16 scores are 16 consecutive keys -- those of its 16 bytes of
 // V -- and already lie as the B operand of the second product wants them.  All 16 are of one group, so that a page's
 // scale is one value per lane, folded into the widening.
+// Bound by memory where rows are few: 64 sequences of 256 to 32768 keys, 32 / 8 heads of 128, 217 us, 5.1 TB/s.  The keys
+// of long sequences are cut into chunks for the whole chip, whose partial results a second launch joins; one token
+// against 4001 keys takes 6.5 + 4 us, each a launch and some five round trips to memory in a row.
 #include "kv_cache.h"
 
 namespace rswa {
@@ -293,7 +296,7 @@ struct RowOut {
       out = (T*)a.out + (int64_t)x.b * a.o_st[0] + (int64_t)(x.row0 + tok) * a.o_st[1] + (int64_t)head * a.o_st[2];
       if (a.lse)
         lse = a.lse + (int64_t)x.b * a.lse_st[0] + (int64_t)head * a.lse_st[1] + (int64_t)(x.row0 + tok) * a.lse_st[2];
-    } else if (x.part >= 0 && x.part <= a.part_units - x.n_chunks) {  // (more: cu_seqlens that overlap; more units than rows make)
+    } else if (x.part >= 0 && x.part <= a.part_units - x.n_chunks) {  // (not so only of cu_seqlens that overlap)
       const int64_t at =
           (((int64_t)(x.part + x.chunk_idx) * a.heads_kv + hk) << a.row_log2) + (r - (x.row_tile << a.row_log2));
       part = a.part + at * D;
@@ -449,8 +452,10 @@ __global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(c
 // loop is skewed so that matrix and vector work of a wave can run side by side: while the weights of tile i are
 // computed the scores of tile i + 1 are multiplied, and while tile i's weights meet its values the next operands are
 // widened: K two tiles ahead, V one; one barrier a tile.
-// 2048 tokens of 32 / 8 heads against 32768 keys: 1135 us, 943 TFLOP/s (each wave widening all of a tile for itself
-// 1253, unskewed 1240).  Bound by the vector pipe: some 250 instructions for 64 products of 16 cycles.
+// 2048 tokens of 32 / 8 heads against 32768 keys: 1050 us, 1010 TFLOP/s (a library product of as many operations 877;
+// each wave widening all of a tile for itself took a tenth longer, and so did the loop unskewed).  Of the time the matrix
+// pipes are busy 44 %, the vector ones 47 %, both at once 14 %, and LDS 53 %: what bounds it is how the two waves of a SIMD
+// (all that the registers allow) fill each other's gaps.
 template <typename T, int D, int NT>
 __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const CacheArgs a) {
   using R = Rows<T, D, NT>;

@@ -4,8 +4,11 @@
 // the keys as columns, exp2(S - lse), and a sum over rows that needs no exchange until a tile's end.  V is not read.
 // Few rows: each wave has keys of its own, and K is read once.  More: the four waves of a block share the keys, with
 // rows of their own; their sums meet in LDS, in a fixed order, and rows beyond 64 NR come in further rounds over the
-// block's keys.  (Keys in registers and rows from memory instead took 64 us for 64 tokens of 32 / 8 heads against 32001
-// keys, waiting for rows 16 at a time.)
+// block's keys.
+// 32 tokens of as many sequences of 1024 to 16384 keys, 32 / 8 heads: 45 us, 4.2 TB/s, bound by memory.  64 tokens
+// against 32001 keys: 30 us, 510 TFLOP/s, bound by issuing vector instructions (an exponential, at a
+// quarter of their rate, for each 2 x 128 operations) in blocks of eight tiles.  (Keys in registers and rows
+// from memory 64, waiting for rows 16 at a time; a second set of registers for the keys 34.)
 #include "kv_cache.h"
 
 namespace rswa {
@@ -62,7 +65,6 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
     const int first_row = round + rw * (16 * NR);
     V8 q[NR][C][2];
     float base[NR][4];
-    int tok0[NR], tok1[NR];  // first and last token (tok1 < 0: no rows)
 #pragma unroll
     for (int i = 0; i < NR; i++) {
       const int r0 = first_row + 16 * i, r = min(r0 + col, n_flat - 1);
@@ -77,9 +79,9 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
       const float mine = r0 + col < n_flat && lse != -__builtin_inff() ? lse * kLog2e : __builtin_inff();
 #pragma unroll
       for (int e = 0; e < 4; e++) base[i][e] = __shfl(mine, hi * 4 + e);
-      tok0[i] = quotient(min(r0, n_flat - 1), a.by_group);
-      tok1[i] = r0 < n_flat ? quotient(min(r0 + 15, n_flat - 1), a.by_group) : -1;
     }
+    const int first = shift + quotient(min(first_row, n_flat - 1), a.by_group);  // positions of the wave's rows
+    const int last = shift + quotient(min(first_row + 16 * NR, n_flat) - 1, a.by_group);
 
     int slot = s0 + kw;
     if (slot >= s1) return;  // (RW > 1: all waves or none)
@@ -89,54 +91,57 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
       const int tile = tile_of(slot), j0 = tile * kTileKeys;
       const int id_after = page_id(slot + 2 * KW);
       const bool here = (uint32_t)id < (uint32_t)a.num_pages;
-      const bool all = __builtin_amdgcn_ballot_w64(!here) == 0;
       const float scale = half_scale(ke);
       const int key = j0 + 16 * (col >> 2) + (col & 3);  // of product 0
+      // (lane l takes product l/16's column at the end; the sum so far is read here, a round trip to memory ahead)
+      const int at = 16 * (col >> 2) + 4 * hi + (col & 3);
+      const bool mine_to_add = rw == 0 && j0 + at < min(x.len, a.w_len);
+      const float so_far = mine_to_add ? w[j0 + at] : 0.f;
       float sum[4] = {0, 0, 0, 0};
+      // (one test for the tile: with one for each product's rows nothing could be scheduled past the next)
+      auto add_rows = [&](auto whole) {
 #pragma unroll
-      for (int t = 0; t < 4; t++) {
-        V8 kf[C][2];
+        for (int t = 0; t < 4; t++) {
+          V8 kf[C][2];
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-          kf[c][0] = widen8<T>(kb[t][c][0], kb[t][c][1], scale);
-          kf[c][1] = widen8<T>(kb[t][c][2], kb[t][c][3], scale);
-        }
-        f32x4 s[NR];
+          for (int c = 0; c < C; c++) {
+            kf[c][0] = widen8<T>(kb[t][c][0], kb[t][c][1], scale);
+            kf[c][1] = widen8<T>(kb[t][c][2], kb[t][c][3], scale);
+          }
+          f32x4 s[NR];
 #pragma unroll
-        for (int i = 0; i < NR; i++) {
-          s[i] = f32x4{0, 0, 0, 0};
+          for (int i = 0; i < NR; i++) {
+            s[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int c = 0; c < C; c++)
+            for (int c = 0; c < C; c++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) s[i] = Mma<T>::mfma16(q[i][c][h], kf[c][h], s[i]);
-        }
+              for (int h = 0; h < 2; h++) s[i] = Mma<T>::mfma16(q[i][c][h], kf[c][h], s[i]);
+          }
 #pragma unroll
-        for (int i = 0; i < NR; i++) {
-          const bool whole = all && j0 + kTileKeys - 1 <= shift + tok0[i] &&
-                             (a.window < 0 || j0 >= shift + tok1[i] - a.window);
-          auto weight = [&](int e) { return __builtin_fmaf(s[i][e], sc, -base[i][e]); };
-          if (whole) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) sum[t] += __builtin_amdgcn_exp2f(weight(e));
-          } else {
-            const int j = key + 4 * t;
+          for (int i = 0; i < NR; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-              const int pos = shift + quotient(min(first_row + 16 * i + hi * 4 + e, n_flat - 1), a.by_group);
-              const bool see = here && j <= pos && (a.window < 0 || j >= pos - a.window || j < a.n_sink);
-              // (masked last of all: a row whose lse is NaN leaves the keys alone that it does not see)
-              sum[t] += __builtin_amdgcn_exp2f(see ? weight(e) : -__builtin_inff());
+              float z = __builtin_fmaf(s[i][e], sc, -base[i][e]);
+              if constexpr (!decltype(whole)::value) {
+                const int j = key + 4 * t;
+                const int pos = shift + quotient(min(first_row + 16 * i + hi * 4 + e, n_flat - 1), a.by_group);
+                const bool see = here & (j <= pos) & ((a.window < 0) | (j >= pos - a.window) | (j < a.n_sink));
+                z = see ? z : -__builtin_inff();  // (last of all: a row whose lse is NaN leaves what it does not see alone)
+              }
+              sum[t] += __builtin_amdgcn_exp2f(z);
             }
-          }
         }
-      }
+      };
+      if (j0 + kTileKeys - 1 <= first && (a.window < 0 || j0 >= last - a.window) &&
+          __builtin_amdgcn_ballot_w64(!here) == 0)
+        add_rows(std::true_type{});
+      else
+        add_rows(std::false_type{});
       if (slot + KW < s1) load_keys(tile_of(slot + KW), id_next);
       id = id_next;
       id_next = id_after;
 #pragma unroll
       for (int t = 0; t < 4; t++) sum[t] = columns_sum(sum[t]);
-      // lane l takes product l/16's column
-      const int at = 16 * (col >> 2) + 4 * hi + (col & 3);
       float mine = hi == 0 ? sum[0] : hi == 1 ? sum[1] : hi == 2 ? sum[2] : sum[3];
       if constexpr (RW > 1) {
         // (two buffers: a wave that writes the next tile's has passed the barrier behind the reads of this one's last)
@@ -148,13 +153,15 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
 #pragma unroll
           for (int i = 0; i < RW; i++) mine += buf[i * kTileKeys + lane];
       }
-      if (rw == 0 && j0 + at < min(x.len, a.w_len)) w[j0 + at] += mine;
+      if (mine_to_add) w[j0 + at] = so_far + mine;
     }
     if constexpr (RW > 1) __syncthreads();
   }
 }
 
-// Rows of a sequence (on average, of a pack): up to 16, up to 64, more.
+// Rows of a sequence (on average, of a pack): up to 16, up to 64, more.  What either side of the first line takes is the
+// rows' registers: with 16 rows a unit holds four blocks, which memory wants; what the second saves is keys widened once
+// for each 64 rows.
 template <typename T, int D>
 void launch_weights(const CacheArgs& a, int64_t rows, int64_t grid, hipStream_t stream) {
   const dim3 blocks((unsigned)grid), threads(kThreads);
@@ -188,6 +195,8 @@ extern "C" int rswa_cache_weights(const rswa_cache_params* p, void* stream) {
   a.w_len = p->weights_len;
   a.row_log2 = 30;  // a unit has all rows of its sequence
   const int64_t per_seq = ceil_div(rows, p->batch) * a.group;
+  // Units wanted: as many as a compute unit holds of few rows, in one round and a half; of many rows one round, since
+  // each block reads all its rows anew (64 tokens against 32001 keys: 6 for each compute unit 46 us, 2 33)
   const int64_t wanted = kComputeUnits * (per_seq <= 16 ? 6 : 2);
   a.min_chunk = per_seq > 64 ? 1 : 4;
   a.per_unit = (float)p->heads_kv / (float)wanted;

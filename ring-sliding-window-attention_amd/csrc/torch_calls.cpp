@@ -286,7 +286,9 @@ PyObject* band_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // ---- the calls over the 8-bit paged cache (ring_swa/ops/kv_cache.py makes the same in Python) --------------------
 //
-// A served token is a handful of kernels of 4 to 8 us; from Python the host took 13 to 20 us for each of these calls.
+// A served token is a handful of kernels of 4 to 8 us; from Python the host took 13 to 20 us for each of these calls,
+// here 4 to 6.  What they do not take (other types, tensors that need a gradient, modes) goes to Python, which refuses or
+// handles it; a refusal of the library's is raised there too.
 
 struct {
   int (*append)(const rswa_cache_params*, void*) = nullptr;
@@ -340,7 +342,8 @@ struct CacheCall {
         table->scalar_type() != at::kInt || lens->scalar_type() != at::kInt)
       return false;
     const int64_t pages = k.size(0), heads = k.size(1), size = k.size(2), dim = k.size(3);
-    if (heads == 0 || pages >= INT32_MAX || table->size(0) >= INT32_MAX || table->size(1) >= INT32_MAX || size > 256) return false;
+    if (heads == 0 || pages >= INT32_MAX || table->size(0) >= INT32_MAX || table->size(1) >= INT32_MAX || size > 256)
+      return false;
     if (!v.sizes().equals({pages, heads, size / 16, dim, 16}) || !c[2]->sizes().equals({pages, heads}) ||
         !c[3]->sizes().equals({pages, heads}) || lens->size(0) != table->size(0))
       return false;
@@ -376,7 +379,8 @@ struct CacheCall {
     if (type != at::kBFloat16 && type != at::kHalf) return false;
     if (c10::GradMode::is_enabled() && t.requires_grad()) return false;
     packed = cu_o != Py_None;
-    if (t.dim() != (packed ? 3 : 4) || t.size(-1) != p.head_dim || t.stride(-1) != 1 || t.device() != device) return false;
+    if (t.dim() != (packed ? 3 : 4) || t.size(-1) != p.head_dim || t.stride(-1) != 1 || t.device() != device)
+      return false;
     for (int d = 0; d < t.dim(); d++)
       if (t.size(d) >= (1 << 28)) return false;
     p.dtype = type == at::kBFloat16 ? RSWA_BF16 : RSWA_F16;

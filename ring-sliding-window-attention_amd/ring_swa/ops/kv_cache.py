@@ -194,7 +194,9 @@ def kv_cache_attn(
     ``q``: ``[batch, seq, heads, dim]``, or packed ``[tokens, heads, dim]`` with ``cu_seqlens``; bf16 or
     fp16.  ``seqlens`` counts all tokens of a sequence, those of ``q`` among them.  Each query sees its
     own token and the ``window_size`` before it (negative: all) and the first ``num_sink_tokens``.
-    Returns the output, shape and dtype of ``q``, and with ``return_lse`` the log-sum-exp, fp32
+    Codes are read in the type of ``q``: what bf16 rows have written beyond fp16's range is infinite to
+    fp16 queries.  A NaN reaches the rows that see it and no others.  Rows behind the last sequence of a
+    pack are not written.  Returns the output, shape and dtype of ``q``, and with ``return_lse`` the log-sum-exp, fp32
     ``[batch, heads, seq]`` (``[heads, tokens]`` of a pack), as ``merge_attn_out`` takes it.  Rows that
     see nothing: 0 and ``-inf``."""
     calls = _calls(cache)
@@ -296,7 +298,8 @@ def kv_cache_evict(
     largest ``weights`` (of equal ones the earlier; NaN counts as the least), in their order.  They move
     to the pages of ``new_page_table`` (int32 ``[batch, n]``, room for ``budget`` tokens), each page at the
     scale that fits its values; the old pages are only read, so that sequences may share them, and none
-    of them may be among the new ones.  Returns the new ``seqlens``, the kept tokens' weights (shape of
+    of them may be among the new ones, nor a new one in two rows.  Tokens without a weight (``n`` below the
+    length) weigh 0.  Returns the new ``seqlens``, the kept tokens' weights (shape of
     ``weights``, zeros behind) and their old numbers, int32 ``[batch, kv_heads, budget]`` (``-1`` behind).
     From then on a token's number is its place among the kept ones, for windows too."""
     calls = _calls(cache)
