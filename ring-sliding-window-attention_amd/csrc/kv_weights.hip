@@ -6,9 +6,9 @@
 // rows of their own; their sums meet in LDS, in a fixed order, and rows beyond 64 NR come in further rounds over the
 // block's keys.
 // 32 tokens of as many sequences of 1024 to 16384 keys, 32 / 8 heads: 45 us, 4.2 TB/s, bound by memory.  64 tokens
-// against 32001 keys: 30 us, 510 TFLOP/s, bound by issuing vector instructions (an exponential, at a
-// quarter of their rate, for each 2 x 128 operations) in blocks of eight tiles.  (Keys in registers and rows
-// from memory 64, waiting for rows 16 at a time; a second set of registers for the keys 34.)
+// against 32001 keys: 28 us, 600 TFLOP/s, of which 8 are blocks' starts and ends (eight tiles each); 700
+// TFLOP/s against 200000, bound by issuing vector instructions: an exponential, at a quarter of their rate, for each
+// 2 x 128 operations.  (Keys in registers and rows from memory 64 us, waiting for rows 16 at a time.)
 #include "kv_cache.h"
 
 namespace rswa {
@@ -47,9 +47,13 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
   auto page_id = [&](int slot) {
     return table[min(tile_of(min(slot, s1 - 1)) * 4 + (col >> 2), n_groups - 1) >> per_page];
   };
-  u32x4 kb[4][C];
-  int ke;
-  auto load_keys = [&](int tile, int id) {
+  // Of many rows two sets of registers, the next tile's loaded ahead of this one's products (behind the last tile that one
+  // again: a branch here makes the compiler wait for more than it must).  us without / with it, 32 / 8 heads: 64 tokens
+  // against 4000 keys 11.9 / 12.6, 32001 32.6 / 31.3, 200000 155 / 148; 2 sequences of 512 against 4096 100 / 95.
+  constexpr int BUFS = NR > 1 ? 2 : 1;
+  u32x4 kbs[BUFS][4][C];
+  int kes[BUFS];
+  auto load_keys = [&](u32x4 (&kb)[4][C], int& ke, int tile, int id) {
     const int page = (uint32_t)id < (uint32_t)a.num_pages ? id : 0;
     const int g = min(tile * 4 + (col >> 2), n_groups - 1) & in_page;
     const uint8_t* p = k_head + times(page, a.k_st[0]) + (g * kGroupKeys + (col & 3)) * D + hi * 16;
@@ -86,11 +90,12 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
     int slot = s0 + kw;
     if (slot >= s1) return;  // (RW > 1: all waves or none)
     int id = page_id(slot), id_next = page_id(slot + KW);
-    load_keys(tile_of(slot), id);
-    for (; slot < s1; slot += KW) {
+    load_keys(kbs[0], kes[0], tile_of(slot), id);
+    auto step = [&](int slot, u32x4 (&kb)[4][C], int& ke, u32x4 (&kb_next)[4][C], int& ke_next) {
       const int tile = tile_of(slot), j0 = tile * kTileKeys;
       const int id_after = page_id(slot + 2 * KW);
       const bool here = (uint32_t)id < (uint32_t)a.num_pages;
+      if (BUFS > 1) load_keys(kb_next, ke_next, tile_of(min(slot + KW, s1 - 1)), id_next);
       const float scale = half_scale(ke);
       const int key = j0 + 16 * (col >> 2) + (col & 3);  // of product 0
       // (lane l takes product l/16's column at the end; the sum so far is read here, a round trip to memory ahead)
@@ -137,7 +142,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
         add_rows(std::true_type{});
       else
         add_rows(std::false_type{});
-      if (slot + KW < s1) load_keys(tile_of(slot + KW), id_next);
+      if (BUFS == 1 && slot + KW < s1) load_keys(kb, ke, tile_of(slot + KW), id_next);
       id = id_next;
       id_next = id_after;
 #pragma unroll
@@ -154,6 +159,10 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
           for (int i = 0; i < RW; i++) mine += buf[i * kTileKeys + lane];
       }
       if (mine_to_add) w[j0 + at] = so_far + mine;
+    };
+    for (; slot < s1; slot += BUFS * KW) {
+      step(slot, kbs[0], kes[0], kbs[BUFS - 1], kes[BUFS - 1]);
+      if (BUFS > 1 && slot + KW < s1) step(slot + KW, kbs[BUFS - 1], kes[BUFS - 1], kbs[0], kes[0]);
     }
     if constexpr (RW > 1) __syncthreads();
   }
