@@ -183,20 +183,25 @@ struct Rows {
         }
     }
   }
-  // One tile's step of the running softmax (a row's scores are in the four lanes of its column): the maximum, with
-  // what it changes ...
-  __device__ __forceinline__ void raise(const f32x4 (&s)[NT][4]) {
+  // One tile's step of the running softmax (a row's scores are in the four lanes of its column): the maximum ...
+  __device__ __forceinline__ void tops(const f32x4 (&s)[NT][4], float (&top)[NT]) const {
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       // (NaN stays NaN, and its weights are: the other maximum would first quiet each score, an instruction apiece)
-      float top = s[nt][0][0];
+      float x = s[nt][0][0];
 #pragma unroll
       for (int t = 0; t < 4; t++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) top = __builtin_elementwise_maximum(top, s[nt][t][e]);
-      top = columns_max(top);
-      if (__builtin_amdgcn_ballot_w64(top > m[nt])) {
-        const float m_new = __builtin_elementwise_maximum(m[nt], top);
+        for (int e = 0; e < 4; e++) x = __builtin_elementwise_maximum(x, s[nt][t][e]);
+      top[nt] = columns_max(x);
+    }
+  }
+  // ... what it changes ...
+  __device__ __forceinline__ void raise(const float (&top)[NT]) {
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      if (__builtin_amdgcn_ballot_w64(top[nt] > m[nt])) {
+        const float m_new = __builtin_elementwise_maximum(m[nt], top[nt]);
         const float shrink = m[nt] == m_new ? 1.f : __builtin_amdgcn_exp2f((m[nt] - m_new) * sc);
         m[nt] = m_new;
         l[nt] *= shrink;
@@ -388,7 +393,9 @@ __global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(c
     const bool whole = w.whole(a, j0, here);
     if (!whole) w.mask(a, s, j0 + hi * 16, here);
     V8 pf[NT][2];
-    w.raise(s);
+    float top[NT];
+    w.tops(s, top);
+    w.raise(top);
     w.weigh(s, pf);
     // what no row of the wave sees may hold anything, NaN codes included: a weight of zero does not cancel those
     if (!whole) {
@@ -451,10 +458,11 @@ __global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(c
 // each tile and leaves it in LDS as operands (lane after lane, so that reads and writes have no bank conflicts).  The
 // loop is skewed so that matrix and vector work of a wave can run side by side: while the weights of tile i are
 // computed the scores of tile i + 1 are multiplied, and while tile i's weights meet its values the next operands are
-// widened: K two tiles ahead, V one; one barrier a tile.
-// 2048 tokens of 32 / 8 heads against 32768 keys: 1017 us, 1050 TFLOP/s (a library product of as many operations 877;
+// widened, K two tiles ahead, V one, and the largest scores of tile i + 1 found (2.4 % less time than after the barrier);
+// one barrier a tile.
+// 2048 tokens of 32 / 8 heads against 32768 keys: 985 us, 1080 TFLOP/s (a library product of as many operations 877;
 // each wave widening all of a tile for itself took a tenth longer, and so did the loop unskewed).  Of the time the matrix
-// pipes are busy 44 %, the vector ones 47 %, both at once 14 %, and LDS 53 %: what bounds it is how the two waves of a SIMD
+// pipes are busy 49 %, the vector ones 52 %, both at once 15 %, and LDS 59 %: what bounds it is how the two waves of a SIMD
 // (all that the registers allow) fill each other's gaps.
 template <typename T, int D, int NT>
 __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const CacheArgs a) {
@@ -524,6 +532,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
   };
 
   f32x4 s0[NT][4], s1[NT][4];
+  float top[NT];  // of the next tile's scores
   V8 kf[2][2], vf[2][2];
   // S^T of the tile whose operands are in `op`; they are read four products ahead, the first two before the call
   auto scores = [&](const V8 (&op)[KF][64], f32x4 (&z)[NT][4]) {
@@ -541,6 +550,12 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) z[nt][t] = Mma<T>::mfma16(kf[i & 1][h], w.q[nt][c][h], z[nt][t]);
     }
+  };
+
+  auto hide = [&](f32x4 (&s)[NT][4], int i, const Pages& of) {
+    const int j0 = tile_at(i) * kTileKeys;
+    const bool here = keys.there(of.v);
+    if (!w.whole(a, j0, here)) w.mask(a, s, j0 + hi * 16, here);
   };
 
   Pages p[4] = {};  // of tiles i .. i + 3
@@ -561,10 +576,11 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
 #pragma unroll
     for (int h = 0; h < 2; h++) kf[0][h] = k_ops[0][h][lane];
     scores(k_ops[0], s0);
+    hide(s0, 0, p[0]);
+    w.tops(s0, top);
   }
-  // tile i, whose scores are in s; those of the next go to z
+  // tile i, whose scores are in s and their largest in top; those of the next go to z
   auto step = [&](int i, f32x4 (&s)[NT][4], f32x4 (&z)[NT][4]) {
-    const int j0 = list[i] * kTileKeys;
     const Pages after = keys.pages(tile_at(i + 4));
     prepare_v(tile_at(i + 1), p[1].v);
     // K of tile i + 1 and V of tile i are there; K of tile i and V of tile i - 1, in whose places the next go, are read
@@ -573,9 +589,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
     const auto& v_op = v_ops[i & 1];
 #pragma unroll
     for (int h = 0; h < 2; h++) kf[0][h] = k_op[h][lane];
-    const bool here = keys.there(p[0].v);
-    if (!w.whole(a, j0, here)) w.mask(a, s, j0 + hi * 16, here);
-    w.raise(s);
+    w.raise(top);
 
     __builtin_amdgcn_sched_barrier(0);
     V8 pf[NT][2];
@@ -594,6 +608,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
       }
     }
     __builtin_amdgcn_sched_barrier(0);
+    hide(z, i + 1, p[1]);
 
     // (products with little else between them: their wave goes first, the other fills the gaps; us for 2048 tokens against
     // 32768 keys without 1049, for all products 1031, for these 1009)
@@ -608,6 +623,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) w.acc[d][nt] = Mma<T>::mfma16(vf[d & 1][h], pf[nt][h], w.acc[d][nt]);
     }
+    w.tops(z, top);
     widen_k(k_ops[i & 1]);
     widen_v(v_ops[(i + 1) & 1]);
     load_k(tile_at(i + 3), p[3].k);
@@ -618,7 +634,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
 #pragma unroll
       for (int e = 0; e < 2 * NT; e++) {
         __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x2, 1, 0);  // (0.6 % less time than 2, and that 0.9 % less than 3)
+        __builtin_amdgcn_sched_group_barrier(0x2, 2, 0);  // (1 or 3: 2 % more time)
       }
     }
     __builtin_amdgcn_sched_barrier(0);
