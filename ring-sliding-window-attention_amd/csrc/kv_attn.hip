@@ -730,8 +730,9 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheArgs a)
 // How a call is cut.  Rows of a sequence (on average, of a pack): up to 16 in one tile of a wave, more in two; the four
 // waves of a block share the keys.  Above 64, if tiles of 128 rows are a block for every compute unit: each wave has 32
 // rows of its own (us, shared keys / own rows, 32 / 8 heads: 32 sequences of 64 tokens against 1000 keys 78 / 52; 2 of
-// 512 against 4096 96 / 90; half as many tiles as units: 1 of 512 52 / 55, 16 of 32 against 8000 97 / 94; fewer: 4 of 64
-// against 1000 20 / 34, 1 of 64 16 / 22).
+// 512 against 4096 96 / 90.  Half as many tiles as units: 1 of 512 against 1000 26 / 33, 4096 59 / 59, 32768 367 / 310, 16
+// of 32 against 8000 120 / 116, 28 / 4 heads of 64, 3 of 200 against 8000 76 / 98; the host, which does not know the
+// lengths, cannot tell these apart.  Fewer: 4 of 64 against 1000 20 / 34, 1 of 64 16 / 22).
 constexpr int kMinChunk = 4;
 struct Cut {
   int nt, wr, row_tile, wanted, min_chunk;

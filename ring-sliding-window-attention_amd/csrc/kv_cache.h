@@ -38,7 +38,7 @@ struct CacheArgs {
   float* lse;
   int64_t q_st[3], o_st[3], lse_st[3];
   float scale_log2;  // softmax_scale * log2(e)
-  // how the work is cut (see Plan)
+  // how the work is cut (see find_unit)
   int32_t row_log2;   // a unit's row tile has 2^row_log2 rows (token x grouped head)
   int32_t min_chunk;  // least tiles of a unit
   float per_unit;     // heads_kv / units wanted

@@ -101,7 +101,7 @@ __global__ __launch_bounds__(THREADS) void cache_select_kernel(const EvictArgs a
 
   uint32_t least = kStays - 1;  // above every weight: none of the others stays
   if (find > 0) {
-    // the digit of the find-th largest from the counts of COUNT copies
+    // the digit of the find-th largest, from the counts in so many copies
     auto choose = [&](int copies) {
       uint32_t n[MINE], sum = 0;
       const int top = BINS - 1 - MINE * (int)threadIdx.x;  // thread t: MINE bins, from BINS - 1 - MINE t down
