@@ -460,7 +460,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(c
 // computed the scores of tile i + 1 are multiplied, and while tile i's weights meet its values the next operands are
 // widened, K two tiles ahead, V one, and the largest scores of tile i + 1 found (2.4 % less time than after the barrier);
 // one barrier a tile.
-// 2048 tokens of 32 / 8 heads against 32768 keys: 985 us, 1080 TFLOP/s (a library product of as many operations 877;
+// 2048 tokens of 32 / 8 heads against 32768 keys: 977 us, 1090 TFLOP/s (a library product of as many operations 877;
 // each wave widening all of a tile for itself took a tenth longer, and so did the loop unskewed).  Of the time the matrix
 // pipes are busy 49 %, the vector ones 52 %, both at once 15 %, and LDS 59 %: what bounds it is how the two waves of a SIMD
 // (all that the registers allow) fill each other's gaps.

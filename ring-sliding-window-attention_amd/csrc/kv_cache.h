@@ -216,8 +216,11 @@ __device__ __forceinline__ bool find_unit(const CacheArgs& a, int u, Unit& x) {
       // (not so only of cu_seqlens that overlap, whose units can be more than 31 bits count)
       if (in_seq < 0 || in_seq >= of(units)) return false;
       x.row = in_seq * JOIN;
-      x.row_tile = JOIN ? 0 : in_seq / x.n_chunks;
-      x.chunk_idx = JOIN ? 0 : in_seq - x.row_tile * x.n_chunks;
+      const int tile = JOIN ? 0 : in_seq / x.n_chunks;
+      x.chunk_idx = JOIN ? 0 : in_seq - tile * x.n_chunks;
+      // (the last rows, which see the most keys, first, so that the launch ends on small units: 8192 tokens from empty 665 us
+      // from the first row on, 617 from the last; 4 sequences of 2048 239 / 222)
+      x.row_tile = JOIN ? 0 : of(row_tiles) - 1 - tile;
       x.chunk = (of(t.count()) + x.n_chunks - 1) / x.n_chunks;
       x.part = before_part + of(sp) - of(parts) + x.row_tile * x.n_chunks;
       x.row0 = of(row0);
