@@ -42,7 +42,8 @@ __global__ void cache_append_kernel(const AppendArgs a) {
       const int step = (cnt + 63) >> 6;
       const int i = min(lo + lane * step, lo + cnt - 1);
       const int slot = (max(0, min(c.cu[i], c.total_q)) >> c.page_log2) + 2 * i;
-      const int at = max(__popcll(__builtin_amdgcn_ballot_w64(lane * step < cnt && slot <= u)) - 1, 0);
+      // (none: rows ahead of the first sequence; the count is unsigned)
+      const int at = max((int)__popcll(__builtin_amdgcn_ballot_w64(lane * step < cnt && slot <= u)) - 1, 0);
       lo += at * step;
       if (step == 1) break;
       cnt = min(step, cnt - at * step);

@@ -75,6 +75,54 @@ def test_weights_of_many_rows(case):
     assert bool((diff <= bound).all()), f"off by up to {(diff / bound).max().item():.2f} of the bound"
 
 
+def test_cu_seqlens_that_overlap_or_leave_the_tensor():
+    """Any results, but nothing read or written that is not the call's: pages of no sequence stay as they are, and the
+    sums behind a sequence's tokens."""
+    import ring_swa
+
+    cache, table, lens, free = make([500, 700], 8, 64, 16, 815, spare=5, max_pages=120)
+    q = randn(torch.Generator().manual_seed(36), torch.bfloat16, 1100, 32, 64)
+    k, v = (randn(torch.Generator().manual_seed(37 + i), torch.bfloat16, 1100, 8, 64) for i in range(2))
+    kept = [t.view(torch.uint8)[free].clone() for t in cache]
+    for wild in ([0, 1100, 0], [-5, 600, 10 ** 9], [800, 200, 2 ** 31 - 1], [2 ** 31 - 1, -2 ** 31, 5]):
+        cu = ints(wild)
+        out, lse = ring_swa.kv_cache_attn(q, cache, table, lens, -1, cu, return_lse=True)
+        assert out.shape == q.shape and lse.shape == (32, 1100)
+        w = torch.zeros(2, 8, 900, device="cuda")
+        ring_swa.kv_cache_weights(q, cache, table, lens, lse, w, -1, cu)
+        assert bool((w[0, :, 500:] == 0).all()) and bool((w[1, :, 700:] == 0).all())
+        ring_swa.kv_cache_append(cache, k, v, table, lens, cu)
+        for t, was in zip(cache, kept):
+            assert torch.equal(t.view(torch.uint8)[free], was)
+
+
+def test_packs_that_begin_behind_the_first_row():
+    """Rows ahead of cu_seqlens[0] are no sequence's: neither written to the cache nor answered."""
+    import ring_swa
+
+    for cu_list in ([40, 43, 90], [200, 200, 263], [17, 80, 80]):
+        cache, table, lens, _ = make([500, 70], 2, 64, 16, 816, max_pages=40, wild=False)
+        g = torch.Generator().manual_seed(39)
+        k, v = (randn(g, torch.bfloat16, 300, 2, 64) for _ in range(2))
+        q = randn(g, torch.bfloat16, 300, 8, 64)
+        cu = ints(cu_list)
+        held = lens - cu.diff()
+        want = O.append(cache, k, v, table, held, cu)
+        ring_swa.kv_cache_append(cache, k, v, table, held, cu)
+        assert O.same_bytes(cache, want)
+        out, lse = ring_swa.kv_cache_attn(q, cache, table, lens, -1, cu, return_lse=True)
+        at = cu_list[0]
+        w = torch.zeros(2, 2, 500, device="cuda")
+        ring_swa.kv_cache_weights(q, cache, table, lens, lse, w, -1, cu)
+        moved = ints([x - at for x in cu_list])  # the same pack from its first row on
+        out2, lse2 = ring_swa.kv_cache_attn(q[at:], cache, table, lens, -1, moved, return_lse=True)
+        w2 = torch.zeros(2, 2, 500, device="cuda")
+        ring_swa.kv_cache_weights(q[at:], cache, table, lens, lse2, w2, -1, moved)
+        n = cu_list[-1] - at
+        assert torch.equal(out[at:cu_list[-1]], out2[:n]) and torch.equal(lse[:, at:cu_list[-1]], lse2[:, :n])
+        assert torch.equal(w, w2)
+
+
 def test_the_python_route_gives_the_native_one_s_bits(monkeypatch):
     """Every call through the native module, which must take it, and again without the module."""
     import ring_swa
