@@ -315,7 +315,8 @@ __device__ __forceinline__ bool locate_packed(const AttnArgs& a, int t, int tile
     const int step = (n + 63) >> 6;
     const int i = min(lo + lane * step, lo + n - 1);
     const int slot = (cu[i] >> tile_log2) + i;
-    const int at = max(__popcll(__builtin_amdgcn_ballot_w64(lane * step < n && slot <= t)) - 1, 0);
+    // (none: rows ahead of the first sequence; the count is unsigned)
+    const int at = max((int)__popcll(__builtin_amdgcn_ballot_w64(lane * step < n && slot <= t)) - 1, 0);
     lo += at * step;
     if (step == 1) break;
     n = min(step, n - at * step);
@@ -323,7 +324,7 @@ __device__ __forceinline__ bool locate_packed(const AttnArgs& a, int t, int tile
   const int b = lo;
   const int first = cu[b];
   tile_in_seq = t - ((first >> tile_log2) + b);
-  if ((tile_in_seq << tile_log2) >= cu[b + 1] - first) return false;
+  if (tile_in_seq < 0 || (tile_in_seq << tile_log2) >= cu[b + 1] - first) return false;
   s.batch_idx = b;
   s.q_row0 = a.cu_q[b];
   s.k_row0 = a.cu_k[b];
