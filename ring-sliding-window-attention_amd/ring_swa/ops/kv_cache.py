@@ -20,7 +20,8 @@ says which::
 
 Lengths and page ids stay on the device, nothing is read back.  Rows are ``[batch, seq, heads, dim]``,
 or packed ``[tokens, heads, dim]`` with ``cu_seqlens`` (int32 ``[batch + 1]``; sequences may bring
-different numbers of rows, none among them), as in the attention functions.  The new rows' keys are
+different numbers of rows, none among them; rows that are no sequence's are passed over), as in the
+attention functions.  The new rows' keys are
 in the cache already when their queries attend: row ``i`` of ``n`` is token ``seqlens - n + i``.  A
 page id outside the cache (``-1``) is a page that is not there: seen by nobody, never written, so the
 pages that a window has left behind can be given back.  There is no backward.
@@ -195,8 +196,8 @@ def kv_cache_attn(
     fp16.  ``seqlens`` counts all tokens of a sequence, those of ``q`` among them.  Each query sees its
     own token and the ``window_size`` before it (negative: all) and the first ``num_sink_tokens``.
     Codes are read in the type of ``q``: what bf16 rows have written beyond fp16's range is infinite to
-    fp16 queries.  A NaN reaches the rows that see it and no others.  Rows behind the last sequence of a
-    pack are not written.  Returns the output, shape and dtype of ``q``, and with ``return_lse`` the log-sum-exp, fp32
+    fp16 queries.  A NaN reaches the rows that see it and no others.  Rows ahead of a pack's first
+    sequence and behind its last are not written.  Returns the output, shape and dtype of ``q``, and with ``return_lse`` the log-sum-exp, fp32
     ``[batch, heads, seq]`` (``[heads, tokens]`` of a pack), as ``merge_attn_out`` takes it.  Rows that
     see nothing: 0 and ``-inf``."""
     calls = _calls(cache)
