@@ -25,6 +25,8 @@ attention functions.  The new rows' keys are
 in the cache already when their queries attend: row ``i`` of ``n`` is token ``seqlens - n + i``.  A
 page id outside the cache (``-1``) is a page that is not there: seen by nobody, never written, so the
 pages that a window has left behind can be given back.  There is no backward.
+
+A compiled program makes these calls between its graphs (``fullgraph=True`` refuses them).
 """
 from __future__ import annotations
 
@@ -77,9 +79,14 @@ def _dense_from(t: torch.Tensor, dim: int) -> bool:
 
 def _calls(cache):
     """The native module where it may take the call (it answers None to what it leaves to Python)."""
-    if cache[0].is_cuda and not torch.compiler.is_compiling():
-        return _lib.torch_calls()
-    return None
+    return _lib.torch_calls() if cache[0].is_cuda else None
+
+
+@torch._disable_dynamo
+def _uncompiled(call, *args, **kwargs):
+    """Compiled programs make the calls between their graphs, as they make those of the attention functions.  (In a
+    graph, PyTorch's default compiler refuses operators that write beside e8m0 tensors, and others copy the cache.)"""
+    return call(*args, **kwargs)
 
 
 def _no_grad(*tensors) -> None:
@@ -163,6 +170,8 @@ def kv_cache_append(
     smallest normal code change).  Infinities and NaN are stored as NaN.  Tokens beyond the last page
     of ``page_table``, or whose page is not there, are dropped.  ``seqlens`` is left alone; two
     sequences of one call must not have a page written in common."""
+    if torch.compiler.is_dynamo_compiling():
+        return _uncompiled(kv_cache_append, cache, k, v, page_table, seqlens, cu_seqlens)
     calls = _calls(cache)
     if calls is not None and calls.cache_append(cache, k, v, page_table, seqlens, cu_seqlens):
         return
@@ -200,6 +209,9 @@ def kv_cache_attn(
     sequence and behind its last are not written.  Returns the output, shape and dtype of ``q``, and with ``return_lse`` the log-sum-exp, fp32
     ``[batch, heads, seq]`` (``[heads, tokens]`` of a pack), as ``merge_attn_out`` takes it.  Rows that
     see nothing: 0 and ``-inf``."""
+    if torch.compiler.is_dynamo_compiling():
+        return _uncompiled(kv_cache_attn, q, cache, page_table, seqlens, window_size, cu_seqlens, softmax_scale,
+                           num_sink_tokens=num_sink_tokens, return_lse=return_lse)
     calls = _calls(cache)
     if calls is not None:
         got = calls.cache_attn(q, cache, page_table, seqlens, window_size, cu_seqlens, softmax_scale,
@@ -251,6 +263,9 @@ def kv_cache_weights(
 
     ``lse`` is what ``kv_cache_attn(..., return_lse=True)`` returned for the same arguments; ``weights``
     fp32 ``[batch, kv_heads, n]``, entry ``j`` that of token ``j`` (tokens from ``n`` on are passed over)."""
+    if torch.compiler.is_dynamo_compiling():
+        return _uncompiled(kv_cache_weights, q, cache, page_table, seqlens, lse, weights, window_size, cu_seqlens,
+                           softmax_scale, num_sink_tokens=num_sink_tokens)
     calls = _calls(cache)
     if calls is not None and calls.cache_weights(q, cache, page_table, seqlens, lse, weights, window_size, cu_seqlens,
                                                  softmax_scale, num_sink_tokens):
@@ -303,6 +318,9 @@ def kv_cache_evict(
     length) weigh 0.  Returns the new ``seqlens``, the kept tokens' weights (shape of
     ``weights``, zeros behind) and their old numbers, int32 ``[batch, kv_heads, budget]`` (``-1`` behind).
     From then on a token's number is its place among the kept ones, for windows too."""
+    if torch.compiler.is_dynamo_compiling():
+        return _uncompiled(kv_cache_evict, cache, weights, page_table, seqlens, new_page_table, budget,
+                           num_sink_tokens=num_sink_tokens, num_recent=num_recent)
     calls = _calls(cache)
     if calls is not None:
         got = calls.cache_evict(cache, weights, page_table, seqlens, new_page_table, budget, num_sink_tokens,
