@@ -26,7 +26,8 @@ in the cache already when their queries attend: row ``i`` of ``n`` is token ``se
 page id outside the cache (``-1``) is a page that is not there: seen by nobody, never written, so the
 pages that a window has left behind can be given back.  There is no backward.
 
-A compiled program makes these calls between its graphs (``fullgraph=True`` refuses them).
+A compiled program makes these calls between its graphs (``fullgraph=True`` refuses them); in a traced one, and to a
+dispatch mode, they are the operators ``ring_swa::cache_append``, ``cache_attn``, ``cache_weights`` and ``cache_evict``.
 """
 from __future__ import annotations
 
@@ -89,6 +90,24 @@ def _uncompiled(call, *args, **kwargs):
     return call(*args, **kwargs)
 
 
+# What the native module leaves to Python goes through operators that PyTorch knows, so that whatever looks on (a
+# tracer, a dispatch mode) sees one operation with what it reads and writes, and not a launch behind its back.
+_ops = torch.library.Library("ring_swa", "DEF")
+_CACHE = "Tensor k, Tensor v, Tensor k_scale, Tensor v_scale"
+_WRITTEN_CACHE = "Tensor(a!) k, Tensor(b!) v, Tensor(c!) k_scale, Tensor(d!) v_scale"
+
+
+def _operator(schema, fake):
+    """Registers the function under it: ``schema``, and ``fake`` for tensors without data."""
+    def register(fn):
+        name = schema[:schema.index("(")]
+        _ops.define(schema)
+        _ops.impl(name, fn, "CompositeExplicitAutograd")
+        torch.library.register_fake("ring_swa::" + name, fake, lib=_ops)
+        return getattr(torch.ops.ring_swa, name)
+    return register
+
+
 def _no_grad(*tensors) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError("the cache has no backward: call this under torch.no_grad()")
@@ -142,14 +161,26 @@ def _strides3(t: torch.Tensor, packed: bool):
     return (0, st[0], st[1]) if packed else st[:3]
 
 
+def _window(window_size) -> int:
+    return max(-1, min(int(window_size), 1 << 28))  # (2^28 is unbounded)
+
+
+def _sinks(num_sink_tokens) -> int:
+    return min(int(num_sink_tokens), 1 << 28)
+
+
+def _scale(softmax_scale) -> Optional[float]:
+    return None if softmax_scale is None else float(softmax_scale)
+
+
 def _query_params(p, q, heads_kv, softmax_scale, window_size, num_sink_tokens, packed):
     assert q.shape[-2] % heads_kv == 0, "Number of query heads must be divisible by number of key/value heads"
     assert q.stride(-1) == 1, "last dimension must be contiguous"
     assert num_sink_tokens >= 0
     p.heads_q = q.shape[-2]
     p.softmax_scale = float(q.shape[-1] ** (-0.5) if softmax_scale is None else softmax_scale)
-    p.window_left = max(-1, min(int(window_size), 1 << 28))
-    p.num_sink = min(int(num_sink_tokens), 1 << 28)
+    p.window_left = _window(window_size)
+    p.num_sink = _sinks(num_sink_tokens)
     p.q, p.q_stride = q.data_ptr(), _strides3(q, packed)
 
 
@@ -176,14 +207,20 @@ def kv_cache_append(
     if calls is not None and calls.cache_append(cache, k, v, page_table, seqlens, cu_seqlens):
         return
     _no_grad(k, v)
-    p, dev = _cache_params(cache, page_table, seqlens, k, cu_seqlens)
-    assert k.shape == v.shape and k.dtype == v.dtype, "k and v must have the same shape and dtype"
-    assert k.shape[-2] == p.heads_kv, "k and v must have the cache's heads"
-    _lib.require_device(k, v)
-    assert k.stride(-1) == 1 and v.stride(-1) == 1, "last dimension must be contiguous"
+    _append(*cache, k, v, page_table, seqlens, cu_seqlens)
+
+
+@_operator(f"cache_append({_WRITTEN_CACHE}, Tensor new_k, Tensor new_v, Tensor page_table, Tensor seqlens, "
+           "Tensor? cu_seqlens) -> ()", lambda *_: None)
+def _append(k, v, k_scale, v_scale, new_k, new_v, page_table, seqlens, cu_seqlens):
+    p, dev = _cache_params((k, v, k_scale, v_scale), page_table, seqlens, new_k, cu_seqlens)
+    assert new_k.shape == new_v.shape and new_k.dtype == new_v.dtype, "k and v must have the same shape and dtype"
+    assert new_k.shape[-2] == p.heads_kv, "k and v must have the cache's heads"
+    _lib.require_device(new_k, new_v)
+    assert new_k.stride(-1) == 1 and new_v.stride(-1) == 1, "last dimension must be contiguous"
     packed = cu_seqlens is not None
-    p.new_k, p.new_v = k.data_ptr(), v.data_ptr()
-    p.new_k_stride, p.new_v_stride = _strides3(k, packed), _strides3(v, packed)
+    p.new_k, p.new_v = new_k.data_ptr(), new_v.data_ptr()
+    p.new_k_stride, p.new_v_stride = _strides3(new_k, packed), _strides3(new_v, packed)
     _lib.launch(dev, _lib.lib().rswa_cache_append, p)
 
 
@@ -219,22 +256,36 @@ def kv_cache_attn(
         if got is not None:
             return got
     _no_grad(q)
-    p, dev = _cache_params(cache, page_table, seqlens, q, cu_seqlens)
+    out, lse = _attn(q, *cache, page_table, seqlens, _window(window_size), cu_seqlens, _scale(softmax_scale),
+                     _sinks(num_sink_tokens), bool(return_lse))
+    return (out, lse) if return_lse else out
+
+
+def _results(q, packed, return_lse):
+    out = q.new_empty(q.shape)
+    if not return_lse:
+        return out, q.new_empty(0, dtype=torch.float32)
+    qs = q.shape
+    return out, q.new_empty((qs[1], qs[0]) if packed else (qs[0], qs[2], qs[1]), dtype=torch.float32)
+
+
+@_operator(f"cache_attn(Tensor q, {_CACHE}, Tensor page_table, Tensor seqlens, int window_size, Tensor? cu_seqlens, "
+           "float? softmax_scale, int num_sink_tokens, bool return_lse) -> (Tensor, Tensor)",
+           lambda q, *rest: _results(q, rest[7] is not None, rest[10]))
+def _attn(q, k, v, k_scale, v_scale, page_table, seqlens, window_size, cu_seqlens, softmax_scale, num_sink_tokens,
+          return_lse):
+    """(``lse`` is an empty tensor where it is not wanted)"""
+    p, dev = _cache_params((k, v, k_scale, v_scale), page_table, seqlens, q, cu_seqlens)
     packed = cu_seqlens is not None
     _query_params(p, q, p.heads_kv, softmax_scale, window_size, num_sink_tokens, packed)
-    out = q.new_empty(q.shape)
-    lse = None
-    if return_lse:
-        qs = q.shape
-        lse = q.new_empty((qs[1], qs[0]) if packed else (qs[0], qs[2], qs[1]), dtype=torch.float32)
+    out, lse = _results(q, packed, return_lse)
     if q.numel() > 0:
         if p.max_pages == 0:  # no keys at all
             out.zero_()
-            if lse is not None:
-                lse.fill_(float("-inf"))
-            return (out, lse) if return_lse else out
+            lse.fill_(float("-inf"))
+            return out, lse
         p.out, p.out_stride = out.data_ptr(), _strides3(out, packed)
-        if lse is not None:
+        if return_lse:
             p.lse, p.lse_stride = lse.data_ptr(), _strides3(lse, packed)
         L = _lib.lib()
         size = int(L.rswa_cache_attn_workspace_bytes(p))
@@ -242,7 +293,7 @@ def kv_cache_attn(
             workspace = q.new_empty(size, dtype=torch.uint8)
             p.workspace, p.workspace_bytes = workspace.data_ptr(), size
         _lib.launch(dev, L.rswa_cache_attn, p)
-    return (out, lse) if return_lse else out
+    return out, lse
 
 
 def kv_cache_weights(
@@ -271,21 +322,29 @@ def kv_cache_weights(
                                                  softmax_scale, num_sink_tokens):
         return
     _no_grad(q)
-    p, dev = _cache_params(cache, page_table, seqlens, q, cu_seqlens)
+    _weights(weights, q, *cache, page_table, seqlens, lse, _window(window_size), cu_seqlens, _scale(softmax_scale),
+             _sinks(num_sink_tokens))
+
+
+@_operator(f"cache_weights(Tensor(a!) weights, Tensor q, {_CACHE}, Tensor page_table, Tensor seqlens, Tensor lse, "
+           "int window_size, Tensor? cu_seqlens, float? softmax_scale, int num_sink_tokens) -> ()", lambda *_: None)
+def _weights(weights, q, k, v, k_scale, v_scale, page_table, seqlens, lse, window_size, cu_seqlens, softmax_scale,
+             num_sink_tokens):
+    p, dev = _cache_params((k, v, k_scale, v_scale), page_table, seqlens, q, cu_seqlens)
     packed = cu_seqlens is not None
     _query_params(p, q, p.heads_kv, softmax_scale, window_size, num_sink_tokens, packed)
     qs = q.shape
     assert lse.dtype == torch.float32 and tuple(lse.shape) == (
         (qs[1], qs[0]) if packed else (qs[0], qs[2], qs[1])), (
         "lse must be fp32 [batch, heads, seq] ([heads, tokens] when packed)")
-    _weights_params(p, cache, weights)
+    _weights_params(p, k, weights)
     _lib.require_device(q, lse)
     if q.numel() > 0 and p.max_pages > 0:
         p.lse, p.lse_stride = lse.data_ptr(), _strides3(lse, packed)
         _lib.launch(dev, _lib.lib().rswa_cache_weights, p)
 
 
-def _weights_params(p, cache, weights):
+def _weights_params(p, k, weights):
     assert weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (p.batch, p.heads_kv), (
         "weights must be fp32 [batch, kv_heads, n]")
     assert _dense_from(weights, 2), "last dimension must be contiguous"
@@ -293,7 +352,7 @@ def _weights_params(p, cache, weights):
     for size, step in sorted(zip(weights.shape[:2], weights.stride()), key=lambda d: d[1]):
         assert size <= 1 or step >= span, "the sums of different heads overlap"
         span += max(0, size - 1) * step
-    _lib.require_device(cache.k, weights)
+    _lib.require_device(k, weights)
     p.weights, p.weights_stride, p.weights_len = weights.data_ptr(), weights.stride()[:2], weights.shape[2]
 
 
@@ -329,16 +388,27 @@ def kv_cache_evict(
             return got
     assert budget > 0 and num_sink_tokens >= 0 and num_recent >= 0
     assert num_sink_tokens + num_recent <= budget, "budget must hold the sinks and the recent tokens"
-    p, dev = _cache_params(cache, page_table, seqlens, None, None)
-    _weights_params(p, cache, weights)
+    return _evict(*cache, weights, page_table, seqlens, new_page_table, int(budget), int(num_sink_tokens), int(num_recent))
+
+
+def _cut(weights, seqlens, heads, budget):
+    """Lengths, weights and numbers of what stays."""
+    return (torch.empty_like(seqlens), weights.new_empty(weights.shape),
+            seqlens.new_empty((seqlens.shape[0], heads, budget)))
+
+
+@_operator(f"cache_evict({_WRITTEN_CACHE}, Tensor weights, Tensor page_table, Tensor seqlens, Tensor new_page_table, "
+           "int budget, int num_sink_tokens, int num_recent) -> (Tensor, Tensor, Tensor)",
+           lambda k, v, ks, vs, weights, table, seqlens, new, budget, *_: _cut(weights, seqlens, k.shape[1], budget))
+def _evict(k, v, k_scale, v_scale, weights, page_table, seqlens, new_page_table, budget, num_sink_tokens, num_recent):
+    p, dev = _cache_params((k, v, k_scale, v_scale), page_table, seqlens, None, None)
+    _weights_params(p, k, weights)
     assert new_page_table.dim() == 2 and new_page_table.dtype == torch.int32 and \
         new_page_table.shape[0] == p.batch, "new_page_table must be int32 [batch, n]"
     assert _dense_from(new_page_table, 1), "the entries of a row of new_page_table must be adjacent"
-    _lib.require_device(cache.k, new_page_table)
-    new_seqlens = torch.empty_like(seqlens)
-    new_weights = weights.new_empty(weights.shape)
-    kept = seqlens.new_empty(p.batch, p.heads_kv, int(budget))
-    p.num_sink, p.num_recent, p.budget = int(num_sink_tokens), int(num_recent), int(budget)
+    _lib.require_device(k, new_page_table)
+    new_seqlens, new_weights, kept = _cut(weights, seqlens, p.heads_kv, budget)
+    p.num_sink, p.num_recent, p.budget = num_sink_tokens, num_recent, budget
     p.new_page_table, p.new_page_table_stride = new_page_table.data_ptr(), new_page_table.stride(0)
     p.new_max_pages = new_page_table.shape[1]
     p.new_seqlens, p.new_weights, p.kept = new_seqlens.data_ptr(), new_weights.data_ptr(), kept.data_ptr()

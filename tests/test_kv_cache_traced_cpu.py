@@ -1,9 +1,11 @@
-"""The cache's calls in compiled programs, without a GPU: they are made between the graphs.  The launch itself is a stub
-that writes what can be told apart."""
+"""The cache's calls in compiled and traced programs, without a GPU: a compiled program makes them between its graphs,
+and in a traced one each is an operation, whose run makes the launch.  The launch itself is a stub that writes what can
+be told apart."""
 import ctypes
 
 import pytest
 import torch
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import ring_swa
 from ring_swa import KVCache, _lib
@@ -91,6 +93,35 @@ def test_compiled(call, backend, launches):
     run = torch.compile(program(call), backend=backend)
     for _ in range(2):
         check(call, run, launches)
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_traced(call, launches):
+    run = torch.jit.trace(program(call), inputs(), check_trace=False)
+    assert "ring_swa::cache_" + call.split("_")[0] in str(run.graph)
+    check(call, run, launches)
+
+
+@pytest.mark.parametrize("mode", ["real", "fake"])
+@pytest.mark.parametrize("call", CALLS)
+def test_traced_by_dispatch(call, mode, launches):
+    run = make_fx(program(call), tracing_mode=mode)(*inputs())
+    check(call, run, launches)
+
+
+def test_a_mode_sees_the_call(launches):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Mode(TorchDispatchMode):
+        seen = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            Mode.seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    with Mode():
+        program("attn")(*inputs())
+    assert "ring_swa.cache_attn.default" in Mode.seen and launches == ["rswa_cache_attn"]
 
 
 def test_a_program_of_one_graph_is_refused(launches):

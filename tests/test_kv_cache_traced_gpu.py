@@ -1,4 +1,4 @@
-"""A step of the cache's calls compiled: the eager step's bits, on other inputs."""
+"""A step of the cache's calls compiled and traced: the eager step's bits, on inputs that were not traced."""
 import pytest
 import torch
 
@@ -39,3 +39,13 @@ def check(run):
 def test_compiled(backend):
     torch._dynamo.reset()
     check(torch.compile(step, backend=backend))
+
+
+def test_traced():
+    check(torch.jit.trace(step, inputs(2), check_trace=False))
+
+
+def test_traced_by_dispatch():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    check(make_fx(step)(*inputs(2)))
