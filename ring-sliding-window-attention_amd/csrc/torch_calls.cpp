@@ -305,6 +305,9 @@ const Tensor* given(PyObject* o) {
   return plain(t) ? &t : nullptr;
 }
 
+// (the calls have no backward: the Python route says so)
+bool needs_grad(const Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+
 // Dimensions from `from` on without gaps?  (A stride over one element is never used.)
 bool dense_from(const Tensor& t, int64_t from) {
   int64_t step = 1;
@@ -332,7 +335,7 @@ struct CacheCall {
     if (!PyTuple_Check(cache) || PyTuple_GET_SIZE(cache) != 4) return false;
     const Tensor* c[4];
     for (int i = 0; i < 4; i++)
-      if (!(c[i] = given(PyTuple_GET_ITEM(cache, i)))) return false;
+      if (!(c[i] = given(PyTuple_GET_ITEM(cache, i))) || needs_grad(*c[i])) return false;
     const Tensor *table = given(table_o), *lens = given(lens_o);
     if (!table || !lens) return false;
     const Tensor &k = *c[0], &v = *c[1];
@@ -377,7 +380,7 @@ struct CacheCall {
   bool rows(const Tensor& t, PyObject* cu_o) {
     const auto type = t.scalar_type();
     if (type != at::kBFloat16 && type != at::kHalf) return false;
-    if (c10::GradMode::is_enabled() && t.requires_grad()) return false;
+    if (needs_grad(t)) return false;
     packed = cu_o != Py_None;
     if (t.dim() != (packed ? 3 : 4) || t.size(-1) != p.head_dim || t.stride(-1) != 1 || t.device() != device)
       return false;
@@ -415,7 +418,7 @@ struct CacheCall {
 
   bool running_sums(const Tensor* w) {
     if (!w || w->scalar_type() != at::kFloat || w->dim() != 3 || w->size(0) != p.batch || w->size(1) != p.heads_kv ||
-        !dense_from(*w, 2) || w->device() != device || w->size(2) >= INT32_MAX)
+        !dense_from(*w, 2) || w->device() != device || w->size(2) >= INT32_MAX || needs_grad(*w))
       return false;
     int64_t span = w->size(2);  // of what the inner of the two strides has walked over
     const int inner = w->stride(0) < w->stride(1) ? 0 : 1;
@@ -446,7 +449,7 @@ PyObject* cache_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Tensor *k = given(args[1]), *v = given(args[2]);
   if (!k || !v || !c.set(args[0], args[3], args[4]) || !c.rows(*k, args[5])) Py_RETURN_NONE;
   if (v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type() || v->device() != c.device || v->stride(-1) != 1 ||
-      k->size(-2) != c.p.heads_kv || (c10::GradMode::is_enabled() && v->requires_grad()))
+      k->size(-2) != c.p.heads_kv || needs_grad(*v))
     Py_RETURN_NONE;
   c.p.new_k = k->data_ptr();
   c.p.new_v = v->data_ptr();
@@ -495,7 +498,7 @@ PyObject* cache_weights(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 10 || !cache_lib.weights || observed()) Py_RETURN_NONE;
   const Tensor *q = given(args[0]), *lse = given(args[4]);
   if (!q || !lse || !c.set(args[1], args[2], args[3]) || !c.queries(*q, args[7], args[6], args[8], args[9]) ||
-      !c.running_sums(given(args[5])) || !lse_of(*lse, *q, c.packed))
+      !c.running_sums(given(args[5])) || !lse_of(*lse, *q, c.packed) || needs_grad(*lse))
     Py_RETURN_NONE;
   c.p.lse = (float*)lse->data_ptr();
   strides3(c.p.lse_stride, *lse, c.packed);

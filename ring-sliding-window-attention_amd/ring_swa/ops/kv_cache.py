@@ -206,7 +206,7 @@ def kv_cache_append(
     calls = _calls(cache)
     if calls is not None and calls.cache_append(cache, k, v, page_table, seqlens, cu_seqlens):
         return
-    _no_grad(k, v)
+    _no_grad(*cache, k, v)
     _append(*cache, k, v, page_table, seqlens, cu_seqlens)
 
 
@@ -255,7 +255,7 @@ def kv_cache_attn(
                                num_sink_tokens, return_lse)
         if got is not None:
             return got
-    _no_grad(q)
+    _no_grad(*cache, q)
     out, lse = _attn(q, *cache, page_table, seqlens, _window(window_size), cu_seqlens, _scale(softmax_scale),
                      _sinks(num_sink_tokens), bool(return_lse))
     return (out, lse) if return_lse else out
@@ -321,7 +321,7 @@ def kv_cache_weights(
     if calls is not None and calls.cache_weights(q, cache, page_table, seqlens, lse, weights, window_size, cu_seqlens,
                                                  softmax_scale, num_sink_tokens):
         return
-    _no_grad(q)
+    _no_grad(*cache, q, lse, weights)
     _weights(weights, q, *cache, page_table, seqlens, lse, _window(window_size), cu_seqlens, _scale(softmax_scale),
              _sinks(num_sink_tokens))
 
@@ -388,6 +388,7 @@ def kv_cache_evict(
             return got
     assert budget > 0 and num_sink_tokens >= 0 and num_recent >= 0
     assert num_sink_tokens + num_recent <= budget, "budget must hold the sinks and the recent tokens"
+    _no_grad(*cache, weights)
     return _evict(*cache, weights, page_table, seqlens, new_page_table, int(budget), int(num_sink_tokens), int(num_recent))
 
 
