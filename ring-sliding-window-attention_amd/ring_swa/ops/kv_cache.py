@@ -34,6 +34,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -111,6 +112,8 @@ def _operator(schema, fake):
 def _no_grad(*tensors) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError("the cache has no backward: call this under torch.no_grad()")
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors if t.is_floating_point()):
+        raise RuntimeError("the cache has no forward derivative: call this on tensors without tangents")
 
 
 def _cache_params(cache, page_table, seqlens, rows, cu_seqlens):

@@ -1,6 +1,7 @@
-"""The cache's calls have no backward: every floating-point input that needs a gradient is refused."""
+"""The cache's calls have no derivative: every floating-point input that wants one is refused, in both directions."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import ring_swa
 from ring_swa import KVCache, _lib
@@ -48,6 +49,16 @@ def test_tensors_that_need_a_gradient(call, name):
         run(call, x)
 
 
+@pytest.mark.parametrize("call,name", [i for i in INPUTS if i[1] not in KVCache._fields])
+def test_tensors_with_a_tangent(call, name):
+    x = inputs()
+    with forward_ad.dual_level():
+        run(call, x)
+        x[name] = forward_ad.make_dual(x[name].detach(), torch.ones_like(x[name]))
+        with pytest.raises(RuntimeError, match="no forward derivative"):
+            run(call, x)
+
+
 def test_transforms():
     def attn(q):
         return run("attn", dict(inputs(), q=q)).float().sum()
@@ -55,5 +66,7 @@ def test_transforms():
     q = inputs()["q"].detach()
     with pytest.raises(RuntimeError, match="no backward"):
         torch.func.grad(attn)(q)
+    with pytest.raises(RuntimeError, match="no forward derivative"):
+        torch.func.jvp(attn, (q,), (torch.ones_like(q),))
     with pytest.raises(RuntimeError):
         torch.func.jacrev(attn)(q)
