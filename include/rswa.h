@@ -354,7 +354,8 @@ int rswa_attn_fwd_blocks_per_cu(const rswa_attn_params* p);
  * Queries are the last rows of their sequence: row i of n is token seqlens[b] - n + i and sees the keys of tokens
  *   j <= seqlens[b] - n + i  and  (window_left < 0  or  j >= seqlens[b] - n + i - window_left  or  j < num_sink)
  * which is the rule of rswa_attn_fwd with causal != 0, bottom-right aligned.  Rows that see nothing: out = 0,
- * lse = -inf.  A NaN reaches the results that the formula takes it into and no others.  Dense rows are
+ * lse = -inf.  A NaN, or a value that is infinite to q, reaches the results that the formula takes it into (which are
+ * infinite or NaN: a weight too small for its type times infinity is NaN) and no others.  Dense rows are
  * [batch, seqlen_q, heads, head_dim]; with cu_seqlens_q (int32, batch + 1 entries on the device) [total_q, heads,
  * head_dim], and rows ahead of cu_seqlens_q[0] and behind cu_seqlens_q[batch] are left alone.
  */

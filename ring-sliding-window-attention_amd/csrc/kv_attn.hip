@@ -107,23 +107,37 @@ __device__ __forceinline__ u32x4 seen_bytes(const CacheArgs& a, int j, bool here
   return keep;
 }
 
-// A value that is NaN makes those rows NaN that see its key, and no others; but a weight of zero does not cancel it.  So
-// in tiles that some rows see and others do not, the product is taken without such values, and where there were any,
-// spoil() below gives them to their rows afterwards.  (In the loop there are no registers for that.)
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {  // 0xff for each byte that is NaN
-  const uint32_t h = ((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-  return h | (h - (h >> 7));
+// A value that is not finite -- NaN, or a code whose value the type of the queries holds as infinite -- makes those rows
+// not finite that see its key, and no others; but a weight of zero does not cancel it.  So in tiles that some rows see and
+// others do not, the product is taken without such values, and where there were any, spoil() below gives them to their
+// rows afterwards.  (In the loop there are no registers for that.)
+//
+// Half the value of a code of exponent field E at scale byte e is of exponent E + e - 135 and infinite from the type's
+// largest exponent + 1 on (four significant bits: nothing lies between the largest finite value and that power of two).
+// Codes below E = 1 are m * 2^-9 and reach E = 0 with m = 4, E = -1 with 2, E = -2 with 1.  Returned for each byte: 128
+// less the least magnitude that is not finite, so that adding a magnitude carries into the byte's highest bit from there on.
+template <typename T>
+__device__ __forceinline__ uint32_t special_from(int e) {
+  const int n = (std::is_same_v<T, __bf16> ? 128 : 16) + 135 - e;
+  const int least = n > 0 ? min(8 * n, 0x7f) : 4 >> min(-n, 2);
+  return (uint32_t)(0x80 - least) * 0x01010101u;
+}
+__device__ __forceinline__ uint32_t spread(uint32_t highest) {  // bytes' highest bits to all of their bits
+  return highest | (highest - (highest >> 7));
+}
+__device__ __forceinline__ uint32_t special_bytes(uint32_t codes, uint32_t from) {
+  return spread(((codes & 0x7f7f7f7fu) + from) & 0x80808080u);
 }
 template <int N>
-__device__ __forceinline__ bool take_out_nan(u32x4 (&codes)[N]) {
+__device__ __forceinline__ bool take_out_special(u32x4 (&codes)[N], uint32_t from) {
   uint32_t any = 0;
 #pragma unroll
   for (int d = 0; d < N; d++)
 #pragma unroll
     for (int q = 0; q < 4; q++) {
-      const uint32_t nan = nan_bytes(codes[d][q]);
-      codes[d][q] &= ~nan;
-      any |= nan;
+      const uint32_t special = special_bytes(codes[d][q], from);
+      codes[d][q] &= ~special;
+      any |= special;
     }
   return __builtin_amdgcn_ballot_w64(any != 0) != 0;
 }
@@ -232,8 +246,9 @@ struct Rows {
   }
 };
 
-// NaN for the rows that see a NaN among the values of tiles i, i + step, .., of those that rows at positions
-// first .. last do not all see: a product of ones, 1 where a value is NaN and 1 where a row sees its key.
+// What take_out_special() left out of tiles i, i + step, .., of those that rows at positions first .. last do not all
+// see, for the rows that see it: two products of ones, 1 where a value is positive (negative) and infinite, or NaN, and 1
+// where a row sees its key.  A row that has both is NaN.
 template <typename T, int D, int NT>
 __device__ __forceinline__ void spoil(const CacheArgs& a, Rows<T, D, NT>& w, const Keys<D>& keys, const TileList& list,
                                       int i, int step, int first, int last) {
@@ -260,20 +275,38 @@ __device__ __forceinline__ void spoil(const CacheArgs& a, Rows<T, D, NT>& w, con
       }
     }
     const uint8_t* const from = keys.values(tile, id);
+    const uint32_t specials = special_from<T>(keys.value_scale(id));
 #pragma unroll
     for (int d = 0; d < Rows<T, D, NT>::ND; d++) {
       const u32x4 codes = *(const u32x4*)(from + d * 256);
-      V8 nan[2];
+      V8 up[2], down[2];  // (0x38 is the code of 1)
 #pragma unroll
-      for (int h = 0; h < 2; h++)  // (0x38 is the code of 1)
-        nan[h] = widen8<T>(nan_bytes(codes[2 * h]) & 0x38383838u, nan_bytes(codes[2 * h + 1]) & 0x38383838u, 1.f);
+      for (int h = 0; h < 2; h++) {
+        uint32_t u[2], n[2];
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+          const uint32_t c = codes[2 * h + q], below = spread(c & 0x80808080u);
+          const uint32_t special = special_bytes(c, specials), nan = special_bytes(c, 0x01010101u);
+          u[q] = ((special & ~below) | nan) & 0x38383838u;
+          n[q] = ((special & below) | nan) & 0x38383838u;
+        }
+        up[h] = widen8<T>(u[0], u[1], 1.f);
+        down[h] = widen8<T>(n[0], n[1], 1.f);
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
-        f32x4 of = {0, 0, 0, 0};
+        f32x4 ups = {0, 0, 0, 0}, downs = {0, 0, 0, 0};
 #pragma unroll
-        for (int h = 0; h < 2; h++) of = Mma<T>::mfma16(nan[h], sees[nt][h], of);
+        for (int h = 0; h < 2; h++) {
+          ups = Mma<T>::mfma16(up[h], sees[nt][h], ups);
+          downs = Mma<T>::mfma16(down[h], sees[nt][h], downs);
+        }
 #pragma unroll
-        for (int e = 0; e < 4; e++) w.acc[d][nt][e] = of[e] > 0.f ? __builtin_nanf("") : w.acc[d][nt][e];
+        for (int e = 0; e < 4; e++) {
+          float o = w.acc[d][nt][e];
+          o = ups[e] > 0.f ? o + __builtin_inff() : o;
+          w.acc[d][nt][e] = downs[e] > 0.f ? o - __builtin_inff() : o;
+        }
       }
     }
   }
@@ -397,12 +430,12 @@ __global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(c
     w.tops(s, top);
     w.raise(top);
     w.weigh(s, pf);
-    // what no row of the wave sees may hold anything, NaN codes included: a weight of zero does not cancel those
+    // what no row of the wave sees may hold anything, NaN and infinities included: a weight of zero does not cancel those
     if (!whole) {
       const u32x4 keep = seen_bytes(a, j0 + hi * 16, here, w.first, w.last);
 #pragma unroll
       for (int d = 0; d < ND; d++) vb[d] &= keep;
-      if (w.first != w.last) spoiled |= take_out_nan(vb);
+      if (w.first != w.last) spoiled |= take_out_special(vb, special_from<T>(ve));
     }
     const float vscale = half_scale(ve);
 #pragma unroll
@@ -471,7 +504,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
   constexpr int C = R::C, ND = R::ND, NV = ND / 4;
   constexpr int KF = 4 * C * 2, VF = ND * 2;  // operands of a tile
   __shared__ V8 k_ops[2][KF][64], v_ops[2][VF][64];
-  __shared__ uint32_t any_nan;
+  __shared__ uint32_t any_special;
 
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int col = lane & 15, hi = lane >> 4;
@@ -511,7 +544,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
 #pragma unroll
       for (int h = 0; h < 2; h++) to[(wave * C + c) * 2 + h][lane] = widen8<T>(kb[c][2 * h], kb[c][2 * h + 1], f);
   };
-  // (what no row of the block sees may hold anything, NaN codes included: a weight of zero does not cancel those)
+  // (what no row of the block sees may hold anything, NaN and infinities included: a weight of zero does not cancel those)
   bool spoiled = false;
   auto prepare_v = [&](int tile, int id) {
     const int j0 = tile * kTileKeys;
@@ -520,7 +553,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
     const u32x4 keep = seen_bytes(a, j0 + hi * 16, here, first, last);
 #pragma unroll
     for (int d = 0; d < NV; d++) vb[d] &= keep;
-    spoiled |= take_out_nan(vb);
+    spoiled |= take_out_special(vb, special_from<T>(ve));
   };
   auto widen_v = [&](V8 (&to)[VF][64]) {
     const float f = half_scale(ve);
@@ -571,7 +604,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
     load_v(tile_at(1), p[1].v);
     widen_k(k_ops[1]);
     load_k(tile_at(2), p[2].k);
-    if (threadIdx.x == 0) any_nan = 0;
+    if (threadIdx.x == 0) any_special = 0;
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < 2; h++) kf[0][h] = k_ops[0][h][lane];
@@ -650,9 +683,9 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
   }
   const CacheArgs& late = arguments_again();
   if (n > 0) {  // (each wave has looked at its quarter of the values)
-    if (spoiled && lane == 0) any_nan = 1;
+    if (spoiled && lane == 0) any_special = 1;
     __syncthreads();
-    if (__builtin_amdgcn_readfirstlane(any_nan)) spoil(late, w, keys, list, 0, 1, first, last);
+    if (__builtin_amdgcn_readfirstlane(any_special)) spoil(late, w, keys, list, 0, 1, first, last);
   }
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {

@@ -245,10 +245,10 @@ def kv_cache_attn(
     fp16.  ``seqlens`` counts all tokens of a sequence, those of ``q`` among them.  Each query sees its
     own token and the ``window_size`` before it (negative: all) and the first ``num_sink_tokens``.
     Codes are read in the type of ``q``: what bf16 rows have written beyond fp16's range is infinite to
-    fp16 queries.  A NaN reaches the rows that see it and no others.  Rows ahead of a pack's first
-    sequence and behind its last are not written.  Returns the output, shape and dtype of ``q``, and with ``return_lse`` the log-sum-exp, fp32
-    ``[batch, heads, seq]`` (``[heads, tokens]`` of a pack), as ``merge_attn_out`` takes it.  Rows that
-    see nothing: 0 and ``-inf``."""
+    fp16 queries.  A NaN or an infinite value reaches the rows that see it and no others.  Rows ahead of
+    a pack's first sequence and behind its last are not written.  Returns the output, shape and dtype of
+    ``q``, and with ``return_lse`` the log-sum-exp, fp32 ``[batch, heads, seq]`` (``[heads, tokens]`` of a
+    pack), as ``merge_attn_out`` takes it.  Rows that see nothing: 0 and ``-inf``."""
     if torch.compiler.is_dynamo_compiling():
         return _uncompiled(kv_cache_attn, q, cache, page_table, seqlens, window_size, cu_seqlens, softmax_scale,
                            num_sink_tokens=num_sink_tokens, return_lse=return_lse)
