@@ -443,10 +443,12 @@ int rswa_cache_weights(const rswa_cache_params* p, void* stream);
 /*
  * Cuts every sequence to at most `budget` tokens, for each kv head by itself: kept are the first num_sink, the last
  * num_recent, and of the others those with the largest weights (equal ones: the earlier; NaN: as the least), in their
- * order.  (Tokens from weights_len on weigh 0.)  Their codes go to the pages of new_page_table, from place 0 on, at the
- * scale that fits the values in each new page; new_seqlens[b] = min(seqlens[b], budget); new_weights gets their weights, zeros behind; kept gets the tokens'
- * old numbers, -1 behind.  The old pages are only read (they may be shared with other sequences); a page may not be
- * old and new, or new for two sequences.  num_sink + num_recent <= budget.
+ * order.  (Tokens from weights_len on weigh 0.)  Tokens whose page is not there are not kept.  The kept ones' codes go to
+ * the pages of new_page_table, from place 0 on, at the scale that fits the values in each new page; new_seqlens[b] is
+ * their number, the lesser of budget and of the tokens whose page is there; new_weights gets their weights, zeros behind;
+ * kept gets the tokens' old numbers, -1 behind.  The old pages are only read (they may be shared with other sequences);
+ * a page may not be old and new, or new for two sequences.
+ * num_sink + num_recent <= budget.
  */
 int rswa_cache_evict(const rswa_cache_params* p, void* stream);
 

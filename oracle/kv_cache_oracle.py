@@ -195,17 +195,20 @@ def evict(cache, running, page_table, seqlens, new_page_table, budget, sinks=0, 
     kept = torch.full((batch, heads, budget), -1, dtype=torch.int32)
     new_weights = torch.zeros(running.shape, dtype=torch.float32)
     target = new_page_table.tolist()
-    lens = seqlens.tolist()
-    for b, n in enumerate(lens):
+    count = torch.zeros(batch, dtype=torch.int32)
+    for b, (n, row) in enumerate(zip(seqlens.tolist(), page_table.tolist())):
+        n = max(0, min(n, len(row) * size))
+        there = [j for j in range(n) if 0 <= row[j // size] < pages]  # (tokens without a page are not kept)
+        count[b] = min(len(there), budget)
         for h in range(heads):
             w = running[b, h].tolist() + [0.0] * max(0, n - width)
-            if n <= budget:
-                keep = list(range(n))
+            if len(there) <= budget:
+                keep = there
             else:
-                must = set(range(sinks)) | set(range(n - recent, n))
-                rest = sorted((j for j in range(n) if j not in must),
+                must = [j for j in there if j < sinks or j >= n - recent]
+                rest = sorted((j for j in there if sinks <= j < n - recent),
                               key=lambda j: (math.isnan(w[j]), -w[j] if not math.isnan(w[j]) else 0.0, j))
-                keep = sorted(list(must) + rest[:budget - len(must)])
+                keep = sorted(must + rest[:budget - len(must)])
             tokens = torch.tensor(keep, dtype=torch.long, device=page_table.device)
             kept[b, h, :len(keep)] = torch.tensor(keep, dtype=torch.int32)
             for r, j in enumerate(keep):
@@ -224,5 +227,4 @@ def evict(cache, running, page_table, seqlens, new_page_table, budget, sinks=0, 
                     mine[:part.shape[0]] = encode(part * 2.0 ** (127 - byte))
                     _put_page_rows(codes, which, page, h, mine)
                     codes[2 + which][page, h] = byte
-    count = torch.tensor([min(n, budget) for n in lens], dtype=torch.int32)
     return out, count, new_weights, kept

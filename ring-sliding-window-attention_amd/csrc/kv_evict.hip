@@ -43,31 +43,26 @@ __global__ __launch_bounds__(THREADS) void cache_select_kernel(const EvictArgs a
   __shared__ uint32_t list[LIST];
   __shared__ uint32_t listed;
   __shared__ uint32_t chosen[2];  // digit, how many are still to be found among its weights
-  __shared__ int count[WAVES][2];
+  __shared__ int count[WAVES][2], missing[WAVES][2];
   __shared__ uint32_t sums[WAVES];
   const CacheArgs& c = a.c;
   const int b = blockIdx.x / c.heads_kv, hk = blockIdx.x % c.heads_kv;
   const int len = held_tokens(c, c.lens[b]);
-  const int stay = min(len, a.budget);
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int32_t* const table = c.table + (int64_t)b * c.table_st;
   const float* w = c.weights + (int64_t)b * c.w_st[0] + (int64_t)hk * c.w_st[1];
   int32_t* kept = a.kept + (int64_t)blockIdx.x * a.budget;
   float* new_w = a.new_weights + (int64_t)blockIdx.x * c.w_len;
 
-  if (hk == 0 && threadIdx.x == 0) a.new_lens[b] = stay;
-  for (int r = stay + threadIdx.x; r < a.budget; r += THREADS) kept[r] = -1;
-  for (int r = stay + threadIdx.x; r < c.w_len; r += THREADS) new_w[r] = 0.f;  // (the others: see the move)
-  if (len <= a.budget) {
-    for (int j = threadIdx.x; j < len; j += THREADS) kept[j] = j;
-    return;
-  }
-  const int c0 = c.n_sink, c1 = len - a.n_recent;  // the others
-  int find = a.budget - c.n_sink - a.n_recent;     // of which so many stay
-  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  int c0 = c.n_sink, c1 = len - a.n_recent;  // the others
   const int steps = (len + THREADS - 1) / THREADS;
   const int p0 = wave * steps * 64 + lane;  // a lane's first token
   // (loads first and without branches, so that they are all in flight; tokens without a weight of their own have 0)
   const int last = max(0, c.w_len - 1);
   if (c.w_len == 0) w = (const float*)c.lens;  // (any place that can be read)
+  const int n_pages = (len + (1 << c.page_log2) - 1) >> c.page_log2;
+  auto there = [&](int id) { return (uint32_t)id < (uint32_t)c.num_pages; };
+  const int first_id = (int)threadIdx.x < n_pages ? table[threadIdx.x] : 0;
   auto load = [&](int i) { return w[min(p0 + i * 64, last)]; };
   auto number = [&](int i, float x) -> uint32_t {
     const int j = p0 + i * 64;
@@ -76,12 +71,50 @@ __global__ __launch_bounds__(THREADS) void cache_select_kernel(const EvictArgs a
     return j < len ? o : 0;
   };
   uint32_t mine[N];
-  float raw[N];
+  float raw[N] = {};
+  if (len > a.budget)
 #pragma unroll
-  for (int i0 = 0; i0 < N; i0 += 8)
-    if (i0 < steps)
+    for (int i0 = 0; i0 < N; i0 += 8)
+      if (i0 < steps)
 #pragma unroll
-      for (int i = i0; i < i0 + 8; i++) raw[i] = load(i);
+        for (int i = i0; i < i0 + 8; i++) raw[i] = load(i);
+
+  // Tokens whose page is not there are not kept: how many, and how many of them are sinks or recent ones.  (The table's
+  // entries are on their way together with the weights.)
+  int gone = 0, gone_stays = 0;
+  auto look = [&](int p, int id) {
+    if (there(id)) return;
+    const int lo = p << c.page_log2, hi = min(lo + (1 << c.page_log2), len);
+    gone += hi - lo;
+    gone_stays += max(0, min(hi, c0) - lo) + max(0, hi - max(lo, c1));  // (of use only where c0 <= c1)
+  };
+  if ((int)threadIdx.x < n_pages) look(threadIdx.x, first_id);
+  for (int p = threadIdx.x + THREADS; p < n_pages; p += THREADS) look(p, table[p]);
+  gone = wave_scan(gone);
+  gone_stays = wave_scan(gone_stays);
+  if (lane == 63) {
+    missing[wave][0] = gone;
+    missing[wave][1] = gone_stays;
+  }
+  __syncthreads();
+  gone = gone_stays = 0;
+#pragma unroll
+  for (int i = 0; i < WAVES; i++) {
+    gone += missing[i][0];
+    gone_stays += missing[i][1];
+  }
+  const int stay = min(len - gone, a.budget);
+  if (hk == 0 && threadIdx.x == 0) a.new_lens[b] = stay;
+  for (int r = stay + threadIdx.x; r < a.budget; r += THREADS) kept[r] = -1;
+  for (int r = stay + threadIdx.x; r < c.w_len; r += THREADS) new_w[r] = 0.f;  // (the others: see the move)
+  if (gone == 0 && len <= a.budget) {
+    for (int j = threadIdx.x; j < len; j += THREADS) kept[j] = j;
+    return;
+  }
+  const bool all = len - gone <= a.budget;  // all that are there
+  if (all) c0 = c1 = 0;
+  int find = all ? 0 : a.budget - (c.n_sink + a.n_recent - gone_stays);  // so many of the others stay
+
   for (int i = threadIdx.x; i < COPIES * BINS / 4; i += THREADS) ((u32x4*)hist)[i] = u32x4{0, 0, 0, 0};
   if (threadIdx.x == 0) listed = 0;
 #pragma unroll
@@ -89,6 +122,11 @@ __global__ __launch_bounds__(THREADS) void cache_select_kernel(const EvictArgs a
     if (i0 < steps)
 #pragma unroll
       for (int i = i0; i < i0 + 8; i++) mine[i] = i < steps ? number(i, raw[i]) : 0;
+  auto has_page = [&](int i) { return there(table[min(p0 + i * 64, len - 1) >> c.page_log2]); };
+  if (gone > 0)
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      if (i < steps && !has_page(i)) mine[i] = 0;
   // all of a wave's weights, eight steps without a branch at a time (those beyond its part are 0)
   auto each = [&](auto f) {
 #pragma unroll
@@ -96,10 +134,10 @@ __global__ __launch_bounds__(THREADS) void cache_select_kernel(const EvictArgs a
       if (i0 < steps)
 #pragma unroll
         for (int i = i0; i < i0 + 8; i++) f(i, mine[i]);
-    for (int i = N; i < steps; i++) f(i, number(i, load(i)));
+    for (int i = N; i < steps; i++) f(i, gone > 0 && !has_page(i) ? 0u : number(i, load(i)));
   };
 
-  uint32_t least = kStays - 1;  // above every weight: none of the others stays
+  uint32_t least = all ? 0 : kStays - 1;  // below every token's number, or above every weight: none of the others stays
   if (find > 0) {
     // the digit of the find-th largest, from the counts in so many copies
     auto choose = [&](int copies) {
@@ -241,7 +279,7 @@ __global__ __launch_bounds__(512, 4) void cache_move_kernel(const EvictArgs a) {
   const int page_size = 1 << c.page_log2;
   const int hk = blockIdx.x % c.heads_kv;
   const int b = blockIdx.x / c.heads_kv / a.new_max_pages, np = blockIdx.x / c.heads_kv % a.new_max_pages;
-  const int len = held_tokens(c, c.lens[b]), stay = min(len, a.budget);
+  const int len = held_tokens(c, c.lens[b]), stay = a.new_lens[b];
   const int r0 = np << c.page_log2;
   const int n_page = min(page_size, stay - r0);  // tokens of the page
   if (n_page <= 0) return;

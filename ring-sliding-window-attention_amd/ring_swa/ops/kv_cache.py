@@ -373,7 +373,8 @@ def kv_cache_evict(
     """Cut every sequence to at most ``budget`` tokens, for each kv head by itself.
 
     Kept are the first ``num_sink_tokens``, the last ``num_recent``, and of the others those with the
-    largest ``weights`` (of equal ones the earlier; NaN counts as the least), in their order.  They move
+    largest ``weights`` (of equal ones the earlier; NaN counts as the least), in their order.  Tokens whose
+    page is not there are not kept, and a sequence's new length does not count them.  The others move
     to the pages of ``new_page_table`` (int32 ``[batch, n]``, room for ``budget`` tokens), each page at the
     scale that fits its values; the old pages are only read, so that sequences may share them, and none
     of them may be among the new ones, nor a new one in two rows.  Tokens without a weight (``n`` below the
