@@ -801,7 +801,8 @@ Cut cut_call(const rswa_cache_params* p) {
   const int64_t at_most = std::min(ceil_div(8 * per_head, 5), c.row_tiles * most_tiles);
   // few tiles are not split: the join costs what a wave's third tile does (one token: 512 keys 8.0 us whole, 10.1 in two
   // launches, 768 9.2 / 10.2, 1024 10.5 / 10.3; own rows: 500 keys 21.9 / 25.2, 1000 33.2 / 32.7)
-  c.min_chunk = most_tiles <= (c.wr == 1 ? 12 : 8) ? (int)most_tiles : kMinChunk;
+  // (a table without columns has no tiles, and chunks of none could not be counted)
+  c.min_chunk = most_tiles <= (c.wr == 1 ? 12 : 8) ? std::max(1, (int)most_tiles) : kMinChunk;
   c.part_units = most_tiles <= c.min_chunk ? 0 : at_most;
   c.grid = (c.row_tiles + std::min(per_head, c.row_tiles * most_tiles)) * p->heads_kv;
   return c;
