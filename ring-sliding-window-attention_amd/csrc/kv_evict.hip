@@ -487,9 +487,10 @@ extern "C" int rswa_cache_evict(const rswa_cache_params* p, void* stream) {
                p->num_recent, p->budget);
   RSWA_REQUIRE(p->num_pages > 0 && p->weights_len >= 0 && p->new_max_pages >= 0, RSWA_ERR_INVALID,
                "cache_evict: a cache without pages, or a negative size");
-  RSWA_REQUIRE((p->weights && p->new_weights || p->weights_len == 0) && p->new_page_table && p->new_seqlens && p->kept,
+  RSWA_REQUIRE((p->weights && p->new_weights || p->weights_len == 0) && (p->new_page_table || p->new_max_pages == 0) &&
+                   p->new_seqlens && p->kept,
                RSWA_ERR_INVALID, "cache_evict: null tensor");
-  RSWA_REQUIRE(p->new_page_table != p->page_table, RSWA_ERR_INVALID,
+  RSWA_REQUIRE(p->new_page_table != p->page_table || p->new_max_pages == 0, RSWA_ERR_INVALID,
                "cache_evict: the new pages must be others than the old ones");
   const int64_t most = std::min<int64_t>(p->budget, (int64_t)p->max_pages * p->page_size);
   RSWA_REQUIRE((int64_t)p->new_max_pages * p->page_size >= most, RSWA_ERR_INVALID,

@@ -1,5 +1,5 @@
-"""Attention through the C ABI over a page table without columns: no keys at all, so every row of a sequence is 0 and
-its lse -inf.  (The Python function answers such calls by itself.)"""
+"""Page tables without columns.  Attention through the C ABI: no keys at all, so every row of a sequence is 0 and its lse
+-inf (the Python function answers such calls by itself).  Eviction: nothing to keep."""
 import math
 
 import pytest
@@ -30,3 +30,16 @@ def test_a_table_without_columns(new, heads, packed, dtype):
     rows = new - 3 if packed else new
     assert bool((out[..., :rows, :, :] == 0).all()) and bool((lse[..., :rows] == -math.inf).all())
     assert bool((out[..., rows:, :, :] == 7).all()) and bool((lse[..., rows:] == 7).all())
+
+
+@pytest.mark.gpu
+def test_eviction_from_tables_without_columns():
+    from ring_swa import kv_cache_evict
+
+    cache, table, lens, _ = make([40, 7], 2, 128, 16, 2)
+    before = [t.view(torch.uint8).clone() for t in cache]
+    w = torch.rand(2, 2, 50, device="cuda")
+    for new in (table[:, :0].clone(), table):
+        n, new_w, kept = kv_cache_evict(cache, w, table[:, :0], lens, new, 5, num_sink_tokens=1, num_recent=2)
+        assert n.tolist() == [0, 0] and bool((new_w == 0).all()) and bool((kept == -1).all())
+    assert all(torch.equal(t.view(torch.uint8), was) for t, was in zip(cache, before))
