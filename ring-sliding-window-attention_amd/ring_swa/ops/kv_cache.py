@@ -116,6 +116,11 @@ def _no_grad(*tensors) -> None:
         raise RuntimeError("the cache has no forward derivative: call this on tensors without tangents")
 
 
+def _fit(*sizes) -> None:
+    """(the parameter block would cut them to 32 bits without a word; what is too large below that, the library refuses)"""
+    assert max(sizes) < 1 << 31, "sizes must be below 2^31"
+
+
 def _cache_params(cache, page_table, seqlens, rows, cu_seqlens):
     """The fields that every call sets, from its cache, table, lengths and rows (a tensor, or None)."""
     k, v, k_scale, v_scale = cache
@@ -133,6 +138,7 @@ def _cache_params(cache, page_table, seqlens, rows, cu_seqlens):
     assert seqlens.dtype == torch.int32 and seqlens.shape == (batch,) and seqlens.is_contiguous(), (
         "seqlens must be a contiguous int32 tensor [batch]")
     dev = _lib.require_device(k, v, k_scale, v_scale, page_table, seqlens)
+    _fit(*k.shape, *page_table.shape)
     p = _lib.CacheParams()  # (zero-initialised)
     p.head_dim, p.batch, p.heads_q, p.heads_kv = dim, batch, heads, heads
     p.page_size, p.num_pages, p.max_pages = size, pages, page_table.shape[1]
@@ -143,6 +149,7 @@ def _cache_params(cache, page_table, seqlens, rows, cu_seqlens):
     p.seqlens = seqlens.data_ptr()
     if rows is not None:
         assert rows.shape[-1] == dim, "head_dim mismatch"
+        _fit(*rows.shape)
         _lib.require_device(k, rows)
         p.dtype = _lib.dtype_code(rows)
         if cu_seqlens is None:
@@ -351,6 +358,7 @@ def _weights_params(p, k, weights):
     assert weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (p.batch, p.heads_kv), (
         "weights must be fp32 [batch, kv_heads, n]")
     assert _dense_from(weights, 2), "last dimension must be contiguous"
+    _fit(weights.shape[2])
     span = weights.shape[2]  # of what the inner of the two strides has walked over
     for size, step in sorted(zip(weights.shape[:2], weights.stride()), key=lambda d: d[1]):
         assert size <= 1 or step >= span, "the sums of different heads overlap"
@@ -390,6 +398,7 @@ def kv_cache_evict(
                                 num_recent)
         if got is not None:
             return got
+    _fit(budget)
     assert budget > 0 and num_sink_tokens >= 0 and num_recent >= 0
     assert num_sink_tokens + num_recent <= budget, "budget must hold the sinks and the recent tokens"
     _no_grad(*cache, weights)
@@ -411,6 +420,7 @@ def _evict(k, v, k_scale, v_scale, weights, page_table, seqlens, new_page_table,
     assert new_page_table.dim() == 2 and new_page_table.dtype == torch.int32 and \
         new_page_table.shape[0] == p.batch, "new_page_table must be int32 [batch, n]"
     assert _dense_from(new_page_table, 1), "the entries of a row of new_page_table must be adjacent"
+    _fit(new_page_table.shape[1])
     _lib.require_device(k, new_page_table)
     new_seqlens, new_weights, kept = _cut(weights, seqlens, p.heads_kv, budget)
     p.num_sink, p.num_recent, p.budget = num_sink_tokens, num_recent, budget
