@@ -428,7 +428,11 @@ typedef struct rswa_cache_params {
  */
 int rswa_cache_append(const rswa_cache_params* p, void* stream);
 
-/* Attention of q over the cache: out, and the natural-log lse if asked for.  fp32 sums whatever the types. */
+/*
+ * Attention of q over the cache: out, and the natural-log lse if asked for.  fp32 sums whatever the types.
+ * Here and in the weights every block reads all lengths: a part of the time grows with batch^2 * heads_kv (8 kv heads:
+ * 0.1 ms at 1024 sequences, 19 ms at 16384), and beyond 2^36 of that product the call is refused.
+ */
 int rswa_cache_attn(const rswa_cache_params* p, void* stream);
 /* Scratch of such a call: partial results of rows whose keys several blocks share. */
 uint64_t rswa_cache_attn_workspace_bytes(const rswa_cache_params* p);

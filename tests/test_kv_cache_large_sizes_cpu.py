@@ -1,9 +1,11 @@
-"""Sizes that 32 bits do not hold are refused, and not cut to what is left of them."""
+"""Sizes that 32 bits do not hold are refused, and not cut to what is left of them; and batches whose lengths, which
+every block of attention and weights reads, would take seconds."""
 import pytest
 import torch
 
 import ring_swa
 from ring_swa import KVCache, _lib
+from test_kv_cache_cpu import params
 
 
 @pytest.fixture(autouse=True)
@@ -48,3 +50,11 @@ def test_running_sums():
     w = torch.zeros(1, device="meta").as_strided((1, 2, 2 ** 32 + 9), (2 ** 33, 2 ** 33, 1))
     with pytest.raises(AssertionError, match="2.31"):
         ring_swa.ops.kv_cache._weights_params(_lib.CacheParams(batch=1, heads_kv=2), cache.k, w)
+
+
+@pytest.mark.parametrize("batch,heads_q,heads_kv", [(1 << 17, 32, 8), (1 << 18, 4, 2), (1 << 20, 1, 1), (1 << 15, 128, 128)])
+@pytest.mark.parametrize("call", ["attn", "weights"])
+def test_batches(call, batch, heads_q, heads_kv):
+    L = _lib.lib()
+    assert getattr(L, "rswa_cache_" + call)(params({"batch": batch, "heads_q": heads_q, "heads_kv": heads_kv}), None) == -2
+    assert "2^36" in L.rswa_last_error().decode()
