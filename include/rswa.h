@@ -344,7 +344,7 @@ int rswa_attn_fwd_blocks_per_cu(const rswa_attn_params* p);
  * (V lies as the matrix instruction wants it: 16 bytes are 16 keys of one dimension.)  Page and head strides are the
  * caller's, in bytes, below 2^32 (a pool may span any number of bytes), those of k and v multiples of 16; within a
  * (page, head) the bytes are dense.  Attention and weights take the codes' values in the type of q, so that what bf16
- * rows have written beyond fp16's range is infinite to fp16 queries.
+ * rows have written beyond fp16's range is infinite to fp16 queries (and what is below 2^-20, to those, a multiple of 2^-23).
  *
  * Token t of sequence b is in page page_table[b * page_table_stride + t / page_size] at place t % page_size.  An id
  * outside [0, num_pages) (-1, say) is a page that is not there: its keys are seen by nobody, tokens that would go
@@ -451,7 +451,7 @@ int rswa_cache_weights(const rswa_cache_params* p, void* stream);
  * the pages of new_page_table, from place 0 on, at the scale that fits the values in each new page; new_seqlens[b] is
  * their number, the lesser of budget and of the tokens whose page is there; new_weights gets their weights, zeros behind;
  * kept gets the tokens' old numbers, -1 behind.  The old pages are only read (they may be shared with other sequences);
- * a page may not be old and new, or new for two sequences.
+ * a page may not be old and new, or new for two sequences.  What would go to a new page that is not there is lost.
  * num_sink + num_recent <= budget.
  */
 int rswa_cache_evict(const rswa_cache_params* p, void* stream);

@@ -10,7 +10,7 @@
 // scale is one value per lane, folded into the widening.
 // Bound by memory where rows are few: 64 sequences of 256 to 32768 keys, 32 / 8 heads of 128, 217 us, 5.1 TB/s.  The keys
 // of long sequences are cut into chunks for the whole chip, whose partial results a second launch joins; one token
-// against 4001 keys takes 6.5 + 4 us, each a launch and some five round trips to memory in a row.
+// against 4001 keys takes 6.8 + 3.9 us, each a launch and some five round trips to memory in a row.
 #include "kv_cache.h"
 
 namespace rswa {
@@ -493,7 +493,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(c
 // computed the scores of tile i + 1 are multiplied, and while tile i's weights meet its values the next operands are
 // widened, K two tiles ahead, V one, and the largest scores of tile i + 1 found (2.4 % less time than after the barrier);
 // one barrier a tile.
-// 2048 tokens of 32 / 8 heads against 32768 keys: 977 us, 1090 TFLOP/s (a library product of as many operations 877;
+// 2048 tokens of 32 / 8 heads against 32768 keys: 966 us, 1100 TFLOP/s (a library product of as many operations 873;
 // each wave widening all of a tile for itself took a tenth longer, and so did the loop unskewed).  Of the time the matrix
 // pipes are busy 49 %, the vector ones 52 %, both at once 15 %, and LDS 59 %: what bounds it is how the two waves of a SIMD
 // (all that the registers allow) fill each other's gaps.
@@ -765,7 +765,9 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheArgs a)
 // rows of its own (us, shared keys / own rows, 32 / 8 heads: 32 sequences of 64 tokens against 1000 keys 78 / 52; 2 of
 // 512 against 4096 96 / 90.  Half as many tiles as units: 1 of 512 against 1000 26 / 33, 4096 59 / 59, 32768 367 / 310, 16
 // of 32 against 8000 120 / 116, 28 / 4 heads of 64, 3 of 200 against 8000 76 / 98; the host, which does not know the
-// lengths, cannot tell these apart.  Fewer: 4 of 64 against 1000 20 / 34, 1 of 64 16 / 22).
+// lengths, cannot tell these apart.  Fewer: 4 of 64 against 1000 20 / 34, 1 of 64 16 / 22).  All of these have sequences of
+// equal counts.  Of a pack with unlike ones the mean chooses, which suits neither: 63 single tokens and a chunk of 512
+// against 8000 keys each 280, the two parts in calls of their own 175 + 89; a chunk of 2048 580, apart 176 + 239.
 constexpr int kMinChunk = 4;
 struct Cut {
   int nt, wr, row_tile, wanted, min_chunk;

@@ -154,7 +154,8 @@ __device__ __forceinline__ SeenTiles seen_tiles(const CacheArgs& a, int first, i
 //
 // The host knows no length.  Every wave reads all of them (64 at a time), sums the tiles of the whole call, and cuts
 // the tiles of every row tile into chunks of as many as give the launch about the units it was sized for: sequences
-// of any lengths make units of nearly one size, which the hardware then deals.  The grid is sized for the bound
+// of any lengths make units of nearly one number of tiles, which the hardware then deals (for attention, that is; in the
+// weights a row tile is all rows of a sequence, and units of long chunks take longer).  The grid is sized for the bound
 //   sum over sequences of row_tiles * chunks <= units wanted / heads_kv + sum of row_tiles
 // and what is beyond the last unit ends at once.  Rows of sequences with several chunks are joined from partial
 // results; those sequences have at most 8/5 of the units wanted (with x = tiles / chunk, which is above 5/4 there,
@@ -255,7 +256,8 @@ __device__ __forceinline__ typename Mma<T>::V8 widen8(uint32_t lo, uint32_t hi, 
 
 // Half of the power of two that scale byte `e` stands for.  Operands are taken at half their value (and scores and
 // outputs doubled, which costs nothing): rounding to e4m3 can raise a value just below the 16-bit type's largest
-// past it, and half of that is always there.
+// past it, and half of that is always there.  What it costs: fp16 operands below 2^-20 are
+// multiples of 2^-23, where the type has 2^-24 (off by 2^-24 at most).
 __device__ __forceinline__ float half_scale(int e) {
   return __builtin_bit_cast(float, (uint32_t)(max(e, 1) - 1) << 23);
 }

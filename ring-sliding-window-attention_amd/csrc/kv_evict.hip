@@ -1,8 +1,8 @@
 // Eviction from the 8-bit paged cache by running sums of softmax weights.
 //
 // Two launches: the first chooses, for each sequence and kv head, the second moves what stays into the new pages.
-// 32 sequences of 2176 tokens cut to 2048, 8 heads of 128: 10 + 52 us (275 MB, 5 TB/s).  4 of 20000 to
-// 32768 cut to 4096: 23 + 31 us; one in six tokens stays, so that nearly every group of 16 has one and all of V is read
+// 32 sequences of 2176 tokens cut to 2048, 8 heads of 128: 10 + 53 us (275 MB, 5 TB/s).  4 of 20000 to
+// 32768 cut to 4096: 24 + 30 us; one in six tokens stays, so that nearly every group of 16 has one and all of V is read
 // (the price of V in groups, which the attention reads as they are).
 #include "kv_cache.h"
 

@@ -4,11 +4,14 @@
 // the keys as columns, exp2(S - lse), and a sum over rows that needs no exchange until a tile's end.  V is not read.
 // Few rows: each wave has keys of its own, and K is read once.  More: the four waves of a block share the keys, with
 // rows of their own; their sums meet in LDS, in a fixed order, and rows beyond 64 NR come in further rounds over the
-// block's keys.
+// block's keys, whether those rows see them or not: what a window or the sequence's end hides is computed and masked
+// (2048 tokens from an empty cache 184 us whatever the window; against 8192 or 32768 keys with a window of 1000 261).
 // 32 tokens of as many sequences of 1024 to 16384 keys, 32 / 8 heads: 45 us, 4.2 TB/s, bound by memory.  64 tokens
 // against 32001 keys: 28 us, 600 TFLOP/s, of which 8 are blocks' starts and ends (eight tiles each); 700
 // TFLOP/s against 200000, bound by issuing vector instructions: an exponential, at a quarter of their rate, for each
-// 2 x 128 operations.  (Keys in registers and rows from memory 64 us, waiting for rows 16 at a time.)
+// 2 x 128 operations.  (Keys in registers and rows from memory 64 us, waiting for rows 16 at a time.)  Units are equal
+// shares of key tiles, not of rows: a pack's long chunk is left to the few blocks that have its keys (63 single tokens
+// and a chunk of 2048 against 8000 keys each 6600 us, in calls of their own 117 + 357).
 #include "kv_cache.h"
 
 namespace rswa {
@@ -48,8 +51,9 @@ __global__ __launch_bounds__(kThreads, 2) void cache_weights_kernel(const CacheA
     return table[min(tile_of(min(slot, s1 - 1)) * 4 + (col >> 2), n_groups - 1) >> per_page];
   };
   // Of many rows two sets of registers, the next tile's loaded ahead of this one's products (behind the last tile that one
-  // again: a branch here makes the compiler wait for more than it must).  us without / with it, 32 / 8 heads: 64 tokens
-  // against 4000 keys 11.9 / 12.6, 32001 32.6 / 31.3, 200000 155 / 148; 2 sequences of 512 against 4096 100 / 95.
+  // again: a branch here makes the compiler wait for more than it must).  us without / with it, 32 / 8 heads, in bursts of
+  // 20 calls, which run at lower clocks than calls among others: 64 tokens against 4000 keys 11.9 / 12.6, 32001 32.6 / 31.3,
+  // 200000 155 / 148; 2 sequences of 512 against 4096 100 / 95.
   constexpr int BUFS = NR > 1 ? 2 : 1;
   u32x4 kbs[BUFS][4][C];
   int kes[BUFS];
