@@ -286,8 +286,8 @@ PyObject* band_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // ---- the calls over the 8-bit paged cache (ring_swa/ops/kv_cache.py makes the same in Python) --------------------
 //
-// A served token is a handful of kernels of 4 to 8 us; from Python the host took 13 to 20 us for each of these calls,
-// here 4 to 6.  What they do not take (other types, tensors that need a gradient, modes) goes to Python, which refuses or
+// A served token is a handful of kernels of 4 to 8 us; from Python the host takes 16 to 25 us for each of these calls (22
+// to 31 under a torch function mode, such as a default device), here 4 to 9.  What they do not take (other types, tensors that need a gradient, modes) goes to Python, which refuses or
 // handles it; a refusal of the library's is raised there too.
 
 struct {

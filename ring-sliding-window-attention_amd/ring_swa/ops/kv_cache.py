@@ -105,14 +105,14 @@ def _operator(schema, fake):
         _ops.define(schema)
         _ops.impl(name, fn, "CompositeExplicitAutograd")
         torch.library.register_fake("ring_swa::" + name, fake, lib=_ops)
-        return getattr(torch.ops.ring_swa, name)
+        return getattr(torch.ops.ring_swa, name).default
     return register
 
 
 def _no_grad(*tensors) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError("the cache has no backward: call this under torch.no_grad()")
-    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors if t.is_floating_point()):
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError("the cache has no forward derivative: call this on tensors without tangents")
 
 
