@@ -452,6 +452,7 @@ int rswa_cache_weights(const rswa_cache_params* p, void* stream);
  * their number, the lesser of budget and of the tokens whose page is there; new_weights gets their weights, zeros behind;
  * kept gets the tokens' old numbers, -1 behind.  The old pages are only read (they may be shared with other sequences);
  * a page may not be old and new, or new for two sequences.  What would go to a new page that is not there is lost.
+ * new_seqlens and new_weights may not be seqlens and weights.
  * num_sink + num_recent <= budget.
  */
 int rswa_cache_evict(const rswa_cache_params* p, void* stream);

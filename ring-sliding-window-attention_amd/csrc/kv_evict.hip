@@ -492,6 +492,9 @@ extern "C" int rswa_cache_evict(const rswa_cache_params* p, void* stream) {
                RSWA_ERR_INVALID, "cache_evict: null tensor");
   RSWA_REQUIRE(p->new_page_table != p->page_table || p->new_max_pages == 0, RSWA_ERR_INVALID,
                "cache_evict: the new pages must be others than the old ones");
+  // (blocks of other heads still read these while one writes its results)
+  RSWA_REQUIRE(p->new_seqlens != p->seqlens && (p->new_weights != p->weights || p->weights_len == 0), RSWA_ERR_INVALID,
+               "cache_evict: the new lengths and weights must be others than the old ones");
   const int64_t most = std::min<int64_t>(p->budget, (int64_t)p->max_pages * p->page_size);
   RSWA_REQUIRE((int64_t)p->new_max_pages * p->page_size >= most, RSWA_ERR_INVALID,
                "cache_evict: a row of new_page_table holds %lld tokens, %lld may stay",
