@@ -459,6 +459,119 @@ int rswa_cache_evict(const rswa_cache_params* p, void* stream);
 
 uint64_t rswa_sizeof_cache_params(void);
 
+/*
+ * The inverse of rswa_cache_append: rows of new_k and new_v [.., heads_kv, head_dim], which this call WRITES, are
+ * tokens seqlens[b], seqlens[b] + 1, .. of their sequence (below zero counts as zero), their values rounded to dtype
+ * (infinite where it holds them as that).  Rows of tokens that have no page, or lie beyond the table, are zeros.
+ */
+int rswa_cache_read(const rswa_cache_params* p, void* stream);
+
+/*
+ * A step of drafted tokens over the cache.  No counterpart in the upstream package.
+ *
+ * The drafts of a sequence form a tree.  Its n nodes are rows in an order in which parents come first: dense
+ * [batch, nodes, ..], or of a pack [total, ..] with cu_seqlens.  A node's parent is a lower node of its sequence, or -1:
+ * the last cached token.  A node whose chain of parents does not fall, step by step, and end at -1 is not there (padding:
+ * -2); nor is one from the max_nodes-th on.  Node i is token seqlens[b] + depth(i), its depth the number of its ancestors.
+ */
+typedef struct rswa_tree_params {
+  int32_t batch;
+  int32_t nodes;     /* dense: nodes per sequence */
+  int32_t max_nodes; /* 1 .. 1024; dense: at least `nodes` */
+  int64_t total;     /* packed: rows */
+  const int32_t* cu_seqlens;
+  const int32_t* parents;
+  int64_t parents_stride; /* dense: between sequences (0: one tree for all) */
+  /* written, dense in the order of the rows; rows that are no sequence's are left alone */
+  int32_t* tree_parents; /* [rows]: the parent, -2 where the node is not there */
+  int32_t* depths;       /* [rows]: -1 where the node is not there */
+  int64_t* ancestors;    /* [rows, (max_nodes + 63) / 64]: bit j % 64 of word j / 64 for j = the node itself and its
+                            ancestors; none where the node is not there */
+} rswa_tree_params;
+
+int rswa_draft_tree(const rswa_tree_params* p, void* stream);
+
+/*
+ * The parameters of the calls over the cache that take a tree: `cache` as those of rswa_cache_attn (rows are nodes, and
+ * seqlens counts the tokens in the cache, the nodes not among them), with new_k and new_v the nodes' own keys and values,
+ * in their own type and not in the cache.
+ */
+typedef struct rswa_draft_params {
+  rswa_cache_params cache;
+  /* tree_attn: of rswa_draft_tree */
+  const int32_t* depths;
+  int64_t depths_stride; /* dense: between sequences */
+  const int64_t* ancestors;
+  int64_t ancestors_stride; /* dense: between sequences, in words; rows are `words` apart */
+  int32_t words;            /* 1 .. 16; nodes from 64 * words on are seen by nobody */
+  /* accept */
+  int32_t path_len;
+  const int32_t* path; /* [batch, path_len] */
+  int64_t path_stride;
+} rswa_draft_params;
+
+/*
+ * Attention of the nodes: node i sees the cached tokens j with
+ *   window_left < 0  or  j >= seqlens[b] + depth(i) - window_left  or  j < num_sink
+ * and by the same rule, at place seqlens[b] + depth(j), itself and its ancestors.  out and lse as rswa_cache_attn's; nodes
+ * that are not there: out = 0, lse = -inf.  Bits of `ancestors` say who sees whom, whatever the depths.
+ */
+int rswa_cache_tree_attn(const rswa_draft_params* p, void* stream);
+uint64_t rswa_cache_tree_attn_workspace_bytes(const rswa_draft_params* p);
+
+/*
+ * rswa_cache_append of the rows that `path` names: the keys and values of nodes path[b, 0], path[b, 1], .. go behind the
+ * tokens that the sequence holds, as many as there are ahead of the first entry that is no node's number.
+ */
+int rswa_cache_accept(const rswa_draft_params* p, void* stream);
+
+uint64_t rswa_sizeof_tree_params(void);
+uint64_t rswa_sizeof_draft_params(void);
+uint64_t rswa_sizeof_verify_params(void);
+
+/*
+ * Which drafts the target's probabilities take, and the token behind them, so that tokens are distributed as if drawn from
+ * the target one by one.  Rows as in rswa_tree_params.  Node 0 is the root: a token that is chosen already.  target[i, x]
+ * is the probability of token x behind node i, draft[i, x] the one that the children of node i were drawn with
+ * (independently), uniforms[i] a number from [0, 1).  From the root on, at the node reached, with p and q its rows, a = 0
+ * and S = 1, its children i are tried in their order, r(x) = max(0, p(x) - a q(x)):
+ *   uniforms[i] * S * q(tokens[i]) < r(tokens[i]):  child i is reached
+ *   else:  a <- a + S,  S <- sum over x of max(0, p(x) - a q(x))
+ * Without draft (NULL) its drafts are named outright, and r = p but for tokens tried before, where it is 0:
+ *   uniforms[i] * S < r(tokens[i]):  child i is reached;  else:  S <- max(0, S - r(tokens[i]))
+ * Where no child is reached the next token is the least x with  sum over y <= x of r(y)  >  uniforms[0] * sum of r  (r = p if
+ * nothing is left of it, -1 if there is nothing in p).  Sums in 64 bits.  Probabilities that are not positive (NaN) count as
+ * 0; a child whose token is outside [0, vocab) is passed over.
+ */
+typedef struct rswa_verify_params {
+  int32_t dtype;       /* of target and draft: RSWA_BF16, RSWA_F16 or RSWA_F32 */
+  int32_t token_bytes; /* 4 or 8: type of tokens and next_token */
+  int32_t batch;
+  int32_t nodes;     /* dense */
+  int32_t max_nodes; /* 1 .. 1024: nodes of a sequence from there on are not looked at */
+  int32_t vocab;
+  int64_t total; /* packed */
+  const int32_t* cu_seqlens;
+  const int32_t* parents; /* tree_parents of rswa_draft_tree (a node with a parent that is no lower one is passed over) */
+  const void* tokens;
+  const float* uniforms;
+  int64_t parents_stride, tokens_stride, uniforms_stride; /* dense: between sequences */
+  const void* target;
+  const void* draft;          /* NULL: none */
+  int64_t target_stride[2];   /* sequence (dense), node */
+  int64_t draft_stride[2];
+  /* written */
+  int32_t* path;       /* [batch, path_len], dense: the nodes reached, root first, -1 behind */
+  int32_t path_len;    /* at least min(nodes, max_nodes) */
+  int32_t* accepted;   /* [batch]: their number (0 where the root is not there; the next token is -1 then) */
+  void* next_token;    /* [batch] */
+  void* workspace;     /* rswa_verify_drafts_workspace_bytes(), 8-byte aligned, uninitialised */
+  uint64_t workspace_bytes;
+} rswa_verify_params;
+
+int rswa_verify_drafts(const rswa_verify_params* p, void* stream);
+uint64_t rswa_verify_drafts_workspace_bytes(const rswa_verify_params* p);
+
 /* Message of the calling thread's last failed call ("" if none). */
 const char* rswa_last_error(void);
 

@@ -1,0 +1,561 @@
+// Trees of drafted tokens: depths and ancestor bits from parents, and the choice of the drafts that the target's
+// probabilities take.
+//
+// The choice walks down from the root: at a node with target p and draft q its children are tried one after the other, each
+// against what p has left after the rejected ones, norm(max(0, .. - q)) for each.  That residual after k rejections is
+// max(0, p - a q) / S with a_0 = 0, S_0 = 1, a_{k+1} = a_k + S_k, S_k = sum max(0, p - a_k q): two numbers carry it, no row
+// is ever written, and a rejection costs one pass over two rows for the next S.
+//   max(0, max(0, p - a q) / S - q) = max(0, p - (a + S) q) / S
+// Sums and comparisons are in 64 bits: a draw lies next to borders that are closer than 32-bit sums of a vocabulary.
+// The first pass -- a chain has no other -- is one launch over all rows in pieces of 4096 tokens, each of whose blocks walks
+// for itself; a second launch, a block for each sequence, goes on from there and draws the next token by the pieces' sums.
+#include "rswa_common.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace rswa {
+namespace {
+
+constexpr int kMaxNodes = 1024;
+constexpr int kPiece = 4096;  // tokens
+
+// Sequence b's rows, whatever cu_seqlens holds.
+__device__ __forceinline__ void rows_of(const int32_t* cu, int b, int nodes, int64_t total, int64_t& row0, int& n) {
+  row0 = 0;
+  n = nodes;
+  if (cu) {
+    row0 = max((int64_t)0, min((int64_t)cu[b], total));
+    n = (int)(max(row0, min((int64_t)cu[b + 1], total)) - row0);
+  }
+}
+
+// ---- the tree ---------------------------------------------------------------------------------------------------
+struct TreeKernelArgs {
+  int32_t nodes, max_nodes, words;
+  int64_t total;
+  const int32_t* cu;
+  const int32_t* parents;
+  int64_t parents_st;
+  int32_t* tree_parents;
+  int32_t* depths;
+  uint64_t* ancestors;
+};
+
+constexpr int kTreeThreads = 256;
+
+// A block has a sequence.  A node's ancestors among the 64 nodes of its own word are found by walking up, and the first one
+// of a lower word is remembered; the others are that one's, word by word.  (At most 63 + 15 steps through LDS in a row, where
+// a walk up a chain of 1024 would be 1023.)
+__global__ __launch_bounds__(kTreeThreads) void draft_tree_kernel(const TreeKernelArgs a) {
+  __shared__ int32_t up[kMaxNodes];   // the parent; -1: none, -2: the node is not there
+  __shared__ int32_t out[kMaxNodes];  // the first ancestor of a lower word, -1 or -2 as the chain ends
+  __shared__ uint64_t own[kMaxNodes]; // ancestors of its word, and itself
+  const int b = blockIdx.x;
+  int64_t row0;
+  int n;
+  rows_of(a.cu, b, a.nodes, a.total, row0, n);
+  const int m = min(n, a.max_nodes);
+  const int32_t* const parents = a.parents + (a.cu ? row0 : b * a.parents_st);
+  const int64_t row = a.cu ? row0 : (int64_t)b * a.nodes;  // of what is written
+  for (int i = threadIdx.x; i < m; i += kTreeThreads) {
+    const int p = parents[i];
+    up[i] = p >= -1 && p < i ? p : -2;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < m; i += kTreeThreads) {
+    const int low = i & ~63;
+    uint64_t bits = 0;
+    int j = i;
+    while (j >= low) {
+      bits |= 1ull << (j & 63);
+      j = up[j];
+    }
+    own[i] = bits;
+    out[i] = j;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kTreeThreads) {
+    int depth = -1, end = -2;
+    if (i < m)
+      for (int j = i; j >= 0; j = end) {
+        depth += __popcll(own[j]);
+        end = out[j];
+      }
+    const bool there = end == -1;
+    a.tree_parents[row + i] = there ? up[i] : -2;
+    a.depths[row + i] = there ? depth : -1;
+    uint64_t* const to = a.ancestors + (row + i) * a.words;
+    int j = there ? i : -1;
+    for (int w = a.words - 1; w >= 0; w--) {
+      const bool mine = j >= 64 * w;  // (j is of word w or a lower one; none: -1)
+      to[w] = mine ? own[j] : 0;
+      if (mine) j = out[j];
+    }
+  }
+}
+
+// ---- the choice -------------------------------------------------------------------------------------------------
+struct VerifyArgs {
+  int32_t batch, nodes, max_nodes, vocab, pieces, token_bytes, path_len;
+  int64_t total;
+  const int32_t* cu;
+  const int32_t* parents;
+  const void* tokens;
+  const float* uniforms;
+  int64_t parents_st, tokens_st, uniforms_st;
+  const void* target;
+  const void* draft;
+  int64_t target_st[2], draft_st[2];
+  int32_t* path;
+  int32_t* accepted;
+  void* next_token;
+  // from the first launch to the second
+  double* sums;  // [batch][pieces]
+  struct Walk* walks;
+};
+
+// Where the walk of a sequence is: at node `cur`, whose children below `next` are tried, with the residual
+// max(0, p - a q) / mass.
+struct Walk {
+  double a, mass;
+  int32_t cur, next, count;  // count: nodes reached
+  int32_t draw;              // no child is left to try (else: a sum is wanted)
+};
+
+template <typename T>
+__device__ __forceinline__ float positive(T v) {
+  return fmaxf((float)v, 0.f);  // (0 for NaN)
+}
+
+// A sequence's nodes in LDS.
+struct Nodes {
+  int32_t parent[kMaxNodes];  // -2: nobody's child
+  int32_t token[kMaxNodes];
+  float p[kMaxNodes], q[kMaxNodes], u[kMaxNodes];  // the token's probabilities at the parent, and the node's number
+};
+
+template <typename T>
+struct Sequence {
+  const VerifyArgs& a;
+  const T *target, *draft;
+  int64_t row0;
+  int b, n;
+  __device__ __forceinline__ Sequence(const VerifyArgs& args, int b_) : a(args), b(b_) {
+    rows_of(a.cu, b, a.nodes, a.total, row0, n);
+    n = min(n, min(a.max_nodes, a.path_len));
+    target = (const T*)a.target + (a.cu ? row0 * a.target_st[1] : b * a.target_st[0]);
+    draft = a.draft ? (const T*)a.draft + (a.cu ? row0 * a.draft_st[1] : b * a.draft_st[0]) : nullptr;
+  }
+  __device__ __forceinline__ const T* p_row(int node) const { return target + node * a.target_st[1]; }
+  __device__ __forceinline__ const T* q_row(int node) const { return draft ? draft + node * a.draft_st[1] : nullptr; }
+
+  // (`root`: is there one?)
+  __device__ __forceinline__ void load(Nodes& s, int threads) const {
+    const int32_t* const parents = a.parents + (a.cu ? row0 : b * a.parents_st);
+    const float* const uniforms = a.uniforms + (a.cu ? row0 : b * a.uniforms_st);
+    const int64_t at = a.cu ? row0 : b * a.tokens_st;
+    for (int i = threadIdx.x; i < n; i += threads) {
+      const int parent = parents[i];
+      const int64_t x = a.token_bytes == 8 ? ((const int64_t*)a.tokens)[at + i] : ((const int32_t*)a.tokens)[at + i];
+      const bool child = parent >= 0 && parent < i && x >= 0 && x < a.vocab;
+      s.u[i] = uniforms[i];
+      s.token[i] = (int)x;
+      s.parent[i] = i == 0 ? parent : child ? parent : -2;
+      s.p[i] = child ? positive(p_row(parent)[x]) : 0.f;
+      s.q[i] = child && draft ? positive(q_row(parent)[x]) : 0.f;
+    }
+  }
+};
+
+// The first child of `node` from `from` on (n: none).
+__device__ __forceinline__ int next_child(const Nodes& s, int node, int from, int n) {
+  const int lane = threadIdx.x & 63;
+  for (int i = from; i < n; i += 64) {
+    const uint64_t mine = __builtin_amdgcn_ballot_w64(i + lane < n && s.parent[min(i + lane, n - 1)] == node);
+    if (mine) return i + (int)__builtin_ctzll(mine);
+  }
+  return n;
+}
+
+// Without a draft: was the token tried at this node before, by a child below `i`?
+__device__ __forceinline__ bool tried(const Nodes& s, int node, int i) {
+  const int lane = threadIdx.x & 63;
+  for (int j = node + 1; j < i; j += 64)
+    if (__builtin_amdgcn_ballot_w64(j + lane < i && s.parent[min(j + lane, i)] == node && s.token[min(j + lane, i)] == s.token[i]))
+      return true;
+  return false;
+}
+
+// On to where a sum is wanted, or no child is left.  All lanes of a wave do the same; nodes reached go to `path` (null: not
+// written).
+template <bool DRAFT>
+__device__ __forceinline__ void walk_on(const Nodes& s, Walk& w, int n, int32_t* path) {
+  w.draw = 0;
+  for (;;) {
+    const int i = next_child(s, w.cur, w.next, n);
+    if (i == n) {
+      w.draw = 1;
+      w.next = n;
+      return;
+    }
+    w.next = i + 1;
+    const double p = s.p[i], q = s.q[i], u = s.u[i];
+    const double rest = DRAFT ? fmax(0.0, p - w.a * q) : tried(s, w.cur, i) ? 0.0 : p;
+    if (DRAFT ? u * w.mass * q < rest : u * w.mass < rest) {
+      if (path && threadIdx.x == 0) path[w.count] = i;
+      w.count++;
+      w.cur = i;
+      w.a = 0.0;
+      w.mass = 1.0;
+    } else if (DRAFT) {
+      w.a += w.mass;
+      return;
+    } else {
+      w.mass = fmax(0.0, w.mass - rest);
+    }
+  }
+}
+
+// 16 bytes from anywhere an element may lie
+template <typename T>
+struct Piece16 {
+  static constexpr int N = 16 / sizeof(T);
+  T v[N];
+  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(v, p, 16); }
+};
+
+// What is left at a node: r(x) for a vector of tokens from x0 on.
+template <typename T, bool DRAFT>
+struct Rest {
+  static constexpr int N = Piece16<T>::N;
+  const T *p, *q;
+  double a;
+  int vocab;
+  const Nodes& s;
+  int node, n_tried;  // children that `tried` has to look at: up to n_tried
+  __device__ __forceinline__ void at(int x0, double (&r)[N]) const {
+    Piece16<T> pv, qv;
+    if (x0 + N <= vocab) {
+      pv.load(p + x0);
+      if constexpr (DRAFT) qv.load(q + x0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        pv.v[e] = x0 + e < vocab ? p[x0 + e] : (T)0.f;
+        if constexpr (DRAFT) qv.v[e] = x0 + e < vocab ? q[x0 + e] : (T)0.f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      r[e] = positive(pv.v[e]);
+      if constexpr (DRAFT) r[e] = fmax(0.0, r[e] - a * (double)positive(qv.v[e]));
+    }
+    if constexpr (!DRAFT) {
+      for (int i = node + 1; i < n_tried; i++) {
+        const int at = s.parent[i] == node ? s.token[i] - x0 : -1;
+#pragma unroll
+        for (int e = 0; e < N; e++) r[e] = at == e ? 0.0 : r[e];
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
+  return v;
+}
+
+// Sum over a piece, by the threads t of `threads` (whole waves; every wave returns its lanes' share).
+template <typename T, bool DRAFT>
+__device__ __forceinline__ double piece_share(const Rest<T, DRAFT>& rest, int piece, int t, int threads) {
+  constexpr int N = Piece16<T>::N;
+  const int end = min(rest.vocab, (piece + 1) * kPiece);
+  double sum = 0.0;
+#pragma unroll 4
+  for (int x = piece * kPiece + t * N; x < end; x += threads * N) {
+    double r[N];
+    rest.at(x, r);
+    double of = 0.0;
+#pragma unroll
+    for (int e = 0; e < N; e++) of += r[e];
+    sum += of;
+  }
+  return sum;
+}
+
+constexpr int kFirstThreads = 256;
+
+// The walk as far as the first sum, and that sum of one piece.
+template <typename T, bool DRAFT>
+__global__ __launch_bounds__(kFirstThreads) void verify_first_kernel(const VerifyArgs a) {
+  __shared__ Nodes s;
+  __shared__ double share[kFirstThreads / 64];
+  const int b = blockIdx.y, piece = blockIdx.x;
+  const Sequence<T> seq(a, b);
+  Walk w{0.0, 1.0, 0, 1, 0, 0};
+  int32_t* const path = a.path + (int64_t)b * a.path_len;
+  if (seq.n > 0) {
+    seq.load(s, kFirstThreads);
+    __syncthreads();
+    if (s.parent[0] == -1) {
+      if (piece == 0 && threadIdx.x == 0) path[0] = 0;
+      w.count = 1;
+      walk_on<DRAFT>(s, w, seq.n, piece == 0 ? path : nullptr);
+    }
+  }
+  if (piece == 0 && threadIdx.x == 0) a.walks[b] = w;
+  if (w.count == 0) return;
+  const Rest<T, DRAFT> rest{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, s, w.cur, w.next};
+  const double sum = wave_sum(piece_share(rest, piece, threadIdx.x, kFirstThreads));
+  if ((threadIdx.x & 63) == 0) share[threadIdx.x / 64] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double of = 0.0;
+#pragma unroll
+    for (int i = 0; i < kFirstThreads / 64; i++) of += share[i];
+    a.sums[(int64_t)b * a.pieces + piece] = of;
+  }
+}
+
+constexpr int kRestThreads = 1024, kRestWaves = kRestThreads / 64;
+constexpr int kMaxPieces = 4096;
+
+// The rest of the walk, and the draw.
+template <typename T, bool DRAFT>
+__global__ __launch_bounds__(kRestThreads) void verify_rest_kernel(const VerifyArgs a) {
+  constexpr int N = Piece16<T>::N;
+  __shared__ Nodes s;
+  __shared__ double sums[kMaxPieces];
+  __shared__ double share[kRestWaves];
+  __shared__ int found, last_positive;
+  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+  const Sequence<T> seq(a, b);
+  int32_t* const path = a.path + (int64_t)b * a.path_len;
+  Walk w = a.walks[b];
+  if (w.count > 0) {
+    seq.load(s, kRestThreads);
+    for (int i = threadIdx.x; i < a.pieces; i += kRestThreads) sums[i] = a.sums[(int64_t)b * a.pieces + i];
+  }
+  if (threadIdx.x == 0) found = last_positive = -1;
+  __syncthreads();
+  auto pass = [&](const Rest<T, DRAFT>& rest) {  // sums of all pieces
+    __syncthreads();
+    for (int i = wave; i < a.pieces; i += kRestWaves) {
+      const double of = wave_sum(piece_share(rest, i, lane, 64));
+      if (lane == 0) sums[i] = of;
+    }
+    __syncthreads();
+  };
+  auto total = [&] {  // in the order of the pieces, the same in every lane
+    double of = 0.0;
+    for (int i = 0; i < a.pieces; i++) of += sums[i];
+    return of;
+  };
+  auto rest_of = [&](const Walk& at) {
+    return Rest<T, DRAFT>{seq.p_row(at.cur), seq.q_row(at.cur), at.a, a.vocab, s, at.cur, at.next};
+  };
+  int drawn = -1;
+  if (w.count > 0) {
+    if constexpr (DRAFT) {
+      while (!w.draw) {
+        w.mass = total();
+        const int cur = w.cur;
+        walk_on<DRAFT>(s, w, seq.n, path);
+        if (!w.draw || w.cur != cur) pass(rest_of(w));
+      }
+    }
+    Rest<T, DRAFT> rest = rest_of(w);
+    double all = total();
+    if (!(all > 0.0)) {  // nothing is left
+      rest.a = 0.0;
+      rest.n_tried = 0;
+      pass(rest);
+      all = total();
+    }
+    if (all > 0.0) {
+      const double want = (double)s.u[0] * all;
+      // the piece, of those that have anything
+      double before = 0.0, past = 0.0;
+      int piece = 0;
+      for (int i = 0; i < a.pieces; i++) {
+        if (sums[i] > 0.0) {
+          before = past;
+          piece = i;
+          past += sums[i];
+          if (past > want) break;
+        }
+      }
+      // the token: a thread has N tokens in a row, a wave 64 N, one after the other
+      constexpr int kTurn = 64 * N;
+      const int x_end = min(a.vocab, (piece + 1) * kPiece);
+      const int x = piece * kPiece + threadIdx.x * N;
+      static_assert(kTurn * kRestWaves >= kPiece, "a piece in one go");
+      double r[N];
+      double mine = 0.0;
+#pragma unroll
+      for (int e = 0; e < N; e++) r[e] = 0.0;
+      if (threadIdx.x * N < kPiece && x < x_end) {
+        rest.at(x, r);
+#pragma unroll
+        for (int e = 0; e < N; e++) mine += r[e];
+      }
+      double upto = mine;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const double from = __shfl_up(upto, d);
+        if (lane >= d) upto += from;
+      }
+      if (lane == 63) share[wave] = upto;
+      __syncthreads();
+      for (int i = 0; i < wave; i++) before += share[i];
+      double sum = before + (upto - mine);
+      int first = INT32_MAX, positive_at = -1;
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        sum += r[e];
+        if (r[e] > 0.0) {
+          positive_at = x + e;
+          if (sum > want && first == INT32_MAX) first = x + e;
+        }
+      }
+      if (first != INT32_MAX) atomicMin((uint32_t*)&found, (uint32_t)first);  // (-1 is the largest)
+      if (positive_at >= 0) atomicMax(&last_positive, positive_at);
+      __syncthreads();
+      drawn = found != -1 ? found : last_positive;  // (the last: where roundings have the sums end short of their total)
+    }
+  }
+  if (threadIdx.x == 0) {
+    a.accepted[b] = w.count;
+    if (a.token_bytes == 8)
+      ((int64_t*)a.next_token)[b] = drawn;
+    else
+      ((int32_t*)a.next_token)[b] = drawn;
+  }
+  for (int i = w.count + threadIdx.x; i < a.path_len; i += kRestThreads) path[i] = -1;
+}
+
+int pieces_of(int vocab) { return (int)ceil_div(vocab, kPiece); }
+
+uint64_t walk_bytes(const rswa_verify_params* p) {
+  return (uint64_t)p->batch * (sizeof(Walk) + 8 * (uint64_t)pieces_of(p->vocab));
+}
+
+template <typename T>
+void launch_verify(const VerifyArgs& a, hipStream_t stream) {
+  const dim3 first((unsigned)a.pieces, (unsigned)a.batch), rest((unsigned)a.batch);
+  if (a.draft) {
+    hipLaunchKernelGGL((verify_first_kernel<T, true>), first, dim3(kFirstThreads), 0, stream, a);
+    hipLaunchKernelGGL((verify_rest_kernel<T, true>), rest, dim3(kRestThreads), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((verify_first_kernel<T, false>), first, dim3(kFirstThreads), 0, stream, a);
+    hipLaunchKernelGGL((verify_rest_kernel<T, false>), rest, dim3(kRestThreads), 0, stream, a);
+  }
+}
+
+}  // namespace
+}  // namespace rswa
+
+extern "C" int rswa_draft_tree(const rswa_tree_params* p, void* stream) {
+  using namespace rswa;
+  constexpr const char* who = "draft_tree";
+  RSWA_REQUIRE(p, RSWA_ERR_INVALID, "%s: null parameters", who);
+  RSWA_REQUIRE(p->batch >= 0 && p->nodes >= 0 && p->total >= 0, RSWA_ERR_INVALID, "%s: negative size", who);
+  RSWA_REQUIRE(p->max_nodes >= 1 && p->max_nodes <= kMaxNodes, RSWA_ERR_UNSUPPORTED, "%s: max_nodes %d (1 to %d)", who,
+               p->max_nodes, kMaxNodes);
+  RSWA_REQUIRE(p->cu_seqlens || p->nodes <= p->max_nodes, RSWA_ERR_INVALID, "%s: %d nodes, max_nodes %d", who, p->nodes,
+               p->max_nodes);
+  RSWA_REQUIRE(p->total < (1ll << 31) && p->batch <= (1 << 20), RSWA_ERR_UNSUPPORTED, "%s: rows or batch too large", who);
+  const int64_t rows = p->cu_seqlens ? p->total : (int64_t)p->batch * p->nodes;
+  if (rows == 0 || p->batch == 0) return RSWA_OK;
+  RSWA_REQUIRE(p->parents && p->tree_parents && p->depths && p->ancestors, RSWA_ERR_INVALID, "%s: null tensor", who);
+  TreeKernelArgs a{};
+  a.nodes = p->nodes;
+  a.max_nodes = p->max_nodes;
+  a.words = (p->max_nodes + 63) / 64;
+  a.total = p->total;
+  a.cu = p->cu_seqlens;
+  a.parents = p->parents;
+  a.parents_st = p->parents_stride;
+  a.tree_parents = p->tree_parents;
+  a.depths = p->depths;
+  a.ancestors = (uint64_t*)p->ancestors;
+  clear_launch_error();
+  hipLaunchKernelGGL(draft_tree_kernel, dim3((unsigned)p->batch), dim3(kTreeThreads), 0, (hipStream_t)stream, a);
+  return check_launch(who);
+}
+
+extern "C" uint64_t rswa_verify_drafts_workspace_bytes(const rswa_verify_params* p) {
+  using namespace rswa;
+  if (!p || p->batch <= 0 || p->vocab <= 0) return 0;
+  return walk_bytes(p);
+}
+
+extern "C" int rswa_verify_drafts(const rswa_verify_params* p, void* stream) {
+  using namespace rswa;
+  constexpr const char* who = "verify_drafts";
+  RSWA_REQUIRE(p, RSWA_ERR_INVALID, "%s: null parameters", who);
+  RSWA_REQUIRE(p->dtype == RSWA_BF16 || p->dtype == RSWA_F16 || p->dtype == RSWA_F32, RSWA_ERR_UNSUPPORTED, "%s: dtype %d",
+               who, p->dtype);
+  RSWA_REQUIRE(p->token_bytes == 4 || p->token_bytes == 8, RSWA_ERR_UNSUPPORTED, "%s: tokens of %d bytes (4 or 8)", who,
+               p->token_bytes);
+  RSWA_REQUIRE(p->batch >= 0 && p->nodes >= 0 && p->total >= 0 && p->path_len >= 0, RSWA_ERR_INVALID, "%s: negative size",
+               who);
+  RSWA_REQUIRE(p->max_nodes >= 1 && p->max_nodes <= kMaxNodes, RSWA_ERR_UNSUPPORTED, "%s: max_nodes %d (1 to %d)", who,
+               p->max_nodes, kMaxNodes);
+  RSWA_REQUIRE(p->cu_seqlens || p->nodes <= p->max_nodes, RSWA_ERR_INVALID, "%s: %d nodes, max_nodes %d", who, p->nodes,
+               p->max_nodes);
+  RSWA_REQUIRE(p->path_len >= (p->cu_seqlens ? p->max_nodes : p->nodes), RSWA_ERR_INVALID, "%s: path_len %d is too short",
+               who, p->path_len);
+  RSWA_REQUIRE(p->vocab > 0, RSWA_ERR_INVALID, "%s: vocab %d", who, p->vocab);
+  RSWA_REQUIRE(p->vocab <= kPiece * kMaxPieces, RSWA_ERR_UNSUPPORTED, "%s: vocab %d (at most %d)", who, p->vocab,
+               kPiece * kMaxPieces);
+  RSWA_REQUIRE(p->total < (1ll << 31) && p->batch < (1 << 16), RSWA_ERR_UNSUPPORTED, "%s: rows or batch too large", who);
+  if (p->batch == 0) return RSWA_OK;
+  const int64_t rows = p->cu_seqlens ? p->total : (int64_t)p->batch * p->nodes;
+  RSWA_REQUIRE(p->accepted && p->next_token && (p->path || p->path_len == 0), RSWA_ERR_INVALID, "%s: null result", who);
+  RSWA_REQUIRE(rows == 0 || (p->parents && p->tokens && p->uniforms && p->target), RSWA_ERR_INVALID, "%s: null tensor", who);
+  RSWA_REQUIRE(p->workspace && (uintptr_t)p->workspace % 8 == 0 && p->workspace_bytes >= walk_bytes(p), RSWA_ERR_INVALID,
+               "%s: workspace of %llu bytes, %llu needed (8-byte aligned)", who, (unsigned long long)p->workspace_bytes,
+               (unsigned long long)walk_bytes(p));
+  VerifyArgs a{};
+  a.batch = p->batch;
+  a.nodes = p->nodes;
+  a.max_nodes = p->max_nodes;
+  a.vocab = p->vocab;
+  a.pieces = pieces_of(p->vocab);
+  a.token_bytes = p->token_bytes;
+  a.path_len = p->path_len;
+  a.total = p->total;
+  a.cu = p->cu_seqlens;
+  a.parents = p->parents;
+  a.tokens = p->tokens;
+  a.uniforms = p->uniforms;
+  a.parents_st = p->parents_stride;
+  a.tokens_st = p->tokens_stride;
+  a.uniforms_st = p->uniforms_stride;
+  a.target = p->target;
+  a.draft = p->draft;
+  for (int i = 0; i < 2; i++) {
+    a.target_st[i] = p->target_stride[i];
+    a.draft_st[i] = p->draft_stride[i];
+  }
+  a.path = p->path;
+  a.accepted = p->accepted;
+  a.next_token = p->next_token;
+  a.sums = (double*)p->workspace;
+  a.walks = (Walk*)(a.sums + (int64_t)p->batch * a.pieces);
+  clear_launch_error();
+  hipStream_t st = (hipStream_t)stream;
+  if (p->dtype == RSWA_F32)
+    launch_verify<float>(a, st);
+  else if (p->dtype == RSWA_BF16)
+    launch_verify<__bf16>(a, st);
+  else
+    launch_verify<_Float16>(a, st);
+  return check_launch(who);
+}
+
+extern "C" uint64_t rswa_sizeof_tree_params(void) { return sizeof(rswa_tree_params); }
+extern "C" uint64_t rswa_sizeof_verify_params(void) { return sizeof(rswa_verify_params); }

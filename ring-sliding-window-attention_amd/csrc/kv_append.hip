@@ -32,31 +32,7 @@ __global__ void cache_append_kernel(const AppendArgs a) {
   if (id0 >= a.work) return;
   int u = quotient(id0, a.by_heads), b, row0, n;
   const int hk = id0 - u * c.heads_kv;
-  // sequence, and which of its touched pages
-  if (c.cu) {
-    // sequence b owns the slots from cu[b] / page_size + 2 b on: n tokens touch at most n / page_size + 2 pages.
-    // (a search 64 ways at a time, as locate_packed)
-    const int lane = lane_id();
-    int lo = 0, cnt = c.batch;
-    for (;;) {
-      const int step = (cnt + 63) >> 6;
-      const int i = min(lo + lane * step, lo + cnt - 1);
-      const int slot = (max(0, min(c.cu[i], c.total_q)) >> c.page_log2) + 2 * i;
-      // (none: rows ahead of the first sequence; the count is unsigned)
-      const int at = max((int)__popcll(__builtin_amdgcn_ballot_w64(lane * step < cnt && slot <= u)) - 1, 0);
-      lo += at * step;
-      if (step == 1) break;
-      cnt = min(step, cnt - at * step);
-    }
-    b = __builtin_amdgcn_readfirstlane(lo);
-    Sequence(c, b).rows(c, row0, n);
-    u -= (row0 >> c.page_log2) + 2 * b;
-  } else {
-    b = quotient(u, a.by_pages);
-    u -= b * a.pages;
-    row0 = 0;
-    n = c.seqlen_q;
-  }
+  touched_page(c, a.pages, a.by_pages, u, b, row0, n);
   if (u < 0) return;
   const int start = max(0, c.lens[b]);
   const int in_seq = (start >> c.page_log2) + u;  // page of the sequence
@@ -184,6 +160,23 @@ __global__ void cache_append_kernel(const AppendArgs a) {
   }
 }
 
+// The codes of a page's places 0 .. from - 1 at a scale 2^by times as large, by one wave.
+template <int D>
+__device__ __forceinline__ void rescale_page(uint8_t* page, int which, int from, int by, int lane) {
+  const float f = by < 127 ? __builtin_bit_cast(float, (uint32_t)(127 - by) << 23) : 0.f;
+  const int words = which ? (from + 15) / 16 * 4 * D : from * D / 4;
+#pragma unroll 1
+  for (int i = lane; i < words; i += 64) {
+    const int left = which ? from - (i / (4 * D) * 16 + (i & 3) * 4) : 4;  // tokens from before in this word
+    uint32_t* const w = (uint32_t*)page + i;
+    const uint32_t again = left > 0 ? rescale4(*w, f) : 0u;
+    if (left >= 4) *w = again;
+#pragma unroll
+    for (int k = 0; k < 3; k++)
+      if (left < 4 && k < left) ((uint8_t*)w)[k] = (uint8_t)(again >> (8 * k));
+  }
+}
+
 // One token per sequence (dense): a wave has the key or the value of one head.  The same as above in a tenth of the
 // code: such a launch waits for little but memory, and that includes its instructions (one sequence or 128 of 8 heads:
 // 3.5 us, the kernel above 7.5).
@@ -215,26 +208,94 @@ __global__ __launch_bounds__(64) void cache_append_token_kernel(const AppendArgs
   const int e_new = max(was, scale_byte(wave_max(most)));
   const float inv = inverse(e_new);
   const uint32_t code = codes4((float)x[0] * inv, (float)x[E - 1] * inv, 0.f, 0.f);
-  if (from > 0 && e_new > was) {  // the tokens from before at the new scale
-    const float f = e_new - was < 127 ? __builtin_bit_cast(float, (uint32_t)(127 - (e_new - was)) << 23) : 0.f;
-    const int words = which ? (from + 15) / 16 * 4 * D : from * D / 4;
-#pragma unroll 1
-    for (int i = lane; i < words; i += 64) {
-      const int left = which ? from - (i / (4 * D) * 16 + (i & 3) * 4) : 4;  // tokens from before in this word
-      uint32_t* const w = (uint32_t*)page + i;
-      const uint32_t again = left > 0 ? rescale4(*w, f) : 0u;
-      if (left >= 4) *w = again;
-#pragma unroll
-      for (int k = 0; k < 3; k++)
-        if (left < 4 && k < left) ((uint8_t*)w)[k] = (uint8_t)(again >> (8 * k));
-    }
-  }
+  if (from > 0 && e_new > was) rescale_page<D>(page, which, from, e_new - was, lane);
   if (lane == 0) *scale = (uint8_t)e_new;
 #pragma unroll
   for (int i = 0; i < E; i++) {
     const int d = lane * E + i;
     page[which ? from / 16 * (16 * D) + d * 16 + from % 16 : from * D + d] = (uint8_t)(code >> (8 * i));
   }
+}
+
+struct AcceptArgs {
+  AppendArgs n;
+  const int32_t* path;
+  int64_t path_st;
+  int32_t path_len;
+};
+
+// Rows that a path names, as many as there are ahead of its first entry that is no row of the sequence.  As the kernel
+// for single tokens: paths are a few tokens, and their launch waits for little but memory.  A wave has the keys or the
+// values of one head that go to one page, kRows of them in registers (longer paths are read twice, for the scale and for
+// the codes).
+template <typename T, int D>
+__global__ __launch_bounds__(64) void cache_accept_kernel(const AcceptArgs a) {
+  constexpr int E = D / 64, kRows = 16;
+  typedef __attribute__((__vector_size__(E * sizeof(T)))) T VE;
+  const CacheArgs& c = a.n.c;
+  const int which = blockIdx.x & 1, lane = threadIdx.x;
+  int u = blockIdx.x >> 1;
+  const int slot = quotient(u, a.n.by_heads), hk = u - slot * c.heads_kv;
+  const int b = quotient(slot, a.n.by_pages);
+  u = slot - b * a.n.pages;
+  const int page_size = 1 << c.page_log2;
+  const int32_t* const path = a.path + (int64_t)b * a.path_st;
+  const Sequence seq(c, b);
+  int row0, n_rows;
+  seq.rows(c, row0, n_rows);
+  const int start = max(0, seq.len), in_page = start & (page_size - 1);
+  const int64_t in_seq = (int64_t)(start >> c.page_log2) + u;
+  if (in_seq >= c.max_pages) return;
+  const int id = c.table[(int64_t)b * c.table_st + in_seq];
+  const int from = u == 0 ? in_page : 0;               // first place written
+  const int i0 = u == 0 ? 0 : (u << c.page_log2) - in_page;  // its row of the path
+  int n = 0;  // rows of the path
+  for (int i = 0; i < a.path_len; i += 64) {
+    const int node = i + lane < a.path_len ? path[i + lane] : -1;
+    const uint64_t ends = __builtin_amdgcn_ballot_w64((uint32_t)node >= (uint32_t)n_rows);
+    n = i + (ends ? (int)__builtin_ctzll(ends) : 64);
+    if (ends) break;
+  }
+  const int count = min(page_size - from, n - i0);
+  if (count <= 0 || (uint32_t)id >= (uint32_t)c.num_pages) return;
+
+  const T* const x = (const T*)a.n.x[which] + (int64_t)b * a.n.x_st[which][0] + (int64_t)hk * a.n.x_st[which][2] + lane * E;
+  auto row = [&](int i) { return *(const VE*)(x + (int64_t)(row0 + path[i0 + i]) * a.n.x_st[which][1]); };
+  uint8_t* const scale = which ? const_cast<uint8_t*>(c.v_scale) + times(id, c.vs_st[0]) + times(hk, c.vs_st[1])
+                               : const_cast<uint8_t*>(c.k_scale) + times(id, c.ks_st[0]) + times(hk, c.ks_st[1]);
+  uint8_t* const page = which ? const_cast<uint8_t*>(c.v) + times(id, c.v_st[0]) + times(hk, c.v_st[1])
+                              : const_cast<uint8_t*>(c.k) + times(id, c.k_st[0]) + times(hk, c.k_st[1]);
+  const int was = from > 0 ? *scale : 0;
+  VE v[kRows];
+  float most = 0.f;
+  auto largest = [&](const VE& r) {
+#pragma unroll
+    for (int k = 0; k < E; k++) {
+      const float y = __builtin_fabsf((float)r[k]);
+      most = y < __builtin_inff() ? fmaxf(most, y) : most;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kRows; i++) v[i] = row(min(i, count - 1));
+#pragma unroll
+  for (int i = 0; i < kRows; i++) largest(v[i]);
+  for (int i = kRows; i < count; i++) largest(row(i));
+  const int e_new = max(was, scale_byte(wave_max(most)));
+  const float inv = inverse(e_new);
+  if (from > 0 && e_new > was) rescale_page<D>(page, which, from, e_new - was, lane);
+  if (lane == 0) *scale = (uint8_t)e_new;
+  auto put = [&](const VE& r, int place) {
+    const uint32_t code = codes4((float)r[0] * inv, (float)r[E - 1] * inv, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < E; k++) {
+      const int d = lane * E + k;
+      page[which ? place / 16 * (16 * D) + d * 16 + place % 16 : place * D + d] = (uint8_t)(code >> (8 * k));
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kRows; i++)
+    if (i < count) put(v[i], from + i);
+  for (int i = kRows; i < count; i++) put(row(i), from + i);
 }
 
 }  // namespace
@@ -246,18 +307,7 @@ extern "C" int rswa_cache_append(const rswa_cache_params* p, void* stream) {
   if (int rc = cache_args(p, "cache_append", a.c)) return rc;
   const int64_t rows = p->cu_seqlens_q ? p->total_q : (int64_t)p->batch * p->seqlen_q;
   if (rows == 0 || p->batch == 0 || p->max_pages == 0) return RSWA_OK;
-  RSWA_REQUIRE(p->new_k && p->new_v, RSWA_ERR_INVALID, "cache_append: null tensor");
-  a.x[0] = p->new_k;
-  a.x[1] = p->new_v;
-  for (int i = 0; i < 3; i++) {
-    a.x_st[0][i] = p->new_k_stride[i];
-    a.x_st[1][i] = p->new_v_stride[i];
-  }
-  for (int w = 0; w < 2; w++) {
-    RSWA_REQUIRE((uintptr_t)a.x[w] % 16 == 0 && a.x_st[w][0] % 8 == 0 && a.x_st[w][1] % 8 == 0 && a.x_st[w][2] % 8 == 0,
-                 RSWA_ERR_UNSUPPORTED, "cache_append: rows of new_k and new_v must be 16-byte aligned");
-    if (p->cu_seqlens_q) a.x_st[w][0] = 0;
-  }
+  if (int rc = cache_new_rows(p, "cache_append", a.x, a.x_st)) return rc;
   a.pages = (int32_t)((p->seqlen_q + p->page_size - 2) / p->page_size + 1);
   const int64_t slots =
       p->cu_seqlens_q ? p->total_q / p->page_size + 2 * (int64_t)p->batch : (int64_t)p->batch * a.pages;
@@ -285,4 +335,38 @@ extern "C" int rswa_cache_append(const rswa_cache_params* p, void* stream) {
   else
     p->head_dim == 128 ? go(_Float16{}, D128{}) : go(_Float16{}, D64{});
   return check_launch("cache_append");
+}
+
+extern "C" int rswa_cache_accept(const rswa_draft_params* d, void* stream) {
+  using namespace rswa;
+  constexpr const char* who = "cache_accept";
+  AcceptArgs a{};
+  RSWA_REQUIRE(d, RSWA_ERR_INVALID, "%s: null parameters", who);
+  const rswa_cache_params* p = &d->cache;
+  if (int rc = cache_args(p, who, a.n.c)) return rc;
+  RSWA_REQUIRE(d->path_len >= 0, RSWA_ERR_INVALID, "%s: negative size", who);
+  const int64_t rows = p->cu_seqlens_q ? p->total_q : (int64_t)p->batch * p->seqlen_q;
+  if (rows == 0 || p->batch == 0 || p->max_pages == 0 || d->path_len == 0) return RSWA_OK;
+  RSWA_REQUIRE(d->path, RSWA_ERR_INVALID, "%s: null path", who);
+  if (int rc = cache_new_rows(p, who, a.n.x, a.n.x_st)) return rc;
+  a.path = d->path;
+  a.path_st = d->path_stride;
+  a.path_len = d->path_len;
+  a.n.pages = (int32_t)(((int64_t)d->path_len + p->page_size - 2) / p->page_size + 1);
+  const int64_t blocks = 2 * (int64_t)p->batch * a.n.pages * p->heads_kv;
+  RSWA_REQUIRE(blocks < (1ll << 30), RSWA_ERR_UNSUPPORTED, "%s: %lld blocks", who, (long long)blocks);
+  a.n.by_pages = fast_div((uint32_t)a.n.pages);
+  a.n.by_heads = fast_div((uint32_t)p->heads_kv);
+  clear_launch_error();
+  auto go = [&](auto t, auto dim) {
+    hipLaunchKernelGGL((cache_accept_kernel<decltype(t), decltype(dim)::value>), dim3((unsigned)blocks), dim3(64), 0,
+                       (hipStream_t)stream, a);
+  };
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
+  if (p->dtype == RSWA_BF16)
+    p->head_dim == 128 ? go(__bf16{}, D128{}) : go(__bf16{}, D64{});
+  else
+    p->head_dim == 128 ? go(_Float16{}, D128{}) : go(_Float16{}, D64{});
+  return check_launch(who);
 }

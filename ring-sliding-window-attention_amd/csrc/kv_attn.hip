@@ -17,6 +17,7 @@ namespace rswa {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMaxWords = 16;  // of a node's ancestors, at most
 
 // Weights are taken 2^kLift times as large, and their sum with them, so that it cancels.  fp16: relative to the
 // largest they reach down to 2^-38 then instead of 2^-24, below which a long cache's many small weights would be lost.
@@ -24,16 +25,24 @@ constexpr int kThreads = 256;
 template <typename T>
 constexpr float kLift = std::is_same_v<T, _Float16> ? 14.f : -20.f;
 
-// The tiles of one row tile in one chunk: `n_a` from tile `a0`, then n_b from tile b0.
+// The tiles of one row tile in one chunk: `n_a` from tile `a0`, then n_b from tile b0 (and of nodes n_d from tile d0).
 struct TileList {
-  int a0, n_a, b0, n_b;
+  int a0, n_a, b0, n_b, d0, n_d;
   __device__ __forceinline__ int operator[](int i) const { return i < n_a ? a0 + i : b0 + (i - n_a); }
   __device__ __forceinline__ int count() const { return n_a + n_b; }
 };
 
-__device__ __forceinline__ TileList chunk_tiles(const CacheArgs& a, const Unit& x, int first, int last) {
-  const int s0 = x.chunk_idx * x.chunk, s1 = s0 + x.chunk;
+template <typename Args>
+__device__ __forceinline__ TileList chunk_tiles(const Args& a, const Unit& x, int first, int last) {
+  int s0 = x.chunk_idx * x.chunk, s1 = s0 + x.chunk;
   TileList t;
+  t.d0 = t.n_d = 0;
+  if constexpr (std::is_same_v<Args, TreeArgs>) {
+    t.d0 = min(s0, x.tiles.n_draft);
+    t.n_d = last < 0 ? 0 : min(s1, x.tiles.n_draft) - t.d0;
+    s0 = max(0, s0 - x.tiles.n_draft);
+    s1 = max(0, s1 - x.tiles.n_draft);
+  }
   t.a0 = min(s0, x.tiles.n_sink);
   t.n_a = min(s1, x.tiles.n_sink) - t.a0;
   int b0 = x.tiles.t_lo + max(0, s0 - x.tiles.n_sink);
@@ -144,9 +153,14 @@ __device__ __forceinline__ bool take_out_special(u32x4 (&codes)[N], uint32_t fro
 
 // 16 NT rows of a wave from row r0 of the sequence on: B operands of Q (the dimensions in the order in which a lane of
 // A holds K's), what each row sees, and the running softmax and output, O^T.
-template <typename T, int D, int NT>
+//
+// Nodes of a tree (TREE) come behind all cached tokens, at positions that do not follow from the row: a node's is read
+// from memory, where the mask needs it.  `first` is the last cached token, which all nodes see unless the window hides it,
+// and `last` a bound on the nodes' positions.
+template <typename T, int D, int NT, typename Args>
 struct Rows {
   using V8 = typename Mma<T>::V8;
+  static constexpr bool TREE = std::is_same_v<Args, TreeArgs>;
   static constexpr int C = D / 64;  // 16-byte pieces of a lane's key row
   static constexpr int ND = D / 16;
   V8 q[NT][C][2];
@@ -156,17 +170,27 @@ struct Rows {
   float m[NT], l[NT];
   float sc;
 
-  __device__ __forceinline__ Rows(const CacheArgs& a, const Unit& x, int hk, int r0, int col, int hi) {
+  __device__ __forceinline__ Rows(const Args& a, const Unit& x, int hk, int r0, int col, int hi) {
     const int shift = x.len - x.n_rows, n_flat = x.n_rows * a.group;  // shift: position of token 0
-    first = shift + quotient(min(r0, n_flat - 1), a.by_group);
-    last = r0 < n_flat ? shift + quotient(min(r0 + NT * 16, n_flat) - 1, a.by_group) : -1;
+    if constexpr (TREE) {
+      first = x.len - 1;
+      last = r0 < n_flat ? first + x.n_rows : -1;
+    } else {
+      first = shift + quotient(min(r0, n_flat - 1), a.by_group);
+      last = r0 < n_flat ? shift + quotient(min(r0 + NT * 16, n_flat) - 1, a.by_group) : -1;
+    }
     sc = 2.f * a.scale_log2;  // (K at half its value)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       const int r = r0 + nt * 16 + col;
       const int tok = quotient(min(r, n_flat - 1), a.by_group);
       const int head = hk * a.group + min(r, n_flat - 1) - tok * a.group;
-      pos[nt] = r < n_flat ? shift + tok : -1;
+      if constexpr (TREE) {
+        const int depth = a.depths[(int64_t)x.b * a.depths_st + x.row0 + tok];
+        pos[nt] = r < n_flat && depth >= 0 ? x.len + min(depth, x.n_rows - 1) : -1;
+      } else {
+        pos[nt] = r < n_flat ? shift + tok : -1;
+      }
       const T* p = (const T*)a.q + (int64_t)x.b * a.q_st[0] + (int64_t)(x.row0 + tok) * a.q_st[1] +
                    (int64_t)head * a.q_st[2] + hi * 16;
 #pragma unroll
@@ -182,17 +206,19 @@ struct Rows {
   __device__ __forceinline__ bool whole(const CacheArgs& a, int j0, bool here) const {
     return whole_tile(a, j0, here, first, last);
   }
+  // the last cached token that row nt may see
+  __device__ __forceinline__ int upto(int nt) const { return TREE ? (pos[nt] < 0 ? -1 : first) : pos[nt]; }
   // scores of what a row does not see become -inf; j: the lane's first key
   __device__ __forceinline__ void mask(const CacheArgs& a, f32x4 (&s)[NT][4], int j, bool here) const {
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      const int lo = a.window < 0 ? 0 : pos[nt] - a.window;
+      const int lo = a.window < 0 ? 0 : pos[nt] - a.window, end = upto(nt);
 #pragma unroll
       for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const int jj = j + 4 * t + e;
-          const bool see = here && jj <= pos[nt] && (jj >= lo || jj < a.n_sink);
+          const bool see = here && jj <= end && (jj >= lo || jj < a.n_sink);
           s[nt][t][e] = see ? s[nt][t][e] : -__builtin_inff();
         }
     }
@@ -224,7 +250,8 @@ struct Rows {
       }
     }
   }
-  // ... and the weights, P^T
+  // ... and the weights, P^T (or half of them)
+  template <bool HALF = false>
   __device__ __forceinline__ void weigh(const f32x4 (&s)[NT][4], V8 (&pf)[NT][2]) {
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -238,19 +265,55 @@ struct Rows {
           p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][2 * h + e / 4][e % 4], sc, -base));
           sum += p[e];
         }
+        if constexpr (HALF)
+#pragma unroll
+          for (int e = 0; e < 8; e++) p[e] *= 0.5f;
         // (weights are rounded to the type of the values' product: half a step of at most 1)
         pf[nt][h] = Mma<T>::pack(p);
       }
       l[nt] += sum;
     }
   }
+  // nodes that are not there see nothing (tiles that all nodes see are not masked for them)
+  __device__ __forceinline__ void leave_out() {
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+      if (pos[nt] < 0) {
+        m[nt] = -__builtin_inff();
+        l[nt] = 0.f;
+#pragma unroll
+        for (int d = 0; d < ND; d++) acc[d][nt] = f32x4{0, 0, 0, 0};
+      }
+  }
 };
+
+// Dimensions 16 d .. of O^T: `up` and `down` (A operands) are 1 where a value is positive (negative) and infinite, or NaN,
+// `sees` (B) where a row sees its key.
+template <typename T, int D, int NT, typename Args, typename V8 = typename Mma<T>::V8>
+__device__ __forceinline__ void add_specials(Rows<T, D, NT, Args>& w, int d, const V8 (&up)[2], const V8 (&down)[2],
+                                             const V8 (&sees)[NT][2]) {
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    f32x4 ups = {0, 0, 0, 0}, downs = {0, 0, 0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      ups = Mma<T>::mfma16(up[h], sees[nt][h], ups);
+      downs = Mma<T>::mfma16(down[h], sees[nt][h], downs);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      float o = w.acc[d][nt][e];
+      o = ups[e] > 0.f ? o + __builtin_inff() : o;
+      w.acc[d][nt][e] = downs[e] > 0.f ? o - __builtin_inff() : o;
+    }
+  }
+}
 
 // What take_out_special() left out of tiles i, i + step, .., of those that rows at positions first .. last do not all
 // see, for the rows that see it: two products of ones, 1 where a value is positive (negative) and infinite, or NaN, and 1
 // where a row sees its key.  A row that has both is NaN.
-template <typename T, int D, int NT>
-__device__ __forceinline__ void spoil(const CacheArgs& a, Rows<T, D, NT>& w, const Keys<D>& keys, const TileList& list,
+template <typename T, int D, int NT, typename Args>
+__device__ __forceinline__ void spoil(const Args& a, Rows<T, D, NT, Args>& w, const Keys<D>& keys, const TileList& list,
                                       int i, int step, int first, int last) {
   using V8 = typename Mma<T>::V8;
   const int n = list.count();
@@ -262,14 +325,14 @@ __device__ __forceinline__ void spoil(const CacheArgs& a, Rows<T, D, NT>& w, con
     V8 sees[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      const int lo = a.window < 0 ? 0 : w.pos[nt] - a.window;
+      const int lo = a.window < 0 ? 0 : w.pos[nt] - a.window, end = w.upto(nt);
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const int jj = j + 8 * h + e;
-          p[e] = here && jj <= w.pos[nt] && (jj >= lo || jj < a.n_sink) ? 1.f : 0.f;
+          p[e] = here && jj <= end && (jj >= lo || jj < a.n_sink) ? 1.f : 0.f;
         }
         sees[nt][h] = Mma<T>::pack(p);
       }
@@ -277,7 +340,7 @@ __device__ __forceinline__ void spoil(const CacheArgs& a, Rows<T, D, NT>& w, con
     const uint8_t* const from = keys.values(tile, id);
     const uint32_t specials = special_from<T>(keys.value_scale(id));
 #pragma unroll
-    for (int d = 0; d < Rows<T, D, NT>::ND; d++) {
+    for (int d = 0; d < D / 16; d++) {
       const u32x4 codes = *(const u32x4*)(from + d * 256);
       V8 up[2], down[2];  // (0x38 is the code of 1)
 #pragma unroll
@@ -293,31 +356,174 @@ __device__ __forceinline__ void spoil(const CacheArgs& a, Rows<T, D, NT>& w, con
         up[h] = widen8<T>(u[0], u[1], 1.f);
         down[h] = widen8<T>(n[0], n[1], 1.f);
       }
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
-        f32x4 ups = {0, 0, 0, 0}, downs = {0, 0, 0, 0};
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          ups = Mma<T>::mfma16(up[h], sees[nt][h], ups);
-          downs = Mma<T>::mfma16(down[h], sees[nt][h], downs);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          float o = w.acc[d][nt][e];
-          o = ups[e] > 0.f ? o + __builtin_inff() : o;
-          w.acc[d][nt][e] = downs[e] > 0.f ? o - __builtin_inff() : o;
-        }
-      }
+      add_specials(w, d, up, down, sees);
     }
+  }
+}
+
+// ---- the nodes' own keys and values, 64 to a tile, in their own type ------------------------------------------------
+//
+// As a tile of the cache: K from memory to the A operand, who sees whom from the nodes' ancestor bits.  Values lie in rows
+// and are transposed through LDS, by the block together, into the operands that a tile of the cache is widened to.  The
+// running softmax counts operands of the cache at half their value, so the nodes' scores are halved, and their weights for
+// the product with V: exact, but for fp16 weights below 2^-27 of the largest, which are multiples of 2^-37 of it.
+
+// Which of a lane's 16 nodes (from 64 tile + 16 hi on) does row nt see?  A bit for each.
+template <typename T, int D, int NT>
+__device__ __forceinline__ uint32_t seen_nodes(const TreeArgs& a, const Rows<T, D, NT, TreeArgs>& w, const Unit& x, int nt,
+                                               int r0, int tile, int hi) {
+  const int r = min(r0 + nt * 16 + (lane_id() & 15), x.n_rows * a.group - 1);
+  const int64_t row = x.row0 + quotient(r, a.by_group);
+  const int j = tile * kTileKeys + 16 * hi, left = max(0, min(16, x.n_rows - j));
+  const uint64_t word = (uint64_t)a.ancestors[(int64_t)x.b * a.ancestors_st + row * a.words + tile];
+  uint32_t bits = (uint32_t)(word >> (16 * hi)) & ((1u << left) - 1u);
+  if (a.window >= 0 && x.n_rows - 1 > a.window) {  // (else no two depths are that far apart)
+    const int32_t* const depths = a.depths + (int64_t)x.b * a.depths_st + x.row0;
+#pragma unroll 1
+    for (int e = 0; e < left; e++) {
+      const int place = x.len + depths[j + e];
+      if (place < w.pos[nt] - a.window && place >= a.n_sink) bits &= ~(1u << e);
+    }
+  }
+  return w.pos[nt] < 0 ? 0u : bits;
+}
+
+template <typename T>
+__device__ __forceinline__ bool not_finite(T v) {
+  constexpr uint16_t exponent = std::is_same_v<T, __bf16> ? 0x7f80 : 0x7c00;
+  return (__builtin_bit_cast(uint16_t, v) & exponent) == exponent;
+}
+
+// V^T of a tile of nodes as A operands in `ops` [D / 16][2][64 lanes], without values that are not finite; a byte of
+// `special` for each wave says whether it found any.  A thread transposes 8 nodes of 4 dimensions.
+template <typename T, int D>
+__device__ __forceinline__ void stage_node_values(const TreeArgs& a, const Unit& x, int hk, int tile,
+                                                  typename Mma<T>::V8* ops, uint32_t* special) {
+  using V4 = typename Mma<T>::V4;
+  using V8 = typename Mma<T>::V8;
+  constexpr int LANES = D / 4;
+  const int d0 = (int)threadIdx.x % LANES * 4, octet = (int)threadIdx.x / LANES;
+  bool any = false;
+  if (octet < 8) {
+    const T* const p = (const T*)a.v_new + (int64_t)x.b * a.vn_st[0] + (int64_t)hk * a.vn_st[2] + d0;
+    V4 v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      v[e] = *(const V4*)(p + (int64_t)(x.row0 + min(tile * kTileKeys + octet * 8 + e, x.n_rows - 1)) * a.vn_st[1]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      V8 of;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const bool real = tile * kTileKeys + octet * 8 + e < x.n_rows, special_value = not_finite(v[e][i]);
+        of[e] = real && !special_value ? v[e][i] : (T)0.f;
+        any |= real && special_value;
+      }
+      const int d = d0 + i;
+      ops[((d / 16) * 2 + (octet & 1)) * 64 + (octet >> 1) * 16 + d % 16] = of;
+    }
+  }
+  const bool found = __builtin_amdgcn_ballot_w64(any) != 0;
+  if (lane_id() == 0) ((uint8_t*)special)[threadIdx.x / 64] = found;
+}
+
+template <typename T, int D, int NT>
+__device__ __forceinline__ void add_nodes(const TreeArgs& a, Rows<T, D, NT, TreeArgs>& w, const Unit& x, int hk, int r0,
+                                          int tile, const typename Mma<T>::V8* ops) {
+  using R = Rows<T, D, NT, TreeArgs>;
+  using V8 = typename Mma<T>::V8;
+  const int lane = lane_id(), col = lane & 15, hi = lane >> 4;
+  const T* const p = (const T*)a.k_new + (int64_t)x.b * a.kn_st[0] + (int64_t)hk * a.kn_st[2] + hi * 16;
+  uint32_t sees[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) sees[nt] = seen_nodes(a, w, x, nt, r0, tile, hi);
+  f32x4 s[NT][4];
+#pragma unroll
+  for (int t = 0; t < 4; t++) {
+    const int key = min(tile * kTileKeys + 16 * (col >> 2) + 4 * t + (col & 3), x.n_rows - 1);
+    const T* const row = p + (int64_t)(x.row0 + key) * a.kn_st[1];
+    V8 kf[R::C][2];
+#pragma unroll
+    for (int c = 0; c < R::C; c++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) kf[c][h] = *(const V8*)(row + c * 64 + h * 8);
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      s[nt][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < R::C; c++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) s[nt][t] = Mma<T>::mfma16(kf[c][h], w.q[nt][c][h], s[nt][t]);
+    }
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) s[nt][t][e] = sees[nt] >> (4 * t + e) & 1 ? 0.5f * s[nt][t][e] : -__builtin_inff();
+  V8 pf[NT][2];
+  float top[NT];
+  w.tops(s, top);
+  w.raise(top);
+  w.template weigh<true>(s, pf);
+#pragma unroll
+  for (int d = 0; d < R::ND; d++)
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const V8 vf = ops[(d * 2 + h) * 64 + lane];
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) w.acc[d][nt] = Mma<T>::mfma16(vf, pf[nt][h], w.acc[d][nt]);
+    }
+}
+
+// What stage_node_values() left out of a tile, for the rows that see it (as spoil()).
+template <typename T, int D, int NT>
+__device__ __forceinline__ void spoil_nodes(const TreeArgs& a, Rows<T, D, NT, TreeArgs>& w, const Unit& x, int hk, int r0,
+                                            int tile) {
+  using V8 = typename Mma<T>::V8;
+  const int lane = lane_id(), col = lane & 15, hi = lane >> 4;
+  V8 sees[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    const uint32_t bits = seen_nodes(a, w, x, nt, r0, tile, hi);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) p[e] = bits >> (8 * h + e) & 1 ? 1.f : 0.f;
+      sees[nt][h] = Mma<T>::pack(p);
+    }
+  }
+  const T* const p = (const T*)a.v_new + (int64_t)x.b * a.vn_st[0] + (int64_t)hk * a.vn_st[2] + col;
+#pragma unroll
+  for (int d = 0; d < D / 16; d++) {
+    V8 up[2], down[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      float u[8], n[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int key = tile * kTileKeys + 16 * hi + 8 * h + e;
+        const float v = (float)p[(int64_t)(x.row0 + min(key, x.n_rows - 1)) * a.vn_st[1] + d * 16];
+        const bool real = key < x.n_rows, nan = v != v;
+        u[e] = real && (nan || v == __builtin_inff()) ? 1.f : 0.f;
+        n[e] = real && (nan || v == -__builtin_inff()) ? 1.f : 0.f;
+      }
+      up[h] = Mma<T>::pack(u);
+      down[h] = Mma<T>::pack(n);
+    }
+    add_specials(w, d, up, down, sees);
   }
 }
 
 // The kernel's arguments read again: those of the epilogue alone would be loaded ahead of the loop, where they crowd
 // others out of the scalar registers.
-__device__ __forceinline__ const CacheArgs& arguments_again() {
-  auto p = (const __attribute__((address_space(4))) CacheArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+template <typename Args>
+__device__ __forceinline__ const Args& arguments_again() {
+  auto p = (const __attribute__((address_space(4))) Args*)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(p));
-  return *(const CacheArgs*)p;
+  return *(const Args*)p;
 }
 
 // Where row r's result goes: to the output, or to the join if the row has several chunks.
@@ -356,9 +562,10 @@ struct RowOut {
 
 // Few rows: the four waves of a block have the same rows, each its own keys, and everything from memory to the output
 // stays in registers; the waves meet in LDS at the end.
-template <typename T, int D, int NT>
-__global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(const CacheArgs a) {
-  using R = Rows<T, D, NT>;
+template <typename T, int D, int NT, typename Args>
+__global__ __launch_bounds__(kThreads, (NT == 1 && !std::is_same_v<Args, TreeArgs>) ? 3 : 2) void cache_attn_kernel(
+    const Args a) {
+  using R = Rows<T, D, NT, Args>;
   using V8 = typename Mma<T>::V8;
   constexpr int KW = 4, ROWS = NT * 16, C = R::C, ND = R::ND;
   constexpr int LD = D + 4;
@@ -390,7 +597,7 @@ __global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(c
   };
 
   const int n = list.count();
-  int i = wave;
+  int i = R::TREE ? (wave - list.n_d) & (KW - 1) : wave;  // (waves that have a tile of nodes come last)
   Pages next{0, 0};
   bool here = false;  // the lane's group of the tile has its page
   if (i < n) {
@@ -399,6 +606,16 @@ __global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(c
     next = keys.pages(list[min(i + KW, n - 1)]);
     load_k(list[i], now.k);
     load_v(list[i], now.v);
+  }
+  __shared__ uint32_t lds_special[R::TREE ? kMaxWords : 1];
+  if constexpr (R::TREE) {
+#pragma unroll 1
+    for (int t = 0; t < list.n_d; t++) {
+      if (t > 0) __syncthreads();
+      stage_node_values<T, D>(a, x, hk, list.d0 + t, (V8*)lds, &lds_special[t]);
+      __syncthreads();
+      if (wave == (t & (KW - 1))) add_nodes(a, w, x, hk, x.row_tile * ROWS, list.d0 + t, (const V8*)lds);
+    }
   }
   bool spoiled = false;  // (one token's rows see the same keys: nothing to tell apart)
   for (; i < n; i += KW) {
@@ -432,10 +649,10 @@ __global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(c
     w.weigh(s, pf);
     // what no row of the wave sees may hold anything, NaN and infinities included: a weight of zero does not cancel those
     if (!whole) {
-      const u32x4 keep = seen_bytes(a, j0 + hi * 16, here, w.first, w.last);
+      const u32x4 keep = seen_bytes(a, j0 + hi * 16, here, R::TREE ? w.first + 1 : w.first, R::TREE ? w.first : w.last);
 #pragma unroll
       for (int d = 0; d < ND; d++) vb[d] &= keep;
-      if (w.first != w.last) spoiled |= take_out_special(vb, special_from<T>(ve));
+      if (R::TREE ? a.window >= 0 : w.first != w.last) spoiled |= take_out_special(vb, special_from<T>(ve));
     }
     const float vscale = half_scale(ve);
 #pragma unroll
@@ -451,8 +668,14 @@ __global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(c
     next = after;
   }
 
-  const CacheArgs& late = arguments_again();
-  if (spoiled) spoil(late, w, keys, list, wave, KW, w.first, w.last);
+  const Args& late = arguments_again<Args>();
+  if (spoiled) spoil(late, w, keys, list, R::TREE ? (wave - list.n_d) & (KW - 1) : wave, KW, w.first, w.last);
+  if constexpr (R::TREE) {
+    for (int t = wave; t < list.n_d; t += KW)
+      if (lds_special[t]) spoil_nodes(late, w, x, hk, x.row_tile * ROWS, list.d0 + t);
+    w.leave_out();
+    if (list.n_d > 0) __syncthreads();
+  }
   float* ml = lds + KW * ROWS * LD;
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
@@ -497,9 +720,9 @@ __global__ __launch_bounds__(kThreads, NT == 1 ? 3 : 2) void cache_attn_kernel(c
 // each wave widening all of a tile for itself took a tenth longer, and so did the loop unskewed).  Of the time the matrix
 // pipes are busy 49 %, the vector ones 52 %, both at once 15 %, and LDS 59 %: what bounds it is how the two waves of a SIMD
 // (all that the registers allow) fill each other's gaps.
-template <typename T, int D, int NT>
-__global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const CacheArgs a) {
-  using R = Rows<T, D, NT>;
+template <typename T, int D, int NT, typename Args>
+__global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Args a) {
+  using R = Rows<T, D, NT, Args>;
   using V8 = typename Mma<T>::V8;
   constexpr int C = R::C, ND = R::ND, NV = ND / 4;
   constexpr int KF = 4 * C * 2, VF = ND * 2;  // operands of a tile
@@ -515,8 +738,8 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
   R w(a, x, hk, r0 + wave * (NT * 16), col, hi);
   // the block's rows
   const int shift = x.len - x.n_rows, n_flat = x.n_rows * a.group;
-  const int first = shift + quotient(r0, a.by_group);
-  const int last = shift + quotient(min(r0 + 4 * NT * 16, n_flat) - 1, a.by_group);
+  const int first = R::TREE ? x.len - 1 : shift + quotient(r0, a.by_group);
+  const int last = R::TREE ? first + x.n_rows : shift + quotient(min(r0 + 4 * NT * 16, n_flat) - 1, a.by_group);
   const TileList list = chunk_tiles(a, x, first, last);
   const Keys<D> keys(a, x, hk, lane);
   const int n = list.count();
@@ -550,7 +773,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
     const int j0 = tile * kTileKeys;
     const bool here = keys.there(id);
     if (whole_tile(a, j0, here, first, last)) return;
-    const u32x4 keep = seen_bytes(a, j0 + hi * 16, here, first, last);
+    const u32x4 keep = seen_bytes(a, j0 + hi * 16, here, R::TREE ? first + 1 : first, R::TREE ? first : last);
 #pragma unroll
     for (int d = 0; d < NV; d++) vb[d] &= keep;
     spoiled |= take_out_special(vb, special_from<T>(ve));
@@ -591,6 +814,17 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
     if (!w.whole(a, j0, here)) w.mask(a, s, j0 + hi * 16, here);
   };
 
+  __shared__ uint32_t lds_special[R::TREE ? kMaxWords : 1];
+  if constexpr (R::TREE) {
+#pragma unroll 1
+    for (int t = 0; t < list.n_d; t++) {
+      if (t > 0) __syncthreads();
+      stage_node_values<T, D>(a, x, hk, list.d0 + t, &v_ops[0][0][0], &lds_special[t]);
+      __syncthreads();
+      add_nodes(a, w, x, hk, r0 + wave * (NT * 16), list.d0 + t, &v_ops[0][0][0]);
+    }
+    if (list.n_d > 0) __syncthreads();
+  }
   Pages p[4] = {};  // of tiles i .. i + 3
   if (n > 0) {
 #pragma unroll
@@ -681,11 +915,16 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
     step(i, s0, s1);
     if (i + 1 < n) step(i + 1, s1, s0);
   }
-  const CacheArgs& late = arguments_again();
+  const Args& late = arguments_again<Args>();
   if (n > 0) {  // (each wave has looked at its quarter of the values)
     if (spoiled && lane == 0) any_special = 1;
     __syncthreads();
     if (__builtin_amdgcn_readfirstlane(any_special)) spoil(late, w, keys, list, 0, 1, first, last);
+  }
+  if constexpr (R::TREE) {
+    for (int t = 0; t < list.n_d; t++)
+      if (lds_special[t]) spoil_nodes(late, w, x, hk, r0 + wave * (NT * 16), list.d0 + t);
+    w.leave_out();
   }
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
@@ -703,8 +942,8 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Cach
 // meet in LDS.  (A thread that went over all chunks one by one waited for each: 7.4 us for the 16 chunks of one token
 // over 4001, 17 for 16 drafts of 5.)  A block does GROUPS groups of rows in turn: with chunks of a prompt, which mostly
 // are not split, most blocks find nothing to do, and 4 groups are 5 us instead of 9; with drafts 7.5 instead of 4.
-template <typename T, int D, int P, int GROUPS>
-__global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheArgs a) {
+template <typename T, int D, int P, int GROUPS, typename Args>
+__global__ __launch_bounds__(kThreads) void cache_join_kernel(const Args a) {
   constexpr int LANES = D / 4, ROWS = kThreads / LANES / P, N = 4;
   __shared__ f32x4 lds_o[P > 1 ? P : 1][ROWS * LANES];
   __shared__ f32x2 lds_ml[P > 1 ? P : 1][ROWS];
@@ -775,7 +1014,8 @@ struct Cut {
   int64_t part_units;  // at most
   int64_t grid;
 };
-Cut cut_call(const rswa_cache_params* p) {
+// `words`: tiles that a sequence's nodes are at most (0: rows are no nodes).
+Cut cut_call(const rswa_cache_params* p, int words = 0) {
   Cut c;
   const int64_t group = p->heads_q / p->heads_kv;
   const int64_t rows = p->cu_seqlens_q ? ceil_div(p->total_q * group, std::max(1, p->batch)) : p->seqlen_q * group;
@@ -800,6 +1040,7 @@ Cut cut_call(const rswa_cache_params* p) {
     most_tiles = std::min(most_tiles, (p->window_left + rows_seq + kTileKeys - 2) / kTileKeys + 1 +
                                           ceil_div(p->num_sink, kTileKeys));
   }
+  if (words) most_tiles += p->cu_seqlens_q ? words : std::min<int64_t>(words, ceil_div(p->seqlen_q, kTileKeys));
   const int64_t at_most = std::min(ceil_div(8 * per_head, 5), c.row_tiles * most_tiles);
   // few tiles are not split: the join costs what a wave's third tile does (one token: 512 keys 8.0 us whole, 10.1 in two
   // launches, 768 9.2 / 10.2, 1024 10.5 / 10.3; own rows: 500 keys 21.9 / 25.2, 1000 33.2 / 32.7)
@@ -813,16 +1054,16 @@ uint64_t part_bytes(const Cut& c, const rswa_cache_params* p) {
   return (uint64_t)c.part_units * p->heads_kv * c.row_tile * (p->head_dim + 2) * 4;
 }
 
-template <typename T, int D>
-int launch_attn(CacheArgs& a, const Cut& c, hipStream_t stream) {
+template <typename T, int D, typename Args>
+int launch_attn(const Args& a, const Cut& c, hipStream_t stream) {
   const dim3 grid((unsigned)c.grid), block(kThreads);
   clear_launch_error();
   if (c.nt == 1)
-    hipLaunchKernelGGL((cache_attn_kernel<T, D, 1>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((cache_attn_kernel<T, D, 1, Args>), grid, block, 0, stream, a);
   else if (c.wr == 1)
-    hipLaunchKernelGGL((cache_attn_kernel<T, D, 2>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((cache_attn_kernel<T, D, 2, Args>), grid, block, 0, stream, a);
   else
-    hipLaunchKernelGGL((cache_attn_rows_kernel<T, D, 2>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((cache_attn_rows_kernel<T, D, 2, Args>), grid, block, 0, stream, a);
   if (int rc = check_launch("cache_attn")) return rc;
   if (c.part_units == 0) return RSWA_OK;
   // as many chunks a row (on average) as threads that may share one, or one thread for all
@@ -833,39 +1074,27 @@ int launch_attn(CacheArgs& a, const Cut& c, hipStream_t stream) {
     return dim3((unsigned)(per_head * a.heads_kv));
   };
   if (c.row_tiles * a.heads_kv * P <= c.wanted)
-    hipLaunchKernelGGL((cache_join_kernel<T, D, P, 1>), join_blocks(1), block, 0, stream, a);
+    hipLaunchKernelGGL((cache_join_kernel<T, D, P, 1, Args>), join_blocks(1), block, 0, stream, a);
   else if (c.wr == 1)
-    hipLaunchKernelGGL((cache_join_kernel<T, D, 1, 1>), join_blocks(P), block, 0, stream, a);
+    hipLaunchKernelGGL((cache_join_kernel<T, D, 1, 1, Args>), join_blocks(P), block, 0, stream, a);
   else
-    hipLaunchKernelGGL((cache_join_kernel<T, D, 1, 4>), join_blocks(4 * P), block, 0, stream, a);
+    hipLaunchKernelGGL((cache_join_kernel<T, D, 1, 4, Args>), join_blocks(4 * P), block, 0, stream, a);
   return check_launch("cache_attn join");
 }
 
-}  // namespace
-}  // namespace rswa
-
-extern "C" uint64_t rswa_cache_attn_workspace_bytes(const rswa_cache_params* p) {
-  using namespace rswa;
-  if (!p || p->heads_kv <= 0 || p->heads_q < p->heads_kv || p->page_size <= 0) return 0;
-  return part_bytes(cut_call(p), p);
-}
-
-extern "C" int rswa_cache_attn(const rswa_cache_params* p, void* stream) {
-  using namespace rswa;
-  CacheArgs a;
-  if (int rc = cache_args(p, "cache_attn", a)) return rc;
-  const int64_t rows = p->cu_seqlens_q ? p->total_q : (int64_t)p->batch * p->seqlen_q;
-  if (rows == 0 || p->batch == 0) return RSWA_OK;
-  if (int rc = cache_query_args(p, "cache_attn", a)) return rc;
-  RSWA_REQUIRE(p->out, RSWA_ERR_INVALID, "cache_attn: null tensor");
+// The rest of a call whose cache has been looked over.
+template <typename Args>
+int attention(const rswa_cache_params* p, int words, const char* who, Args& a, void* stream) {
+  if (int rc = cache_query_args(p, who, a)) return rc;
+  RSWA_REQUIRE(p->out, RSWA_ERR_INVALID, "%s: null tensor", who);
   RSWA_REQUIRE((uintptr_t)p->out % 16 == 0 && p->out_stride[0] % 8 == 0 && p->out_stride[1] % 8 == 0 &&
                    p->out_stride[2] % 8 == 0,
-               RSWA_ERR_UNSUPPORTED, "cache_attn: rows of out must be 16-byte aligned");
-  const Cut c = cut_call(p);
-  RSWA_REQUIRE(c.grid < (1ll << 31), RSWA_ERR_UNSUPPORTED, "cache_attn: %lld blocks", (long long)c.grid);
+               RSWA_ERR_UNSUPPORTED, "%s: rows of out must be 16-byte aligned", who);
+  const Cut c = cut_call(p, words);
+  RSWA_REQUIRE(c.grid < (1ll << 31), RSWA_ERR_UNSUPPORTED, "%s: %lld blocks", who, (long long)c.grid);
   RSWA_REQUIRE(c.part_units == 0 || (p->workspace && (uintptr_t)p->workspace % 16 == 0 &&
                                      p->workspace_bytes >= part_bytes(c, p)),
-               RSWA_ERR_INVALID, "cache_attn: workspace of %llu bytes, %llu needed (16-byte aligned)",
+               RSWA_ERR_INVALID, "%s: workspace of %llu bytes, %llu needed (16-byte aligned)", who,
                (unsigned long long)p->workspace_bytes, (unsigned long long)part_bytes(c, p));
   a.out = p->out;
   a.lse = p->lse;
@@ -885,3 +1114,62 @@ extern "C" int rswa_cache_attn(const rswa_cache_params* p, void* stream) {
     return p->head_dim == 128 ? launch_attn<__bf16, 128>(a, c, st) : launch_attn<__bf16, 64>(a, c, st);
   return p->head_dim == 128 ? launch_attn<_Float16, 128>(a, c, st) : launch_attn<_Float16, 64>(a, c, st);
 }
+
+}  // namespace
+}  // namespace rswa
+
+extern "C" uint64_t rswa_cache_attn_workspace_bytes(const rswa_cache_params* p) {
+  using namespace rswa;
+  if (!p || p->heads_kv <= 0 || p->heads_q < p->heads_kv || p->page_size <= 0) return 0;
+  return part_bytes(cut_call(p), p);
+}
+
+extern "C" int rswa_cache_attn(const rswa_cache_params* p, void* stream) {
+  using namespace rswa;
+  CacheArgs a;
+  if (int rc = cache_args(p, "cache_attn", a)) return rc;
+  const int64_t rows = p->cu_seqlens_q ? p->total_q : (int64_t)p->batch * p->seqlen_q;
+  if (rows == 0 || p->batch == 0) return RSWA_OK;
+  return attention(p, 0, "cache_attn", a, stream);
+}
+
+extern "C" uint64_t rswa_cache_tree_attn_workspace_bytes(const rswa_draft_params* d) {
+  using namespace rswa;
+  if (!d || d->words <= 0 || d->words > kMaxWords) return 0;
+  const rswa_cache_params* p = &d->cache;
+  if (p->heads_kv <= 0 || p->heads_q < p->heads_kv || p->page_size <= 0) return 0;
+  return part_bytes(cut_call(p, d->words), p);
+}
+
+extern "C" int rswa_cache_tree_attn(const rswa_draft_params* d, void* stream) {
+  using namespace rswa;
+  constexpr const char* who = "cache_tree_attn";
+  TreeArgs a{};
+  RSWA_REQUIRE(d, RSWA_ERR_INVALID, "%s: null parameters", who);
+  const rswa_cache_params* p = &d->cache;
+  if (int rc = cache_args(p, who, a)) return rc;
+  const int64_t rows = p->cu_seqlens_q ? p->total_q : (int64_t)p->batch * p->seqlen_q;
+  if (rows == 0 || p->batch == 0) return RSWA_OK;
+  RSWA_REQUIRE(d->words >= 1 && d->words <= kMaxWords, RSWA_ERR_UNSUPPORTED, "%s: %d words of ancestors (1 to %d)", who,
+               d->words, kMaxWords);
+  RSWA_REQUIRE(p->cu_seqlens_q || p->seqlen_q <= 64 * d->words, RSWA_ERR_INVALID, "%s: %d nodes, and ancestors of %d", who,
+               p->seqlen_q, 64 * d->words);
+  RSWA_REQUIRE(d->depths && d->ancestors, RSWA_ERR_INVALID, "%s: null tree", who);
+  const void* x[2];
+  int64_t st[2][3];
+  if (int rc = cache_new_rows(p, who, x, st)) return rc;
+  a.depths = d->depths;
+  a.ancestors = d->ancestors;
+  a.depths_st = a.cu ? 0 : d->depths_stride;
+  a.ancestors_st = a.cu ? 0 : d->ancestors_stride;
+  a.words = d->words;
+  a.k_new = x[0];
+  a.v_new = x[1];
+  for (int i = 0; i < 3; i++) {
+    a.kn_st[i] = st[0][i];
+    a.vn_st[i] = st[1][i];
+  }
+  return attention(p, d->words, who, a, stream);
+}
+
+extern "C" uint64_t rswa_sizeof_draft_params(void) { return sizeof(rswa_draft_params); }

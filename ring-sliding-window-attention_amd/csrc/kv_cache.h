@@ -52,6 +52,17 @@ struct CacheArgs {
   int32_t w_len;
 };
 
+// ... and of rswa_draft_params: queries that are nodes of a tree of drafted tokens.
+struct TreeArgs : CacheArgs {
+  const int32_t* depths;
+  const int64_t* ancestors;
+  int64_t depths_st, ancestors_st;  // sequence
+  int32_t words;                    // of a node's ancestors, and tiles of 64 nodes that a sequence has at most
+  const void* k_new;                // the nodes' own
+  const void* v_new;
+  int64_t kn_st[3], vn_st[3];
+};
+
 __device__ __forceinline__ int lane_id() {
   return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
 }
@@ -135,17 +146,27 @@ struct Sequence {
 };
 
 // The tiles that rows at positions first .. last (the end of the sequence) see: those of the sink keys ahead of the
-// band, from tile 0 on, then n_band from tile t_lo on.
+// band, from tile 0 on, then n_band from tile t_lo on.  Ahead of them all, n_draft tiles of nodes.
 struct SeenTiles {
-  int n_sink, t_lo, n_band;
-  __device__ __forceinline__ int count() const { return n_sink + n_band; }
+  int n_sink, t_lo, n_band, n_draft;
+  __device__ __forceinline__ int count() const { return n_draft + n_sink + n_band; }
 };
 __device__ __forceinline__ SeenTiles seen_tiles(const CacheArgs& a, int first, int last) {
-  SeenTiles t{0, 0, 0};
+  SeenTiles t{0, 0, 0, 0};
   if (last < 0) return t;
   const int lo = a.window < 0 ? 0 : max(0, first - a.window);
   t.t_lo = lo / kTileKeys;
   t.n_band = last / kTileKeys - t.t_lo + 1;
+  t.n_sink = min((min(a.n_sink, lo) + kTileKeys - 1) / kTileKeys, t.t_lo);
+  return t;
+}
+// ... and that a sequence's nodes do: all come behind its tokens, the first of them at position `len`.
+__device__ __forceinline__ SeenTiles seen_tiles(const TreeArgs& a, int len, int nodes) {
+  SeenTiles t{0, 0, 0, min((nodes + kTileKeys - 1) / kTileKeys, a.words)};
+  if (len <= 0) return t;
+  const int lo = a.window < 0 ? 0 : max(0, len - a.window);
+  t.t_lo = lo / kTileKeys;
+  t.n_band = (len - 1) / kTileKeys - t.t_lo + 1;  // (0 where the window holds no token and a tile ends with the last)
   t.n_sink = min((min(a.n_sink, lo) + kTileKeys - 1) / kTileKeys, t.t_lo);
   return t;
 }
@@ -170,18 +191,22 @@ struct Unit {
 };
 
 // JOIN > 0: units are JOIN rows from x.row on, and `part` is the sequence's first partial result.
-template <int JOIN>
-__device__ __forceinline__ bool find_unit(const CacheArgs& a, int u, Unit& x) {
+template <int JOIN, typename Args>
+__device__ __forceinline__ bool find_unit(const Args& a, int u, Unit& x) {
+  constexpr bool TREE = std::is_same_v<Args, TreeArgs>;
   const int lane = lane_id();
   int row0 = 0, n = 0, len = 0, row_tiles = 0;
-  SeenTiles t{0, 0, 0};
+  SeenTiles t{0, 0, 0, 0};
   auto load = [&](int b) { return Sequence(a, min(b, a.batch - 1)); };
   auto take = [&](const Sequence& s, int b) {
     s.rows(a, row0, n);
     len = s.tokens(a);
     n = b < a.batch ? n : 0;
     row_tiles = (n * a.group + (1 << a.row_log2) - 1) >> a.row_log2;  // (below 2^30 rows)
-    t = n > 0 ? seen_tiles(a, len - n, len - 1) : SeenTiles{0, 0, 0};
+    if constexpr (TREE)
+      t = n > 0 ? seen_tiles(a, len, n) : SeenTiles{0, 0, 0, 0};
+    else
+      t = n > 0 ? seen_tiles(a, len - n, len - 1) : SeenTiles{0, 0, 0, 0};
   };
   // (fused by hand: attention and join must come to the same chunk)
   float total = 0.f;
@@ -230,12 +255,43 @@ __device__ __forceinline__ bool find_unit(const CacheArgs& a, int u, Unit& x) {
       x.tiles.n_sink = of(t.n_sink);
       x.tiles.t_lo = of(t.t_lo);
       x.tiles.n_band = of(t.n_band);
+      x.tiles.n_draft = TREE ? of(t.n_draft) : 0;
       return true;
     }
     before += __builtin_amdgcn_readlane(su, 63);
     before_part += __builtin_amdgcn_readlane(sp, 63);
   }
   return false;
+}
+
+// Of rows that lie behind `held` tokens of their sequences: sequence b, its rows, and which of the pages that they touch
+// (u, from 0 on; below 0: none) is slot u's.  `pages`: of a sequence at most (dense).
+__device__ __forceinline__ void touched_page(const CacheArgs& c, int pages, const FastDiv& by_pages, int& u, int& b,
+                                             int& row0, int& n) {
+  if (c.cu) {
+    // sequence b owns the slots from cu[b] / page_size + 2 b on: n tokens touch at most n / page_size + 2 pages.
+    // (a search 64 ways at a time, as locate_packed)
+    const int lane = lane_id();
+    int lo = 0, cnt = c.batch;
+    for (;;) {
+      const int step = (cnt + 63) >> 6;
+      const int i = min(lo + lane * step, lo + cnt - 1);
+      const int slot = (max(0, min(c.cu[i], c.total_q)) >> c.page_log2) + 2 * i;
+      // (none: rows ahead of the first sequence; the count is unsigned)
+      const int at = max((int)__popcll(__builtin_amdgcn_ballot_w64(lane * step < cnt && slot <= u)) - 1, 0);
+      lo += at * step;
+      if (step == 1) break;
+      cnt = min(step, cnt - at * step);
+    }
+    b = __builtin_amdgcn_readfirstlane(lo);
+    Sequence(c, b).rows(c, row0, n);
+    u -= (row0 >> c.page_log2) + 2 * b;
+  } else {
+    b = quotient(u, by_pages);
+    u -= b * pages;
+    row0 = 0;
+    n = c.seqlen_q;
+  }
 }
 
 // Two e4m3 codes (the low or the high half of a word) times a power of two, in the matrix operand's type: one
@@ -286,5 +342,7 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float f) {
 // Checks of rswa_cache_params that every call makes, and the kernels' view of them.
 int cache_args(const rswa_cache_params* p, const char* who, CacheArgs& a);
 int cache_query_args(const rswa_cache_params* p, const char* who, CacheArgs& a);
+// Rows that a call's new keys and values are, or go to.
+int cache_new_rows(const rswa_cache_params* p, const char* who, const void* (&x)[2], int64_t (&st)[2][3]);
 
 }  // namespace rswa

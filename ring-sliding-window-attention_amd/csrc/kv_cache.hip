@@ -85,6 +85,22 @@ int cache_query_args(const rswa_cache_params* p, const char* who, CacheArgs& a) 
   return RSWA_OK;
 }
 
+int cache_new_rows(const rswa_cache_params* p, const char* who, const void* (&x)[2], int64_t (&st)[2][3]) {
+  RSWA_REQUIRE(p->new_k && p->new_v, RSWA_ERR_INVALID, "%s: null tensor", who);
+  x[0] = p->new_k;
+  x[1] = p->new_v;
+  for (int i = 0; i < 3; i++) {
+    st[0][i] = p->new_k_stride[i];
+    st[1][i] = p->new_v_stride[i];
+  }
+  for (int w = 0; w < 2; w++) {
+    RSWA_REQUIRE((uintptr_t)x[w] % 16 == 0 && st[w][0] % 8 == 0 && st[w][1] % 8 == 0 && st[w][2] % 8 == 0,
+                 RSWA_ERR_UNSUPPORTED, "%s: rows of new_k and new_v must be 16-byte aligned", who);
+    if (p->cu_seqlens_q) st[w][0] = 0;
+  }
+  return RSWA_OK;
+}
+
 }  // namespace rswa
 
 extern "C" uint64_t rswa_sizeof_cache_params(void) { return sizeof(rswa_cache_params); }

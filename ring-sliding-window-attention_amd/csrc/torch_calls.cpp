@@ -296,6 +296,13 @@ struct {
   int (*weights)(const rswa_cache_params*, void*) = nullptr;
   int (*evict)(const rswa_cache_params*, void*) = nullptr;
   uint64_t (*attn_bytes)(const rswa_cache_params*) = nullptr;
+  int (*read)(const rswa_cache_params*, void*) = nullptr;
+  int (*draft_tree)(const rswa_tree_params*, void*) = nullptr;
+  int (*tree_attn)(const rswa_draft_params*, void*) = nullptr;
+  uint64_t (*tree_attn_bytes)(const rswa_draft_params*) = nullptr;
+  int (*accept)(const rswa_draft_params*, void*) = nullptr;
+  int (*verify)(const rswa_verify_params*, void*) = nullptr;
+  uint64_t (*verify_bytes)(const rswa_verify_params*) = nullptr;
 } cache_lib;
 
 // A tensor argument that the calls take as it is; null: the Python route sees to it.
@@ -323,6 +330,14 @@ bool int_arg(PyObject* o, int64_t& v) {
   int over = 0;
   v = PyLong_AsLongLongAndOverflow(o, &over);
   return !over;
+}
+
+// 0, or the library's status with nothing launched
+template <typename Params>
+int launch_call(int (*entry)(const Params*, void*), const Params& p, c10::Device device) {
+  void* const stream = (void*)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device.index()).stream();
+  pybind11::gil_scoped_release others_run;
+  return entry(&p, stream);
 }
 
 struct CacheCall {
@@ -403,7 +418,7 @@ struct CacheCall {
 
   bool queries(const Tensor& q, PyObject* cu, PyObject* window_o, PyObject* scale_o, PyObject* sinks_o) {
     int64_t window, sinks;
-    if (!rows(q, cu) || q.numel() == 0 || p.max_pages == 0 || q.size(-2) % p.heads_kv != 0) return false;
+    if (!rows(q, cu) || q.numel() == 0 || q.size(-2) % p.heads_kv != 0) return false;
     if (!int_arg(window_o, window) || !int_arg(sinks_o, sinks) || sinks < 0) return false;
     if (scale_o == Py_None) p.softmax_scale = (float)std::pow((double)p.head_dim, -0.5);
     else if (PyFloat_CheckExact(scale_o)) p.softmax_scale = (float)PyFloat_AS_DOUBLE(scale_o);
@@ -414,6 +429,19 @@ struct CacheCall {
     p.q = q.data_ptr();
     strides3(p.q_stride, q, packed);
     return true;
+  }
+
+  Tensor results(const Tensor& q, bool want_lse, Tensor& lse) {
+    Tensor out = at::empty(q.sizes(), q.options());
+    p.out = out.data_ptr();
+    strides3(p.out_stride, out, packed);
+    if (want_lse) {
+      const auto f32 = q.options().dtype(at::kFloat);
+      lse = packed ? at::empty({q.size(1), q.size(0)}, f32) : at::empty({q.size(0), q.size(2), q.size(1)}, f32);
+      p.lse = (float*)lse.data_ptr();
+      strides3(p.lse_stride, lse, packed);
+    }
+    return out;
   }
 
   bool running_sums(const Tensor* w) {
@@ -433,13 +461,29 @@ struct CacheCall {
     return true;
   }
 
-  // 0, or the library's status with nothing launched
-  int launch(int (*entry)(const rswa_cache_params*, void*)) {
-    void* const stream = (void*)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device.index()).stream();
-    pybind11::gil_scoped_release others_run;
-    return entry(&p, stream);
+  // new keys and values, whose rows are `like`'s
+  bool new_rows(const Tensor* k, const Tensor* v, const Tensor& like) {
+    if (!k || !v || k->dim() != like.dim() || v->sizes() != k->sizes() || k->size(-2) != p.heads_kv) return false;
+    for (int d = 0; d < k->dim(); d++)
+      if (d != k->dim() - 2 && k->size(d) != like.size(d)) return false;
+    for (const Tensor* t : {k, v})
+      if (t->scalar_type() != like.scalar_type() || t->device() != device || t->stride(-1) != 1 || needs_grad(*t)) return false;
+    p.new_k = k->data_ptr();
+    p.new_v = v->data_ptr();
+    strides3(p.new_k_stride, *k, packed);
+    strides3(p.new_v_stride, *v, packed);
+    return true;
   }
+
+  // 0, or the library's status with nothing launched
+  int launch(int (*entry)(const rswa_cache_params*, void*)) { return launch_call(entry, p, device); }
 };
+
+// An integer tensor whose rows are dense from `from` on, on the device; null otherwise.
+const Tensor* ints(PyObject* o, at::ScalarType type, c10::IntArrayRef sizes, int64_t from, c10::Device device) {
+  const Tensor* t = given(o);
+  return t && t->scalar_type() == type && t->sizes() == sizes && t->device() == device && dense_from(*t, from) ? t : nullptr;
+}
 
 // cache_append(cache, k, v, page_table, seqlens, cu_seqlens or None) -> True, or None: not taken
 PyObject* cache_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -448,13 +492,7 @@ PyObject* cache_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 6 || !cache_lib.append || observed()) Py_RETURN_NONE;
   const Tensor *k = given(args[1]), *v = given(args[2]);
   if (!k || !v || !c.set(args[0], args[3], args[4]) || !c.rows(*k, args[5])) Py_RETURN_NONE;
-  if (v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type() || v->device() != c.device || v->stride(-1) != 1 ||
-      k->size(-2) != c.p.heads_kv || needs_grad(*v))
-    Py_RETURN_NONE;
-  c.p.new_k = k->data_ptr();
-  c.p.new_v = v->data_ptr();
-  strides3(c.p.new_k_stride, *k, c.packed);
-  strides3(c.p.new_v_stride, *v, c.packed);
+  if (!c.new_rows(k, v, *k)) Py_RETURN_NONE;
   c10::DeviceGuard guard(c.device);
   if (c.launch(cache_lib.append) != RSWA_OK) Py_RETURN_NONE;
   Py_RETURN_TRUE;
@@ -468,17 +506,10 @@ PyObject* cache_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   CacheCall c;
   if (n != 9 || !cache_lib.attn || observed() || !PyBool_Check(args[8])) Py_RETURN_NONE;
   const Tensor* q = given(args[0]);
-  if (!q || !c.set(args[1], args[2], args[3]) || !c.queries(*q, args[5], args[4], args[6], args[7])) Py_RETURN_NONE;
+  if (!q || !c.set(args[1], args[2], args[3]) || !c.queries(*q, args[5], args[4], args[6], args[7]) || c.p.max_pages == 0)
+    Py_RETURN_NONE;
   c10::DeviceGuard guard(c.device);
-  Tensor out = at::empty(q->sizes(), q->options()), lse, workspace;
-  c.p.out = out.data_ptr();
-  strides3(c.p.out_stride, out, c.packed);
-  if (args[8] == Py_True) {
-    const auto f32 = q->options().dtype(at::kFloat);
-    lse = c.packed ? at::empty({q->size(1), q->size(0)}, f32) : at::empty({q->size(0), q->size(2), q->size(1)}, f32);
-    c.p.lse = (float*)lse.data_ptr();
-    strides3(c.p.lse_stride, lse, c.packed);
-  }
+  Tensor lse, workspace, out = c.results(*q, args[8] == Py_True, lse);
   if (const uint64_t bytes = cache_lib.attn_bytes(&c.p)) {
     workspace = at::empty({(int64_t)bytes}, q->options().dtype(at::kByte));
     c.p.workspace = workspace.data_ptr();
@@ -498,7 +529,7 @@ PyObject* cache_weights(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 10 || !cache_lib.weights || observed()) Py_RETURN_NONE;
   const Tensor *q = given(args[0]), *lse = given(args[4]);
   if (!q || !lse || !c.set(args[1], args[2], args[3]) || !c.queries(*q, args[7], args[6], args[8], args[9]) ||
-      !c.running_sums(given(args[5])) || !lse_of(*lse, *q, c.packed) || needs_grad(*lse))
+      c.p.max_pages == 0 || !c.running_sums(given(args[5])) || !lse_of(*lse, *q, c.packed) || needs_grad(*lse))
     Py_RETURN_NONE;
   c.p.lse = (float*)lse->data_ptr();
   strides3(c.p.lse_stride, *lse, c.packed);
@@ -541,17 +572,223 @@ PyObject* cache_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind_cache(rswa_cache_append, .._attn, .._weights, .._evict, .._attn_workspace_bytes): addresses
+// cache_read(cache, k, v, page_table, first, cu_seqlens or None) -> True, or None: not taken
+PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  CacheCall c;
+  if (n != 6 || !cache_lib.read || observed()) Py_RETURN_NONE;
+  const Tensor *k = given(args[1]), *v = given(args[2]);
+  if (!k || !v || !c.set(args[0], args[3], args[4]) || !c.rows(*k, args[5]) || !c.new_rows(k, v, *k)) Py_RETURN_NONE;
+  for (const Tensor* t : {k, v})
+    for (int64_t d = 0; d < t->dim(); d++)
+      if (t->size(d) > 1 && t->stride(d) == 0) Py_RETURN_NONE;  // (rows that are one another's)
+  c10::DeviceGuard guard(c.device);
+  if (c.launch(cache_lib.read) != RSWA_OK) Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- drafted tokens (ring_swa/ops/drafts.py makes the same in Python) ---------------------------------------------
+
+// cu_seqlens of a pack, or None
+bool pack_of(PyObject* o, c10::Device device, const Tensor*& cu) {
+  cu = nullptr;
+  if (o == Py_None) return true;
+  cu = given(o);
+  return cu && cu->scalar_type() == at::kInt && cu->dim() == 1 && cu->size(0) >= 1 && cu->size(0) < (1 << 28) &&
+         cu->is_contiguous() && cu->device() == device;
+}
+
+// draft_tree(parents, cu_seqlens or None, max_nodes) -> (parents, depths, ancestors), or None: not taken
+PyObject* draft_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t max_nodes;
+  if (n != 3 || !cache_lib.draft_tree || observed() || !int_arg(args[2], max_nodes)) Py_RETURN_NONE;
+  const Tensor *parents = given(args[0]), *cu;
+  if (!parents || parents->scalar_type() != at::kInt || !pack_of(args[1], parents->device(), cu)) Py_RETURN_NONE;
+  if (parents->dim() != (cu ? 1 : 2) || !dense_from(*parents, parents->dim() - 1) || max_nodes < 1 || max_nodes > 1024)
+    Py_RETURN_NONE;
+  for (int64_t d = 0; d < parents->dim(); d++)
+    if (parents->size(d) >= (1 << 28)) Py_RETURN_NONE;
+  rswa_tree_params p{};
+  if (cu) {
+    p.batch = (int32_t)(cu->size(0) - 1);
+    p.total = parents->size(0);
+    p.cu_seqlens = (const int32_t*)cu->data_ptr();
+  } else {
+    p.batch = (int32_t)parents->size(0);
+    p.nodes = (int32_t)parents->size(1);
+    p.parents_stride = parents->stride(0);
+  }
+  p.max_nodes = (int32_t)max_nodes;
+  p.parents = (const int32_t*)parents->data_ptr();
+  c10::DeviceGuard guard(parents->device());
+  auto sizes = parents->sizes().vec();
+  Tensor up = at::empty(sizes, parents->options()), depths = at::empty(sizes, parents->options());
+  sizes.push_back((max_nodes + 63) / 64);
+  Tensor ancestors = at::empty(sizes, parents->options().dtype(at::kLong));
+  p.tree_parents = (int32_t*)up.data_ptr();
+  p.depths = (int32_t*)depths.data_ptr();
+  p.ancestors = (int64_t*)ancestors.data_ptr();
+  if (launch_call(cache_lib.draft_tree, p, parents->device()) != RSWA_OK) Py_RETURN_NONE;
+  return Py_BuildValue("NNN", THPVariable_Wrap(std::move(up)), THPVariable_Wrap(std::move(depths)),
+                       THPVariable_Wrap(std::move(ancestors)));
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_tree_attn(q, k, v, tree, cache, page_table, seqlens, window, cu_seqlens or None, scale or None, sinks, return_lse)
+//   -> out or (out, lse), or None: not taken
+PyObject* cache_tree_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  CacheCall c;
+  if (n != 12 || !cache_lib.tree_attn || observed() || !PyBool_Check(args[11])) Py_RETURN_NONE;
+  if (!PyTuple_Check(args[3]) || PyTuple_GET_SIZE(args[3]) != 3) Py_RETURN_NONE;
+  const Tensor* q = given(args[0]);
+  if (!q || !c.set(args[4], args[5], args[6]) || !c.queries(*q, args[8], args[7], args[9], args[10])) Py_RETURN_NONE;
+  if (!c.new_rows(given(args[1]), given(args[2]), *q)) Py_RETURN_NONE;
+  const auto rows = q->sizes().slice(0, q->dim() - 2);
+  const int64_t nd = (int64_t)rows.size();
+  const Tensor* depths = ints(PyTuple_GET_ITEM(args[3], 1), at::kInt, rows, nd - 1, c.device);
+  const Tensor* ancestors = given(PyTuple_GET_ITEM(args[3], 2));
+  if (!depths || !ancestors || ancestors->dim() != nd + 1) Py_RETURN_NONE;
+  const int64_t words = ancestors->size(-1);
+  auto sizes = rows.vec();
+  sizes.push_back(words);
+  if (!ints(PyTuple_GET_ITEM(args[3], 2), at::kLong, sizes, nd - 1, c.device)) Py_RETURN_NONE;
+  if (words < 1 || words > 16 || (!c.packed && rows[1] > 64 * words)) Py_RETURN_NONE;
+  c10::DeviceGuard guard(c.device);
+  Tensor lse, workspace, out = c.results(*q, args[11] == Py_True, lse);
+  rswa_draft_params p{};
+  p.cache = c.p;
+  p.depths = (const int32_t*)depths->data_ptr();
+  p.ancestors = (const int64_t*)ancestors->data_ptr();
+  if (!c.packed) {
+    p.depths_stride = depths->stride(0);
+    p.ancestors_stride = ancestors->stride(0);
+  }
+  p.words = (int32_t)words;
+  if (const uint64_t bytes = cache_lib.tree_attn_bytes(&p)) {
+    workspace = at::empty({(int64_t)bytes}, q->options().dtype(at::kByte));
+    p.cache.workspace = workspace.data_ptr();
+    p.cache.workspace_bytes = bytes;
+  }
+  if (launch_call(cache_lib.tree_attn, p, c.device) != RSWA_OK) Py_RETURN_NONE;
+  if (!lse.defined()) return THPVariable_Wrap(std::move(out));
+  return Py_BuildValue("NN", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lse)));
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_accept(cache, k, v, path, page_table, seqlens, cu_seqlens or None) -> True, or None: not taken
+PyObject* cache_accept(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  CacheCall c;
+  if (n != 7 || !cache_lib.accept || observed()) Py_RETURN_NONE;
+  const Tensor *k = given(args[1]), *v = given(args[2]), *path = given(args[3]);
+  if (!k || !v || !path || path->dim() != 2 || path->size(1) >= (1 << 28)) Py_RETURN_NONE;
+  if (!c.set(args[0], args[4], args[5]) || !c.rows(*k, args[6]) || !c.new_rows(k, v, *k)) Py_RETURN_NONE;
+  if (!ints(args[3], at::kInt, {c.p.batch, path->size(1)}, 1, c.device)) Py_RETURN_NONE;
+  rswa_draft_params p{};
+  p.cache = c.p;
+  p.path = (const int32_t*)path->data_ptr();
+  p.path_stride = path->stride(0);
+  p.path_len = (int32_t)path->size(1);
+  c10::DeviceGuard guard(c.device);
+  if (launch_call(cache_lib.accept, p, c.device) != RSWA_OK) Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// verify_drafts(tree, tokens, target, draft or None, uniforms, cu_seqlens or None) -> (path, accepted, next), or None: not taken
+PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !cache_lib.verify || observed()) Py_RETURN_NONE;
+  if (!PyTuple_Check(args[0]) || PyTuple_GET_SIZE(args[0]) != 3) Py_RETURN_NONE;
+  const Tensor *target = given(args[2]), *draft = args[3] == Py_None ? nullptr : given(args[3]), *cu;
+  const Tensor *tokens = given(args[1]), *ancestors = given(PyTuple_GET_ITEM(args[0], 2));
+  if (!target || !tokens || !ancestors || (!draft && args[3] != Py_None)) Py_RETURN_NONE;
+  const c10::Device device = target->device();
+  if (!pack_of(args[5], device, cu) || target->dim() != (cu ? 2 : 3) || ancestors->dim() != target->dim()) Py_RETURN_NONE;
+  const auto type = target->scalar_type(), token_type = tokens->scalar_type();
+  if ((type != at::kFloat && type != at::kBFloat16 && type != at::kHalf) ||
+      (token_type != at::kInt && token_type != at::kLong))
+    Py_RETURN_NONE;
+  for (const Tensor* t : {target, draft})
+    if (t && (t->sizes() != target->sizes() || t->scalar_type() != type || t->device() != device || needs_grad(*t) ||
+              (t->stride(-1) != 1 && t->size(-1) != 1)))
+      Py_RETURN_NONE;
+  for (int64_t d = 0; d < target->dim(); d++)
+    if (target->size(d) >= (1 << 28)) Py_RETURN_NONE;
+  const auto rows = target->sizes().slice(0, target->dim() - 1);
+  const int64_t nd = (int64_t)rows.size();
+  const Tensor* parents = ints(PyTuple_GET_ITEM(args[0], 0), at::kInt, rows, nd - 1, device);
+  const Tensor* uniforms = ints(args[4], at::kFloat, rows, nd - 1, device);
+  if (!parents || !uniforms || needs_grad(*uniforms) || !ints(args[1], token_type, rows, nd - 1, device)) Py_RETURN_NONE;
+  rswa_verify_params p{};
+  p.dtype = type == at::kFloat ? RSWA_F32 : type == at::kBFloat16 ? RSWA_BF16 : RSWA_F16;
+  p.token_bytes = token_type == at::kInt ? 4 : 8;
+  p.vocab = (int32_t)target->size(-1);
+  p.max_nodes = (int32_t)std::min<int64_t>(64 * ancestors->size(-1), INT32_MAX);
+  const auto strides = [&](int64_t(&to)[2], const Tensor& t) {
+    to[0] = cu ? 0 : t.stride(0);
+    to[1] = t.stride(cu ? 0 : 1);
+  };
+  if (cu) {
+    p.batch = (int32_t)(cu->size(0) - 1);
+    p.total = rows[0];
+    p.cu_seqlens = (const int32_t*)cu->data_ptr();
+  } else {
+    p.batch = (int32_t)rows[0];
+    p.nodes = (int32_t)rows[1];
+    p.parents_stride = parents->stride(0);
+    p.tokens_stride = tokens->stride(0);
+    p.uniforms_stride = uniforms->stride(0);
+  }
+  p.parents = (const int32_t*)parents->data_ptr();
+  p.tokens = tokens->data_ptr();
+  p.uniforms = (const float*)uniforms->data_ptr();
+  p.target = target->data_ptr();
+  strides(p.target_stride, *target);
+  if (draft) {
+    p.draft = draft->data_ptr();
+    strides(p.draft_stride, *draft);
+  }
+  c10::DeviceGuard guard(device);
+  p.path_len = cu ? p.max_nodes : p.nodes;
+  if (p.max_nodes < 1 || p.max_nodes > 1024) Py_RETURN_NONE;
+  Tensor path = at::empty({p.batch, p.path_len}, parents->options()), accepted = at::empty({p.batch}, parents->options());
+  Tensor next = at::empty({p.batch}, tokens->options());
+  p.path = (int32_t*)path.data_ptr();
+  p.accepted = (int32_t*)accepted.data_ptr();
+  p.next_token = next.data_ptr();
+  const uint64_t bytes = cache_lib.verify_bytes(&p);
+  Tensor workspace = at::empty({(int64_t)bytes}, target->options().dtype(at::kByte));
+  p.workspace = workspace.data_ptr();
+  p.workspace_bytes = bytes;
+  if (launch_call(cache_lib.verify, p, device) != RSWA_OK) Py_RETURN_NONE;
+  return Py_BuildValue("NNN", THPVariable_Wrap(std::move(path)), THPVariable_Wrap(std::move(accepted)),
+                       THPVariable_Wrap(std::move(next)));
+  END_HANDLE_TH_ERRORS
+}
+
+// bind_cache(rswa_cache_append, .._attn, .._weights, .._evict, .._attn_workspace_bytes, .._read, rswa_draft_tree,
+//   rswa_cache_tree_attn, .._tree_attn_workspace_bytes, .._accept, rswa_verify_drafts, .._workspace_bytes): addresses
 PyObject* bind_cache(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 5) {
-    PyErr_SetString(PyExc_TypeError, "bind_cache takes five addresses");
+  if (n != 12) {
+    PyErr_SetString(PyExc_TypeError, "bind_cache takes twelve addresses");
     return nullptr;
   }
-  void* at[5];
-  for (int i = 0; i < 5; i++) {
+  void* at[12];
+  for (int i = 0; i < 12; i++) {
     at[i] = PyLong_AsVoidPtr(args[i]);
     if (PyErr_Occurred()) return nullptr;
   }
+  cache_lib.read = reinterpret_cast<decltype(cache_lib.read)>(at[5]);
+  cache_lib.draft_tree = reinterpret_cast<decltype(cache_lib.draft_tree)>(at[6]);
+  cache_lib.tree_attn_bytes = reinterpret_cast<decltype(cache_lib.tree_attn_bytes)>(at[8]);
+  cache_lib.tree_attn = reinterpret_cast<decltype(cache_lib.tree_attn)>(at[7]);
+  cache_lib.accept = reinterpret_cast<decltype(cache_lib.accept)>(at[9]);
+  cache_lib.verify_bytes = reinterpret_cast<decltype(cache_lib.verify_bytes)>(at[11]);
+  cache_lib.verify = reinterpret_cast<decltype(cache_lib.verify)>(at[10]);
   cache_lib.attn_bytes = reinterpret_cast<decltype(cache_lib.attn_bytes)>(at[4]);
   cache_lib.append = reinterpret_cast<decltype(cache_lib.append)>(at[0]);
   cache_lib.attn = reinterpret_cast<decltype(cache_lib.attn)>(at[1]);
@@ -589,14 +826,26 @@ PyObject* params_bytes(PyObject*, PyObject*) { return PyLong_FromSize_t(sizeof(r
 
 PyObject* cache_params_bytes(PyObject*, PyObject*) { return PyLong_FromSize_t(sizeof(rswa_cache_params)); }
 
+// of the trees, the calls that take one, and the verification
+PyObject* draft_params_bytes(PyObject*, PyObject*) {
+  return Py_BuildValue("nnn", (Py_ssize_t)sizeof(rswa_tree_params), (Py_ssize_t)sizeof(rswa_draft_params),
+                       (Py_ssize_t)sizeof(rswa_verify_params));
+}
+
 PyMethodDef methods[] = {
     {"band_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&band_attn)), METH_FASTCALL, nullptr},
     {"cache_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&cache_append)), METH_FASTCALL, nullptr},
     {"cache_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&cache_attn)), METH_FASTCALL, nullptr},
     {"cache_weights", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&cache_weights)), METH_FASTCALL, nullptr},
     {"cache_evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&cache_evict)), METH_FASTCALL, nullptr},
+    {"cache_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&cache_read)), METH_FASTCALL, nullptr},
+    {"draft_tree", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&draft_tree)), METH_FASTCALL, nullptr},
+    {"cache_tree_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&cache_tree_attn)), METH_FASTCALL, nullptr},
+    {"cache_accept", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&cache_accept)), METH_FASTCALL, nullptr},
+    {"verify_drafts", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&verify_drafts)), METH_FASTCALL, nullptr},
     {"bind_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&bind_cache)), METH_FASTCALL, nullptr},
     {"cache_params_bytes", &cache_params_bytes, METH_NOARGS, nullptr},
+    {"draft_params_bytes", &draft_params_bytes, METH_NOARGS, nullptr},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&bind)), METH_FASTCALL, nullptr},
     {"params_bytes", &params_bytes, METH_NOARGS, nullptr},
     {"torch_build", &torch_build, METH_NOARGS, nullptr},

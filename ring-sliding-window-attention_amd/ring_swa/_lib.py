@@ -146,6 +146,70 @@ class CacheParams(Structure):
     ]
 
 
+class TreeParams(Structure):
+    """Mirror of ``rswa_tree_params`` (include/rswa.h); field order is the ABI."""
+
+    _fields_ = [
+        ("batch", c_int32),
+        ("nodes", c_int32),
+        ("max_nodes", c_int32),
+        ("total", c_int64),
+        ("cu_seqlens", c_void_p),
+        ("parents", c_void_p),
+        ("parents_stride", c_int64),
+        ("tree_parents", c_void_p),
+        ("depths", c_void_p),
+        ("ancestors", c_void_p),
+    ]
+
+
+class DraftParams(Structure):
+    """Mirror of ``rswa_draft_params`` (include/rswa.h); field order is the ABI."""
+
+    _fields_ = [
+        ("cache", CacheParams),
+        ("depths", c_void_p),
+        ("depths_stride", c_int64),
+        ("ancestors", c_void_p),
+        ("ancestors_stride", c_int64),
+        ("words", c_int32),
+        ("path_len", c_int32),
+        ("path", c_void_p),
+        ("path_stride", c_int64),
+    ]
+
+
+class VerifyParams(Structure):
+    """Mirror of ``rswa_verify_params`` (include/rswa.h); field order is the ABI."""
+
+    _fields_ = [
+        ("dtype", c_int32),
+        ("token_bytes", c_int32),
+        ("batch", c_int32),
+        ("nodes", c_int32),
+        ("max_nodes", c_int32),
+        ("vocab", c_int32),
+        ("total", c_int64),
+        ("cu_seqlens", c_void_p),
+        ("parents", c_void_p),
+        ("tokens", c_void_p),
+        ("uniforms", c_void_p),
+        ("parents_stride", c_int64),
+        ("tokens_stride", c_int64),
+        ("uniforms_stride", c_int64),
+        ("target", c_void_p),
+        ("draft", c_void_p),
+        ("target_stride", _I64x2),
+        ("draft_stride", _I64x2),
+        ("path", c_void_p),
+        ("path_len", c_int32),
+        ("accepted", c_void_p),
+        ("next_token", c_void_p),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_uint64),
+    ]
+
+
 WIDE_OUT, WIDE_DQ, WIDE_DKV = 1, 2, 4
 DKDV_FORMS = {"wide": 1, "short": 2}
 
@@ -206,19 +270,30 @@ def load(path: str) -> ctypes.CDLL:
     L.rswa_attn_fwd_blocks_per_cu.argtypes = [POINTER(AttnParams)]
     L.rswa_attn_bwd_dkdv_keys.restype = c_int
     L.rswa_attn_bwd_dkdv_keys.argtypes = [POINTER(AttnParams)]
-    for name in ("rswa_cache_append", "rswa_cache_attn", "rswa_cache_weights", "rswa_cache_evict"):
+    for name in ("rswa_cache_append", "rswa_cache_attn", "rswa_cache_weights", "rswa_cache_evict", "rswa_cache_read"):
         fn = getattr(L, name)
         fn.restype = c_int
         fn.argtypes = [POINTER(CacheParams), c_void_p]
     L.rswa_cache_attn_workspace_bytes.restype = c_uint64
     L.rswa_cache_attn_workspace_bytes.argtypes = [POINTER(CacheParams)]
-    L.rswa_sizeof_cache_params.restype = c_uint64
-    if L.rswa_sizeof_cache_params() != ctypes.sizeof(CacheParams):
-        raise ImportError(
-            "rswa_cache_params layout mismatch between librswa.so "
-            f"({L.rswa_sizeof_cache_params()} bytes) and the Python binding "
-            f"({ctypes.sizeof(CacheParams)} bytes): rebuild the library"
-        )
+    for name, params in (("rswa_draft_tree", TreeParams), ("rswa_cache_tree_attn", DraftParams),
+                         ("rswa_cache_accept", DraftParams), ("rswa_verify_drafts", VerifyParams)):
+        fn = getattr(L, name)
+        fn.restype = c_int
+        fn.argtypes = [POINTER(params), c_void_p]
+    L.rswa_cache_tree_attn_workspace_bytes.restype = c_uint64
+    L.rswa_cache_tree_attn_workspace_bytes.argtypes = [POINTER(DraftParams)]
+    L.rswa_verify_drafts_workspace_bytes.restype = c_uint64
+    L.rswa_verify_drafts_workspace_bytes.argtypes = [POINTER(VerifyParams)]
+    for name, params in (("cache", CacheParams), ("tree", TreeParams), ("draft", DraftParams), ("verify", VerifyParams)):
+        size = getattr(L, f"rswa_sizeof_{name}_params")
+        size.restype = c_uint64
+        if size() != ctypes.sizeof(params):
+            raise ImportError(
+                f"rswa_{name}_params layout mismatch between librswa.so "
+                f"({size()} bytes) and the Python binding "
+                f"({ctypes.sizeof(params)} bytes): rebuild the library"
+            )
     if L.rswa_sizeof_attn_params() != ctypes.sizeof(AttnParams):
         raise ImportError(
             "rswa_attn_params layout mismatch between librswa.so "
@@ -275,9 +350,13 @@ def _load_torch_calls():
              check, band_backward)
     if mod.cache_params_bytes() != ctypes.sizeof(CacheParams):
         raise ImportError(f"{path} was built for another rswa_cache_params: rebuild it")
+    if mod.draft_params_bytes() != tuple(ctypes.sizeof(p) for p in (TreeParams, DraftParams, VerifyParams)):
+        raise ImportError(f"{path} was built for other parameters of the calls on drafts: rebuild it")
     mod.bind_cache(*[ctypes.cast(fn, c_void_p).value
                      for fn in (L.rswa_cache_append, L.rswa_cache_attn, L.rswa_cache_weights, L.rswa_cache_evict,
-                                L.rswa_cache_attn_workspace_bytes)])
+                                L.rswa_cache_attn_workspace_bytes, L.rswa_cache_read, L.rswa_draft_tree,
+                                L.rswa_cache_tree_attn, L.rswa_cache_tree_attn_workspace_bytes, L.rswa_cache_accept,
+                                L.rswa_verify_drafts, L.rswa_verify_drafts_workspace_bytes)])
     return mod
 
 

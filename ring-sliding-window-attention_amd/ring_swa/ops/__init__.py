@@ -14,7 +14,9 @@ from .band_attn import (
     wrapped_flash_attn_fwd,
     wrapped_flash_attn_fwd_varlen,
 )
-from .kv_cache import KVCache, kv_cache_append, kv_cache_attn, kv_cache_evict, kv_cache_weights
+from .drafts import DraftTree, draft_tree, kv_cache_accept, kv_cache_tree_attn, verify_drafts
+from .kv_cache import (KVCache, kv_cache_append, kv_cache_attn, kv_cache_evict, kv_cache_read,
+                       kv_cache_weights)
 from .lse_merge import merge_attn_out
 from .p2p import (
     broadcast_tensor_to_group,
@@ -41,6 +43,12 @@ __all__ = [
     "kv_cache_attn",
     "kv_cache_weights",
     "kv_cache_evict",
+    "kv_cache_read",
+    "DraftTree",
+    "draft_tree",
+    "kv_cache_tree_attn",
+    "verify_drafts",
+    "kv_cache_accept",
     "ring_attn_p2p_communicate",
     "broadcast_tensor_to_group",
     "reduce_sum_tesnsor_to_rank",

@@ -18,6 +18,7 @@ says which::
         ...                                                                     # now and then:
         held, weights, kept = kv_cache_evict(cache, weights, page_table, held, new_page_table, budget)
 
+``kv_cache_read`` gives cached tokens back in 16 bits; drafted tokens are in ``drafts.py``.
 Lengths and page ids stay on the device, nothing is read back.  Rows are ``[batch, seq, heads, dim]``,
 or packed ``[tokens, heads, dim]`` with ``cu_seqlens`` (int32 ``[batch + 1]``; sequences may bring
 different numbers of rows, none among them; rows that are no sequence's are passed over), as in the
@@ -27,7 +28,8 @@ page id outside the cache (``-1``) is a page that is not there: seen by nobody, 
 pages that a window has left behind can be given back.  There is no backward.
 
 A compiled program makes these calls between its graphs (``fullgraph=True`` refuses them); in a traced one, and to a
-dispatch mode, they are the operators ``ring_swa::cache_append``, ``cache_attn``, ``cache_weights`` and ``cache_evict``.
+dispatch mode, they are the operators ``ring_swa::cache_append``, ``cache_attn``, ``cache_weights``, ``cache_evict`` and
+``cache_read``.
 """
 from __future__ import annotations
 
@@ -194,6 +196,15 @@ def _query_params(p, q, heads_kv, softmax_scale, window_size, num_sink_tokens, p
     p.q, p.q_stride = q.data_ptr(), _strides3(q, packed)
 
 
+def _new_rows(p, k, v, packed):
+    assert k.shape == v.shape and k.dtype == v.dtype, "k and v must have the same shape and dtype"
+    assert k.shape[-2] == p.heads_kv, "k and v must have the cache's heads"
+    _lib.require_device(k, v)
+    assert k.stride(-1) == 1 and v.stride(-1) == 1, "last dimension must be contiguous"
+    p.new_k, p.new_v = k.data_ptr(), v.data_ptr()
+    p.new_k_stride, p.new_v_stride = _strides3(k, packed), _strides3(v, packed)
+
+
 def kv_cache_append(
     cache: KVCache,
     k: torch.Tensor,
@@ -224,14 +235,42 @@ def kv_cache_append(
            "Tensor? cu_seqlens) -> ()", lambda *_: None)
 def _append(k, v, k_scale, v_scale, new_k, new_v, page_table, seqlens, cu_seqlens):
     p, dev = _cache_params((k, v, k_scale, v_scale), page_table, seqlens, new_k, cu_seqlens)
-    assert new_k.shape == new_v.shape and new_k.dtype == new_v.dtype, "k and v must have the same shape and dtype"
-    assert new_k.shape[-2] == p.heads_kv, "k and v must have the cache's heads"
-    _lib.require_device(new_k, new_v)
-    assert new_k.stride(-1) == 1 and new_v.stride(-1) == 1, "last dimension must be contiguous"
-    packed = cu_seqlens is not None
-    p.new_k, p.new_v = new_k.data_ptr(), new_v.data_ptr()
-    p.new_k_stride, p.new_v_stride = _strides3(new_k, packed), _strides3(new_v, packed)
+    _new_rows(p, new_k, new_v, cu_seqlens is not None)
     _lib.launch(dev, _lib.lib().rswa_cache_append, p)
+
+
+def kv_cache_read(
+    cache: KVCache,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    page_table: torch.Tensor,
+    first: torch.Tensor,
+    cu_seqlens: Optional[torch.Tensor] = None,
+) -> None:
+    """Read tokens back: the inverse of ``kv_cache_append``, with the same arguments.
+
+    ``k`` and ``v`` (``[batch, seq, kv_heads, dim]``, or packed ``[tokens, kv_heads, dim]`` with ``cu_seqlens``;
+    bf16 or fp16) are written: row ``i`` of a sequence is its token ``first + i`` (``first``: int32 ``[batch]``, below
+    zero counts as zero), a code times its page's scale rounded to the type (infinite where the type holds it as that).
+    Rows of tokens that have no page are zeros; rows of a pack that are no sequence's are left alone.  So a cached
+    prefix goes to the attention functions, to another page size or to another device."""
+    if torch.compiler.is_dynamo_compiling():
+        return _uncompiled(kv_cache_read, cache, k, v, page_table, first, cu_seqlens)
+    calls = _calls(cache)
+    if calls is not None and calls.cache_read(cache, k, v, page_table, first, cu_seqlens):
+        return
+    _no_grad(*cache, k, v)
+    _read(k, v, *cache, page_table, first, cu_seqlens)
+
+
+@_operator(f"cache_read(Tensor(a!) to_k, Tensor(b!) to_v, {_CACHE}, Tensor page_table, Tensor first, "
+           "Tensor? cu_seqlens) -> ()", lambda *_: None)
+def _read(to_k, to_v, k, v, k_scale, v_scale, page_table, first, cu_seqlens):
+    p, dev = _cache_params((k, v, k_scale, v_scale), page_table, first, to_k, cu_seqlens)
+    _new_rows(p, to_k, to_v, cu_seqlens is not None)
+    for t in (to_k, to_v):
+        assert all(n <= 1 or s != 0 for n, s in zip(t.shape, t.stride())), "k and v are written: their rows must not overlap"
+    _lib.launch(dev, _lib.lib().rswa_cache_read, p)
 
 
 def kv_cache_attn(
