@@ -560,6 +560,27 @@ struct RowOut {
   static __device__ __forceinline__ float inverse_of(float sum) { return sum == 0.f ? 0.f : 2.f / sum; }  // (V halved)
 };
 
+// A tile of `n` rows from r0 on none of whose nodes is there (padding): is it, and its results.  (Trees padded to twice
+// their nodes, 32 sequences of 512 to 16384 keys, 64 nodes: TIMES.)
+__device__ __forceinline__ bool no_nodes(const TreeArgs& a, const Unit& x, int r0, int n) {
+  const int n_flat = x.n_rows * a.group;
+  const int first = quotient(min(r0, n_flat - 1), a.by_group), last = quotient(min(r0 + n, n_flat) - 1, a.by_group);
+  const int32_t* const depths = a.depths + (int64_t)x.b * a.depths_st + x.row0;
+  uint64_t there = 0;
+  for (int i = first; i <= last; i += 64) there |= __builtin_amdgcn_ballot_w64(depths[min(i + lane_id(), last)] >= 0);
+  return there == 0;
+}
+template <typename T, int D>
+__device__ __forceinline__ void put_nothing(const TreeArgs& a, const Unit& x, int hk, int r0, int n) {
+#pragma unroll 1
+  for (int at = threadIdx.x; at < n * (D / 4); at += kThreads) {
+    const int d0 = at % (D / 4) * 4;
+    const RowOut<T, D> to(a, x, hk, r0 + at / (D / 4), x.n_chunks == 1);
+    if (to.out) to.put(d0, f32x4{0, 0, 0, 0}, 0.f);
+    if (d0 == 0) to.finish(-__builtin_inff(), 0.f);
+  }
+}
+
 // Few rows: the four waves of a block have the same rows, each its own keys, and everything from memory to the output
 // stays in registers; the waves meet in LDS at the end.
 template <typename T, int D, int NT, typename Args>
@@ -600,6 +621,8 @@ __global__ __launch_bounds__(kThreads, (NT == 1 && !std::is_same_v<Args, TreeArg
   int i = R::TREE ? (wave - list.n_d) & (KW - 1) : wave;  // (waves that have a tile of nodes come last)
   Pages next{0, 0};
   bool here = false;  // the lane's group of the tile has its page
+  if constexpr (R::TREE)
+    if (no_nodes(a, x, x.row_tile * ROWS, ROWS)) return put_nothing<T, D>(arguments_again<Args>(), x, hk, x.row_tile * ROWS, ROWS);
   if (i < n) {
     const Pages now = keys.pages(list[i]);
     here = keys.there(now.v);
@@ -815,16 +838,13 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Args
   };
 
   __shared__ uint32_t lds_special[R::TREE ? kMaxWords : 1];
-  if constexpr (R::TREE) {
-#pragma unroll 1
-    for (int t = 0; t < list.n_d; t++) {
-      if (t > 0) __syncthreads();
-      stage_node_values<T, D>(a, x, hk, list.d0 + t, &v_ops[0][0][0], &lds_special[t]);
-      __syncthreads();
-      add_nodes(a, w, x, hk, r0 + wave * (NT * 16), list.d0 + t, &v_ops[0][0][0]);
-    }
-    if (list.n_d > 0) __syncthreads();
-  }
+  // Nodes' values go through the part of LDS that the first step writes, so that the first tiles' loads and the nodes' are
+  // on their way together.
+  auto& node_ops = v_ops[1];
+  if constexpr (R::TREE)
+    if (no_nodes(a, x, r0, 4 * NT * 16)) return put_nothing<T, D>(arguments_again<Args>(), x, hk, r0, 4 * NT * 16);
+  if constexpr (R::TREE)
+    if (list.n_d > 0) stage_node_values<T, D>(a, x, hk, list.d0, &node_ops[0][0], &lds_special[0]);
   Pages p[4] = {};  // of tiles i .. i + 3
   if (n > 0) {
 #pragma unroll
@@ -836,6 +856,19 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Args
     prepare_v(tile_at(0), p[0].v);
     widen_v(v_ops[0]);
     load_v(tile_at(1), p[1].v);
+  }
+  if constexpr (R::TREE) {
+#pragma unroll 1
+    for (int t = 0; t < list.n_d; t++) {
+      if (t > 0) {
+        __syncthreads();
+        stage_node_values<T, D>(a, x, hk, list.d0 + t, &node_ops[0][0], &lds_special[t]);
+      }
+      __syncthreads();
+      add_nodes(a, w, x, hk, r0 + wave * (NT * 16), list.d0 + t, &node_ops[0][0]);
+    }
+  }
+  if (n > 0) {
     widen_k(k_ops[1]);
     load_k(tile_at(2), p[2].k);
     if (threadIdx.x == 0) any_special = 0;
