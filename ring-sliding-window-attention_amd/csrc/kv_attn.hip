@@ -561,7 +561,8 @@ struct RowOut {
 };
 
 // A tile of `n` rows from r0 on none of whose nodes is there (padding): is it, and its results.  (Trees padded to twice
-// their nodes, 32 sequences of 512 to 16384 keys, 64 nodes: TIMES.)
+// their nodes, 32 sequences of 512 to 16384 keys, 64 nodes: 306 us without this and the order of the rows kernel's first
+// loads, 239 with both.)
 __device__ __forceinline__ bool no_nodes(const TreeArgs& a, const Unit& x, int r0, int n) {
   const int n_flat = x.n_rows * a.group;
   const int first = quotient(min(r0, n_flat - 1), a.by_group), last = quotient(min(r0 + n, n_flat) - 1, a.by_group);
@@ -1047,14 +1048,44 @@ struct Cut {
   int64_t part_units;  // at most
   int64_t grid;
 };
-// `words`: tiles that a sequence's nodes are at most (0: rows are no nodes).
+//
+// Nodes of trees (`words` != 0: tiles that a sequence's nodes are at most) are cut by the tiles of keys that a unit gets in
+// a launch of two for each compute unit (32 / 8 heads of 128; us):
+//   up to 20 with row tiles of 16: those.  One sequence of 32 nodes against 4001 keys 18.9 (tiles of 32: 20.3), 8 of 6 22 / 27, 2 of
+//     32 21 / 24; with 32 tiles a unit, 4 of 32, 31 / 27
+//   33 to 64 rows and a tile of 64 for every resident block: waves with 16 rows of their own.  64 sequences of 14 nodes
+//     against 1000 keys 47 (shared keys: 61), of 12 against 4001 127 / 134, 128 of 16 against 512 to 4096 161 / 174; fewer, 16 of
+//     12, 44 / 40
+//   more rows, three quarters of tiles of 128 or more, and from 24 tiles on: waves with 32 rows.  8 of 64 against 8000 91 (shared
+//     101), 1 of 64 against 131072 166 / 192, 64 of 24 against 2000 102 / 117; with 8 tiles, 8 of 32, 51 / 37; 64 packed trees of up to
+//     24, 28 / 4 heads of 64, window 4092, which fill them less, 106 / 83
+// The last are cut twice as fine where they are a block for every compute unit, since then sequences of unlike lengths are not
+// evened by their splitting: 32 padded trees of 64 nodes against 512 to 16384 keys 239 -> 218, 16 128 -> 118 (equal lengths lose by
+// it: 64 of 24 against 2000 102 -> 120).  Shared keys are not cut finer than once (the packed trees 83; twice as fine 91).
 Cut cut_call(const rswa_cache_params* p, int words = 0) {
   Cut c;
+  const int resident = 2 * kComputeUnits;
   const int64_t group = p->heads_q / p->heads_kv;
   const int64_t rows = p->cu_seqlens_q ? ceil_div(p->total_q * group, std::max(1, p->batch)) : p->seqlen_q * group;
-  c.nt = rows <= 16 ? 1 : 2;
-  const int64_t all_rows = (p->cu_seqlens_q ? p->total_q : (int64_t)p->batch * p->seqlen_q) * p->heads_q;
-  c.wr = rows <= 64 || all_rows < 128 * kComputeUnits ? 1 : 4;
+  // tiles that a sequence's rows see at most: what its pages hold, or its rows' windows and the sinks; and its nodes
+  int64_t most_tiles = ceil_div((int64_t)p->max_pages * p->page_size, kTileKeys);
+  if (p->window_left >= 0) {
+    const int64_t rows_seq = p->cu_seqlens_q ? p->total_q : p->seqlen_q;
+    most_tiles = std::min(most_tiles, (p->window_left + rows_seq + kTileKeys - 2) / kTileKeys + 1 +
+                                          ceil_div(p->num_sink, kTileKeys));
+  }
+  if (words) {
+    most_tiles += p->cu_seqlens_q ? words : std::min<int64_t>(words, ceil_div(p->seqlen_q, kTileKeys));
+    auto blocks = [&](int row_tile) { return p->batch * ceil_div(rows, row_tile) * p->heads_kv; };
+    const bool own = rows > 64 ? 4 * rows >= 3 * 128 * ceil_div(rows, 128) && blocks(128) * most_tiles >= 24 * resident
+                               : rows > 32 && blocks(64) >= resident;
+    c.wr = own ? 4 : 1;
+    c.nt = own ? (rows > 64 ? 2 : 1) : rows <= 16 || blocks(16) * most_tiles <= 20 * resident ? 1 : 2;
+  } else {
+    c.nt = rows <= 16 ? 1 : 2;
+    const int64_t all_rows = (p->cu_seqlens_q ? p->total_q : (int64_t)p->batch * p->seqlen_q) * p->heads_q;
+    c.wr = rows <= 64 || all_rows < 128 * kComputeUnits ? 1 : 4;
+  }
   c.row_tile = c.nt * 16 * c.wr;
   c.row_tiles = p->cu_seqlens_q ? p->total_q * group / c.row_tile + p->batch
                                 : p->batch * ceil_div(p->seqlen_q * group, c.row_tile);
@@ -1062,18 +1093,10 @@ Cut cut_call(const rswa_cache_params* p, int words = 0) {
   // one sequence of 131072 48 / 50 / 53 / 55, 128 of head_dim 64 56 / 59 / 62 / 60, 8 of 8192 28 / 28 / 30 / 30, 64 ragged
   // ones, which finer shares even out, 217 / 218 / 207 / 207) and two of more (16 x 5 drafts 37 / 43 / 45 / 46); where those
   // have more row tiles than that, whole rounds.
-  const int resident = 2 * kComputeUnits;
-  c.wanted =
-      c.nt == 1 ? resident : (int)std::min<int64_t>(4, ceil_div(c.row_tiles * p->heads_kv, resident)) * resident;
+  int64_t rounds = (words ? c.wr : c.nt) == 1 ? 1 : std::min<int64_t>(4, ceil_div(c.row_tiles * p->heads_kv, resident));
+  if (words && c.row_tile == 128 && c.row_tiles * p->heads_kv >= kComputeUnits) rounds = std::max<int64_t>(2, rounds);
+  c.wanted = (int)rounds * resident;
   const int64_t per_head = ceil_div(c.wanted, p->heads_kv) + 1;
-  // tiles that a sequence's rows see at most: what its pages hold, or its rows' windows and the sinks
-  int64_t most_tiles = ceil_div((int64_t)p->max_pages * p->page_size, kTileKeys);
-  if (p->window_left >= 0) {
-    const int64_t rows_seq = p->cu_seqlens_q ? p->total_q : p->seqlen_q;
-    most_tiles = std::min(most_tiles, (p->window_left + rows_seq + kTileKeys - 2) / kTileKeys + 1 +
-                                          ceil_div(p->num_sink, kTileKeys));
-  }
-  if (words) most_tiles += p->cu_seqlens_q ? words : std::min<int64_t>(words, ceil_div(p->seqlen_q, kTileKeys));
   const int64_t at_most = std::min(ceil_div(8 * per_head, 5), c.row_tiles * most_tiles);
   // few tiles are not split: the join costs what a wave's third tile does (one token: 512 keys 8.0 us whole, 10.1 in two
   // launches, 768 9.2 / 10.2, 1024 10.5 / 10.3; own rows: 500 keys 21.9 / 25.2, 1000 33.2 / 32.7)
@@ -1091,7 +1114,10 @@ template <typename T, int D, typename Args>
 int launch_attn(const Args& a, const Cut& c, hipStream_t stream) {
   const dim3 grid((unsigned)c.grid), block(kThreads);
   clear_launch_error();
-  if (c.nt == 1)
+  constexpr bool TREE = std::is_same_v<Args, TreeArgs>;
+  if (TREE && c.nt == 1 && c.wr == 4)
+    hipLaunchKernelGGL((cache_attn_rows_kernel<T, D, TREE ? 1 : 2, Args>), grid, block, 0, stream, a);
+  else if (c.nt == 1)
     hipLaunchKernelGGL((cache_attn_kernel<T, D, 1, Args>), grid, block, 0, stream, a);
   else if (c.wr == 1)
     hipLaunchKernelGGL((cache_attn_kernel<T, D, 2, Args>), grid, block, 0, stream, a);

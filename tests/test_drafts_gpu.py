@@ -111,6 +111,14 @@ TREES = [
     ([77 * i for i in range(12)], 100, 9, 32, 4, 64, 32, 300, 3, "fp16"),
     ([1500, 0, 31, 800, 64, 9], [300, 2, 0, 130, 64, 257], 20, 48, 2, 128, 64, 100, 70, "bf16"),
     ([9000], 1024, 1, 32, 8, 128, 64, -1, 0, "fp16"),                     # the largest tree, a chain
+    # 32 rows a wave, over row tiles of several chunks
+    ([4000 + 100 * i for i in range(12)], 100, 9, 32, 4, 128, 32, 3000, 3, "fp16"),
+    ([7000, 0, 31, 6800, 64, 6000], [300, 2, 0, 330, 64, 257], 20, 48, 2, 128, 64, -1, 0, "bf16"),
+    ([9000, 12000, 700, 0], 130, 30, 16, 1, 64, 16, 8000, 2, "bf16"),
+    # 16 rows a wave
+    ([11 * i for i in range(64)], 12, 5, 32, 8, 128, 64, -1, 0, "bf16"),
+    ([(37 * i) % 900 for i in range(128)], 10, 4, 16, 4, 64, 32, 100, 3, "fp16"),
+    ([(61 * i) % 900 for i in range(70)], [(7 * i) % 25 for i in range(70)], 4, 32, 8, 128, 16, 9, 2, "fp16"),
 ]
 
 
@@ -206,7 +214,7 @@ def test_a_chain_whose_values_the_cache_holds_exactly(window):
     check_attn(q, cache, table, lens, *kv_cache_attn(q, cache, table, lens, window, num_sink_tokens=3, return_lse=True), window, sinks=3)
 
 
-@pytest.mark.parametrize("case", [1, 4, 11, 13])
+@pytest.mark.parametrize("case", [1, 4, 11, 13, 15, 17, 19, 20])
 def test_what_is_not_finite_reaches_the_descendants_alone(case):
     args, parents = tree_case(case, wild=False)
     q, k, v, tree, cache, table, lens, window, cu, sinks = args
