@@ -7,7 +7,7 @@
 // is ever written, and a rejection costs one pass over two rows for the next S.
 //   max(0, max(0, p - a q) / S - q) = max(0, p - (a + S) q) / S
 // Sums and comparisons are in 64 bits: a draw lies next to borders that are closer than 32-bit sums of a vocabulary.
-// The first pass -- a chain has no other -- is one launch over all rows in pieces of 4096 tokens, each of whose blocks walks
+// The first pass -- a chain has no other -- is one launch over all rows in pieces of 1024 tokens, each of whose blocks walks
 // for itself; a second launch, a block for each sequence, goes on from there and draws the next token by the pieces' sums.
 #include "rswa_common.h"
 
@@ -18,7 +18,7 @@ namespace rswa {
 namespace {
 
 constexpr int kMaxNodes = 1024;
-constexpr int kPiece = 4096;  // tokens
+constexpr int kPiece = 1024;  // tokens whose probabilities are summed by one wave
 
 // Sequence b's rows, whatever cu_seqlens holds.
 __device__ __forceinline__ void rows_of(const int32_t* cu, int b, int nodes, int64_t total, int64_t& row0, int& n) {
@@ -120,7 +120,7 @@ struct VerifyArgs {
 struct Walk {
   double a, mass;
   int32_t cur, next, count;  // count: nodes reached
-  int32_t draw;              // no child is left to try (else: a sum is wanted)
+  int32_t draw;              // no child is left to try
 };
 
 template <typename T>
@@ -133,6 +133,8 @@ struct Nodes {
   int32_t parent[kMaxNodes];  // -2: nobody's child
   int32_t token[kMaxNodes];
   float p[kMaxNodes], q[kMaxNodes], u[kMaxNodes];  // the token's probabilities at the parent, and the node's number
+  int32_t tried[kMaxNodes];   // tokens that were tried at a node
+  int32_t n_tried;
 };
 
 template <typename T>
@@ -150,7 +152,6 @@ struct Sequence {
   __device__ __forceinline__ const T* p_row(int node) const { return target + node * a.target_st[1]; }
   __device__ __forceinline__ const T* q_row(int node) const { return draft ? draft + node * a.draft_st[1] : nullptr; }
 
-  // (`root`: is there one?)
   __device__ __forceinline__ void load(Nodes& s, int threads) const {
     const int32_t* const parents = a.parents + (a.cu ? row0 : b * a.parents_st);
     const float* const uniforms = a.uniforms + (a.cu ? row0 : b * a.uniforms_st);
@@ -179,7 +180,7 @@ __device__ __forceinline__ int next_child(const Nodes& s, int node, int from, in
 }
 
 // Without a draft: was the token tried at this node before, by a child below `i`?
-__device__ __forceinline__ bool tried(const Nodes& s, int node, int i) {
+__device__ __forceinline__ bool tried_before(const Nodes& s, int node, int i) {
   const int lane = threadIdx.x & 63;
   for (int j = node + 1; j < i; j += 64)
     if (__builtin_amdgcn_ballot_w64(j + lane < i && s.parent[min(j + lane, i)] == node && s.token[min(j + lane, i)] == s.token[i]))
@@ -187,8 +188,8 @@ __device__ __forceinline__ bool tried(const Nodes& s, int node, int i) {
   return false;
 }
 
-// On to where a sum is wanted, or no child is left.  All lanes of a wave do the same; nodes reached go to `path` (null: not
-// written).
+// On to where a sum is wanted: the mass that a rejection leaves for the next child, or what the next token is drawn from.
+// All lanes of a wave do the same; nodes reached go to `path` (null: not written).
 template <bool DRAFT>
 __device__ __forceinline__ void walk_on(const Nodes& s, Walk& w, int n, int32_t* path) {
   w.draw = 0;
@@ -201,7 +202,7 @@ __device__ __forceinline__ void walk_on(const Nodes& s, Walk& w, int n, int32_t*
     }
     w.next = i + 1;
     const double p = s.p[i], q = s.q[i], u = s.u[i];
-    const double rest = DRAFT ? fmax(0.0, p - w.a * q) : tried(s, w.cur, i) ? 0.0 : p;
+    const double rest = DRAFT ? fmax(0.0, p - w.a * q) : tried_before(s, w.cur, i) ? 0.0 : p;
     if (DRAFT ? u * w.mass * q < rest : u * w.mass < rest) {
       if (path && threadIdx.x == 0) path[w.count] = i;
       w.count++;
@@ -210,6 +211,7 @@ __device__ __forceinline__ void walk_on(const Nodes& s, Walk& w, int n, int32_t*
       w.mass = 1.0;
     } else if (DRAFT) {
       w.a += w.mass;
+      w.draw = next_child(s, w.cur, w.next, n) == n;  // (the sum wanted is that of what is drawn from)
       return;
     } else {
       w.mass = fmax(0.0, w.mass - rest);
@@ -217,47 +219,65 @@ __device__ __forceinline__ void walk_on(const Nodes& s, Walk& w, int n, int32_t*
   }
 }
 
-// 16 bytes from anywhere an element may lie
-template <typename T>
-struct Piece16 {
-  static constexpr int N = 16 / sizeof(T);
-  T v[N];
-  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(v, p, 16); }
-};
+// The tokens of the children of `node` below `next`, in any order.
+__device__ __forceinline__ void list_tried(Nodes& s, int node, int next, int threads) {
+  if (threadIdx.x == 0) s.n_tried = 0;
+  __syncthreads();
+  for (int i = node + 1 + threadIdx.x; i < next; i += threads)
+    if (s.parent[i] == node) s.tried[atomicAdd(&s.n_tried, 1)] = s.token[i];
+  __syncthreads();
+}
 
-// What is left at a node: r(x) for a vector of tokens from x0 on.
+// What is left at a node, r(x), for 16 bytes of tokens.  They are read from anywhere an element may lie; the last ones are
+// the row's last 16 bytes, of which those ahead of x0 are not taken.
 template <typename T, bool DRAFT>
 struct Rest {
-  static constexpr int N = Piece16<T>::N;
+  static constexpr int N = 16 / sizeof(T);
   const T *p, *q;
   double a;
   int vocab;
-  const Nodes& s;
-  int node, n_tried;  // children that `tried` has to look at: up to n_tried
-  __device__ __forceinline__ void at(int x0, double (&r)[N]) const {
-    Piece16<T> pv, qv;
-    if (x0 + N <= vocab) {
-      pv.load(p + x0);
-      if constexpr (DRAFT) qv.load(q + x0);
+  const int32_t* tried;
+  int n_tried;
+  typedef __attribute__((__vector_size__(16), aligned(sizeof(T)))) T Vec;
+  struct Raw {
+    Vec p, q;
+  };
+  __device__ __forceinline__ int base(int x0) const { return min(x0, vocab - N); }
+  // vectors from x0 on, `step` apart, all on their way at once
+  template <int M>
+  __device__ __forceinline__ void load(int x0, int step, Raw (&v)[M]) const {
+    if (vocab >= N) {
+#pragma unroll
+      for (int i = 0; i < M; i++) {
+        v[i].p = *(const Vec*)(p + base(x0 + i * step));
+        if constexpr (DRAFT) v[i].q = *(const Vec*)(q + base(x0 + i * step));
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < N; e++) {
-        pv.v[e] = x0 + e < vocab ? p[x0 + e] : (T)0.f;
-        if constexpr (DRAFT) qv.v[e] = x0 + e < vocab ? q[x0 + e] : (T)0.f;
-      }
+      for (int i = 0; i < M; i++)
+#pragma unroll 1
+        for (int e = 0; e < N; e++) {
+          const int x = max(0, base(x0 + i * step) + e);
+          v[i].p[e] = p[x];
+          if constexpr (DRAFT) v[i].q[e] = q[x];
+        }
     }
+  }
+  // (of tokens base(x0) ..; 0 for those below x0)
+  __device__ __forceinline__ void values(int x0, const Raw& v, double (&r)[N]) const {
+    const int from = base(x0);
 #pragma unroll
     for (int e = 0; e < N; e++) {
-      r[e] = positive(pv.v[e]);
-      if constexpr (DRAFT) r[e] = fmax(0.0, r[e] - a * (double)positive(qv.v[e]));
+      r[e] = positive(v.p[e]);
+      if constexpr (DRAFT) r[e] = fmax(0.0, r[e] - a * (double)positive(v.q[e]));
+      r[e] = from + e >= x0 ? r[e] : 0.0;
     }
-    if constexpr (!DRAFT) {
-      for (int i = node + 1; i < n_tried; i++) {
-        const int at = s.parent[i] == node ? s.token[i] - x0 : -1;
+    if constexpr (!DRAFT)
+      for (int i = 0; i < n_tried; i++) {
+        const int at = tried[i] - from;
 #pragma unroll
         for (int e = 0; e < N; e++) r[e] = at == e ? 0.0 : r[e];
       }
-    }
   }
 };
 
@@ -266,33 +286,42 @@ __device__ __forceinline__ double wave_sum(double v) {
   for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
   return v;
 }
-
-// Sum over a piece, by the threads t of `threads` (whole waves; every wave returns its lanes' share).
-template <typename T, bool DRAFT>
-__device__ __forceinline__ double piece_share(const Rest<T, DRAFT>& rest, int piece, int t, int threads) {
-  constexpr int N = Piece16<T>::N;
-  const int end = min(rest.vocab, (piece + 1) * kPiece);
-  double sum = 0.0;
-#pragma unroll 4
-  for (int x = piece * kPiece + t * N; x < end; x += threads * N) {
-    double r[N];
-    rest.at(x, r);
-    double of = 0.0;
+__device__ __forceinline__ double wave_scan(double v) {  // of the lanes up to each
+  const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int e = 0; e < N; e++) of += r[e];
-    sum += of;
+  for (int d = 1; d < 64; d <<= 1) {
+    const double from = __shfl_up(v, d);
+    if (lane >= d) v += from;
   }
-  return sum;
+  return v;
 }
 
-constexpr int kFirstThreads = 256;
+// Sum over a piece, by one wave: all of its loads first.
+template <typename T, bool DRAFT>
+__device__ __forceinline__ double piece_sum(const Rest<T, DRAFT>& rest, int piece) {
+  using R = Rest<T, DRAFT>;
+  constexpr int TURNS = kPiece / (64 * R::N);
+  const int x = piece * kPiece + (threadIdx.x & 63) * R::N;
+  typename R::Raw v[TURNS];
+  rest.load(x, 64 * R::N, v);
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < TURNS; i++) {
+    double r[R::N];
+    rest.values(x + i * 64 * R::N, v[i], r);
+#pragma unroll
+    for (int e = 0; e < R::N; e++) sum += r[e];
+  }
+  return wave_sum(sum);
+}
 
-// The walk as far as the first sum, and that sum of one piece.
+constexpr int kFirstThreads = 256, kFirstPieces = kFirstThreads / 64;
+
+// The walk as far as the first sum, and that sum over the waves' pieces.
 template <typename T, bool DRAFT>
 __global__ __launch_bounds__(kFirstThreads) void verify_first_kernel(const VerifyArgs a) {
   __shared__ Nodes s;
-  __shared__ double share[kFirstThreads / 64];
-  const int b = blockIdx.y, piece = blockIdx.x;
+  const int b = blockIdx.y, piece = blockIdx.x * kFirstPieces + threadIdx.x / 64;
   const Sequence<T> seq(a, b);
   Walk w{0.0, 1.0, 0, 1, 0, 0};
   int32_t* const path = a.path + (int64_t)b * a.path_len;
@@ -300,23 +329,18 @@ __global__ __launch_bounds__(kFirstThreads) void verify_first_kernel(const Verif
     seq.load(s, kFirstThreads);
     __syncthreads();
     if (s.parent[0] == -1) {
-      if (piece == 0 && threadIdx.x == 0) path[0] = 0;
+      if (blockIdx.x == 0 && threadIdx.x == 0) path[0] = 0;
       w.count = 1;
-      walk_on<DRAFT>(s, w, seq.n, piece == 0 ? path : nullptr);
+      walk_on<DRAFT>(s, w, seq.n, blockIdx.x == 0 ? path : nullptr);
     }
   }
-  if (piece == 0 && threadIdx.x == 0) a.walks[b] = w;
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.walks[b] = w;
   if (w.count == 0) return;
-  const Rest<T, DRAFT> rest{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, s, w.cur, w.next};
-  const double sum = wave_sum(piece_share(rest, piece, threadIdx.x, kFirstThreads));
-  if ((threadIdx.x & 63) == 0) share[threadIdx.x / 64] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double of = 0.0;
-#pragma unroll
-    for (int i = 0; i < kFirstThreads / 64; i++) of += share[i];
-    a.sums[(int64_t)b * a.pieces + piece] = of;
-  }
+  if constexpr (!DRAFT) list_tried(s, w.cur, w.next, kFirstThreads);
+  if (piece >= a.pieces) return;
+  const Rest<T, DRAFT> rest{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, s.tried, DRAFT ? 0 : s.n_tried};
+  const double sum = piece_sum(rest, piece);
+  if ((threadIdx.x & 63) == 0) a.sums[(int64_t)b * a.pieces + piece] = sum;
 }
 
 constexpr int kRestThreads = 1024, kRestWaves = kRestThreads / 64;
@@ -325,7 +349,8 @@ constexpr int kMaxPieces = 4096;
 // The rest of the walk, and the draw.
 template <typename T, bool DRAFT>
 __global__ __launch_bounds__(kRestThreads) void verify_rest_kernel(const VerifyArgs a) {
-  constexpr int N = Piece16<T>::N;
+  using R = Rest<T, DRAFT>;
+  constexpr int N = R::N;
   __shared__ Nodes s;
   __shared__ double sums[kMaxPieces];
   __shared__ double share[kRestWaves];
@@ -334,94 +359,93 @@ __global__ __launch_bounds__(kRestThreads) void verify_rest_kernel(const VerifyA
   const Sequence<T> seq(a, b);
   int32_t* const path = a.path + (int64_t)b * a.path_len;
   Walk w = a.walks[b];
+  const float u_root = w.count > 0 ? a.uniforms[a.cu ? seq.row0 : b * a.uniforms_st] : 0.f;
   if (w.count > 0) {
-    seq.load(s, kRestThreads);
     for (int i = threadIdx.x; i < a.pieces; i += kRestThreads) sums[i] = a.sums[(int64_t)b * a.pieces + i];
+    if (!DRAFT || !w.draw) seq.load(s, kRestThreads);
   }
   if (threadIdx.x == 0) found = last_positive = -1;
   __syncthreads();
-  auto pass = [&](const Rest<T, DRAFT>& rest) {  // sums of all pieces
+  auto pass = [&](const R& rest) {  // sums of all pieces
     __syncthreads();
     for (int i = wave; i < a.pieces; i += kRestWaves) {
-      const double of = wave_sum(piece_share(rest, i, lane, 64));
+      const double of = piece_sum(rest, i);
       if (lane == 0) sums[i] = of;
     }
     __syncthreads();
   };
-  auto total = [&] {  // in the order of the pieces, the same in every lane
+  // A lane has PER pieces in a row.  All waves do the same.
+  const int per = (a.pieces + 63) / 64;
+  auto lane_total = [&] {
     double of = 0.0;
-    for (int i = 0; i < a.pieces; i++) of += sums[i];
+    for (int i = lane * per; i < min(a.pieces, (lane + 1) * per); i++) of += sums[i];
     return of;
-  };
-  auto rest_of = [&](const Walk& at) {
-    return Rest<T, DRAFT>{seq.p_row(at.cur), seq.q_row(at.cur), at.a, a.vocab, s, at.cur, at.next};
   };
   int drawn = -1;
   if (w.count > 0) {
     if constexpr (DRAFT) {
       while (!w.draw) {
-        w.mass = total();
-        const int cur = w.cur;
+        w.mass = wave_sum(lane_total());
         walk_on<DRAFT>(s, w, seq.n, path);
-        if (!w.draw || w.cur != cur) pass(rest_of(w));
+        pass(R{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, nullptr, 0});
       }
+    } else {
+      list_tried(s, w.cur, w.next, kRestThreads);
     }
-    Rest<T, DRAFT> rest = rest_of(w);
-    double all = total();
+    R rest{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, s.tried, DRAFT ? 0 : s.n_tried};
+    double of_lane = lane_total(), upto = wave_scan(of_lane), all = __shfl(upto, 63);
     if (!(all > 0.0)) {  // nothing is left
       rest.a = 0.0;
       rest.n_tried = 0;
       pass(rest);
-      all = total();
+      of_lane = lane_total();
+      upto = wave_scan(of_lane);
+      all = __shfl(upto, 63);
     }
     if (all > 0.0) {
-      const double want = (double)s.u[0] * all;
-      // the piece, of those that have anything
-      double before = 0.0, past = 0.0;
-      int piece = 0;
-      for (int i = 0; i < a.pieces; i++) {
+      const double want = (double)u_root * all;
+      // the piece: the first whose running sum is above, or the last that has anything
+      const uint64_t past = __builtin_amdgcn_ballot_w64(upto > want && of_lane > 0.0);
+      const uint64_t any = __builtin_amdgcn_ballot_w64(of_lane > 0.0);
+      const int at = past ? (int)__builtin_ctzll(past) : 63 - (int)__builtin_clzll(any);
+      double before = 0.0, upto_piece = at == 0 ? 0.0 : __shfl(upto, max(at - 1, 0));
+      int piece = at * per;
+      for (int i = at * per; i < min(a.pieces, (at + 1) * per); i++)
         if (sums[i] > 0.0) {
-          before = past;
+          before = upto_piece;
           piece = i;
-          past += sums[i];
-          if (past > want) break;
+          upto_piece += sums[i];
+          if (upto_piece > want) break;
         }
-      }
-      // the token: a thread has N tokens in a row, a wave 64 N, one after the other
-      constexpr int kTurn = 64 * N;
-      const int x_end = min(a.vocab, (piece + 1) * kPiece);
+      // the token: a thread has N tokens in a row
       const int x = piece * kPiece + threadIdx.x * N;
-      static_assert(kTurn * kRestWaves >= kPiece, "a piece in one go");
-      double r[N];
-      double mine = 0.0;
+      const bool mine = (int)threadIdx.x * N < kPiece;
+      double r[N], of = 0.0;
+      if (mine) {
+        typename R::Raw v[1];
+        rest.load(x, 0, v);
+        rest.values(x, v[0], r);
 #pragma unroll
-      for (int e = 0; e < N; e++) r[e] = 0.0;
-      if (threadIdx.x * N < kPiece && x < x_end) {
-        rest.at(x, r);
-#pragma unroll
-        for (int e = 0; e < N; e++) mine += r[e];
+        for (int e = 0; e < N; e++) of += r[e];
       }
-      double upto = mine;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const double from = __shfl_up(upto, d);
-        if (lane >= d) upto += from;
-      }
-      if (lane == 63) share[wave] = upto;
+      const double in_wave = wave_scan(of);
+      if (lane == 63) share[wave] = in_wave;
       __syncthreads();
-      for (int i = 0; i < wave; i++) before += share[i];
-      double sum = before + (upto - mine);
-      int first = INT32_MAX, positive_at = -1;
+      if (mine) {
+        for (int i = 0; i < wave; i++) before += share[i];
+        double sum = before + (in_wave - of);
+        int first = -1, positive_at = -1;
 #pragma unroll
-      for (int e = 0; e < N; e++) {
-        sum += r[e];
-        if (r[e] > 0.0) {
-          positive_at = x + e;
-          if (sum > want && first == INT32_MAX) first = x + e;
+        for (int e = 0; e < N; e++) {
+          sum += r[e];
+          if (r[e] > 0.0) {
+            positive_at = rest.base(x) + e;
+            if (sum > want && first < 0) first = positive_at;
+          }
         }
+        if (first >= 0) atomicMin((uint32_t*)&found, (uint32_t)first);  // (-1 is the largest)
+        if (positive_at >= 0) atomicMax(&last_positive, positive_at);
       }
-      if (first != INT32_MAX) atomicMin((uint32_t*)&found, (uint32_t)first);  // (-1 is the largest)
-      if (positive_at >= 0) atomicMax(&last_positive, positive_at);
       __syncthreads();
       drawn = found != -1 ? found : last_positive;  // (the last: where roundings have the sums end short of their total)
     }
@@ -444,7 +468,7 @@ uint64_t walk_bytes(const rswa_verify_params* p) {
 
 template <typename T>
 void launch_verify(const VerifyArgs& a, hipStream_t stream) {
-  const dim3 first((unsigned)a.pieces, (unsigned)a.batch), rest((unsigned)a.batch);
+  const dim3 first((unsigned)ceil_div(a.pieces, kFirstPieces), (unsigned)a.batch), rest((unsigned)a.batch);
   if (a.draft) {
     hipLaunchKernelGGL((verify_first_kernel<T, true>), first, dim3(kFirstThreads), 0, stream, a);
     hipLaunchKernelGGL((verify_rest_kernel<T, true>), rest, dim3(kRestThreads), 0, stream, a);
