@@ -226,8 +226,9 @@ struct AcceptArgs {
 
 // Rows that a path names, as many as there are ahead of its first entry that is no row of the sequence.  As the kernel
 // for single tokens: paths are a few tokens, and their launch waits for little but memory.  A wave has the keys or the
-// values of one head that go to one page, kRows of them in registers (longer paths are read twice, for the scale and for
-// the codes).
+// values of one head that go to one page, 16 rows at a time, the first of them in registers from the scale to the codes
+// (longer paths are read twice).  Of the values 16 rows are bytes of two groups of 16 places, which are read while the rows
+// are, and written whole.
 template <typename T, int D>
 __global__ __launch_bounds__(64) void cache_accept_kernel(const AcceptArgs a) {
   constexpr int E = D / 64, kRows = 16;
@@ -247,7 +248,7 @@ __global__ __launch_bounds__(64) void cache_accept_kernel(const AcceptArgs a) {
   const int64_t in_seq = (int64_t)(start >> c.page_log2) + u;
   if (in_seq >= c.max_pages) return;
   const int id = c.table[(int64_t)b * c.table_st + in_seq];
-  const int from = u == 0 ? in_page : 0;               // first place written
+  const int from = u == 0 ? in_page : 0;                     // first place written
   const int i0 = u == 0 ? 0 : (u << c.page_log2) - in_page;  // its row of the path
   int n = 0;  // rows of the path
   for (int i = 0; i < a.path_len; i += 64) {
@@ -260,42 +261,98 @@ __global__ __launch_bounds__(64) void cache_accept_kernel(const AcceptArgs a) {
   if (count <= 0 || (uint32_t)id >= (uint32_t)c.num_pages) return;
 
   const T* const x = (const T*)a.n.x[which] + (int64_t)b * a.n.x_st[which][0] + (int64_t)hk * a.n.x_st[which][2] + lane * E;
-  auto row = [&](int i) { return *(const VE*)(x + (int64_t)(row0 + path[i0 + i]) * a.n.x_st[which][1]); };
   uint8_t* const scale = which ? const_cast<uint8_t*>(c.v_scale) + times(id, c.vs_st[0]) + times(hk, c.vs_st[1])
                                : const_cast<uint8_t*>(c.k_scale) + times(id, c.ks_st[0]) + times(hk, c.ks_st[1]);
   uint8_t* const page = which ? const_cast<uint8_t*>(c.v) + times(id, c.v_st[0]) + times(hk, c.v_st[1])
                               : const_cast<uint8_t*>(c.k) + times(id, c.k_st[0]) + times(hk, c.k_st[1]);
-  const int was = from > 0 ? *scale : 0;
-  VE v[kRows];
-  float most = 0.f;
-  auto largest = [&](const VE& r) {
+  auto load = [&](VE (&v)[kRows], int i) {  // rows i .. (the last again behind it)
 #pragma unroll
-    for (int k = 0; k < E; k++) {
-      const float y = __builtin_fabsf((float)r[k]);
-      most = y < __builtin_inff() ? fmaxf(most, y) : most;
-    }
+    for (int e = 0; e < kRows; e++)
+      v[e] = *(const VE*)(x + (int64_t)(row0 + path[i0 + min(i + e, count - 1)]) * a.n.x_st[which][1]);
   };
+  float most = 0.f;
+  auto largest = [&](const VE (&v)[kRows]) {
 #pragma unroll
-  for (int i = 0; i < kRows; i++) v[i] = row(min(i, count - 1));
+    for (int e = 0; e < kRows; e++)
 #pragma unroll
-  for (int i = 0; i < kRows; i++) largest(v[i]);
-  for (int i = kRows; i < count; i++) largest(row(i));
+      for (int k = 0; k < E; k++) {
+        const float y = __builtin_fabsf((float)v[e][k]);
+        most = y < __builtin_inff() ? fmaxf(most, y) : most;
+      }
+  };
+  // groups of places of rows i ..: the first, and the one behind it (or itself, at the page's end)
+  auto group = [&](int i, int which_of) { return min((from + i) / 16 + which_of, (page_size >> 4) - 1); };
+  u32x4 held[2][E];
+  auto load_groups = [&](int i) {
+#pragma unroll
+    for (int g = 0; g < 2; g++)
+#pragma unroll
+      for (int k = 0; k < E; k++) held[g][k] = *(const u32x4*)(page + (group(i, g) * D + lane * E + k) * 16);
+  };
+  VE v[kRows];
+  load(v, 0);
+  if (which) load_groups(0);
+  const int was = from > 0 ? *scale : 0;
+  largest(v);
+  for (int i = kRows; i < count; i += kRows) {
+    VE more[kRows];
+    load(more, i);
+    largest(more);
+  }
   const int e_new = max(was, scale_byte(wave_max(most)));
   const float inv = inverse(e_new);
-  if (from > 0 && e_new > was) rescale_page<D>(page, which, from, e_new - was, lane);
+  const bool grown = from > 0 && e_new > was;
+  if (grown) rescale_page<D>(page, which, which ? from & ~15 : from, e_new - was, lane);
+  const float shrink = grown && e_new - was < 127 ? __builtin_bit_cast(float, (uint32_t)(127 - (e_new - was)) << 23) : 0.f;
   if (lane == 0) *scale = (uint8_t)e_new;
-  auto put = [&](const VE& r, int place) {
-    const uint32_t code = codes4((float)r[0] * inv, (float)r[E - 1] * inv, 0.f, 0.f);
+  for (int i = 0;;) {
+    const int rows = min(kRows, count - i);
+    if (!which) {
 #pragma unroll
-    for (int k = 0; k < E; k++) {
-      const int d = lane * E + k;
-      page[which ? place / 16 * (16 * D) + d * 16 + place % 16 : place * D + d] = (uint8_t)(code >> (8 * k));
+      for (int e = 0; e < kRows; e++)
+        if (e < rows) {
+          const uint32_t code = codes4((float)v[e][0] * inv, (float)v[e][E - 1] * inv, 0.f, 0.f);
+          uint8_t* const to = page + (from + i + e) * D + lane * E;
+          if constexpr (E == 2)
+            *(uint16_t*)to = (uint16_t)code;
+          else
+            *to = (uint8_t)code;
+        }
+    } else {
+      typedef unsigned __int128 u128;
+      const int at = (from + i) & 15, old = from + i - at < from ? at : 0;  // places of the first group from before the call
+      const u128 low = rows < 16 ? ((u128)1 << (8 * rows)) - 1 : ~(u128)0;
+#pragma unroll
+      for (int k = 0; k < E; k++) {
+        u32x4 fresh;
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+          fresh[q] = codes4((float)v[4 * q][k] * inv, (float)v[4 * q + 1][k] * inv, (float)v[4 * q + 2][k] * inv,
+                            (float)v[4 * q + 3][k] * inv);
+        const u128 codes = __builtin_bit_cast(u128, fresh);
+        u32x4 before = held[0][k];
+        if (grown && old > 0) {
+#pragma unroll
+          for (int q = 0; q < 4; q++) before[q] = rescale4(before[q], shrink);
+        }
+        const u128 mine = low << (8 * at), keep = ((u128)1 << (8 * old)) - 1;
+        u128 w = __builtin_bit_cast(u128, held[0][k]);
+        w = (w & ~keep) | (__builtin_bit_cast(u128, before) & keep);
+        w = (w & ~mine) | ((codes << (8 * at)) & mine);
+        *(u32x4*)(page + (group(i, 0) * D + lane * E + k) * 16) = __builtin_bit_cast(u32x4, w);
+        if (at + rows > 16) {
+          const u128 rest = low >> (8 * (16 - at)), next = codes >> (8 * (16 - at));
+          w = __builtin_bit_cast(u128, held[1][k]);
+          w = (w & ~rest) | (next & rest);
+          *(u32x4*)(page + (group(i, 1) * D + lane * E + k) * 16) = __builtin_bit_cast(u32x4, w);
+        }
+      }
     }
-  };
-#pragma unroll
-  for (int i = 0; i < kRows; i++)
-    if (i < count) put(v[i], from + i);
-  for (int i = kRows; i < count; i++) put(row(i), from + i);
+    i += kRows;
+    if (i >= count) break;
+    load(v, i);
+    if (which) load_groups(i);
+  }
 }
 
 }  // namespace
