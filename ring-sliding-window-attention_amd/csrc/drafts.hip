@@ -9,10 +9,7 @@
 // Sums and comparisons are in 64 bits: a draw lies next to borders that are closer than 32-bit sums of a vocabulary.
 // The first pass -- a chain has no other -- is one launch over all rows in pieces of 1024 tokens, each of whose blocks walks
 // for itself; a second launch, a block for each sequence, goes on from there and draws the next token by the pieces' sums.
-#include "rswa_common.h"
-
-#include <algorithm>
-#include <type_traits>
+#include "kv_cache.h"
 
 namespace rswa {
 namespace {
@@ -281,38 +278,49 @@ struct Rest {
   }
 };
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
+// Sums over the lanes up to each, in the vector pipe (as wave_scan of floats).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v) {
+  const u32x2 w = __builtin_bit_cast(u32x2, v);
+  return __builtin_bit_cast(double, u32x2{(uint32_t)dpp_or_zero<CTRL, ROWS>((int)w[0]), (uint32_t)dpp_or_zero<CTRL, ROWS>((int)w[1])});
+}
+__device__ __forceinline__ double wave_scan(double v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  v += moved<0x143, 0xc>(v);
   return v;
 }
-__device__ __forceinline__ double wave_scan(double v) {  // of the lanes up to each
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double from = __shfl_up(v, d);
-    if (lane >= d) v += from;
-  }
-  return v;
+__device__ __forceinline__ double of_lane(double v, int lane) {  // (the same lane for all)
+  const u32x2 w = __builtin_bit_cast(u32x2, v);
+  return __builtin_bit_cast(double, u32x2{(uint32_t)__builtin_amdgcn_readlane((int)w[0], lane),
+                                          (uint32_t)__builtin_amdgcn_readlane((int)w[1], lane)});
 }
+__device__ __forceinline__ double wave_sum(double v) { return of_lane(wave_scan(v), 63); }
 
-// Sum over a piece, by one wave: all of its loads first.
-template <typename T, bool DRAFT>
-__device__ __forceinline__ double piece_sum(const Rest<T, DRAFT>& rest, int piece) {
+// Sums over M pieces, `step` apart, by one wave: all of their loads first.
+template <int M, typename T, bool DRAFT>
+__device__ __forceinline__ void piece_sums(const Rest<T, DRAFT>& rest, int piece, int step, double (&sum)[M]) {
   using R = Rest<T, DRAFT>;
   constexpr int TURNS = kPiece / (64 * R::N);
-  const int x = piece * kPiece + (threadIdx.x & 63) * R::N;
-  typename R::Raw v[TURNS];
-  rest.load(x, 64 * R::N, v);
-  double sum = 0.0;
+  typename R::Raw v[M][TURNS];
+  auto first = [&](int m) { return (piece + m * step) * kPiece + lane_id() * R::N; };
 #pragma unroll
-  for (int i = 0; i < TURNS; i++) {
-    double r[R::N];
-    rest.values(x + i * 64 * R::N, v[i], r);
+  for (int m = 0; m < M; m++) rest.load(first(m), 64 * R::N, v[m]);
 #pragma unroll
-    for (int e = 0; e < R::N; e++) sum += r[e];
+  for (int m = 0; m < M; m++) {
+    sum[m] = 0.0;
+#pragma unroll
+    for (int i = 0; i < TURNS; i++) {
+      double r[R::N];
+      rest.values(first(m) + i * 64 * R::N, v[m][i], r);
+#pragma unroll
+      for (int e = 0; e < R::N; e++) sum[m] += r[e];
+    }
+    sum[m] = wave_sum(sum[m]);
   }
-  return wave_sum(sum);
 }
 
 constexpr int kFirstThreads = 256, kFirstPieces = kFirstThreads / 64;
@@ -339,8 +347,9 @@ __global__ __launch_bounds__(kFirstThreads) void verify_first_kernel(const Verif
   if constexpr (!DRAFT) list_tried(s, w.cur, w.next, kFirstThreads);
   if (piece >= a.pieces) return;
   const Rest<T, DRAFT> rest{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, s.tried, DRAFT ? 0 : s.n_tried};
-  const double sum = piece_sum(rest, piece);
-  if ((threadIdx.x & 63) == 0) a.sums[(int64_t)b * a.pieces + piece] = sum;
+  double sum[1];
+  piece_sums(rest, piece, 0, sum);
+  if ((threadIdx.x & 63) == 0) a.sums[(int64_t)b * a.pieces + piece] = sum[0];
 }
 
 constexpr int kRestThreads = 1024, kRestWaves = kRestThreads / 64;
@@ -358,19 +367,22 @@ __global__ __launch_bounds__(kRestThreads) void verify_rest_kernel(const VerifyA
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x / 64;
   const Sequence<T> seq(a, b);
   int32_t* const path = a.path + (int64_t)b * a.path_len;
+  // (all on their way at once: sums that the first launch has not written are not looked at)
+  const float u_root = seq.n > 0 ? a.uniforms[a.cu ? seq.row0 : b * a.uniforms_st] : 0.f;
+  for (int i = threadIdx.x; i < a.pieces; i += kRestThreads) sums[i] = a.sums[(int64_t)b * a.pieces + i];
   Walk w = a.walks[b];
-  const float u_root = w.count > 0 ? a.uniforms[a.cu ? seq.row0 : b * a.uniforms_st] : 0.f;
-  if (w.count > 0) {
-    for (int i = threadIdx.x; i < a.pieces; i += kRestThreads) sums[i] = a.sums[(int64_t)b * a.pieces + i];
-    if (!DRAFT || !w.draw) seq.load(s, kRestThreads);
-  }
+  if (w.count > 0 && (!DRAFT || !w.draw)) seq.load(s, kRestThreads);
   if (threadIdx.x == 0) found = last_positive = -1;
   __syncthreads();
   auto pass = [&](const R& rest) {  // sums of all pieces
     __syncthreads();
-    for (int i = wave; i < a.pieces; i += kRestWaves) {
-      const double of = piece_sum(rest, i);
-      if (lane == 0) sums[i] = of;
+    for (int i = wave; i < a.pieces; i += 2 * kRestWaves) {  // (a piece behind the last: 0, as the row's end)
+      double of[2];
+      piece_sums(rest, i, kRestWaves, of);
+      if (lane == 0) {
+        sums[i] = of[0];
+        if (i + kRestWaves < a.pieces) sums[i + kRestWaves] = of[1];
+      }
     }
     __syncthreads();
   };
@@ -393,22 +405,22 @@ __global__ __launch_bounds__(kRestThreads) void verify_rest_kernel(const VerifyA
       list_tried(s, w.cur, w.next, kRestThreads);
     }
     R rest{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, s.tried, DRAFT ? 0 : s.n_tried};
-    double of_lane = lane_total(), upto = wave_scan(of_lane), all = __shfl(upto, 63);
+    double own = lane_total(), upto = wave_scan(own), all = of_lane(upto, 63);
     if (!(all > 0.0)) {  // nothing is left
       rest.a = 0.0;
       rest.n_tried = 0;
       pass(rest);
-      of_lane = lane_total();
-      upto = wave_scan(of_lane);
-      all = __shfl(upto, 63);
+      own = lane_total();
+      upto = wave_scan(own);
+      all = of_lane(upto, 63);
     }
     if (all > 0.0) {
       const double want = (double)u_root * all;
       // the piece: the first whose running sum is above, or the last that has anything
-      const uint64_t past = __builtin_amdgcn_ballot_w64(upto > want && of_lane > 0.0);
-      const uint64_t any = __builtin_amdgcn_ballot_w64(of_lane > 0.0);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(upto > want && own > 0.0);
+      const uint64_t any = __builtin_amdgcn_ballot_w64(own > 0.0);
       const int at = past ? (int)__builtin_ctzll(past) : 63 - (int)__builtin_clzll(any);
-      double before = 0.0, upto_piece = at == 0 ? 0.0 : __shfl(upto, max(at - 1, 0));
+      double before = 0.0, upto_piece = at == 0 ? 0.0 : of_lane(upto, max(at - 1, 0));
       int piece = at * per;
       for (int i = at * per; i < min(a.pieces, (at + 1) * per); i++)
         if (sums[i] > 0.0) {
