@@ -584,6 +584,8 @@ PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
       if (t->size(d) > 1 && t->stride(d) == 0) Py_RETURN_NONE;  // (rows that are one another's)
   c10::DeviceGuard guard(c.device);
   if (c.launch(cache_lib.read) != RSWA_OK) Py_RETURN_NONE;
+  for (const Tensor* t : {k, v})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();  // (a graph that has saved them is to notice)
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }

@@ -270,6 +270,9 @@ def _read(to_k, to_v, k, v, k_scale, v_scale, page_table, first, cu_seqlens):
     _new_rows(p, to_k, to_v, cu_seqlens is not None)
     for t in (to_k, to_v):
         assert all(n <= 1 or s != 0 for n, s in zip(t.shape, t.stride())), "k and v are written: their rows must not overlap"
+    for t in (to_k, to_v):
+        if not t.is_inference():  # (a graph that has saved them for its backward is to notice)
+            torch.autograd.graph.increment_version(t)
     _lib.launch(dev, _lib.lib().rswa_cache_read, p)
 
 

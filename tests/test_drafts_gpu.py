@@ -892,3 +892,65 @@ def test_derivatives_are_refused():
     with pytest.raises(RuntimeError, match="no backward"):
         kv_cache_read(cache, k.clone().requires_grad_(), v, table, held)
     assert isinstance(tree, DraftTree)
+
+
+def test_pools_beyond_4_gib():
+    """Pages whose offsets pass 32 bits, at the pool's both ends: what a small pool gives."""
+    from ring_swa import KVCache, kv_cache_accept, kv_cache_append, kv_cache_read
+
+    pages = (5 << 30) // (8 * 64 * 128)
+    pools = (KVCache.empty(pages, 8, 128, device="cuda"), ints([[pages - 1, 0, pages - 2], [1, pages - 3, 2]])), \
+        (KVCache.empty(6, 8, 128, device="cuda"), ints([[0, 1, 2], [3, 4, 5]]))
+    parents = [some_parents(random.Random(b), 40, 7) for b in range(2)]
+    tree = tree_tensors(parents, False)
+    path = ints([[0, 5, 30, -1], [0, 1, 2, 39]])
+    results = []
+    for cache, table in pools:
+        g = torch.Generator().manual_seed(10)
+        kv_cache_append(cache, *(randn(g, torch.bfloat16, 2, 126, 8, 128) for _ in range(2)), table, ints([0, 0]))
+        q, (k, v) = randn(g, torch.bfloat16, 2, 40, 32, 128), (randn(g, torch.bfloat16, 2, 40, 8, 128) for _ in range(2))
+        out, lse = attend((q, k, v, tree, cache, table, ints([126, 126]), -1, None, 0), return_lse=True)
+        kv_cache_accept(cache, k, v, path, table, ints([126, 126]))
+        back = [torch.empty(2, 129, 8, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        kv_cache_read(cache, *back, table, ints([0, 0]))
+        results.append((out, lse, *back))
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+
+
+def test_a_tree_with_room_for_more_nodes():
+    from ring_swa import draft_tree, verify_drafts
+
+    args, parents = tree_case(3)
+    q, k, v, tree, cache, table, lens, window, cu, sinks = args
+    wide = draft_tree(tree.parents, max_nodes=1000)
+    assert wide.ancestors.shape == (1, 32, 16) and bool((wide.ancestors[..., 1:] == 0).all())
+    assert torch.equal(wide.ancestors[..., :1], tree.ancestors)
+    for x, y in zip(attend(args, return_lse=True), attend((q, k, v, wide, *args[4:]), return_lse=True)):
+        assert (x - y).abs().max() <= 2.0 ** -7 * x.abs().max()  # (cut elsewhere: other sums, within a rounding of each)
+    p = torch.rand(1, 32, 900, device="cuda")
+    tokens, u = torch.randint(0, 900, (1, 32), device="cuda"), torch.rand(1, 32, device="cuda")
+    for x, y in zip(verify_drafts(tree, tokens, p, p, u), verify_drafts(wide, tokens, p, p, u)):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_graph_that_has_saved_the_rows_notices_a_read(native, monkeypatch):
+    from ring_swa import kv_cache_read, ring_sliding_window_attn
+    from ring_swa.ops import kv_cache
+
+    if not native:
+        monkeypatch.setattr(kv_cache, "_calls", lambda *_: None)
+    cache, table, lens, _ = make([100], 2, 64, 32, 77)
+    k, v = (torch.empty(1, 100, 2, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    first = torch.zeros_like(lens)
+    kv_cache_read(cache, k, v, table, first)
+    q = torch.randn(1, 100, 4, 64, device="cuda").bfloat16().requires_grad_()
+    ring_sliding_window_attn(q, k, v, 50).float().sum().backward()
+    out = ring_sliding_window_attn(q, k, v, 50)
+    kv_cache_read(cache, k, v, table, first)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.float().sum().backward()
+    with torch.inference_mode():
+        k, v = (torch.empty(1, 100, 2, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        kv_cache_read(cache, k, v, table, first)
+    kv_cache_read(cache, k, v, table, first)
