@@ -8,7 +8,10 @@
 //   max(0, max(0, p - a q) / S - q) = max(0, p - (a + S) q) / S
 // Sums and comparisons are in 64 bits: a draw lies next to borders that are closer than 32-bit sums of a vocabulary.
 // The first pass -- a chain has no other -- is one launch over all rows in pieces of 1024 tokens, each of whose blocks walks
-// for itself; a second launch, a block for each sequence, goes on from there and draws the next token by the pieces' sums.
+// for itself; a second launch, a block for each sequence, goes on from there and draws the next token by the pieces' sums (for
+// large vocabularies some more passes are launches like the first, see stages_of).
+// Few sequences are launches and round trips: a chain of 6 over 131072 tokens 11.5 us, 4.0 + 6.7 of kernels.  Where siblings are
+// rejected the passes come one after the other: 32 trees of 32 nodes over 32768 tokens 31 us, up to 4 passes behind the first.
 #include "kv_cache.h"
 
 namespace rswa {
@@ -107,9 +110,10 @@ struct VerifyArgs {
   int32_t* path;
   int32_t* accepted;
   void* next_token;
-  // from the first launch to the second
-  double* sums;  // [batch][pieces]
-  struct Walk* walks;
+  // from one launch to the next: of `stage` launches behind the first
+  double* sums;  // [stage][batch][pieces]
+  struct Walk* walks;  // [stage][batch]
+  int32_t stage;
 };
 
 // Where the walk of a sequence is: at node `cur`, whose children below `next` are tried, with the residual
@@ -352,6 +356,38 @@ __global__ __launch_bounds__(kFirstThreads) void verify_first_kernel(const Verif
   if ((threadIdx.x & 63) == 0) a.sums[(int64_t)b * a.pieces + piece] = sum[0];
 }
 
+// A lane's share of the sums of `pieces` pieces: as many as each in a row.
+__device__ __forceinline__ double lane_total(const double* sums, int pieces) {
+  const int per = (pieces + 63) / 64, lane = threadIdx.x & 63;
+  double of = 0.0;
+  for (int i = lane * per; i < min(pieces, (lane + 1) * per); i++) of += sums[i];
+  return of;
+}
+
+// One rejection further, where that wants a sum: as the first launch, from where the one before it has come.
+template <typename T>
+__global__ __launch_bounds__(kFirstThreads) void verify_next_kernel(const VerifyArgs a) {
+  __shared__ Nodes s;
+  const int b = blockIdx.y, piece = blockIdx.x * kFirstPieces + threadIdx.x / 64;
+  const Walk* const walks = a.walks + (int64_t)(a.stage - 1) * a.batch;
+  const double* const sums = a.sums + ((int64_t)(a.stage - 1) * a.batch + b) * a.pieces;
+  double* const to = a.sums + ((int64_t)a.stage * a.batch + b) * a.pieces;
+  Walk w = walks[b];
+  const bool wanted = w.count > 0 && !w.draw;
+  const Sequence<T> seq(a, b);
+  if (wanted) {
+    seq.load(s, kFirstThreads);
+    __syncthreads();
+    w.mass = wave_sum(lane_total(sums, a.pieces));
+    walk_on<true>(s, w, seq.n, blockIdx.x == 0 ? a.path + (int64_t)b * a.path_len : nullptr);
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.walks[(int64_t)a.stage * a.batch + b] = w;
+  if (piece >= a.pieces || w.count == 0) return;
+  double sum[1] = {wanted ? 0.0 : sums[piece]};
+  if (wanted) piece_sums(Rest<T, true>{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, nullptr, 0}, piece, 0, sum);
+  if ((threadIdx.x & 63) == 0) to[piece] = sum[0];
+}
+
 constexpr int kRestThreads = 1024, kRestWaves = kRestThreads / 64;
 constexpr int kMaxPieces = 4096;
 
@@ -369,8 +405,9 @@ __global__ __launch_bounds__(kRestThreads) void verify_rest_kernel(const VerifyA
   int32_t* const path = a.path + (int64_t)b * a.path_len;
   // (all on their way at once: sums that the first launch has not written are not looked at)
   const float u_root = seq.n > 0 ? a.uniforms[a.cu ? seq.row0 : b * a.uniforms_st] : 0.f;
-  for (int i = threadIdx.x; i < a.pieces; i += kRestThreads) sums[i] = a.sums[(int64_t)b * a.pieces + i];
-  Walk w = a.walks[b];
+  const double* const known = a.sums + ((int64_t)a.stage * a.batch + b) * a.pieces;
+  for (int i = threadIdx.x; i < a.pieces; i += kRestThreads) sums[i] = known[i];
+  Walk w = a.walks[(int64_t)a.stage * a.batch + b];
   if (w.count > 0 && (!DRAFT || !w.draw)) seq.load(s, kRestThreads);
   if (threadIdx.x == 0) found = last_positive = -1;
   __syncthreads();
@@ -386,18 +423,13 @@ __global__ __launch_bounds__(kRestThreads) void verify_rest_kernel(const VerifyA
     }
     __syncthreads();
   };
-  // A lane has PER pieces in a row.  All waves do the same.
+  // (all waves do the same)
   const int per = (a.pieces + 63) / 64;
-  auto lane_total = [&] {
-    double of = 0.0;
-    for (int i = lane * per; i < min(a.pieces, (lane + 1) * per); i++) of += sums[i];
-    return of;
-  };
   int drawn = -1;
   if (w.count > 0) {
     if constexpr (DRAFT) {
       while (!w.draw) {
-        w.mass = wave_sum(lane_total());
+        w.mass = wave_sum(lane_total(sums, a.pieces));
         walk_on<DRAFT>(s, w, seq.n, path);
         pass(R{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, nullptr, 0});
       }
@@ -405,12 +437,12 @@ __global__ __launch_bounds__(kRestThreads) void verify_rest_kernel(const VerifyA
       list_tried(s, w.cur, w.next, kRestThreads);
     }
     R rest{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, s.tried, DRAFT ? 0 : s.n_tried};
-    double own = lane_total(), upto = wave_scan(own), all = of_lane(upto, 63);
+    double own = lane_total(sums, a.pieces), upto = wave_scan(own), all = of_lane(upto, 63);
     if (!(all > 0.0)) {  // nothing is left
       rest.a = 0.0;
       rest.n_tried = 0;
       pass(rest);
-      own = lane_total();
+      own = lane_total(sums, a.pieces);
       upto = wave_scan(own);
       all = of_lane(upto, 63);
     }
@@ -474,15 +506,27 @@ __global__ __launch_bounds__(kRestThreads) void verify_rest_kernel(const VerifyA
 
 int pieces_of(int vocab) { return (int)ceil_div(vocab, kPiece); }
 
+// Launches between the first and the last: a pass over all compute units takes 4 us (2.5 if no sequence wants it), one by the
+// last launch's block for a sequence 4.5 of 32768 tokens and 15 of 131072.  So three for large vocabularies and trees, of
+// whose sequences some reject a few siblings: 8 sequences of 32 nodes over 131072 tokens 65 us without, 31 with three, 32 with
+// five; 32 of 8 over 32768 22.0 and 24.8.  Not for what is likely a chain, which rejects once (6 nodes over 131072 11.6, 19.3).
+int stages_of(const rswa_verify_params* p) {
+  return p->draft && p->vocab >= 65536 && (p->cu_seqlens ? p->max_nodes : p->nodes) > 8 ? 3 : 0;
+}
+
 uint64_t walk_bytes(const rswa_verify_params* p) {
-  return (uint64_t)p->batch * (sizeof(Walk) + 8 * (uint64_t)pieces_of(p->vocab));
+  return (uint64_t)(stages_of(p) + 1) * p->batch * (sizeof(Walk) + 8 * (uint64_t)pieces_of(p->vocab));
 }
 
 template <typename T>
-void launch_verify(const VerifyArgs& a, hipStream_t stream) {
+void launch_verify(VerifyArgs& a, int stages, hipStream_t stream) {
   const dim3 first((unsigned)ceil_div(a.pieces, kFirstPieces), (unsigned)a.batch), rest((unsigned)a.batch);
   if (a.draft) {
     hipLaunchKernelGGL((verify_first_kernel<T, true>), first, dim3(kFirstThreads), 0, stream, a);
+    while (a.stage < stages) {
+      a.stage++;
+      hipLaunchKernelGGL((verify_next_kernel<T>), first, dim3(kFirstThreads), 0, stream, a);
+    }
     hipLaunchKernelGGL((verify_rest_kernel<T, true>), rest, dim3(kRestThreads), 0, stream, a);
   } else {
     hipLaunchKernelGGL((verify_first_kernel<T, false>), first, dim3(kFirstThreads), 0, stream, a);
@@ -581,15 +625,16 @@ extern "C" int rswa_verify_drafts(const rswa_verify_params* p, void* stream) {
   a.accepted = p->accepted;
   a.next_token = p->next_token;
   a.sums = (double*)p->workspace;
-  a.walks = (Walk*)(a.sums + (int64_t)p->batch * a.pieces);
+  const int stages = stages_of(p);
+  a.walks = (Walk*)(a.sums + (int64_t)(stages + 1) * p->batch * a.pieces);
   clear_launch_error();
   hipStream_t st = (hipStream_t)stream;
   if (p->dtype == RSWA_F32)
-    launch_verify<float>(a, st);
+    launch_verify<float>(a, stages, st);
   else if (p->dtype == RSWA_BF16)
-    launch_verify<__bf16>(a, st);
+    launch_verify<__bf16>(a, stages, st);
   else
-    launch_verify<_Float16>(a, st);
+    launch_verify<_Float16>(a, stages, st);
   return check_launch(who);
 }
 

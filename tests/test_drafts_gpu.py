@@ -954,3 +954,28 @@ def test_a_graph_that_has_saved_the_rows_notices_a_read(native, monkeypatch):
         k, v = (torch.empty(1, 100, 2, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
         kv_cache_read(cache, k, v, table, first)
     kv_cache_read(cache, k, v, table, first)
+
+
+@pytest.mark.parametrize("nodes,vocab", [(8, 70000), (9, 65536), (9, 65535), (24, 65537), (24, 131072)])
+def test_verification_over_large_vocabularies(nodes, vocab):
+    """(Passes of several launches from 65536 tokens and 9 nodes on.)  All siblings of the root, most of them rejected."""
+    from ring_swa import verify_drafts
+
+    g = torch.Generator().manual_seed(nodes + vocab)
+    batch = 6
+    parents = [[-1] + [0] * (nodes - 3) + [1, 2]] * batch
+    tree = tree_tensors(parents, False)
+    p, q = (t.view(batch, nodes, vocab).cuda() for t in probabilities(g, batch * nodes, vocab, torch.float32, 1.0))
+    # drafts that the target likes less than the draft does, which are all rejected, and of the last sequences what it draws
+    tokens = (q / p).topk(nodes, -1).indices[:, 0].contiguous()
+    for b in range(3, batch):
+        tokens[b] = torch.tensor(drawn(random.Random(b + vocab), parents[b], q[b].cpu()))
+    u = torch.rand(batch, nodes, generator=g)
+    u[0] = 0.9999
+    path, accepted, token = verify_drafts(tree, tokens, p, q, u.cuda())
+    counts = set()
+    for b in range(batch):
+        want = R.verify(parents[b], tokens[b].tolist(), p[b].cpu(), q[b].cpu(), u[b].tolist())
+        assert path[b, :int(accepted[b])].tolist() == want[0] and int(token[b]) == want[1], b
+        counts.add(want[0][1] if len(want[0]) > 1 else 0)
+    assert 0 in counts and len(counts) > 1  # (some with all rejected, some not)
