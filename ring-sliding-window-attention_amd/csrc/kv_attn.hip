@@ -1103,20 +1103,21 @@ struct Cut {
   int64_t part_units;  // at most
   int64_t grid;
 };
-//
+
 // Nodes of trees (`words` != 0: tiles that a sequence's nodes are at most) are cut by the tiles of keys that a unit gets in
 // a launch of two for each compute unit (32 / 8 heads of 128; us):
-//   up to 20 with row tiles of 16: those.  One sequence of 32 nodes against 4001 keys 18.9 (tiles of 32: 20.3), 8 of 6 22 / 27, 2 of
+//   up to 20 with row tiles of 16: those.  One sequence of 32 nodes against 4001 keys 18.7 (tiles of 32: 20.3), 8 of 6 22 / 27, 2 of
 //     32 21 / 24; with 32 tiles a unit, 4 of 32, 31 / 27
 //   33 to 64 rows and a tile of 64 for every resident block: waves with 16 rows of their own.  64 sequences of 14 nodes
-//     against 1000 keys 47 (shared keys: 61), of 12 against 4001 127 / 134, 128 of 16 against 512 to 4096 161 / 174; fewer, 16 of
+//     against 1000 keys 44 (shared keys: 61), of 12 against 4001 110 / 134, 128 of 16 against 512 to 4096 158 / 174; fewer, 16 of
 //     12, 44 / 40
-//   more rows, three quarters of tiles of 128 or more, and from 24 tiles on: waves with 32 rows.  8 of 64 against 8000 91 (shared
-//     101), 1 of 64 against 131072 166 / 192, 64 of 24 against 2000 102 / 117; with 8 tiles, 8 of 32, 51 / 37; 64 packed trees of up to
-//     24, 28 / 4 heads of 64, window 4092, which fill them less, 106 / 83
+//   more rows, three quarters of tiles of 128 or more, of packs 128 or more, and from 24 tiles on: waves with 32 rows.  8 of 64
+//     against 8000 91 (shared 101), 1 of 64 against 131072 165 / 192, 64 of 24 against 2000 102 / 117, a pack of 32 trees of 16 to 64
+//     against 512 to 16384 201 / 245; with 8 tiles, 8 of 32, 51 / 37; packs of 32 trees of 11 to 44 against 2000 to 6000 145 / 136, of
+//     64 of up to 24, 28 / 4 heads of 64, window 4092, 106 / 83
 // The last are cut twice as fine where they are a block for every compute unit, since then sequences of unlike lengths are not
-// evened by their splitting: 32 padded trees of 64 nodes against 512 to 16384 keys 239 -> 218, 16 128 -> 118 (equal lengths lose by
-// it: 64 of 24 against 2000 102 -> 120).  Shared keys are not cut finer than once (the packed trees 83; twice as fine 91).
+// evened by their splitting: 32 padded trees of 64 nodes against 512 to 16384 keys 239 -> 213, 16 128 -> 116 (equal lengths lose by
+// it: 64 of 24 against 2000 102 -> 113).  Shared keys are not cut finer than once (the packed trees 83; twice as fine 91).
 Cut cut_call(const rswa_cache_params* p, int words = 0) {
   Cut c;
   const int resident = 2 * kComputeUnits;
@@ -1132,8 +1133,8 @@ Cut cut_call(const rswa_cache_params* p, int words = 0) {
   if (words) {
     most_tiles += p->cu_seqlens_q ? words : std::min<int64_t>(words, ceil_div(p->seqlen_q, kTileKeys));
     auto blocks = [&](int row_tile) { return p->batch * ceil_div(rows, row_tile) * p->heads_kv; };
-    const bool own = rows > 64 ? 4 * rows >= 3 * 128 * ceil_div(rows, 128) && blocks(128) * most_tiles >= 24 * resident
-                               : rows > 32 && blocks(64) >= resident;
+    const bool filled = p->cu_seqlens_q ? rows >= 128 : 4 * rows >= 3 * 128 * ceil_div(rows, 128);
+    const bool own = rows > 64 ? filled && blocks(128) * most_tiles >= 24 * resident : rows > 32 && blocks(64) >= resident;
     c.wr = own ? 4 : 1;
     c.nt = own ? (rows > 64 ? 2 : 1) : rows <= 16 || blocks(16) * most_tiles <= 20 * resident ? 1 : 2;
   } else {

@@ -119,6 +119,7 @@ TREES = [
     ([11 * i for i in range(64)], 12, 5, 32, 8, 128, 64, -1, 0, "bf16"),
     ([(37 * i) % 900 for i in range(128)], 10, 4, 16, 4, 64, 32, 100, 3, "fp16"),
     ([(61 * i) % 900 for i in range(70)], [(7 * i) % 25 for i in range(70)], 4, 32, 8, 128, 16, 9, 2, "fp16"),
+    ([9000, 12000, 700, 0], 130, 30, 32, 2, 64, 16, 8000, 2, "bf16"),     # 32 rows a wave again, of head_dim 64
 ]
 
 
@@ -244,9 +245,10 @@ def test_what_is_not_finite_reaches_the_descendants_alone(case):
                 assert bool(((there == hit[0]) | there.isnan()).all()), (b, r)
 
 
-def test_cached_values_that_are_not_finite():
+@pytest.mark.parametrize("case", [12, 15, 19, 21])
+def test_cached_values_that_are_not_finite(case):
     """NaN codes in the window of some nodes and not of others."""
-    args, parents = tree_case(12, wild=False, holes=0)
+    args, parents = tree_case(case, wild=False, holes=0)
     q, k, v, tree, cache, table, lens, window, cu, sinks = args
     clean = attend(args)
     size = cache[0].shape[2]
