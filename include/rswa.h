@@ -499,7 +499,7 @@ int rswa_draft_tree(const rswa_tree_params* p, void* stream);
 typedef struct rswa_draft_params {
   rswa_cache_params cache;
   /* tree_attn: of rswa_draft_tree */
-  const int32_t* depths;
+  const int32_t* depths; /* below the number of the sequence's nodes */
   int64_t depths_stride; /* dense: between sequences */
   const int64_t* ancestors;
   int64_t ancestors_stride; /* dense: between sequences, in words; rows are `words` apart */
@@ -546,10 +546,10 @@ uint64_t rswa_sizeof_verify_params(void);
 typedef struct rswa_verify_params {
   int32_t dtype;       /* of target and draft: RSWA_BF16, RSWA_F16 or RSWA_F32 */
   int32_t token_bytes; /* 4 or 8: type of tokens and next_token */
-  int32_t batch;
+  int32_t batch;     /* below 2^16 */
   int32_t nodes;     /* dense */
   int32_t max_nodes; /* 1 .. 1024: nodes of a sequence from there on are not looked at */
-  int32_t vocab;
+  int32_t vocab;     /* at most 2^22 */
   int64_t total; /* packed */
   const int32_t* cu_seqlens;
   const int32_t* parents; /* tree_parents of rswa_draft_tree (a node with a parent that is no lower one is passed over) */

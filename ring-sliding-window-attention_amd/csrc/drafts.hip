@@ -10,7 +10,7 @@
 // The first pass -- a chain has no other -- is one launch over all rows in pieces of 1024 tokens, each of whose blocks walks
 // for itself; a second launch, a block for each sequence, goes on from there and draws the next token by the pieces' sums (for
 // large vocabularies some more passes are launches like the first, see stages_of).
-// Few sequences are launches and round trips: a chain of 6 over 131072 tokens 11.5 us, 4.0 + 6.7 of kernels.  Where siblings are
+// Few sequences are launches and round trips: a chain of 6 over 131072 tokens 10.1 us, 4.0 + 6.3 of kernels.  Where siblings are
 // rejected the passes come one after the other: 32 trees of 32 nodes over 32768 tokens 31 us, up to 4 passes behind the first.
 #include "kv_cache.h"
 
@@ -46,7 +46,8 @@ constexpr int kTreeThreads = 256;
 
 // A block has a sequence.  A node's ancestors among the 64 nodes of its own word are found by walking up, and the first one
 // of a lower word is remembered; the others are that one's, word by word.  (At most 63 + 15 steps through LDS in a row, where
-// a walk up a chain of 1024 would be 1023.)
+// a walk up a chain of 1024 would be 1023.)  One tree of 32 nodes 2.0 us, 256 packed ones of up to 512 7.6; the call, with its
+// three results, 6.2 and 7.2 among others.
 __global__ __launch_bounds__(kTreeThreads) void draft_tree_kernel(const TreeKernelArgs a) {
   __shared__ int32_t up[kMaxNodes];   // the parent; -1: none, -2: the node is not there
   __shared__ int32_t out[kMaxNodes];  // the first ancestor of a lower word, -1 or -2 as the chain ends

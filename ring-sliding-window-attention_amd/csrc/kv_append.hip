@@ -228,7 +228,8 @@ struct AcceptArgs {
 // for single tokens: paths are a few tokens, and their launch waits for little but memory.  A wave has the keys or the
 // values of one head that go to one page, 16 rows at a time, the first of them in registers from the scale to the codes
 // (longer paths are read twice).  Of the values 16 rows are bytes of two groups of 16 places, which are read while the rows
-// are, and written whole.
+// are, and written whole: 128 sequences of 1 to 9 rows, 8 heads of 128, 7.8 us (bytes stored one by one 12.2), one sequence
+// 5.0, a launch and four round trips (lengths, path and page, rows and groups).
 template <typename T, int D>
 __global__ __launch_bounds__(64) void cache_accept_kernel(const AcceptArgs a) {
   constexpr int E = D / 64, kRows = 16;

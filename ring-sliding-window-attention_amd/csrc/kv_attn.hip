@@ -11,6 +11,13 @@
 // Bound by memory where rows are few: 64 sequences of 256 to 32768 keys, 32 / 8 heads of 128, 217 us, 5.1 TB/s.  The keys
 // of long sequences are cut into chunks for the whole chip, whose partial results a second launch joins; one token
 // against 4001 keys takes 6.8 + 3.9 us, each a launch and some five round trips to memory in a row.
+//
+// Queries that are nodes of a tree of drafted tokens (TreeArgs) are the same kernels: their own keys and values, in 16 bits,
+// are up to 16 tiles more, of which ancestor bits say who sees whom.  One tree of 32 nodes against 4001 keys 18 us, 12.4 of the
+// first kernel: finding its unit 1.6, rows, pages and first keys 2.5, nodes 2.8 (the blocks that have them), two tiles a wave
+// 3.5, meeting in LDS 1.4.  64 trees of up to 24 with a window of 4092 (28 / 4 heads of 64, fp16) 83 us, bound by vector work and
+// by the second, half-full round of blocks; 32 of 16 to 64, padded to 64, against 512 to 16384 keys 213, 2.3 us a tile (0.92
+// PFLOP/s), the rest 13 us before and after each block's loop and unlike blocks.
 #include "kv_cache.h"
 
 namespace rswa {
@@ -624,7 +631,7 @@ __global__ __launch_bounds__(kThreads, (NT == 1 && !std::is_same_v<Args, TreeArg
   Pages next{0, 0};
   bool here = false;  // the lane's group of the tile has its page
   if constexpr (R::TREE)
-    if (no_nodes(a, x, x.row_tile * ROWS, ROWS)) 
+    if (no_nodes(a, x, x.row_tile * ROWS, ROWS))
       return put_nothing<T, D>(arguments_again<Args>(), x, hk, x.row_tile * ROWS, ROWS, threadIdx.x, kThreads);
   if (i < n) {
     const Pages now = keys.pages(list[i]);
@@ -845,7 +852,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_attn_rows_kernel(const Args
   // on their way together.
   auto& node_ops = v_ops[1];
   if constexpr (R::TREE)
-    if (no_nodes(a, x, r0, 4 * NT * 16)) 
+    if (no_nodes(a, x, r0, 4 * NT * 16))
       return put_nothing<T, D>(arguments_again<Args>(), x, hk, r0, 4 * NT * 16, threadIdx.x, kThreads);
   if constexpr (R::TREE)
     if (list.n_d > 0) stage_node_values<T, D>(a, x, hk, list.d0, &node_ops[0][0], &lds_special[0]);

@@ -126,7 +126,7 @@ def kv_cache_tree_attn(
     """Attention of a tree's nodes over their sequences' caches and over each other.
 
     ``q``: ``[batch, nodes, heads, dim]``, ``k``, ``v``: ``[batch, nodes, kv_heads, dim]`` (packed ``[tokens, ...]`` with
-    ``cu_seqlens``), bf16 or fp16; ``tree``: of ``draft_tree`` for the same rows.  ``seqlens`` counts the tokens in the
+    ``cu_seqlens``), bf16 or fp16; ``tree``: of ``draft_tree`` for the same rows (depths are below their number).  ``seqlens`` counts the tokens in the
     cache, the nodes not among them; node ``i`` is token ``seqlens + depth(i)``.  It sees the cached tokens, itself and its
     ancestors, of these the ``window_size`` before it (negative: all) and the first ``num_sink_tokens``.  Everything else
     is as in ``kv_cache_attn``; nodes that are not there: 0 and ``-inf``."""
@@ -202,8 +202,10 @@ def verify_drafts(
     the node reached, its children are tried in their order: with ``draft`` a token ``x`` is taken if ``uniform * q(x) <
     p(x)``, and a rejected one leaves ``norm(max(0, p - q))`` for ``p``; without, if ``uniform < p(x)``, and a rejected one
     leaves ``p`` without it, normalised.  What is left for ``p`` when no child is taken is what the next token is drawn from:
-    the least ``x`` at which its running sum is above the root's uniform times its sum.  So tokens are distributed as if
-    drawn from the target one after the other.  Sums and comparisons are in 64 bits.
+    the least ``x`` at which its running sum is above the root's uniform times its sum (``p`` itself, where nothing is left of
+    it).  So tokens are distributed as if drawn from the target one after the other.  Sums and comparisons are in 64 bits;
+    probabilities that are not positive count as 0, and none may be infinite.  At most 2^22 tokens of vocabulary, and fewer
+    than 2^16 sequences.
 
     Returns the nodes taken, root first (int32 ``[batch, nodes]``, of a pack ``[batch, 64 * words]``; -1 behind), their
     number (int32 ``[batch]``) and the next token (type of ``tokens``; -1 where the target has no probabilities, or the
