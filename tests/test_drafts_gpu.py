@@ -981,3 +981,118 @@ def test_verification_over_large_vocabularies(nodes, vocab):
         assert path[b, :int(accepted[b])].tolist() == want[0] and int(token[b]) == want[1], b
         counts.add(want[0][1] if len(want[0]) > 1 else 0)
     assert 0 in counts and len(counts) > 1  # (some with all rejected, some not)
+
+
+# ---- packs that begin behind the first row (cu_seqlens[0] > 0) -----------------------------------
+AHEAD = 37  # rows that are no sequence's, ahead of the first
+
+
+def behind(t, fill):
+    return torch.cat((t.new_full((AHEAD, *t.shape[1:]), fill), t))
+
+
+@pytest.mark.parametrize("case", [8, 9, 10, 13, 16, 20])
+def test_attention_of_packs_from_a_later_row(case):
+    from ring_swa import DraftTree, draft_tree
+
+    args, parents = tree_case(case)
+    q, k, v, tree, cache, table, lens, window, cu, sinks = args
+    later = DraftTree(behind(tree[0], 0), behind(tree[1], 5), behind(tree[2], -1))
+    out, lse = attend((*(behind(t, math.nan) for t in (q, k, v)), later, cache, table, lens, window, cu + AHEAD, sinks),
+                      return_lse=True)
+    check_tree(args, parents, out[AHEAD:], lse[:, AHEAD:])
+    most = max(map(len, parents))
+    made = draft_tree(behind(ints([x for p in parents for x in p] + [-2, -2]), -1), cu + AHEAD, max_nodes=most)
+    for mine, want in zip(made, tree):
+        assert torch.equal(mine[AHEAD:-2], want[:-2])
+
+
+@pytest.mark.parametrize("sampled", [True, False])
+def test_the_other_calls_of_packs_from_a_later_row(sampled):
+    from ring_swa import DraftTree, kv_cache_accept, kv_cache_read, verify_drafts
+
+    sizes, vocab = [9, 1, 0, 70, 3, 64], 3001
+    rng = random.Random(5)
+    g = torch.Generator().manual_seed(5)
+    parents = [some_parents(rng, n, 20, 0.02) for n in sizes]
+    tree = tree_tensors(parents, True)
+    p, q = (t.cuda() for t in probabilities(g, sum(sizes), vocab, torch.float32, 1.0))
+    base = [sum(sizes[:i]) for i in range(len(sizes) + 1)]
+    tokens = ints([x for b, own in enumerate(parents) for x in drawn(
+        rng, [i if -1 <= i < n else -2 for n, i in enumerate(own)], q[base[b]:base[b + 1]].cpu())])
+    u, cu = torch.rand(sum(sizes), generator=g).cuda(), ints(base)
+    want = verify_drafts(tree, tokens, p, q if sampled else None, u, cu)
+    later = DraftTree(behind(tree[0], -1), behind(tree[1], 0), behind(tree[2], 1))
+    got = verify_drafts(later, behind(tokens, 0), behind(p, math.nan), behind(q, math.nan) if sampled else None,
+                        behind(u, 0.0), cu + AHEAD)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert int(want[1].max()) > 1 or not sampled  # (tokens drawn from the draft: few are taken without it)
+
+    held = [10, 0, 200, 77, 63, 64]
+    k, v = (randn(g, torch.bfloat16, sum(sizes), 3, 64) for _ in range(2))
+    made = [make([h + 70 for h in held], 3, 64, 32, 44, wild=False) for _ in range(2)]
+    for (cache, table, _, _), ahead in zip(made, (0, AHEAD)):
+        kv_cache_accept(cache, behind(k, math.nan)[AHEAD - ahead:], behind(v, math.inf)[AHEAD - ahead:], want[0], table,
+                        ints(held), cu + ahead)
+    assert O.same_bytes(made[0][0], made[1][0])
+    cache, table, _, _ = made[0]
+    rows = [torch.full((sum(sizes) + ahead, 3, 64), 7.0, dtype=torch.bfloat16, device="cuda") for ahead in (0, 0, AHEAD, AHEAD)]
+    kv_cache_read(cache, *rows[:2], table, ints(held), cu)
+    kv_cache_read(cache, *rows[2:], table, ints(held), cu + AHEAD)
+    for mine, other in zip(rows[:2], rows[2:]):
+        assert torch.equal(mine, other[AHEAD:]) and bool((other[:AHEAD] == 7).all())
+
+
+@pytest.mark.parametrize("shape", [([0, 70, 500], 40, 4, 2), ([900, 64], 130, 8, 1), ([3000] * 8, 64, 16, 4)])
+def test_bits_of_any_kind_say_who_sees_whom(shape, monkeypatch):
+    """Ancestor bits that are no tree's (descendants, no node itself, nobody, nodes behind the last) and depths that are none's."""
+    from ring_swa import DraftTree
+
+    held, nodes, hq, hk = shape
+    g = torch.Generator().manual_seed(nodes)
+    words = (nodes + 63) // 64
+    bits = torch.rand(len(held), nodes, 64 * words, generator=g) < 0.3
+    bits[:, 3] = False
+    depths = torch.randint(0, nodes, (len(held), nodes), generator=g, dtype=torch.int32)
+    depths[:, 5] = -1
+    weights = torch.ones(64, dtype=torch.int64) << torch.arange(64)
+    packed = (bits.view(len(held), nodes, words, 64).long() * weights).sum(-1)
+    cache, table, seqlens, _ = make(held, hk, 64, 32, 9, max_pages=max(held) // 32 + 1)
+    q = randn(g, torch.bfloat16, len(held), nodes, hq, 64)
+    k, v = (randn(g, torch.bfloat16, len(held), nodes, hk, 64) for _ in range(2))
+    tree = DraftTree(depths.cuda(), depths.cuda(), packed.cuda())
+
+    def seen(b, length, window, sinks, there):
+        see = torch.cat((there.expand(nodes, length), bits[b, :, :nodes]), 1).clone()
+        see[depths[b] < 0] = False
+        return see
+
+    monkeypatch.setattr(R, "seen", seen)
+    args = (q, k, v, tree, cache, table, seqlens, -1, None, 0)
+    out, lse = attend(args, return_lse=True)
+    check_tree(args, list(range(len(held))), out, lse)
+
+
+@pytest.mark.parametrize("sampled", [True, False])
+def test_probabilities_beyond_2_to_31_elements(sampled):
+    """The last sequences of a batch: what they give alone."""
+    from ring_swa import DraftTree, verify_drafts
+
+    batch, nodes, vocab = 34, 32, 1 << 21
+    assert (batch - 2) * nodes * vocab >= 2 ** 31
+    g = torch.Generator(device="cuda").manual_seed(3)
+    parents = [[-1] + [max(0, i - 3) for i in range(1, nodes)]] * batch
+    tree = tree_tensors(parents, False)
+    p = torch.zeros(batch, nodes, vocab, dtype=torch.bfloat16, device="cuda")
+    q = torch.zeros_like(p) if sampled else None
+    for t in (p, q) if sampled else (p,):
+        t[-2:] = torch.softmax(3 * torch.randn(2, nodes, vocab, generator=g, device="cuda"), -1).bfloat16()
+    tokens = torch.randint(0, vocab, (batch, nodes), generator=g, device="cuda")
+    tokens[-1, 1::2] = p[-1, 0].argmax()
+    u = torch.rand(batch, nodes, generator=g, device="cuda")
+    u[-1, 1:] = 0
+    got = verify_drafts(tree, tokens, p, q, u)
+    alone = verify_drafts(DraftTree(*(t[-2:] for t in tree)), tokens[-2:], p[-2:].clone(), q[-2:].clone() if sampled else None, u[-2:])
+    assert all(torch.equal(a[-2:], b) for a, b in zip(got, alone))
+    assert int(alone[1].max()) > 1 and int(alone[2].min()) >= 0
+    assert got[1][:-2].tolist() == [1] * (batch - 2) and got[2][:-2].tolist() == [-1] * (batch - 2)  # (nothing in their rows)
