@@ -11,7 +11,7 @@
 // for itself; a second launch, a block for each sequence, goes on from there and draws the next token by the pieces' sums (for
 // large vocabularies some more passes are launches like the first, see stages_of).
 // Few sequences are launches and round trips: a chain of 6 over 131072 tokens 10.1 us, 4.0 + 6.3 of kernels.  Where siblings are
-// rejected the passes come one after the other: 32 trees of 32 nodes over 32768 tokens 31 us, up to 4 passes behind the first.
+// rejected the passes come one after the other: 32 trees of 32 nodes over 32768 tokens 30 us, up to 4 passes behind the first.
 #include "kv_cache.h"
 
 namespace rswa {
@@ -245,15 +245,19 @@ struct Rest {
     Vec p, q;
   };
   __device__ __forceinline__ int base(int x0) const { return min(x0, vocab - N); }
-  // vectors from x0 on, `step` apart, all on their way at once
+  // vectors from x0 on, `step` apart, all on their way at once (of rows of N tokens or more)
+  template <int M>
+  __device__ __forceinline__ void load_row(int x0, int step, Raw (&v)[M]) const {
+#pragma unroll
+    for (int i = 0; i < M; i++) {
+      v[i].p = *(const Vec*)(p + base(x0 + i * step));
+      if constexpr (DRAFT) v[i].q = *(const Vec*)(q + base(x0 + i * step));
+    }
+  }
   template <int M>
   __device__ __forceinline__ void load(int x0, int step, Raw (&v)[M]) const {
     if (vocab >= N) {
-#pragma unroll
-      for (int i = 0; i < M; i++) {
-        v[i].p = *(const Vec*)(p + base(x0 + i * step));
-        if constexpr (DRAFT) v[i].q = *(const Vec*)(q + base(x0 + i * step));
-      }
+      load_row(x0, step, v);
     } else {
 #pragma unroll
       for (int i = 0; i < M; i++)
@@ -305,27 +309,38 @@ __device__ __forceinline__ double of_lane(double v, int lane) {  // (the same la
 }
 __device__ __forceinline__ double wave_sum(double v) { return of_lane(wave_scan(v), 63); }
 
-// Sums over M pieces, `step` apart, by one wave: all of their loads first.
-template <int M, typename T, bool DRAFT>
-__device__ __forceinline__ void piece_sums(const Rest<T, DRAFT>& rest, int piece, int step, double (&sum)[M]) {
-  using R = Rest<T, DRAFT>;
-  constexpr int TURNS = kPiece / (64 * R::N);
-  typename R::Raw v[M][TURNS];
-  auto first = [&](int m) { return (piece + m * step) * kPiece + lane_id() * R::N; };
+// M pieces, `step` apart, as one wave has them ...
+template <typename R>
+constexpr int kTurns = kPiece / (64 * R::N);
+template <int M, typename R>
+__device__ __forceinline__ void load_pieces(const R& rest, int piece, int step, typename R::Raw (&v)[M][kTurns<R>]) {
 #pragma unroll
-  for (int m = 0; m < M; m++) rest.load(first(m), 64 * R::N, v[m]);
+  for (int m = 0; m < M; m++) rest.load((piece + m * step) * kPiece + lane_id() * R::N, 64 * R::N, v[m]);
+}
+// ... and their sums.
+template <int M, typename R>
+__device__ __forceinline__ void sum_pieces(const R& rest, int piece, int step, const typename R::Raw (&v)[M][kTurns<R>],
+                                           double (&sum)[M]) {
 #pragma unroll
   for (int m = 0; m < M; m++) {
     sum[m] = 0.0;
 #pragma unroll
-    for (int i = 0; i < TURNS; i++) {
+    for (int i = 0; i < kTurns<R>; i++) {
       double r[R::N];
-      rest.values(first(m) + i * 64 * R::N, v[m][i], r);
+      rest.values((piece + m * step) * kPiece + (lane_id() + i * 64) * R::N, v[m][i], r);
 #pragma unroll
       for (int e = 0; e < R::N; e++) sum[m] += r[e];
     }
     sum[m] = wave_sum(sum[m]);
   }
+}
+template <typename R>
+__device__ __forceinline__ double piece_sum(const R& rest, int piece) {
+  typename R::Raw v[1][kTurns<R>];
+  double sum[1];
+  load_pieces(rest, piece, 0, v);
+  sum_pieces(rest, piece, 0, v, sum);
+  return sum[0];
 }
 
 constexpr int kFirstThreads = 256, kFirstPieces = kFirstThreads / 64;
@@ -352,9 +367,8 @@ __global__ __launch_bounds__(kFirstThreads) void verify_first_kernel(const Verif
   if constexpr (!DRAFT) list_tried(s, w.cur, w.next, kFirstThreads);
   if (piece >= a.pieces) return;
   const Rest<T, DRAFT> rest{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, s.tried, DRAFT ? 0 : s.n_tried};
-  double sum[1];
-  piece_sums(rest, piece, 0, sum);
-  if ((threadIdx.x & 63) == 0) a.sums[(int64_t)b * a.pieces + piece] = sum[0];
+  const double sum = piece_sum(rest, piece);
+  if ((threadIdx.x & 63) == 0) a.sums[(int64_t)b * a.pieces + piece] = sum;
 }
 
 // A lane's share of the sums of `pieces` pieces: as many as each in a row.
@@ -384,9 +398,9 @@ __global__ __launch_bounds__(kFirstThreads) void verify_next_kernel(const Verify
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) a.walks[(int64_t)a.stage * a.batch + b] = w;
   if (piece >= a.pieces || w.count == 0) return;
-  double sum[1] = {wanted ? 0.0 : sums[piece]};
-  if (wanted) piece_sums(Rest<T, true>{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, nullptr, 0}, piece, 0, sum);
-  if ((threadIdx.x & 63) == 0) to[piece] = sum[0];
+  const double sum = wanted ? piece_sum(Rest<T, true>{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, nullptr, 0}, piece)
+                            : sums[piece];
+  if ((threadIdx.x & 63) == 0) to[piece] = sum;
 }
 
 constexpr int kRestThreads = 1024, kRestWaves = kRestThreads / 64;
@@ -412,28 +426,55 @@ __global__ __launch_bounds__(kRestThreads) void verify_rest_kernel(const VerifyA
   if (w.count > 0 && (!DRAFT || !w.draw)) seq.load(s, kRestThreads);
   if (threadIdx.x == 0) found = last_positive = -1;
   __syncthreads();
-  auto pass = [&](const R& rest) {  // sums of all pieces
-    __syncthreads();
-    for (int i = wave; i < a.pieces; i += 2 * kRestWaves) {  // (a piece behind the last: 0, as the row's end)
-      double of[2];
-      piece_sums(rest, i, kRestWaves, of);
-      if (lane == 0) {
-        sums[i] = of[0];
-        if (i + kRestWaves < a.pieces) sums[i + kRestWaves] = of[1];
-      }
-    }
-    __syncthreads();
-  };
   // (all waves do the same)
   const int per = (a.pieces + 63) / 64;
   int drawn = -1;
   if (w.count > 0) {
     if constexpr (DRAFT) {
-      while (!w.draw) {
-        w.mass = wave_sum(lane_total(sums, a.pieces));
-        walk_on<DRAFT>(s, w, seq.n, path);
-        pass(R{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, nullptr, 0});
-      }
+      // Rows of up to two pieces a wave stay in registers from one sibling to the next (32 trees of 32 nodes, us: over 32768
+      // tokens 31.7 -> 29.7, over 8192 23.8 -> 18.9).
+      auto rejections = [&](auto few) {
+        [[maybe_unused]] typename R::Raw v[2][1][kTurns<R>];
+        [[maybe_unused]] int held_node = -1;
+        while (!w.draw) {
+          w.mass = wave_sum(lane_total(sums, a.pieces));
+          walk_on<DRAFT>(s, w, seq.n, path);
+          const R rest{seq.p_row(w.cur), seq.q_row(w.cur), w.a, a.vocab, nullptr, 0};
+          __syncthreads();
+          if constexpr (few) {
+            if (w.cur != held_node) {
+#pragma unroll
+              for (int m = 0; m < 2; m++)
+                if (wave + m * kRestWaves < a.pieces)
+                  rest.load_row((wave + m * kRestWaves) * kPiece + lane * N, 64 * N, v[m][0]);
+            }
+            held_node = w.cur;
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+              if (wave + m * kRestWaves < a.pieces) {
+                double of[1];
+                sum_pieces(rest, wave + m * kRestWaves, 0, v[m], of);
+                if (lane == 0) sums[wave + m * kRestWaves] = of[0];
+              }
+          } else {
+            for (int i = wave; i < a.pieces; i += 2 * kRestWaves) {  // (a piece behind the last: 0, as the row's end)
+              typename R::Raw both[2][kTurns<R>];
+              double of[2];
+              load_pieces(rest, i, kRestWaves, both);
+              sum_pieces(rest, i, kRestWaves, both, of);
+              if (lane == 0) {
+                sums[i] = of[0];
+                if (i + kRestWaves < a.pieces) sums[i + kRestWaves] = of[1];
+              }
+            }
+          }
+          __syncthreads();
+        }
+      };
+      if (a.pieces <= 2 * kRestWaves && a.vocab >= N)
+        rejections(std::true_type{});
+      else
+        rejections(std::false_type{});
     } else {
       list_tried(s, w.cur, w.next, kRestThreads);
     }
@@ -442,7 +483,12 @@ __global__ __launch_bounds__(kRestThreads) void verify_rest_kernel(const VerifyA
     if (!(all > 0.0)) {  // nothing is left
       rest.a = 0.0;
       rest.n_tried = 0;
-      pass(rest);
+      __syncthreads();
+      for (int i = wave; i < a.pieces; i += kRestWaves) {
+        const double of = piece_sum(rest, i);
+        if (lane == 0) sums[i] = of;
+      }
+      __syncthreads();
       own = lane_total(sums, a.pieces);
       upto = wave_scan(own);
       all = of_lane(upto, 63);

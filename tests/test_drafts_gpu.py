@@ -958,9 +958,10 @@ def test_a_graph_that_has_saved_the_rows_notices_a_read(native, monkeypatch):
     kv_cache_read(cache, k, v, table, first)
 
 
-@pytest.mark.parametrize("nodes,vocab", [(8, 70000), (9, 65536), (9, 65535), (24, 65537), (24, 131072)])
+@pytest.mark.parametrize("nodes,vocab", [(8, 70000), (9, 65536), (9, 65535), (24, 65537), (24, 131072),
+                                         (24, 32768), (24, 32769), (24, 16385), (24, 16384), (9, 8191)])
 def test_verification_over_large_vocabularies(nodes, vocab):
-    """(Passes of several launches from 65536 tokens and 9 nodes on.)  All siblings of the root, most of them rejected."""
+    """(Passes of several launches from 65536 tokens and 9 nodes on; rows held in registers up to 32768.)  All siblings of the root, most of them rejected."""
     from ring_swa import verify_drafts
 
     g = torch.Generator().manual_seed(nodes + vocab)
