@@ -556,9 +556,11 @@ int pieces_of(int vocab) { return (int)ceil_div(vocab, kPiece); }
 // Launches between the first and the last: a pass over all compute units takes 4 us (2.5 if no sequence wants it), one by the
 // last launch's block for a sequence 4.5 of 32768 tokens and 15 of 131072.  So three for large vocabularies and trees, of
 // whose sequences some reject a few siblings: 8 sequences of 32 nodes over 131072 tokens 65 us without, 31 with three, 32 with
-// five; 32 of 8 over 32768 22.0 and 24.8.  Not for what is likely a chain, which rejects once (6 nodes over 131072 11.6, 19.3).
+// five; 32 of 8 over 32768 22.0 and 24.8.  Not for what is likely a chain, which rejects once (6 nodes over 131072 9.9, 19.0).
+// Of a pack the mean count of nodes says which it is: its max_nodes is that of whole words of ancestors, 64 at least.
 int stages_of(const rswa_verify_params* p) {
-  return p->draft && p->vocab >= 65536 && (p->cu_seqlens ? p->max_nodes : p->nodes) > 8 ? 3 : 0;
+  const int64_t nodes = p->cu_seqlens ? ceil_div(p->total, std::max(1, p->batch)) : p->nodes;
+  return p->draft && p->vocab >= 65536 && nodes > 8 ? 3 : 0;
 }
 
 uint64_t walk_bytes(const rswa_verify_params* p) {
