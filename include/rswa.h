@@ -462,9 +462,12 @@ uint64_t rswa_sizeof_cache_params(void);
 /*
  * The inverse of rswa_cache_append: rows of new_k and new_v [.., heads_kv, head_dim], which this call WRITES, are
  * tokens seqlens[b], seqlens[b] + 1, .. of their sequence (below zero counts as zero), their values rounded to dtype
- * (infinite where it holds them as that).  Rows of tokens that have no page, or lie beyond the table, are zeros.
+ * (infinite where it holds them as that).  Rows of tokens that have no page, or lie beyond the table, are zeros.  No two
+ * rows may share an element, new_k's with new_v's neither (nor with the cache, which is not checked).
  */
 int rswa_cache_read(const rswa_cache_params* p, void* stream);
+/* 1 if rows do, by the sizes, strides and addresses of new_k and new_v alone (no device is asked). */
+int rswa_cache_read_rows_meet(const rswa_cache_params* p);
 
 /*
  * A step of drafted tokens over the cache.  No counterpart in the upstream package.

@@ -6,6 +6,8 @@
 // Bound by memory, of which two thirds are written: prefixes of 31300 tokens together, 8 heads of 128, 193 MB in 33 us, 5.8
 // TB/s with the codes partly in the last-level cache.  The values go past the caches (through them 47 us, and with
 // codes that do not stay there 56).
+#include <algorithm>
+
 #include "kv_cache.h"
 
 namespace rswa {
@@ -98,8 +100,86 @@ __global__ void cache_read_kernel(const ReadArgs a) {
       __builtin_nontemporal_store(values8<T>(codes[e][0], codes[e][1], exponent), (V8*)(x + e * a.x_st[which][1]));
 }
 
+// ---- rows that share an element ----
+// They are written by many blocks at once, so that none may.  A row's address is a sum of counts times strides: two rows meet
+// where the difference of two such sums, with the counts' differences in their ranges, is below head_dim.  It is looked for from the
+// largest stride down, as far as the smaller ones reach: of dimensions that lie inside one another a count or two at each.
+struct Differences {
+  typedef __int128 wide;  // (strides and counts are the caller's)
+  struct Step {
+    wide by, lo, hi;  // lo .. hi times `by`
+  };
+  Step of[6];
+  wide lo_behind[7], hi_behind[7];  // what the steps from each on reach
+  int n = 0, looked = 0, dim;
+  explicit Differences(int dim_) : dim(dim_) {}
+
+  void add(wide by, wide lo, wide hi, bool join) {
+    if (by < 0) {
+      by = -by;
+      std::swap(lo, hi);
+      lo = -lo;
+      hi = -hi;
+    }
+    for (int i = 0; join && i < n; i++)
+      if (of[i].by == by) {
+        of[i].lo += lo;
+        of[i].hi += hi;
+        return;
+      }
+    of[n++] = {by, lo, hi};
+  }
+  // Is from + some sum below `dim`?  (`other`: of counts that are not all 0)
+  bool found(wide from, bool other) {
+    std::sort(of, of + n, [](const Step& a, const Step& b) { return a.by > b.by; });
+    lo_behind[n] = hi_behind[n] = 0;
+    for (int i = n - 1; i >= 0; i--) {
+      lo_behind[i] = lo_behind[i + 1] + of[i].by * of[i].lo;
+      hi_behind[i] = hi_behind[i + 1] + of[i].by * of[i].hi;
+    }
+    return look(0, from, other);
+  }
+  bool look(int i, wide from, bool other) {
+    if (++looked > 4096) return true;  // (no layout of tensors in use comes near it)
+    if (i == n) return !other && from < dim && -from < dim;
+    const Step& s = of[i];
+    wide lo = s.lo, hi = s.hi;
+    if (s.by > 0) {
+      const wide least = -dim + 1 - from - hi_behind[i + 1], most = dim - 1 - from - lo_behind[i + 1];
+      const auto down = [&](wide v) { return v >= 0 ? v / s.by : -((-v + s.by - 1) / s.by); };
+      lo = std::max(lo, -down(-least));
+      hi = std::min(hi, down(most));
+    }
+    for (wide c = lo; c <= hi; c++)
+      if (look(i + 1, from + c * s.by, other && c == 0)) return true;
+    return false;
+  }
+};
+
+bool rows_meet(const rswa_cache_params* p) {
+  const bool packed = p->cu_seqlens_q != nullptr;
+  const int64_t count[3] = {packed ? 1 : p->batch, packed ? p->total_q : p->seqlen_q, p->heads_kv};
+  for (int64_t c : count)
+    if (c <= 0) return false;
+  Differences both(p->head_dim);
+  for (const int64_t* st : {p->new_k_stride, p->new_v_stride}) {
+    Differences own(p->head_dim);
+    for (int d = 0; d < 3; d++)
+      if (count[d] > 1) {
+        own.add(st[d], 1 - count[d], count[d] - 1, false);
+        st == p->new_k_stride ? both.add(st[d], 1 - count[d], 0, true) : both.add(st[d], 0, count[d] - 1, true);
+      }
+    if (own.found(0, true)) return true;
+  }
+  // (an element is two bytes: addresses apart by an odd number share one too if they are less than dim elements apart)
+  const intptr_t apart = (intptr_t)p->new_v - (intptr_t)p->new_k;
+  return both.found(apart / 2, false);
+}
+
 }  // namespace
 }  // namespace rswa
+
+extern "C" int rswa_cache_read_rows_meet(const rswa_cache_params* p) { return p && rswa::rows_meet(p); }
 
 extern "C" int rswa_cache_read(const rswa_cache_params* p, void* stream) {
   using namespace rswa;
@@ -110,6 +190,7 @@ extern "C" int rswa_cache_read(const rswa_cache_params* p, void* stream) {
   if (rows == 0 || p->batch == 0) return RSWA_OK;
   const void* x[2];
   if (int rc = cache_new_rows(p, who, x, a.x_st)) return rc;
+  RSWA_REQUIRE(!rows_meet(p), RSWA_ERR_INVALID, "%s: rows of new_k and new_v, which are written, overlap", who);
   for (int w = 0; w < 2; w++) a.x[w] = const_cast<void*>(x[w]);
   a.pages = (int32_t)((p->seqlen_q + (int64_t)p->page_size - 2) / p->page_size + 1);
   const int64_t slots =

@@ -579,9 +579,6 @@ PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 6 || !cache_lib.read || observed()) Py_RETURN_NONE;
   const Tensor *k = given(args[1]), *v = given(args[2]);
   if (!k || !v || !c.set(args[0], args[3], args[4]) || !c.rows(*k, args[5]) || !c.new_rows(k, v, *k)) Py_RETURN_NONE;
-  for (const Tensor* t : {k, v})
-    for (int64_t d = 0; d < t->dim(); d++)
-      if (t->size(d) > 1 && t->stride(d) == 0) Py_RETURN_NONE;  // (rows that are one another's)
   c10::DeviceGuard guard(c.device);
   if (c.launch(cache_lib.read) != RSWA_OK) Py_RETURN_NONE;
   for (const Tensor* t : {k, v})

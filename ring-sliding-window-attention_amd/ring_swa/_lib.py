@@ -274,6 +274,8 @@ def load(path: str) -> ctypes.CDLL:
         fn = getattr(L, name)
         fn.restype = c_int
         fn.argtypes = [POINTER(CacheParams), c_void_p]
+    L.rswa_cache_read_rows_meet.restype = c_int
+    L.rswa_cache_read_rows_meet.argtypes = [POINTER(CacheParams)]
     L.rswa_cache_attn_workspace_bytes.restype = c_uint64
     L.rswa_cache_attn_workspace_bytes.argtypes = [POINTER(CacheParams)]
     for name, params in (("rswa_draft_tree", TreeParams), ("rswa_cache_tree_attn", DraftParams),

@@ -250,8 +250,9 @@ def kv_cache_read(
     """Read tokens back: the inverse of ``kv_cache_append``, with the same arguments.
 
     ``k`` and ``v`` (``[batch, seq, kv_heads, dim]``, or packed ``[tokens, kv_heads, dim]`` with ``cu_seqlens``;
-    bf16 or fp16) are written: row ``i`` of a sequence is its token ``first + i`` (``first``: int32 ``[batch]``, below
-    zero counts as zero), a code times its page's scale rounded to the type (infinite where the type holds it as that).
+    bf16 or fp16) are written, and may not overlap, themselves or each other: row ``i`` of a sequence is its token
+    ``first + i`` (``first``: int32 ``[batch]``, below zero counts as zero), a code times its page's scale rounded to the type
+    (infinite where the type holds it as that).
     Rows of tokens that have no page are zeros; rows of a pack that are no sequence's are left alone.  So a cached
     prefix goes to the attention functions, to another page size or to another device."""
     if torch.compiler.is_dynamo_compiling():
@@ -268,8 +269,7 @@ def kv_cache_read(
 def _read(to_k, to_v, k, v, k_scale, v_scale, page_table, first, cu_seqlens):
     p, dev = _cache_params((k, v, k_scale, v_scale), page_table, first, to_k, cu_seqlens)
     _new_rows(p, to_k, to_v, cu_seqlens is not None)
-    for t in (to_k, to_v):
-        assert all(n <= 1 or s != 0 for n, s in zip(t.shape, t.stride())), "k and v are written: their rows must not overlap"
+    assert not _lib.lib().rswa_cache_read_rows_meet(p), "k and v are written: their rows must not overlap"
     for t in (to_k, to_v):
         if not t.is_inference():  # (a graph that has saved them for its backward is to notice)
             torch.autograd.graph.increment_version(t)
