@@ -534,7 +534,8 @@ uint64_t rswa_sizeof_verify_params(void);
 
 /*
  * Which drafts the target's probabilities take, and the token behind them, so that tokens are distributed as if drawn from
- * the target one by one.  Rows as in rswa_tree_params.  Node 0 is the root: a token that is chosen already.  target[i, x]
+ * the target one by one, if rows sum to 1 (they are not made to: a token's distribution is off, in total variation, by no
+ * more than what the target's sum differs from 1, and the draft's for each child that is tried).  Rows as in rswa_tree_params.  Node 0 is the root: a token that is chosen already.  target[i, x]
  * is the probability of token x behind node i, draft[i, x] the one that the children of node i were drawn with
  * (independently), uniforms[i] a number from [0, 1).  From the root on, at the node reached, with p and q its rows, a = 0
  * and S = 1, its children i are tried in their order, r(x) = max(0, p(x) - a q(x)):

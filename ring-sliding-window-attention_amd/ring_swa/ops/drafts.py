@@ -199,11 +199,14 @@ def verify_drafts(
     ``target``: ``[batch, nodes, vocab]``, the probabilities behind each node, fp32, bf16 or fp16; ``draft``: the same of
     the draft model, which the children of a node were drawn from, independently, or None: the children were named outright
     (its likeliest tokens, say); ``uniforms``: fp32 ``[batch, nodes]``, numbers from [0, 1).  With ``p`` and ``q`` the rows of
-    the node reached, its children are tried in their order: with ``draft`` a token ``x`` is taken if ``uniform * q(x) <
-    p(x)``, and a rejected one leaves ``norm(max(0, p - q))`` for ``p``; without, if ``uniform < p(x)``, and a rejected one
-    leaves ``p`` without it, normalised.  What is left for ``p`` when no child is taken is what the next token is drawn from:
-    the least ``x`` at which its running sum is above the root's uniform times its sum (``p`` itself, where nothing is left of
-    it).  So tokens are distributed as if drawn from the target one after the other.  Sums and comparisons are in 64 bits;
+    the node reached, its children are tried in their order: with ``draft`` a token ``x`` is taken if ``uniform * S * q(x) <
+    p(x)``, S = 1 for the first, and a rejected one leaves ``max(0, p - S * q)`` for ``p`` and its sum for S; without, if
+    ``uniform * S < p(x)``, and a rejected one leaves ``p`` without it and ``S - p(x)`` for S.  What is left of ``p`` when no child
+    is taken is what the next token is drawn from: the least ``x`` at which its running sum is above the root's uniform times its
+    sum (``p`` itself, where nothing is left of it).  So tokens are distributed as if drawn from the target one after the other,
+    if rows sum to 1.  They are not made to: a token's distribution is off (in total variation) by no more than what the
+    target's sum differs from 1, and the draft's for each child tried (rows rounded to 16 bits: some 1e-3); without ``draft`` a
+    child that has all of S is taken, whatever is left of ``p`` beside it.  Sums and comparisons are in 64 bits;
     probabilities that are not positive count as 0, and none may be infinite.  At most 2^22 tokens of vocabulary, and fewer
     than 2^16 sequences.
 
