@@ -10,8 +10,9 @@
 // The first pass -- a chain has no other -- is one launch over all rows in pieces of 1024 tokens, each of whose blocks walks
 // for itself; a second launch, a block for each sequence, goes on from there and draws the next token by the pieces' sums (for
 // large vocabularies some more passes are launches like the first, see stages_of).
-// Few sequences are launches and round trips: a chain of 6 over 131072 tokens 10.1 us, 4.0 + 6.3 of kernels.  Where siblings are
-// rejected the passes come one after the other: 32 trees of 32 nodes over 32768 tokens 30 us, up to 4 passes behind the first.
+// Few sequences are launches and round trips: a chain of 6 over 131072 tokens 9.1 to 10.6 us among other calls, its kernels by
+// themselves 4.0 + 6.4 at least.  Where siblings are rejected the passes come one after the other: 32 trees of 32 nodes over 32768
+// tokens 28 to 31 us, up to 4 passes behind the first (5.3 + 23.6).
 #include "kv_cache.h"
 
 namespace rswa {
@@ -431,8 +432,9 @@ __global__ __launch_bounds__(kRestThreads) void verify_rest_kernel(const VerifyA
   int drawn = -1;
   if (w.count > 0) {
     if constexpr (DRAFT) {
-      // Rows of up to two pieces a wave stay in registers from one sibling to the next (32 trees of 32 nodes, us: over 32768
-      // tokens 31.7 -> 29.7, over 8192 23.8 -> 18.9).
+      // Rows of up to two pieces a wave stay in registers from one sibling to the next (32 trees of 32 nodes over 8192 tokens 23.8 ->
+      // 18.9 us; the same rows over 32768 tokens and, with one more, read again, three inputs: 23.0 / 24.3, 19.4 / 21.6, 23.3 /
+      // 27.0, 64 trees 34.0 / 37.2, 25.1 / 28.5, 29.0 / 33.8).
       auto rejections = [&](auto few) {
         [[maybe_unused]] typename R::Raw v[2][1][kTurns<R>];
         [[maybe_unused]] int held_node = -1;
@@ -556,7 +558,10 @@ int pieces_of(int vocab) { return (int)ceil_div(vocab, kPiece); }
 // Launches between the first and the last: a pass over all compute units takes 4 us (2.5 if no sequence wants it), one by the
 // last launch's block for a sequence 4.5 of 32768 tokens and 15 of 131072.  So three for large vocabularies and trees, of
 // whose sequences some reject a few siblings: 8 sequences of 32 nodes over 131072 tokens 65 us without, 31 with three, 32 with
-// five; 32 of 8 over 32768 22.0 and 24.8.  Not for what is likely a chain, which rejects once (6 nodes over 131072 9.9, 19.0).
+// five; 32 of 8 over 32768 22.0 and 24.8.  The same rows over 65535 tokens without and over 65536 with, three inputs: 32 of 32 nodes
+// 37.2 / 27.8, 45.7 / 34.9, 38.9 / 29.1, 8 of 32 28.6 / 24.0, 38.2 / 26.7, 35.1 / 25.9, 8 of 16 21.2 / 22.1, 30.4 / 24.7, 21.2 / 22.1,
+// one of 32 20.2 / 21.4, 10.6 / 19.0, 27.0 / 21.9, as rejections come.  (Between 32768 and 65536
+// tokens launches have not been timed.)  Not for what is likely a chain, which rejects once (6 nodes over 131072 9.9, 19.0).
 // Of a pack the mean count of nodes says which it is: its max_nodes is that of whole words of ancestors, 64 at least.
 int stages_of(const rswa_verify_params* p) {
   const int64_t nodes = p->cu_seqlens ? ceil_div(p->total, std::max(1, p->batch)) : p->nodes;
