@@ -140,7 +140,7 @@ struct Differences {
     return look(0, from, other);
   }
   bool look(int i, wide from, bool other) {
-    if (++looked > 4096) return true;  // (no layout of tensors in use comes near it)
+    if (++looked > 4096) return true;  // (refused unproven: no layout of tensors in use comes near it)
     if (i == n) return !other && from < dim && -from < dim;
     const Step& s = of[i];
     wide lo = s.lo, hi = s.hi;
@@ -171,7 +171,7 @@ bool rows_meet(const rswa_cache_params* p) {
       }
     if (own.found(0, true)) return true;
   }
-  // (an element is two bytes: addresses apart by an odd number share one too if they are less than dim elements apart)
+  // (elements of two bytes, and of addresses that are 16-byte aligned, or refused before)
   const intptr_t apart = (intptr_t)p->new_v - (intptr_t)p->new_k;
   return both.found(apart / 2, false);
 }
